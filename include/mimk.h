@@ -333,6 +333,40 @@ typedef struct mimk_mlp_desc {
 } mimk_mlp_desc;
 int mimk_mlp_gated(const mimk_mlp_desc* desc, void* stream);
 
+/* ---- training ------------------------------------------------------------------------------------------
+ * The operators from here to the generic operation are the ends of a training step: they have no counterpart in the reference,
+ * whose `tensor` plugin has no gradients. Their scratch is the caller's: a `workspace` of at least the bytes that the operator's size
+ * query answers for the same descriptor, aligned to 16 bytes (MIMK_E_ALIGN otherwise, MIMK_E_WORKSPACE if it is missing or too small), of any
+ * content, free again once the call's work on `stream` is done. They allocate nothing and may be captured.
+ *
+ * The gated MLP block with its gradients, bf16:
+ *   fwd: a = X W1, b = X W3, h = silu(a) * b, Y = h W2, with a, b (f32) and h (bf16) left in `kept`;
+ *   bwd: from dY and the same `kept`, X and weights: dX, dW1, dW3, dW2, the weights' gradients in the weights' own layout.
+ * h, da and db are rounded to bf16 between the products, a and b are not; sums are f32. Any extents, zero included (gradients of no
+ * rows are zeros); rows that are no multiple of 16 bytes, and unaligned matrices, are copied into the workspace first.
+ * Equal descriptors give equal bits call after call. */
+typedef struct mimk_mlp_train_desc {
+    int64_t m, k, f, n;
+    const void* x;  /* [m, k] */
+    const void* w1; /* [k, f], or [f, k] with MIMK_B_NK; so w3 */
+    const void* w3;
+    const void* w2; /* [f, n], or [n, f] */
+    void* y;        /* fwd: [m, n] */
+    void* kept;     /* fwd writes it, bwd reads it; aligned to 16 bytes */
+    const void* dy; /* bwd: [m, n] */
+    void* dx;       /* bwd */
+    void* dw1;
+    void* dw3;
+    void* dw2;
+    void* workspace;
+    uint64_t workspace_bytes;
+    int32_t dtype, b_layout;
+} mimk_mlp_train_desc;
+/* Bytes of `kept` and of the two calls' workspaces; any of the three may be NULL. The matrices' addresses count (their alignment). */
+int mimk_mlp_gated_train_sizes(const mimk_mlp_train_desc* desc, uint64_t* kept, uint64_t* forward, uint64_t* backward);
+int mimk_mlp_gated_fwd(const mimk_mlp_train_desc* desc, void* stream);
+int mimk_mlp_gated_bwd(const mimk_mlp_train_desc* desc, void* stream);
+
 /* ---- the generic operation ------------------------------------------------------------------------------
  * out[map_out(o)] = post(fold_r f(acc, (in_i[maps_i(o, r)])_i), (post_in_j[post_maps_j(map_out(o))])_j)
  * over the loop vector (o..., r...) with bounds `sr`: the leading `ro` loops are the output loops, the trailing

@@ -25,7 +25,7 @@ ROWS_SOFTMAX, ROWS_RMSNORM, ROWS_SOFTMAX_RMSNORM = 0, 1, 2
 SYMBOLS = (
     "mimk_status_str", "mimk_abi_version", "mimk_last_cuda_error", "mimk_device_check", "mimk_device_status", "mimk_selftest_wait_expiry",
     "mimk_gemm", "mimk_gemm_flat", "mimk_gemm_gather", "mimk_gemm_reduce_scatter", "mimk_gemm_kpanels", "mimk_reduce", "mimk_reduce_fused", "mimk_reduce_plan", "mimk_reduce_tiles", "mimk_reduce_static", "mimk_softmax", "mimk_rmsnorm", "mimk_softmax_rmsnorm", "mimk_map", "mimk_map_t",
-    "mimk_splat", "mimk_select", "mimk_generate_affine", "mimk_gather", "mimk_scatter", "mimk_attn_fwd", "mimk_conv", "mimk_conv_laid_out", "mimk_mlp_gated", "mimk_map_reduce_post", "mimk_mrp_classify", "mimk_mrp_cell_kernel", "mimk_program_classify", "mimk_program_run", "mimk_chain_order", "mimk_chain_cost",
+    "mimk_splat", "mimk_select", "mimk_generate_affine", "mimk_gather", "mimk_scatter", "mimk_attn_fwd", "mimk_conv", "mimk_conv_laid_out", "mimk_mlp_gated", "mimk_mlp_gated_train_sizes", "mimk_mlp_gated_fwd", "mimk_mlp_gated_bwd", "mimk_map_reduce_post", "mimk_mrp_classify", "mimk_mrp_cell_kernel", "mimk_program_classify", "mimk_program_run", "mimk_chain_order", "mimk_chain_cost",
     "mimk_host_rows", "mimk_host_rows_pair", "mimk_host_gemm", "mimk_host_attn_fwd", "mimk_host_mlp_gated", "mimk_host_map_reduce_post", "mimk_host_register",
     "mimk_host_unregister", "mimk_host_release",
 )
@@ -79,6 +79,15 @@ class MlpDesc(C.Structure):
         ("m", C.c_int64), ("k", C.c_int64), ("f", C.c_int64), ("n", C.c_int64),
         ("x", C.c_void_p), ("w1", C.c_void_p), ("w3", C.c_void_p), ("w2", C.c_void_p), ("y", C.c_void_p),
         ("h", C.c_void_p), ("dtype", C.c_int32), ("b_layout", C.c_int32),
+    ]
+
+
+class MlpTrainDesc(C.Structure):
+    _fields_ = [
+        ("m", C.c_int64), ("k", C.c_int64), ("f", C.c_int64), ("n", C.c_int64),
+        ("x", C.c_void_p), ("w1", C.c_void_p), ("w3", C.c_void_p), ("w2", C.c_void_p), ("y", C.c_void_p), ("kept", C.c_void_p),
+        ("dy", C.c_void_p), ("dx", C.c_void_p), ("dw1", C.c_void_p), ("dw3", C.c_void_p), ("dw2", C.c_void_p),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64), ("dtype", C.c_int32), ("b_layout", C.c_int32),
     ]
 
 
@@ -167,6 +176,9 @@ def lib() -> C.CDLL:
         L.mimk_gather.argtypes = [vp, vp, vp, ci, ci, ci, C.POINTER(i64), C.POINTER(i64), ci, vp]
         L.mimk_scatter.argtypes = [vp, vp, vp, vp, ci, ci, ci, C.POINTER(i64), C.POINTER(i64), C.POINTER(i64), ci, vp]
         L.mimk_mlp_gated.argtypes = [C.POINTER(MlpDesc), vp]
+        u64p = C.POINTER(C.c_uint64)
+        L.mimk_mlp_gated_train_sizes.argtypes = [C.POINTER(MlpTrainDesc), u64p, u64p, u64p]
+        L.mimk_mlp_gated_fwd.argtypes = L.mimk_mlp_gated_bwd.argtypes = [C.POINTER(MlpTrainDesc), vp]
         L.mimk_map_reduce_post.argtypes = [C.POINTER(MrpDesc), vp]
         L.mimk_mrp_classify.argtypes = [C.POINTER(MrpDesc)]
         L.mimk_mrp_cell_kernel.argtypes = [C.POINTER(MrpDesc), C.POINTER(C.c_int32)]

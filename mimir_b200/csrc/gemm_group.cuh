@@ -1,0 +1,496 @@
+// Products of a training step on paired SMs: the pipeline of gemm_tc2.cu (TMA producer, one issuer of tcgen05.mma.cta_group::2, four epilogue
+// warps per CTA, two accumulators in tensor memory) with what gradients need beyond a forward product:
+//   - either operand K-major or MN-major, so that x^T dy reads both matrices where the forward pass left them;
+//   - two operand pairs added in one accumulator (da W1^T + db W3^T);
+//   - several products in one launch (the three weight gradients and the input's), so that the last, half empty round of tiles comes once;
+//   - the k-blocks of a tile dealt out over several tiles, each with an f32 partial result of its own, where there are few tiles;
+//   - extents that are known on the device only (the rows that are left once those without a target are taken out);
+//   - epilogues that keep what a gradient needs, or turn an accumulator into one, without the product ever being written.
+// A tile is 256 rows (128 per CTA) by 256 columns (128 + 128 of two right operands for the gated form).
+#pragma once
+
+#include "common.cuh"
+#include "sm100_pair.cuh"
+
+namespace mimk {
+namespace group {
+
+using namespace sm100;
+
+enum Epilogue {
+    STORE,      // the result as bf16, or as f32 (stored or added to what is there)
+    GATED_FWD,  // two right operands: a, b -> a and b as f32, silu(a) b as bf16
+    GATED_BWD,  // dh, with a and b read -> da = dh b silu'(a) and db = dh silu(a), as bf16
+    CE_STATS,   // logits -> per row and tile the maximum and the sum of exp(l - maximum), and the target's logit
+    CE_GRAD,    // logits -> g (exp(l - lse) - [column is the target]) as bf16
+};
+
+constexpr int BM = 128, BK = 64, BN = 256;
+constexpr int ACC_COLS = 256;
+constexpr int A_BYTES = BM * BK * 2, B_BYTES = 128 * BK * 2, STAGE_BYTES = A_BYTES + B_BYTES;
+constexpr int THREADS = 192;
+constexpr int GROUP_M = 8;
+constexpr int SLOT = 4096;  // a [32 rows x 128 bytes] tile of an epilogue warp
+constexpr int MAX_PROBLEMS = 4;
+
+template <int EPI>
+struct Shape {
+    static constexpr bool GATED = EPI == GATED_FWD;
+    static constexpr int WIDTH  = GATED ? 128 : 256;                        // result columns of a tile
+    static constexpr int SLOTS  = EPI == GATED_FWD || EPI == GATED_BWD ? 4 : EPI == CE_STATS ? 0 : 2;  // per epilogue warp
+    static constexpr int STAGES = SLOTS == 4 ? 5 : 6;
+    static constexpr int SMEM   = STAGES * STAGE_BYTES + 4 * SLOTS * SLOT + 1024 + 256;
+};
+
+struct Problem {
+    int M, N;
+    int kb[2];             // k-blocks of 64 of the first and the second operand pair
+    int a_mn, b_mn;        // operand stored with its M (N) axis contiguous
+    int splits, rows_pad;  // the k-blocks dealt out over that many tiles; partial result s starts at row s * rows_pad
+    int out_f32, add;      // STORE: f32 result; added to what is there
+    const int* dyn_m;      // rows that there are, at most M; null: M
+    const int* dyn_k;      // K of the first pair, at most 64 kb[0]; null: all of it
+};
+struct Maps {
+    CUtensorMap a[MAX_PROBLEMS][2], b[MAX_PROBLEMS][2], out[MAX_PROBLEMS], extra[2];
+};
+struct Args {
+    Problem p[MAX_PROBLEMS];
+    int count;
+    // CE_STATS, CE_GRAD
+    const int* target;   // [rows] column of the whole matrix, or -1
+    const float* lse;    // [rows]
+    const float* scale;  // [rows]
+    float2* part;        // [rows][tiles of columns]
+    float* target_logit;  // [rows]
+    int column0;          // first column of this piece
+    int* status;
+};
+// (a kernel's parameters: 4 KiB at most)
+static_assert(sizeof(Maps) + sizeof(Args) <= 4096, "too many parameters");
+
+#ifdef __CUDACC__
+
+struct Bars {
+    uint64_t full[6], empty[6], acc_full[2], acc_empty[2], in[4];
+    uint32_t tmem_base;
+    int abort_flag;
+};
+static_assert(sizeof(Bars) <= 256, "barrier block too large");
+
+struct Tile {
+    int prob, m, n;     // problem; row and column the pair's tile starts at
+    int rows;           // rows that the problem has
+    int kb0, kb1;       // k-blocks [kb0, kb1) of both pairs' kfirst + kb[1]
+    int kfirst, split;  // k-blocks of the first pair
+};
+
+__device__ __forceinline__ int rows_of(const Problem& p) { return p.dyn_m ? min(p.M, *p.dyn_m) : p.M; }
+
+// The `index`-th tile of the launch; false: there is none.
+template <int WIDTH>
+__device__ __forceinline__ bool locate(const Args& g, int index, Tile& t) {
+    for (int q = 0; q < g.count; ++q) {
+        const Problem& p  = g.p[q];
+        const int rows    = rows_of(p);
+        const int tiles_m = (rows + 2 * BM - 1) / (2 * BM), tiles_n = (p.N + WIDTH - 1) / WIDTH;
+        const int each    = tiles_m * tiles_n;
+        if (index >= each * p.splits) {
+            index -= each * p.splits;
+            continue;
+        }
+        const int split = index / each, at = index - split * each;
+        const int per_group = GROUP_M * tiles_n, first_m = at / per_group * GROUP_M;
+        const int size = min(tiles_m - first_m, GROUP_M), in_group = at % per_group;
+        t.prob = q, t.rows = rows, t.split = split;
+        t.m      = (first_m + in_group % size) * 2 * BM;
+        t.n      = in_group / size * WIDTH;
+        t.kfirst = p.dyn_k ? min(p.kb[0], (*p.dyn_k + BK - 1) / BK) : p.kb[0];
+        const int all = t.kfirst + p.kb[1], per = (all + p.splits - 1) / p.splits;
+        t.kb0 = min(all, split * per), t.kb1 = min(all, t.kb0 + per);
+        return true;
+    }
+    return false;
+}
+
+__device__ __forceinline__ void st_shared_v4(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+// This lane's row of a 128-byte-swizzled slot: 32 f32, or 32 bf16 from 16-byte piece `piece0` on.
+__device__ __forceinline__ void put_f32(uint32_t slot, int lane, const float (&v)[32]) {
+#pragma unroll
+    for (int i = 0; i < 32; i += 4)
+        st_shared_v4(slot + lane * 128 + ((uint32_t(i >> 2) ^ uint32_t(lane & 7)) << 4), __float_as_uint(v[i]), __float_as_uint(v[i + 1]),
+                     __float_as_uint(v[i + 2]), __float_as_uint(v[i + 3]));
+}
+__device__ __forceinline__ void put_bf16(uint32_t slot, int lane, int piece0, const float (&v)[32]) {
+#pragma unroll
+    for (int i = 0; i < 32; i += 8)
+        st_shared_v4(slot + lane * 128 + ((uint32_t(piece0 + (i >> 3)) ^ uint32_t(lane & 7)) << 4), pack_bf16x2(v[i], v[i + 1]),
+                     pack_bf16x2(v[i + 2], v[i + 3]), pack_bf16x2(v[i + 4], v[i + 5]), pack_bf16x2(v[i + 6], v[i + 7]));
+}
+__device__ __forceinline__ void get_f32(uint32_t slot, int lane, float (&v)[32]) {
+#pragma unroll
+    for (int i = 0; i < 32; i += 4)
+        asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                     : "=f"(v[i]), "=f"(v[i + 1]), "=f"(v[i + 2]), "=f"(v[i + 3])
+                     : "r"(slot + lane * 128 + ((uint32_t(i >> 2) ^ uint32_t(lane & 7)) << 4))
+                     : "memory");
+}
+__device__ __forceinline__ void get_acc(uint32_t at, float (&v)[32], bool empty) {
+    uint32_t r[32];
+    tmem_ld_32x32(at, r);
+    tmem_ld_wait();
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = empty ? 0.f : __uint_as_float(r[i]);
+}
+// 1 / (1 + exp(-a)): 0 where exp(-a) overflows
+__device__ __forceinline__ float sigmoid(float a) { return __fdividef(1.f, 1.f + __expf(-a)); }
+
+template <int EPI>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
+group_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args g) {
+    using S = Shape<EPI>;
+    constexpr int STAGES = S::STAGES, WIDTH = S::WIDTH;
+    constexpr int BH = WIDTH / 2, BH_BYTES = BH * BK * 2;  // columns (of each right operand) staged by this CTA
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t raw_addr = smem_u32(smem_raw), tile_base = (raw_addr + 1023u) & ~1023u;
+    Bars* bars = reinterpret_cast<Bars*>(smem_raw + (tile_base - raw_addr) + STAGES * STAGE_BYTES + 4 * S::SLOTS * SLOT);
+    volatile int* abort_flag = &bars->abort_flag;
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_ctarank();
+    const int pair = blockIdx.x >> 1, num_pairs = gridDim.x >> 1;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; ++s) {
+            mbar_init(smem_u32(&bars->full[s]), 1);
+            mbar_init(smem_u32(&bars->empty[s]), 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(smem_u32(&bars->acc_full[b]), 1);
+            mbar_init(smem_u32(&bars->acc_empty[b]), 256);
+        }
+        for (int w = 0; w < 4; ++w) mbar_init(smem_u32(&bars->in[w]), 1);
+        bars->abort_flag = 0;
+        fence_barrier_init();
+    }
+    if (warp == 1) {
+        tmem_alloc_pair(smem_u32(&bars->tmem_base), 512);
+        tmem_relinquish_pair();
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();
+    tc_fence_after();
+    const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(&bars->tmem_base);
+
+    Tile t;
+    if (warp == 0) {
+        // ---------------- TMA producer (both CTAs) ----------------
+        if (lane == 0) {
+            uint32_t stage = 0, phase = 0;
+            bool ok = true;
+            for (int tile = pair; ok && locate<WIDTH>(g, tile, t); tile += num_pairs) {
+                const Problem& p = g.p[t.prob];
+                const int m0 = t.m + int(rank) * BM, n0 = t.n + int(rank) * BH;
+                for (int kb = t.kb0; kb < t.kb1; ++kb) {
+                    if (!(ok = mbar_wait(smem_u32(&bars->empty[stage]), phase ^ 1u, abort_flag))) break;
+                    const uint32_t full_even = map_to_cta(smem_u32(&bars->full[stage]), 0);
+                    const uint32_t sa = tile_base + stage * STAGE_BYTES, sb = sa + A_BYTES;
+                    if (rank == 0) mbar_expect_tx(smem_u32(&bars->full[stage]), 2 * STAGE_BYTES);
+                    const int second = kb >= t.kfirst, k = (second ? kb - t.kfirst : kb) * BK;
+                    const CUtensorMap* ma = &maps.a[t.prob][second];
+                    const CUtensorMap* mb = &maps.b[t.prob][S::GATED ? 0 : second];
+                    if (!p.a_mn) {
+                        tma_load_2d_pair(sa, ma, k, m0, full_even);
+                    } else {
+                        tma_load_2d_pair(sa, ma, m0, k, full_even);
+                        tma_load_2d_pair(sa + BK * 128, ma, m0 + 64, k, full_even);
+                    }
+#pragma unroll
+                    for (int o = 0; o < (S::GATED ? 2 : 1); ++o, mb = &maps.b[t.prob][1]) {
+                        const uint32_t at = sb + o * BH_BYTES;
+                        if (!p.b_mn) {
+                            tma_load_2d_pair(at, mb, k, n0, full_even);
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < BH / 64; ++j) tma_load_2d_pair(at + j * (BK * 128), mb, n0 + j * 64, k, full_even);
+                        }
+                    }
+                    if (++stage == STAGES) stage = 0, phase ^= 1u;
+                }
+            }
+        }
+    } else if (warp == 1) {
+        // ---------------- MMA issuer (even CTA only) ----------------
+        if (lane == 0 && rank == 0) {
+            uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0;
+            bool ok = true;
+            for (int tile = pair; ok && locate<WIDTH>(g, tile, t); tile += num_pairs) {
+                const Problem& p     = g.p[t.prob];
+                const uint32_t idesc = idesc_bf16_f32(2 * BM, BN, p.a_mn, p.b_mn);
+                const uint32_t a_step = p.a_mn ? 2048 : 32, a_lead = p.a_mn ? BK * 128 : 16;
+                const uint32_t b_step = p.b_mn ? 2048 : 32, b_lead = p.b_mn ? BK * 128 : 16;
+                if (!(ok = mbar_wait(smem_u32(&bars->acc_empty[acc]), acc_phase ^ 1u, abort_flag))) break;
+                tc_fence_after();
+                for (int kb = t.kb0; kb < t.kb1; ++kb) {
+                    if (!(ok = mbar_wait(smem_u32(&bars->full[stage]), phase, abort_flag))) break;
+                    tc_fence_after();
+                    const uint32_t sa = tile_base + stage * STAGE_BYTES, sb = sa + A_BYTES;
+#pragma unroll
+                    for (int k = 0; k < BK / 16; ++k)
+                        mma_f16_ss_pair(tmem_base + acc * ACC_COLS, smem_desc_sw128(sa + k * a_step, a_lead, 1024),
+                                        smem_desc_sw128(sb + k * b_step, b_lead, 1024), idesc, kb > t.kb0 || k > 0);
+                    mma_commit_pair(smem_u32(&bars->empty[stage]));
+                    if (++stage == STAGES) stage = 0, phase ^= 1u;
+                }
+                if (!ok) break;
+                mma_commit_pair(smem_u32(&bars->acc_full[acc]));
+                if (++acc == 2) acc = 0, acc_phase ^= 1u;
+            }
+        }
+    } else {
+        // ---------------- epilogue (warps 2..5, both CTAs): 32 rows each, one per lane ----------------
+        const int quarter = warp & 3;
+        const uint32_t slots = tile_base + STAGES * STAGE_BYTES + quarter * S::SLOTS * SLOT;
+        const uint32_t in_bar = smem_u32(&bars->in[quarter]);
+        uint32_t acc = 0, acc_phase = 0, turn = 0, in_phase = 0;
+        bool ok = true;
+        bool have = locate<WIDTH>(g, pair, t);
+        // GATED_BWD: a and b of the 32 columns that come next, requested as soon as the slots are free
+        auto request = [&](const Tile& at, int c) {
+            if constexpr (EPI == GATED_BWD) {
+                const int row = at.m + int(rank) * BM + quarter * 32;
+                if (lane == 0 && row < at.rows) {
+                    mbar_expect_tx(in_bar, 2 * SLOT);
+                    tma_load_2d(slots, &maps.extra[0], at.n + c, row, in_bar);
+                    tma_load_2d(slots + SLOT, &maps.extra[1], at.n + c, row, in_bar);
+                }
+            }
+        };
+        if (have) request(t, 0);
+        for (int tile = pair; have && ok;) {
+            const Problem& p = g.p[t.prob];
+            const int row0 = t.m + int(rank) * BM + quarter * 32, row = row0 + lane;
+            const bool empty = t.kb0 == t.kb1, there = row0 < t.rows;
+            const int at_tile = t.n / WIDTH, n0 = t.n;
+            if (!(ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&bars->acc_full[acc]), acc_phase, abort_flag)))) break;
+            tc_fence_after();
+            const uint32_t t0 = tmem_base + acc * ACC_COLS + (uint32_t(quarter * 32) << 16);
+            const uint32_t acc_empty_even = map_to_cta(smem_u32(&bars->acc_empty[acc]), 0);
+            auto release = [&] {  // after the last read of this accumulator
+                tc_fence_before();
+                mbar_arrive_cluster(acc_empty_even);
+            };
+            // one slot's tile to a matrix, as a bulk group of its own (an empty one where the tile lies past the last column: a slot is free
+            // by the number of groups committed since)
+            auto send = [&](const CUtensorMap* m, uint32_t slot, int x, bool add = false, int down = 0) {
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) {
+                    if (x < p.N) {
+                        if (add) tma_reduce_add_2d(m, slot, x, row0 + down);
+                        else tma_store_2d(m, slot, x, row0 + down);
+                    }
+                    bulk_commit();
+                }
+            };
+            if (!there) {
+                release();
+            } else if constexpr (EPI == STORE) {
+                const int step = p.out_f32 ? 32 : 64;
+#pragma unroll 1
+                for (int c0 = 0; c0 < WIDTH; c0 += step, ++turn) {
+                    const uint32_t slot = slots + (turn & 1u) * SLOT;
+                    if (lane == 0) bulk_wait_read_1();
+                    __syncwarp();
+                    float v[32];
+                    get_acc(t0 + c0, v, empty);
+                    if (p.out_f32) {
+                        if (c0 + 32 >= WIDTH) release();
+                        put_f32(slot, lane, v);
+                    } else {
+                        put_bf16(slot, lane, 0, v);
+                        get_acc(t0 + c0 + 32, v, empty);
+                        if (c0 + 64 >= WIDTH) release();
+                        put_bf16(slot, lane, 4, v);
+                    }
+                    send(&maps.out[t.prob], slot, n0 + c0, p.add, t.split * p.rows_pad);
+                }
+            } else if constexpr (EPI == GATED_FWD) {
+                // the accumulator's columns: [a | b] of the even CTA's columns, then [a | b] of the odd one's
+#pragma unroll 1
+                for (int c = 0; c < WIDTH; c += 32) {
+                    const int ac = (c / BH) * 2 * BH + c % BH;
+                    float a[32], b[32];
+                    get_acc(t0 + ac, a, empty);
+                    get_acc(t0 + ac + BH, b, empty);
+                    if (c + 32 >= WIDTH) release();
+                    // slots: a, b, h, h; whichever is next was last sent at least two groups ago
+                    if (lane == 0) bulk_wait_read_1();
+                    __syncwarp();
+                    put_f32(slots, lane, a);
+                    send(&maps.extra[0], slots, n0 + c);
+                    if (lane == 0) bulk_wait_read_1();
+                    __syncwarp();
+                    put_f32(slots + SLOT, lane, b);
+                    send(&maps.extra[1], slots + SLOT, n0 + c);
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) a[i] = a[i] * sigmoid(a[i]) * b[i];
+                    const uint32_t slot = slots + (2 + (turn & 1u)) * SLOT;
+                    put_bf16(slot, lane, (c & 32) ? 4 : 0, a);
+                    if (c & 32) {
+                        send(&maps.out[t.prob], slot, n0 + c - 32);
+                        ++turn;
+                    }
+                }
+            } else if constexpr (EPI == GATED_BWD) {
+#pragma unroll 1
+                for (int c = 0; c < WIDTH; c += 32) {
+                    float a[32], b[32], d[32];
+                    if (!(ok = __all_sync(0xffffffffu, mbar_wait(in_bar, in_phase, abort_flag)))) break;
+                    in_phase ^= 1u;
+                    get_f32(slots, lane, a);
+                    get_f32(slots + SLOT, lane, b);
+                    __syncwarp();
+                    if (c + 32 < WIDTH) request(t, c + 32);
+                    get_acc(t0 + c, d, empty);
+                    if (c + 32 >= WIDTH) release();
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        const float e = sigmoid(a[i]), gate = a[i] * e, db = d[i] * gate;
+                        a[i] = d[i] * b[i] * (e + gate * (1.f - e));
+                        b[i] = db;
+                    }
+                    if (!(c & 32)) {
+                        if (lane == 0) bulk_wait_read_0();
+                        __syncwarp();
+                    }
+                    put_bf16(slots + 2 * SLOT, lane, (c & 32) ? 4 : 0, a);
+                    put_bf16(slots + 3 * SLOT, lane, (c & 32) ? 4 : 0, b);
+                    if (c & 32) {
+                        send(&maps.out[0], slots + 2 * SLOT, n0 + c - 32);
+                        send(&maps.out[1], slots + 3 * SLOT, n0 + c - 32);
+                    }
+                }
+                if (!ok) break;
+            } else if constexpr (EPI == CE_STATS) {
+                const int tcol = row < t.rows ? g.target[row] - g.column0 - n0 : -1, left = p.N - n0;
+                float top = -INFINITY, sum = 0.f;
+                float v[32];
+#pragma unroll 1
+                for (int c = 0; c < WIDTH; c += 32) {
+                    get_acc(t0 + c, v, empty);
+                    if (c + 32 > left) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) v[i] = c + i < left ? v[i] : -INFINITY;
+                    }
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) top = fmaxf(top, v[i]);
+                }
+                const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll 1
+                for (int c = 0; c < WIDTH; c += 32) {
+                    get_acc(t0 + c, v, empty);
+                    if (c + 32 >= WIDTH) release();
+                    if (__any_sync(0xffffffffu, tcol >= c && tcol < c + 32)) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i)
+                            if (tcol == c + i) g.target_logit[row] = v[i];
+                    }
+                    if (c + 32 > left) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) v[i] = c + i < left ? v[i] : -INFINITY;
+                    }
+                    float part = 0.f;
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) part += __expf(v[i] - base);
+                    sum += part;
+                }
+                if (row < t.rows) g.part[int64_t(row) * ((p.N + WIDTH - 1) / WIDTH) + at_tile] = make_float2(top, sum);
+            } else {
+                const bool mine = row < t.rows;
+                const int tcol  = mine ? g.target[row] - g.column0 - n0 : -1;
+                const float lse = mine ? g.lse[row] : 0.f, scale = mine ? g.scale[row] : 0.f;
+#pragma unroll 1
+                for (int c = 0; c < WIDTH; c += 32) {
+                    const uint32_t slot = slots + (turn & 1u) * SLOT;
+                    if (!(c & 32)) {
+                        if (lane == 0) bulk_wait_read_1();
+                        __syncwarp();
+                    }
+                    float v[32];
+                    get_acc(t0 + c, v, empty);
+                    if (c + 32 >= WIDTH) release();
+                    // rows past the last one are zeros, which the products over rows read
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) v[i] = mine ? scale * (__expf(v[i] - lse) - (tcol == c + i ? 1.f : 0.f)) : 0.f;
+                    put_bf16(slot, lane, (c & 32) ? 4 : 0, v);
+                    if (c & 32) {
+                        send(&maps.out[0], slot, n0 + c - 32);
+                        ++turn;
+                    }
+                }
+            }
+            if (++acc == 2) acc = 0, acc_phase ^= 1u;
+            tile += num_pairs;
+            have = locate<WIDTH>(g, tile, t);
+            if (have) request(t, 0);
+        }
+        if (lane == 0) bulk_wait_all();
+    }
+
+    // Neither CTA may release shared or tensor memory while the other can still touch it: meet first.
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();
+    if (warp == 1) {
+        __syncwarp();
+        tc_fence_after();
+        tmem_dealloc_pair(tmem_base, 512);
+    }
+    if (threadIdx.x == 0 && *abort_flag) *g.status = MIMK_E_DEVICE_WAIT;
+}
+
+#endif
+
+// ---- host ------------------------------------------------------------------------------------------------------------------------
+// A row-major bf16 matrix whose rows are `pitch` elements apart.
+struct Mat {
+    const void* p;
+    int64_t rows, cols, pitch;
+};
+inline bool tma_can_read(const void* p, int64_t pitch, int size = 2) { return aligned16(p) && (pitch * size) % 16 == 0; }
+
+// The operand's map: `mn`: the matrix is [K, M or N], else [M or N, K]; `staged`: M or N values that a CTA stages.
+inline int operand_map(CUtensorMap* map, const Mat& x, bool mn, int staged) {
+    return make_tmap_2d(map, false, x.p, uint64_t(x.cols), uint64_t(x.rows), uint64_t(x.pitch) * 2, 64, mn ? 64u : uint32_t(staged));
+}
+inline int result_map(CUtensorMap* map, void* p, bool f32, int64_t rows, int64_t cols, int64_t pitch) {
+    return make_tmap_2d(map, f32, p, uint64_t(cols), uint64_t(rows), uint64_t(pitch) * (f32 ? 4 : 2), f32 ? 32 : 64, 32);
+}
+
+template <int EPI>
+int launch_group(const Maps& maps, const Args& args, const DeviceInfo& dev, cudaStream_t s) {
+    auto kern = group_kernel<EPI>;
+    static bool configured[64] = {};
+    if (!configured[dev.device & 63]) {
+        MIMK_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<EPI>::SMEM));
+        configured[dev.device & 63] = true;
+    }
+    int64_t tiles = 0;
+    for (int q = 0; q < args.count; ++q) {
+        const Problem& p = args.p[q];
+        tiles += int64_t((p.M + 2 * BM - 1) / (2 * BM)) * ((p.N + Shape<EPI>::WIDTH - 1) / Shape<EPI>::WIDTH) * p.splits;
+    }
+    if (tiles > (1 << 30)) return MIMK_E_UNSUPPORTED;
+    const int64_t pairs = dev.sm_count / 2;
+    const int grid      = int(2 * (tiles < pairs ? tiles : pairs));
+    if (!grid) return MIMK_OK;
+    kern<<<grid, THREADS, Shape<EPI>::SMEM, s>>>(maps, args);
+    return launch_status();
+}
+
+}  // namespace group
+}  // namespace mimk

@@ -353,6 +353,86 @@ def mlp_gated(x: torch.Tensor, w1: torch.Tensor, w3: torch.Tensor, w2: torch.Ten
     return y
 
 
+# ------------------------------------------------------------------------------------------------------- training
+class MlpKept:
+    """What mlp_gated_fwd keeps for mlp_gated_bwd: a buffer of the library's own layout and the extents it is for."""
+    __slots__ = ("buffer", "extents")
+
+    def __init__(self, buffer: torch.Tensor, extents):
+        self.buffer, self.extents = buffer, extents
+
+
+def _bytes(n: int, device) -> torch.Tensor:
+    """Scratch of torch's allocator, which orders its reuse on the current stream."""
+    return torch.empty((n,), dtype=torch.uint8, device=device)
+
+
+def _weight_layout(what: str, *ws):
+    """The weights as they lie in memory (copied only where they are neither row-major nor a transposed view of row-major) and their layout."""
+    stored = [_b_layout(w) for w in ws]
+    if any(lay != stored[0][1] for _, lay in stored):
+        raise ValueError(f"{what}: the weights must share one storage layout")
+    return [w for w, _ in stored], stored[0][1]
+
+
+def _like_weight(w: torch.Tensor, layout: int) -> torch.Tensor:
+    """An uninitialised gradient of w's shape in w's storage layout."""
+    rows, cols = w.shape
+    return torch.empty((rows, cols), dtype=w.dtype, device=w.device) if layout == L.B_KN else torch.empty((cols, rows), dtype=w.dtype, device=w.device).t()
+
+
+def _mlp_train_desc(x, w1, w3, w2):
+    _dev(x, w1, w3, w2)
+    if any(t.dim() != 2 for t in (x, w1, w3, w2)):
+        raise ValueError("the gated MLP expects rank-2 tensors")
+    if x.shape[1] != w1.shape[0] or w1.shape != w3.shape or w1.shape[1] != w2.shape[0]:
+        raise ValueError("contracting dims don't match")
+    if any(t.dtype != x.dtype for t in (w1, w3, w2)):
+        raise TypeError("the gated MLP's operands share one element type")
+    x = x.contiguous()
+    stored, layout = _weight_layout("the gated MLP", w1, w3, w2)
+    d = L.MlpTrainDesc()
+    (d.m, d.k), (d.f, d.n) = x.shape, w2.shape
+    d.x, (d.w1, d.w3, d.w2) = x.data_ptr(), (w.data_ptr() for w in stored)
+    d.dtype, d.b_layout = _dt(x), layout
+    return d, (x, *stored)
+
+
+def mlp_gated_fwd(x: torch.Tensor, w1: torch.Tensor, w3: torch.Tensor, w2: torch.Tensor):
+    """mlp_gated for training, bf16: (y, kept), `kept` being what mlp_gated_bwd needs of this pass (10 bytes per row and hidden column)."""
+    d, held = _mlp_train_desc(x, w1, w3, w2)
+    y = torch.empty((d.m, d.n), dtype=x.dtype, device=x.device)
+    d.y = y.data_ptr()
+    kept, scratch = C.c_uint64(), C.c_uint64()
+    L.check(L.lib().mimk_mlp_gated_train_sizes(C.byref(d), C.byref(kept), C.byref(scratch), None), "mlp_gated_fwd")
+    buffer, ws = _bytes(kept.value, x.device), _bytes(scratch.value, x.device)
+    d.kept, d.workspace, d.workspace_bytes = buffer.data_ptr(), ws.data_ptr(), scratch.value
+    L.check(L.lib().mimk_mlp_gated_fwd(C.byref(d), _stream()), "mlp_gated_fwd")
+    return y, MlpKept(buffer, (d.m, d.k, d.f, d.n))
+
+
+def mlp_gated_bwd(dy: torch.Tensor, x: torch.Tensor, w1: torch.Tensor, w3: torch.Tensor, w2: torch.Tensor, kept: MlpKept):
+    """The gradients (dx, dw1, dw3, dw2) of the mlp_gated_fwd call that gave `kept`, from its result's gradient; the weights' have the
+    weights' storage layout."""
+    d, held = _mlp_train_desc(x, w1, w3, w2)
+    _dev(dy)
+    if (d.m, d.k, d.f, d.n) != kept.extents:
+        raise ValueError("mlp_gated_bwd: `kept` is of a call with other extents")
+    if tuple(dy.shape) != (d.m, d.n):
+        raise ValueError("mlp_gated_bwd: dy must have the result's shape")
+    if dy.dtype != x.dtype:
+        raise TypeError("the gated MLP's operands share one element type")
+    dy = dy.contiguous()
+    dx, grads = torch.empty((d.m, d.k), dtype=x.dtype, device=x.device), [_like_weight(w, d.b_layout) for w in (w1, w3, w2)]
+    d.dy, d.dx, (d.dw1, d.dw3, d.dw2) = dy.data_ptr(), dx.data_ptr(), (g.data_ptr() for g in grads)
+    scratch = C.c_uint64()
+    L.check(L.lib().mimk_mlp_gated_train_sizes(C.byref(d), None, None, C.byref(scratch)), "mlp_gated_bwd")
+    ws = _bytes(scratch.value, x.device)
+    d.kept, d.workspace, d.workspace_bytes = kept.buffer.data_ptr(), ws.data_ptr(), scratch.value
+    L.check(L.lib().mimk_mlp_gated_bwd(C.byref(d), _stream()), "mlp_gated_bwd")
+    return (dx, *grads)
+
+
 # ------------------------------------------------------------------------------------------------ the generic op
 def proj_map(n_loops: int, subs):
     """`proj_map subs`: result j reads loop variable subs[j] (tensor.mim:196-203), as a coefficient matrix."""
