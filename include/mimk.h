@@ -367,6 +367,48 @@ int mimk_mlp_gated_train_sizes(const mimk_mlp_train_desc* desc, uint64_t* kept, 
 int mimk_mlp_gated_fwd(const mimk_mlp_train_desc* desc, void* stream);
 int mimk_mlp_gated_bwd(const mimk_mlp_train_desc* desc, void* stream);
 
+/* Softmax cross-entropy of a linear layer, logits = X W, without the logits in memory (bf16) or with those of a piece of at most
+ * 512 MiB (f32): loss_i = log sum_j exp(l_ij) - l_i,target(i), and its gradients with respect to X and W.
+ *   fwd: loss and, unless NULL, lse (log sum exp per row); bwd: dX and dW from lse; fwd_bwd: loss, lse unless NULL, dX and dW.
+ * reduction: one loss per row, their mean over the rows that have a target (0 if none has), or their sum. dloss: the gradient that arrives at the
+ * loss, one value or one per row; NULL: ones.
+ * has_ignore: a row whose target is ignore_index has none: its loss, lse and dX are zeros, nothing of it enters dW, and its X is not read. Any other target
+ * outside [0, v) is recorded (mimk_device_status: MIMK_E_SHAPE); the row's loss is NaN, and it enters no gradient.
+ * Losses, lse and all sums are f32; bf16 gradients are rounded once from f32 sums of products whose factor p = dloss (softmax - onehot) is
+ * rounded to bf16. Equal descriptors give equal bits. Workspace as above, from the query; bf16: 16 bytes per row, 8 per row and 256 classes, and
+ * up to 512 MiB of p (8 KiB per row where that is more) and 4 bytes per value of X for gradients. */
+enum { MIMK_REDUCTION_NONE = 0, MIMK_REDUCTION_MEAN = 1, MIMK_REDUCTION_SUM = 2 };
+typedef struct mimk_linear_ce_desc {
+    int64_t n, d, v;     /* rows, features, classes */
+    const void* x;       /* [n, d] */
+    const void* w;       /* [d, v], or [v, d] with MIMK_B_NK; so dw */
+    const void* targets; /* [n] of target_dtype */
+    const float* dloss;
+    float* loss;
+    float* lse;
+    void* dx;
+    void* dw;
+    void* workspace;
+    uint64_t workspace_bytes;
+    int64_t ignore_index;
+    int32_t dtype, target_dtype, w_layout, reduction, has_ignore;
+} mimk_linear_ce_desc;
+int mimk_linear_ce_workspace(const mimk_linear_ce_desc* desc, int forward, int backward, uint64_t* bytes);
+int mimk_linear_ce_fwd(const mimk_linear_ce_desc* desc, void* stream);
+int mimk_linear_ce_bwd(const mimk_linear_ce_desc* desc, void* stream);
+int mimk_linear_ce_fwd_bwd(const mimk_linear_ce_desc* desc, void* stream);
+
+/* The 2-norm of all values of `count` tensors together (of any length, each dense: tensors[i] has lengths[i] elements of dtypes[i], F32 or BF16), and
+ * the tensors scaled so that it is at most `limit`: out[i] = tensors[i] * c, c = min(1, limit / (norm + eps)); out[i] may be tensors[i]. A norm that
+ * is NaN makes c NaN, one that is infinite makes it zero. `norm`: one f32 on the device. The arrays are on the
+ * host and are read before the call returns. Squares are summed in f32 over 16 values at most and in f64 from there, and over again in
+ * f64 where an f32 sum overflows or all but vanishes. Equal calls give equal bits. Workspace as above. */
+int mimk_clip_grads_workspace(int64_t count, uint64_t* bytes); /* of either call */
+int mimk_grad_norm(const void* const* tensors, const int64_t* lengths, const int32_t* dtypes, int64_t count, float* norm, void* workspace,
+                   uint64_t workspace_bytes, void* stream);
+int mimk_clip_grads(const void* const* tensors, void* const* out, const int64_t* lengths, const int32_t* dtypes, int64_t count, float limit, float eps,
+                    float* norm, void* workspace, uint64_t workspace_bytes, void* stream);
+
 /* ---- the generic operation ------------------------------------------------------------------------------
  * out[map_out(o)] = post(fold_r f(acc, (in_i[maps_i(o, r)])_i), (post_in_j[post_maps_j(map_out(o))])_j)
  * over the loop vector (o..., r...) with bounds `sr`: the leading `ro` loops are the output loops, the trailing

@@ -25,7 +25,8 @@ ROWS_SOFTMAX, ROWS_RMSNORM, ROWS_SOFTMAX_RMSNORM = 0, 1, 2
 SYMBOLS = (
     "mimk_status_str", "mimk_abi_version", "mimk_last_cuda_error", "mimk_device_check", "mimk_device_status", "mimk_selftest_wait_expiry",
     "mimk_gemm", "mimk_gemm_flat", "mimk_gemm_gather", "mimk_gemm_reduce_scatter", "mimk_gemm_kpanels", "mimk_reduce", "mimk_reduce_fused", "mimk_reduce_plan", "mimk_reduce_tiles", "mimk_reduce_static", "mimk_softmax", "mimk_rmsnorm", "mimk_softmax_rmsnorm", "mimk_map", "mimk_map_t",
-    "mimk_splat", "mimk_select", "mimk_generate_affine", "mimk_gather", "mimk_scatter", "mimk_attn_fwd", "mimk_conv", "mimk_conv_laid_out", "mimk_mlp_gated", "mimk_mlp_gated_train_sizes", "mimk_mlp_gated_fwd", "mimk_mlp_gated_bwd", "mimk_map_reduce_post", "mimk_mrp_classify", "mimk_mrp_cell_kernel", "mimk_program_classify", "mimk_program_run", "mimk_chain_order", "mimk_chain_cost",
+    "mimk_splat", "mimk_select", "mimk_generate_affine", "mimk_gather", "mimk_scatter", "mimk_attn_fwd", "mimk_conv", "mimk_conv_laid_out", "mimk_mlp_gated", "mimk_mlp_gated_train_sizes", "mimk_mlp_gated_fwd", "mimk_mlp_gated_bwd", "mimk_linear_ce_workspace", "mimk_linear_ce_fwd", "mimk_linear_ce_bwd", "mimk_linear_ce_fwd_bwd",
+    "mimk_clip_grads_workspace", "mimk_grad_norm", "mimk_clip_grads", "mimk_map_reduce_post", "mimk_mrp_classify", "mimk_mrp_cell_kernel", "mimk_program_classify", "mimk_program_run", "mimk_chain_order", "mimk_chain_cost",
     "mimk_host_rows", "mimk_host_rows_pair", "mimk_host_gemm", "mimk_host_attn_fwd", "mimk_host_mlp_gated", "mimk_host_map_reduce_post", "mimk_host_register",
     "mimk_host_unregister", "mimk_host_release",
 )
@@ -88,6 +89,18 @@ class MlpTrainDesc(C.Structure):
         ("x", C.c_void_p), ("w1", C.c_void_p), ("w3", C.c_void_p), ("w2", C.c_void_p), ("y", C.c_void_p), ("kept", C.c_void_p),
         ("dy", C.c_void_p), ("dx", C.c_void_p), ("dw1", C.c_void_p), ("dw3", C.c_void_p), ("dw2", C.c_void_p),
         ("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64), ("dtype", C.c_int32), ("b_layout", C.c_int32),
+    ]
+
+
+REDUCTION_NONE, REDUCTION_MEAN, REDUCTION_SUM = range(3)
+
+
+class LinearCeDesc(C.Structure):
+    _fields_ = [
+        ("n", C.c_int64), ("d", C.c_int64), ("v", C.c_int64), ("x", C.c_void_p), ("w", C.c_void_p), ("targets", C.c_void_p), ("dloss", C.c_void_p),
+        ("loss", C.c_void_p), ("lse", C.c_void_p), ("dx", C.c_void_p), ("dw", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64),
+        ("ignore_index", C.c_int64), ("dtype", C.c_int32), ("target_dtype", C.c_int32), ("w_layout", C.c_int32), ("reduction", C.c_int32),
+        ("has_ignore", C.c_int32),
     ]
 
 
@@ -179,6 +192,12 @@ def lib() -> C.CDLL:
         u64p = C.POINTER(C.c_uint64)
         L.mimk_mlp_gated_train_sizes.argtypes = [C.POINTER(MlpTrainDesc), u64p, u64p, u64p]
         L.mimk_mlp_gated_fwd.argtypes = L.mimk_mlp_gated_bwd.argtypes = [C.POINTER(MlpTrainDesc), vp]
+        L.mimk_linear_ce_workspace.argtypes = [C.POINTER(LinearCeDesc), ci, ci, u64p]
+        L.mimk_linear_ce_fwd.argtypes = L.mimk_linear_ce_bwd.argtypes = L.mimk_linear_ce_fwd_bwd.argtypes = [C.POINTER(LinearCeDesc), vp]
+        vpp, i64p, i32p = C.POINTER(vp), C.POINTER(i64), C.POINTER(C.c_int32)
+        L.mimk_clip_grads_workspace.argtypes = [i64, u64p]
+        L.mimk_grad_norm.argtypes = [vpp, i64p, i32p, i64, vp, vp, C.c_uint64, vp]
+        L.mimk_clip_grads.argtypes = [vpp, vpp, i64p, i32p, i64, cf, cf, vp, vp, C.c_uint64, vp]
         L.mimk_map_reduce_post.argtypes = [C.POINTER(MrpDesc), vp]
         L.mimk_mrp_classify.argtypes = [C.POINTER(MrpDesc)]
         L.mimk_mrp_cell_kernel.argtypes = [C.POINTER(MrpDesc), C.POINTER(C.c_int32)]

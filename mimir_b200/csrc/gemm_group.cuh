@@ -273,7 +273,8 @@ group_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args g) 
         for (int tile = pair; have && ok;) {
             const Problem& p = g.p[t.prob];
             const int row0 = t.m + int(rank) * BM + quarter * 32, row = row0 + lane;
-            const bool empty = t.kb0 == t.kb1, there = row0 < t.rows;
+            // (products over rows read whole k-blocks of them: CE_GRAD writes zeros up to the end of the last one)
+            const bool empty = t.kb0 == t.kb1, there = row0 < (EPI == CE_GRAD ? (t.rows + BK - 1) / BK * BK : t.rows);
             const int at_tile = t.n / WIDTH, n0 = t.n;
             if (!(ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&bars->acc_full[acc]), acc_phase, abort_flag)))) break;
             tc_fence_after();

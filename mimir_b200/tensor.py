@@ -433,6 +433,134 @@ def mlp_gated_bwd(dy: torch.Tensor, x: torch.Tensor, w1: torch.Tensor, w3: torch
     return (dx, *grads)
 
 
+_REDUCTION = {"none": L.REDUCTION_NONE, "mean": L.REDUCTION_MEAN, "sum": L.REDUCTION_SUM}
+
+
+def _linear_ce(what, x, w, targets, ignore_index, reduction, dloss, lse, forward, backward, want_lse=False):
+    _dev(x, w, targets, dloss, lse)
+    if reduction not in _REDUCTION:
+        raise ValueError(f"{what}: reduction is one of {', '.join(_REDUCTION)}")
+    if x.dim() < 1 or w.dim() != 2 or x.shape[-1] != w.shape[0]:
+        raise ValueError("contracting dims don't match")
+    if x.dtype != w.dtype:
+        raise TypeError(f"{what}: x and w share one element type")
+    if targets.shape != x.shape[:-1]:
+        raise ValueError(f"{what}: one target for each row of x")
+    if targets.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"{what}: targets are I32 or I64")
+    lead = x.shape[:-1]
+    x, targets = x.contiguous(), targets.contiguous()
+    (stored,), layout = _weight_layout(what, w)
+    d = L.LinearCeDesc()
+    d.n, (d.d, d.v) = math.prod(lead), w.shape
+    d.x, d.w, d.targets = x.data_ptr(), stored.data_ptr(), targets.data_ptr()
+    d.dtype, d.target_dtype, d.w_layout, d.reduction = _dt(x), _dt(targets), layout, _REDUCTION[reduction]
+    if ignore_index is not None:
+        d.has_ignore, d.ignore_index = 1, ignore_index
+    each = lead if reduction == "none" else ()
+    f32 = dict(dtype=torch.float32, device=x.device)
+    if dloss is not None:
+        if tuple(dloss.shape) != tuple(each):
+            raise ValueError(f"{what}: dloss must have the loss's shape")
+        dloss = dloss.to(torch.float32).contiguous()
+        d.dloss = dloss.data_ptr()
+    out = []
+    if forward:
+        out.append(torch.empty(each, **f32))
+        d.loss = out[0].data_ptr()
+        if want_lse:
+            out.append(torch.empty(lead, **f32))
+            d.lse = out[1].data_ptr()
+    else:
+        if lse.shape != lead or lse.dtype != torch.float32:
+            raise ValueError(f"{what}: lse is what linear_cross_entropy returned, one F32 for each row")
+        lse = lse.contiguous()
+        d.lse = lse.data_ptr()
+    if backward:
+        out += [torch.empty(x.shape, dtype=x.dtype, device=x.device), _like_weight(w, layout)]
+        d.dx, d.dw = out[-2].data_ptr(), out[-1].data_ptr()
+    scratch, lib = C.c_uint64(), L.lib()
+    L.check(lib.mimk_linear_ce_workspace(C.byref(d), int(forward), int(backward), C.byref(scratch)), what)
+    ws = _bytes(scratch.value, x.device)
+    d.workspace, d.workspace_bytes = ws.data_ptr(), scratch.value
+    call = lib.mimk_linear_ce_fwd_bwd if forward and backward else lib.mimk_linear_ce_fwd if forward else lib.mimk_linear_ce_bwd
+    L.check(call(C.byref(d), _stream()), what)
+    return out
+
+
+def linear_cross_entropy(x: torch.Tensor, w: torch.Tensor, targets: torch.Tensor, *, ignore_index: int | None = None, reduction: str = "mean",
+                         return_lse: bool = False):
+    """The softmax cross-entropy of the logits x w (w: [features, classes] row-major, or a transpose_2d view of [classes, features]) against class
+    numbers, F32 or BF16, without the logits in memory. reduction: "mean" over the rows that have a target (0 if none has), "sum", or "none" for one
+    loss per row; losses are F32. A row whose target is `ignore_index` has none: loss and lse 0. return_lse: also each row's log sum exp, which
+    linear_cross_entropy_grad takes. A target that is neither a class nor `ignore_index` gives NaN, and device_status() raises."""
+    out = _linear_ce("linear_cross_entropy", x, w, targets, ignore_index, reduction, None, None, True, False, return_lse)
+    return tuple(out) if return_lse else out[0]
+
+
+def linear_cross_entropy_grad(x: torch.Tensor, w: torch.Tensor, targets: torch.Tensor, lse: torch.Tensor, *, ignore_index: int | None = None,
+                              reduction: str = "mean", dloss: torch.Tensor | None = None):
+    """(dx, dw) of linear_cross_entropy with the same arguments, from its lse. dloss: the gradient that arrives at the loss (of its shape; ones if None).
+    dw has w's storage layout."""
+    return tuple(_linear_ce("linear_cross_entropy_grad", x, w, targets, ignore_index, reduction, dloss, lse, False, True))
+
+
+def linear_cross_entropy_with_grad(x: torch.Tensor, w: torch.Tensor, targets: torch.Tensor, *, ignore_index: int | None = None, reduction: str = "mean",
+                                   dloss: torch.Tensor | None = None):
+    """(loss, dx, dw): linear_cross_entropy and its gradients in one call."""
+    return tuple(_linear_ce("linear_cross_entropy_with_grad", x, w, targets, ignore_index, reduction, dloss, None, True, True))
+
+
+def _gaps(t: torch.Tensor) -> bool:
+    """Whether the tensor's elements are other than all of a run of memory, each once."""
+    expected = 1
+    for stride, size in sorted((st, sz) for st, sz in zip(t.stride(), t.shape) if sz != 1):
+        if stride != expected:
+            return t.numel() > 0
+        expected *= size
+    return False
+
+
+def _grad_list(what, grads, out=None):
+    grads = list(grads)
+    out = grads if out is None else list(out)
+    if len(out) != len(grads):
+        raise ValueError(f"{what}: one result for each gradient")
+    device = grads[0].device if grads else torch.device("cuda", torch.cuda.current_device())
+    for t, o in zip(grads, out):
+        _dev(t, o)
+        if t.device != device or o.device != device:
+            raise ValueError(f"{what}: the gradients lie on one device")
+        if t.dtype not in (torch.float32, torch.bfloat16) or o.dtype != t.dtype:
+            raise TypeError(f"{what}: gradients are F32 or BF16, and results of the same element type")
+        if o.shape != t.shape or (o is not t and o.stride() != t.stride()) or _gaps(t):
+            raise ValueError(f"{what}: gradients are dense, and results of the same shape and strides")
+    n = len(grads)
+    ptrs = lambda ts: (C.c_void_p * n)(*(t.data_ptr() for t in ts))  # noqa: E731
+    scratch = C.c_uint64()
+    L.check(L.lib().mimk_clip_grads_workspace(n, C.byref(scratch)), what)
+    ws = _bytes(scratch.value, device)
+    norm = torch.empty((), dtype=torch.float32, device=device)
+    return (ptrs(grads), ptrs(out), (C.c_int64 * n)(*(t.numel() for t in grads)), (C.c_int32 * n)(*(_dt(t) for t in grads)), n, norm, ws, scratch.value)
+
+
+def grad_norm(grads) -> torch.Tensor:
+    """The 2-norm of all values of the tensors (F32 and BF16 ones, of any number) together, as an F32 tensor without axes."""
+    ins, _, lengths, dtypes, n, norm, ws, size = _grad_list("grad_norm", grads)
+    L.check(L.lib().mimk_grad_norm(ins, lengths, dtypes, n, norm.data_ptr(), ws.data_ptr(), size, _stream()), "grad_norm")
+    return norm
+
+
+def clip_grad_norm(grads, limit: float, *, eps: float = 1e-6, out=None) -> torch.Tensor:
+    """Scales the tensors by min(1, limit / (norm + eps)), in place or into the tensors `out`, and returns their norm from before
+    (grad_norm). A norm of NaN makes every value NaN, an infinite one zeros, and NaN of what was infinite."""
+    ins, outs, lengths, dtypes, n, norm, ws, size = _grad_list("clip_grad_norm", grads, out)
+    if not (limit >= 0 and eps >= 0):
+        raise ValueError("clip_grad_norm: limit and eps are at least 0")
+    L.check(L.lib().mimk_clip_grads(ins, outs, lengths, dtypes, n, limit, eps, norm.data_ptr(), ws.data_ptr(), size, _stream()), "clip_grad_norm")
+    return norm
+
+
 # ------------------------------------------------------------------------------------------------ the generic op
 def proj_map(n_loops: int, subs):
     """`proj_map subs`: result j reads loop variable subs[j] (tensor.mim:196-203), as a coefficient matrix."""
