@@ -28,7 +28,7 @@ enum Epilogue {
 constexpr int BM = 128, BK = 64, BN = 256;
 constexpr int ACC_COLS = 256;
 constexpr int A_BYTES = BM * BK * 2, B_BYTES = 128 * BK * 2, STAGE_BYTES = A_BYTES + B_BYTES;
-constexpr int THREADS = 192;
+constexpr int THREADS = 224;
 constexpr int GROUP_M = 8;
 constexpr int SLOT = 4096;  // a [32 rows x 128 bytes] tile of an epilogue warp
 constexpr int MAX_PROBLEMS = 4;
@@ -144,6 +144,11 @@ __device__ __forceinline__ void get_acc(uint32_t at, float (&v)[32], bool empty)
 #pragma unroll
     for (int i = 0; i < 32; ++i) v[i] = empty ? 0.f : __uint_as_float(r[i]);
 }
+// A parameter in a register: asked for again in every k-block, it is read from constant memory again.
+__device__ __forceinline__ int held(int v) {
+    asm volatile("" : "+r"(v));
+    return v;
+}
 // 1 / (1 + exp(-a)): 0 where exp(-a) overflows
 __device__ __forceinline__ float sigmoid(float a) { return __fdividef(1.f, 1.f + __expf(-a)); }
 
@@ -186,39 +191,45 @@ group_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args g) 
     const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(&bars->tmem_base);
 
     Tile t;
-    if (warp == 0) {
-        // ---------------- TMA producer (both CTAs) ----------------
+    if (warp == 0 || warp == 6) {
+        // ---------------- TMA producers (both CTAs): warp 0 the left operand, warp 6 the right one or ones ----------------
+        // (one thread for both took longer over a k-block than the multiplication)
         if (lane == 0) {
+            const bool left = warp == 0;
             uint32_t stage = 0, phase = 0;
             bool ok = true;
             for (int tile = pair; ok && locate<WIDTH>(g, tile, t); tile += num_pairs) {
                 const Problem& p = g.p[t.prob];
-                const int m0 = t.m + int(rank) * BM, n0 = t.n + int(rank) * BH;
-                for (int kb = t.kb0; kb < t.kb1; ++kb) {
-                    if (!(ok = mbar_wait(smem_u32(&bars->empty[stage]), phase ^ 1u, abort_flag))) break;
-                    const uint32_t full_even = map_to_cta(smem_u32(&bars->full[stage]), 0);
-                    const uint32_t sa = tile_base + stage * STAGE_BYTES, sb = sa + A_BYTES;
-                    if (rank == 0) mbar_expect_tx(smem_u32(&bars->full[stage]), 2 * STAGE_BYTES);
-                    const int second = kb >= t.kfirst, k = (second ? kb - t.kfirst : kb) * BK;
-                    const CUtensorMap* ma = &maps.a[t.prob][second];
-                    const CUtensorMap* mb = &maps.b[t.prob][S::GATED ? 0 : second];
-                    if (!p.a_mn) {
-                        tma_load_2d_pair(sa, ma, k, m0, full_even);
-                    } else {
-                        tma_load_2d_pair(sa, ma, m0, k, full_even);
-                        tma_load_2d_pair(sa + BK * 128, ma, m0 + 64, k, full_even);
-                    }
-#pragma unroll
-                    for (int o = 0; o < (S::GATED ? 2 : 1); ++o, mb = &maps.b[t.prob][1]) {
-                        const uint32_t at = sb + o * BH_BYTES;
-                        if (!p.b_mn) {
-                            tma_load_2d_pair(at, mb, k, n0, full_even);
+                const int mn = held(left ? p.a_mn : p.b_mn), first = left ? t.m + int(rank) * BM : t.n + int(rank) * BH;
+                const uint32_t base = tile_base + (left ? 0 : A_BYTES);
+                // the k-blocks of one operand pair after those of the other
+                const auto run = [&](const CUtensorMap* map, const CUtensorMap* second, int k, int end) {
+                    for (; k < end; k += BK) {
+                        if (!(ok = mbar_wait(smem_u32(&bars->empty[stage]), phase ^ 1u, abort_flag))) break;
+                        const uint32_t full_even = map_to_cta(smem_u32(&bars->full[stage]), 0), at = base + stage * STAGE_BYTES;
+                        if (left && rank == 0) mbar_expect_tx(smem_u32(&bars->full[stage]), 2 * STAGE_BYTES);  // all four producers' bytes
+                        if (!mn) {
+                            tma_load_2d_pair(at, map, k, first, full_even);
+                            if (second) tma_load_2d_pair(at + BH_BYTES, second, k, first, full_even);
+                        } else if (second) {
+                            tma_load_2d_pair(at, map, first, k, full_even);
+                            tma_load_2d_pair(at + BH_BYTES, second, first, k, full_even);
                         } else {
-#pragma unroll
-                            for (int j = 0; j < BH / 64; ++j) tma_load_2d_pair(at + j * (BK * 128), mb, n0 + j * 64, k, full_even);
+                            tma_load_2d_pair(at, map, first, k, full_even);
+                            tma_load_2d_pair(at + BK * 128, map, first + 64, k, full_even);
                         }
+                        if (++stage == STAGES) stage = 0, phase ^= 1u;
                     }
-                    if (++stage == STAGES) stage = 0, phase ^= 1u;
+                };
+                const CUtensorMap* m = left ? maps.a[t.prob] : maps.b[t.prob];
+                if (S::GATED && left) {
+                    // (128 rows of one left operand)
+                    run(m, nullptr, t.kb0 * BK, t.kb1 * BK);
+                } else if (S::GATED) {
+                    run(m, m + 1, t.kb0 * BK, t.kb1 * BK);
+                } else {
+                    run(m, nullptr, t.kb0 * BK, min(t.kb1, t.kfirst) * BK);
+                    if (ok) run(m + 1, nullptr, max(t.kb0 - t.kfirst, 0) * BK, (t.kb1 - t.kfirst) * BK);
                 }
             }
         }
@@ -227,21 +238,23 @@ group_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args g) 
         if (lane == 0 && rank == 0) {
             uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0;
             bool ok = true;
+            const uint64_t high = smem_desc_sw128(0, 0, 1024);
             for (int tile = pair; ok && locate<WIDTH>(g, tile, t); tile += num_pairs) {
                 const Problem& p     = g.p[t.prob];
                 const uint32_t idesc = idesc_bf16_f32(2 * BM, BN, p.a_mn, p.b_mn);
-                const uint32_t a_step = p.a_mn ? 2048 : 32, a_lead = p.a_mn ? BK * 128 : 16;
-                const uint32_t b_step = p.b_mn ? 2048 : 32, b_lead = p.b_mn ? BK * 128 : 16;
+                // a descriptor's low word is the address >> 4 with the leading offset >> 4 above it, its high word is the same for all
+                const uint32_t a_step = p.a_mn ? 2048 >> 4 : 32 >> 4, b_step = p.b_mn ? 2048 >> 4 : 32 >> 4;
+                const uint32_t a_low = (p.a_mn ? BK * 128 >> 4 : 1) << 16, b_low = ((p.b_mn ? BK * 128 >> 4 : 1) << 16) + (A_BYTES >> 4);
                 if (!(ok = mbar_wait(smem_u32(&bars->acc_empty[acc]), acc_phase ^ 1u, abort_flag))) break;
                 tc_fence_after();
                 for (int kb = t.kb0; kb < t.kb1; ++kb) {
                     if (!(ok = mbar_wait(smem_u32(&bars->full[stage]), phase, abort_flag))) break;
                     tc_fence_after();
-                    const uint32_t sa = tile_base + stage * STAGE_BYTES, sb = sa + A_BYTES;
+                    const uint32_t at = (tile_base + stage * STAGE_BYTES) >> 4;
 #pragma unroll
                     for (int k = 0; k < BK / 16; ++k)
-                        mma_f16_ss_pair(tmem_base + acc * ACC_COLS, smem_desc_sw128(sa + k * a_step, a_lead, 1024),
-                                        smem_desc_sw128(sb + k * b_step, b_lead, 1024), idesc, kb > t.kb0 || k > 0);
+                        mma_f16_ss_pair(tmem_base + acc * ACC_COLS, high | (at + a_low + k * a_step), high | (at + b_low + k * b_step), idesc,
+                                        kb > t.kb0 || k > 0);
                     mma_commit_pair(smem_u32(&bars->empty[stage]));
                     if (++stage == STAGES) stage = 0, phase ^= 1u;
                 }
@@ -251,7 +264,7 @@ group_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args g) 
             }
         }
     } else {
-        // ---------------- epilogue (warps 2..5, both CTAs): 32 rows each, one per lane ----------------
+        // ---------------- epilogue (warps 2 to 5, both CTAs): 32 rows each, one per lane ----------------
         const int quarter = warp & 3;
         const uint32_t slots = tile_base + STAGES * STAGE_BYTES + quarter * S::SLOTS * SLOT;
         const uint32_t in_bar = smem_u32(&bars->in[quarter]);
