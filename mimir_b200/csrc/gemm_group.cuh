@@ -21,14 +21,14 @@ enum Epilogue {
     STORE,      // the result as bf16, or as f32 (stored or added to what is there)
     GATED_FWD,  // two right operands: a, b -> a and b as f32, silu(a) b as bf16
     GATED_BWD,  // dh, with a and b read -> da = dh b silu'(a) and db = dh silu(a), as bf16
-    CE_STATS,   // logits -> per row and tile the maximum and the sum of exp(l - maximum), and the target's logit
+    CE_STATS,   // logits -> per row and 128 columns the maximum and the sum of exp(l - maximum), and the target's logit
+    CE_EXP,     // the same, and exp(l - maximum) in 16 bits of its own (exp_code)
     CE_GRAD,    // logits -> g (exp(l - lse) - [column is the target]) as bf16
 };
 
 constexpr int BM = 128, BK = 64, BN = 256;
 constexpr int ACC_COLS = 256;
 constexpr int A_BYTES = BM * BK * 2, B_BYTES = 128 * BK * 2, STAGE_BYTES = A_BYTES + B_BYTES;
-constexpr int THREADS = 224;
 constexpr int GROUP_M = 8;
 constexpr int SLOT = 4096;  // a [32 rows x 128 bytes] tile of an epilogue warp
 constexpr int MAX_PROBLEMS = 4;
@@ -36,10 +36,20 @@ constexpr int MAX_PROBLEMS = 4;
 template <int EPI>
 struct Shape {
     static constexpr bool GATED = EPI == GATED_FWD;
+    // The loss is f32, and the tensor cores cut sums off where f32 rounds: an error of some 2^-25 of the value for each 16 terms, always towards zero
+    // (4096 of them: 1.2e-6 of the loss). For the loss k-blocks are therefore summed in runs, which the epilogue adds up in registers: a quarter
+    // the error at 4096, and no time, as an accumulator is read while the other one fills. That takes two warps for a row's 256 columns.
+    static constexpr bool LOSS  = EPI == CE_STATS || EPI == CE_EXP;
+    static constexpr int RUN    = LOSS ? 16 : 1 << 30;                      // k-blocks in one accumulator
+    static constexpr int WARPS  = LOSS ? 8 : 4;                             // of the epilogue
+    // one warp for each operand's loads and one for the multiplications, then the epilogue's. Eight of those hold 128 accumulators a thread: they come
+    // in whole groups of four, which pass registers on (168 a thread at launch, 3 x 168 = 56 + 2 x 224).
+    static constexpr int FIRST   = LOSS ? 4 : 3;
+    static constexpr int THREADS = (FIRST + WARPS) * 32;
     static constexpr int WIDTH  = GATED ? 128 : 256;                        // result columns of a tile
-    static constexpr int SLOTS  = EPI == GATED_FWD || EPI == GATED_BWD ? 4 : EPI == CE_STATS ? 0 : 2;  // per epilogue warp
-    static constexpr int STAGES = SLOTS == 4 ? 5 : 6;
-    static constexpr int SMEM   = STAGES * STAGE_BYTES + 4 * SLOTS * SLOT + 1024 + 256;
+    static constexpr int SLOTS  = EPI == GATED_FWD || EPI == GATED_BWD ? 16 : EPI == CE_STATS ? 0 : 8;  // of all epilogue warps
+    static constexpr int STAGES = SLOTS == 16 ? 5 : 6;
+    static constexpr int SMEM   = STAGES * STAGE_BYTES + SLOTS * SLOT + 1024 + 256;
 };
 
 struct Problem {
@@ -149,18 +159,22 @@ __device__ __forceinline__ int held(int v) {
     asm volatile("" : "+r"(v));
     return v;
 }
+// A value from 0 to 1 in 16 bits: the low seven bits of an f32's exponent and nine of its fraction (the bits above are zero), rounded half up. Ten
+// significant bits down to 2^-126, where f16 has eleven down to 2^-14 only and bf16 has eight.
+__device__ __forceinline__ uint32_t exp_code(float v) { return (__float_as_uint(v) + 0x2000u) >> 14; }
+__device__ __forceinline__ float exp_of(uint32_t code) { return __uint_as_float(code << 14); }
 // 1 / (1 + exp(-a)): 0 where exp(-a) overflows
 __device__ __forceinline__ float sigmoid(float a) { return __fdividef(1.f, 1.f + __expf(-a)); }
 
 template <int EPI>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Shape<EPI>::THREADS, 1)
 group_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args g) {
     using S = Shape<EPI>;
     constexpr int STAGES = S::STAGES, WIDTH = S::WIDTH;
     constexpr int BH = WIDTH / 2, BH_BYTES = BH * BK * 2;  // columns (of each right operand) staged by this CTA
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw_addr = smem_u32(smem_raw), tile_base = (raw_addr + 1023u) & ~1023u;
-    Bars* bars = reinterpret_cast<Bars*>(smem_raw + (tile_base - raw_addr) + STAGES * STAGE_BYTES + 4 * S::SLOTS * SLOT);
+    Bars* bars = reinterpret_cast<Bars*>(smem_raw + (tile_base - raw_addr) + STAGES * STAGE_BYTES + S::SLOTS * SLOT);
     volatile int* abort_flag = &bars->abort_flag;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -174,7 +188,7 @@ group_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args g) 
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(smem_u32(&bars->acc_full[b]), 1);
-            mbar_init(smem_u32(&bars->acc_empty[b]), 256);
+            mbar_init(smem_u32(&bars->acc_empty[b]), 2 * S::WARPS * 32);
         }
         for (int w = 0; w < 4; ++w) mbar_init(smem_u32(&bars->in[w]), 1);
         bars->abort_flag = 0;
@@ -191,8 +205,10 @@ group_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args g) 
     const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(&bars->tmem_base);
 
     Tile t;
-    if (warp == 0 || warp == 6) {
-        // ---------------- TMA producers (both CTAs): warp 0 the left operand, warp 6 the right one or ones ----------------
+    if (warp < S::FIRST) {
+      if constexpr (S::LOSS) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+      if (warp == 0 || warp == 2) {
+        // ---------------- TMA producers (both CTAs): warp 0 the left operand, warp 2 the right one or ones ----------------
         // (one thread for both took longer over a k-block than the multiplication)
         if (lane == 0) {
             const bool left = warp == 0;
@@ -233,7 +249,7 @@ group_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args g) 
                 }
             }
         }
-    } else if (warp == 1) {
+      } else if (warp == 1) {
         // ---------------- MMA issuer (even CTA only) ----------------
         if (lane == 0 && rank == 0) {
             uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0;
@@ -245,28 +261,35 @@ group_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args g) 
                 // a descriptor's low word is the address >> 4 with the leading offset >> 4 above it, its high word is the same for all
                 const uint32_t a_step = p.a_mn ? 2048 >> 4 : 32 >> 4, b_step = p.b_mn ? 2048 >> 4 : 32 >> 4;
                 const uint32_t a_low = (p.a_mn ? BK * 128 >> 4 : 1) << 16, b_low = ((p.b_mn ? BK * 128 >> 4 : 1) << 16) + (A_BYTES >> 4);
-                if (!(ok = mbar_wait(smem_u32(&bars->acc_empty[acc]), acc_phase ^ 1u, abort_flag))) break;
-                tc_fence_after();
-                for (int kb = t.kb0; kb < t.kb1; ++kb) {
-                    if (!(ok = mbar_wait(smem_u32(&bars->full[stage]), phase, abort_flag))) break;
+                int from = t.kb0;
+                do {  // (once for a tile without k-blocks, whose accumulator is not read)
+                    const int to = min(t.kb1, from + S::RUN);
+                    if (!(ok = mbar_wait(smem_u32(&bars->acc_empty[acc]), acc_phase ^ 1u, abort_flag))) break;
                     tc_fence_after();
-                    const uint32_t at = (tile_base + stage * STAGE_BYTES) >> 4;
+                    for (int kb = from; kb < to; ++kb) {
+                        if (!(ok = mbar_wait(smem_u32(&bars->full[stage]), phase, abort_flag))) break;
+                        tc_fence_after();
+                        const uint32_t at = (tile_base + stage * STAGE_BYTES) >> 4;
 #pragma unroll
-                    for (int k = 0; k < BK / 16; ++k)
-                        mma_f16_ss_pair(tmem_base + acc * ACC_COLS, high | (at + a_low + k * a_step), high | (at + b_low + k * b_step), idesc,
-                                        kb > t.kb0 || k > 0);
-                    mma_commit_pair(smem_u32(&bars->empty[stage]));
-                    if (++stage == STAGES) stage = 0, phase ^= 1u;
-                }
-                if (!ok) break;
-                mma_commit_pair(smem_u32(&bars->acc_full[acc]));
-                if (++acc == 2) acc = 0, acc_phase ^= 1u;
+                        for (int k = 0; k < BK / 16; ++k)
+                            mma_f16_ss_pair(tmem_base + acc * ACC_COLS, high | (at + a_low + k * a_step), high | (at + b_low + k * b_step), idesc,
+                                            kb > from || k > 0);
+                        mma_commit_pair(smem_u32(&bars->empty[stage]));
+                        if (++stage == STAGES) stage = 0, phase ^= 1u;
+                    }
+                    if (!ok) break;
+                    mma_commit_pair(smem_u32(&bars->acc_full[acc]));
+                    if (++acc == 2) acc = 0, acc_phase ^= 1u;
+                    from = to;
+                } while (from < t.kb1);
             }
         }
+      }
     } else {
-        // ---------------- epilogue (warps 2 to 5, both CTAs): 32 rows each, one per lane ----------------
+        if constexpr (S::LOSS) asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+        // ---------------- epilogue (both CTAs): 32 rows for each warp (for each two of them, where there are eight), one per lane ----------------
         const int quarter = warp & 3;
-        const uint32_t slots = tile_base + STAGES * STAGE_BYTES + quarter * S::SLOTS * SLOT;
+        const uint32_t slots = tile_base + STAGES * STAGE_BYTES + (warp - S::FIRST) * (S::SLOTS / S::WARPS) * SLOT;
         const uint32_t in_bar = smem_u32(&bars->in[quarter]);
         uint32_t acc = 0, acc_phase = 0, turn = 0, in_phase = 0;
         bool ok = true;
@@ -288,15 +311,21 @@ group_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args g) 
             const int row0 = t.m + int(rank) * BM + quarter * 32, row = row0 + lane;
             // (products over rows read whole k-blocks of them: CE_GRAD writes zeros up to the end of the last one)
             const bool empty = t.kb0 == t.kb1, there = row0 < (EPI == CE_GRAD ? (t.rows + BK - 1) / BK * BK : t.rows);
-            const int at_tile = t.n / WIDTH, n0 = t.n;
-            if (!(ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&bars->acc_full[acc]), acc_phase, abort_flag)))) break;
-            tc_fence_after();
-            const uint32_t t0 = tmem_base + acc * ACC_COLS + (uint32_t(quarter * 32) << 16);
-            const uint32_t acc_empty_even = map_to_cta(smem_u32(&bars->acc_empty[acc]), 0);
+            const int n0 = t.n;
+            uint32_t t0, acc_empty_even;
+            auto next_acc = [&] {
+                const bool full = __all_sync(0xffffffffu, mbar_wait(smem_u32(&bars->acc_full[acc]), acc_phase, abort_flag));
+                tc_fence_after();
+                t0             = tmem_base + acc * ACC_COLS + (uint32_t(quarter * 32) << 16);
+                acc_empty_even = map_to_cta(smem_u32(&bars->acc_empty[acc]), 0);
+                if (++acc == 2) acc = 0, acc_phase ^= 1u;
+                return full;
+            };
             auto release = [&] {  // after the last read of this accumulator
                 tc_fence_before();
                 mbar_arrive_cluster(acc_empty_even);
             };
+            if (!(ok = next_acc())) break;
             // one slot's tile to a matrix, as a bulk group of its own (an empty one where the tile lies past the last column: a slot is free
             // by the number of groups committed since)
             auto send = [&](const CUtensorMap* m, uint32_t slot, int x, bool add = false, int down = 0) {
@@ -312,6 +341,10 @@ group_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args g) 
             };
             if (!there) {
                 release();
+                for (int kb = t.kb0 + min(S::RUN, t.kb1 - t.kb0); ok && kb < t.kb1; kb += S::RUN) {  // the tile's other accumulators
+                    if ((ok = next_acc())) release();
+                }
+                if (!ok) break;
             } else if constexpr (EPI == STORE) {
                 const int step = p.out_f32 ? 32 : 64;
 #pragma unroll 1
@@ -389,40 +422,65 @@ group_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args g) 
                     }
                 }
                 if (!ok) break;
-            } else if constexpr (EPI == CE_STATS) {
-                const int tcol = row < t.rows ? g.target[row] - g.column0 - n0 : -1, left = p.N - n0;
-                float top = -INFINITY, sum = 0.f;
-                float v[32];
+            } else if constexpr (S::LOSS) {
+                // this warp's 128 of the columns, in registers: the runs of k-blocks added up
+                const int half = (warp - S::FIRST) >> 2 << 7, n1 = n0 + half, left = p.N - n1;
+                const int tcol = row < t.rows ? g.target[row] - n1 : -1;
+                uint32_t raw[128];
+#pragma unroll
+                for (int c = 0; c < 128; c += 32) tmem_ld_32x32(t0 + half + c, *reinterpret_cast<uint32_t(*)[32]>(raw + c));
+                tmem_ld_wait();
+                release();
 #pragma unroll 1
-                for (int c = 0; c < WIDTH; c += 32) {
-                    get_acc(t0 + c, v, empty);
-                    if (c + 32 > left) {
+                for (int kb = t.kb0 + S::RUN; kb < t.kb1; kb += S::RUN) {
+                    if (!(ok = next_acc())) break;
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) v[i] = c + i < left ? v[i] : -INFINITY;
+                    for (int c = 0; c < 128; c += 16) {
+                        uint32_t r[16];
+                        tmem_ld_32x16(t0 + half + c, r);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) raw[c + i] = __float_as_uint(__uint_as_float(raw[c + i]) + __uint_as_float(r[i]));
                     }
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) top = fmaxf(top, v[i]);
+                    release();
                 }
+                if (!ok) break;
+                float v[128];
+#pragma unroll
+                for (int i = 0; i < 128; ++i) v[i] = __uint_as_float(raw[i]);
+                if (left < 128) {
+#pragma unroll
+                    for (int i = 0; i < 128; ++i) v[i] = i < left ? v[i] : -INFINITY;
+                }
+                if (__any_sync(0xffffffffu, tcol >= 0 && tcol < 128)) {
+#pragma unroll
+                    for (int i = 0; i < 128; ++i)
+                        if (tcol == i) g.target_logit[row] = v[i];
+                }
+                float top = -INFINITY, sum = 0.f;
+#pragma unroll
+                for (int i = 0; i < 128; ++i) top = fmaxf(top, v[i]);
                 const float base = top == -INFINITY ? 0.f : top;
-#pragma unroll 1
-                for (int c = 0; c < WIDTH; c += 32) {
-                    get_acc(t0 + c, v, empty);
-                    if (c + 32 >= WIDTH) release();
-                    if (__any_sync(0xffffffffu, tcol >= c && tcol < c + 32)) {
 #pragma unroll
-                        for (int i = 0; i < 32; ++i)
-                            if (tcol == c + i) g.target_logit[row] = v[i];
-                    }
-                    if (c + 32 > left) {
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) v[i] = c + i < left ? v[i] : -INFINITY;
-                    }
+                for (int c = 0; c < 128; c += 32) {
                     float part = 0.f;
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) part += __expf(v[i] - base);
+                    for (int i = c; i < c + 32; ++i) v[i] = __expf(v[i] - base), part += v[i];
                     sum += part;
                 }
-                if (row < t.rows) g.part[int64_t(row) * ((p.N + WIDTH - 1) / WIDTH) + at_tile] = make_float2(top, sum);
+                if (row < t.rows) g.part[int64_t(row) * ((p.N + 255) / 256 * 2) + (n1 >> 7)] = make_float2(top, sum);
+                if constexpr (EPI == CE_EXP) {
+#pragma unroll
+                    for (int c = 0; c < 128; c += 64) {
+                        if (lane == 0) bulk_wait_read_0();
+                        __syncwarp();
+#pragma unroll
+                        for (int i = 0; i < 64; i += 8)
+                            st_shared_v4(slots + lane * 128 + ((uint32_t(i >> 3) ^ uint32_t(lane & 7)) << 4), __byte_perm(exp_code(v[c + i]), exp_code(v[c + i + 1]), 0x5410),
+                                         __byte_perm(exp_code(v[c + i + 2]), exp_code(v[c + i + 3]), 0x5410), __byte_perm(exp_code(v[c + i + 4]), exp_code(v[c + i + 5]), 0x5410), __byte_perm(exp_code(v[c + i + 6]), exp_code(v[c + i + 7]), 0x5410));
+                        send(&maps.out[0], slots, n1 + c);
+                    }
+                }
             } else {
                 const bool mine = row < t.rows;
                 const int tcol  = mine ? g.target[row] - g.column0 - n0 : -1;
@@ -447,7 +505,6 @@ group_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args g) 
                     }
                 }
             }
-            if (++acc == 2) acc = 0, acc_phase ^= 1u;
             tile += num_pairs;
             have = locate<WIDTH>(g, tile, t);
             if (have) request(t, 0);
@@ -502,7 +559,7 @@ int launch_group(const Maps& maps, const Args& args, const DeviceInfo& dev, cuda
     const int64_t pairs = dev.sm_count / 2;
     const int grid      = int(2 * (tiles < pairs ? tiles : pairs));
     if (!grid) return MIMK_OK;
-    kern<<<grid, THREADS, Shape<EPI>::SMEM, s>>>(maps, args);
+    kern<<<grid, Shape<EPI>::THREADS, Shape<EPI>::SMEM, s>>>(maps, args);
     return launch_status();
 }
 

@@ -3,10 +3,12 @@
 //   lse_i = log sum_j exp(l_ij),  loss_i = lse_i - l_i,t(i)
 //   p_ij = g_i (exp(l_ij - lse_i) - [j = t(i)]),  dx = p W^T,  dW = x^T p        g: the loss's gradient, over the count for a mean
 //
-// bf16: the logits exist as accumulators only. A first product reduces each tile of 256 columns to a maximum and a sum of exponentials per row
-// (8 bytes for 256 logits); a kernel over rows joins them. The gradient goes by pieces of the classes: a second product writes p of the piece
-// as bf16, and one launch then makes the piece's rows of dW and adds to dx in f32. 8 n d v operations, two of them logits over again: kept, they
-// would be n v values of 32 bits (4 GiB for 8192 x 131072), or of 16 with an error of 2^-9 |l| in every exponent.
+// bf16: the logits exist as accumulators only. A first product reduces each 128 columns of a row to a maximum and a sum of exponentials
+// (8 bytes for 128 logits); a kernel over rows joins them. Loss and gradients in one call: where n v is at most 2^30, that product also leaves
+// the exponentials themselves in 16 bits (ten of them significant, where p has eight: as bf16 they would round p twice), which a pass over them turns into p once the sums are
+// known (the targets' p from their logits, in f32), and one launch makes dW and dx: 6 n d v operations. Beyond that, and for gradients from an earlier call's lse, by pieces
+// of the classes: a product writes p of the piece as bf16, and one launch makes the piece's rows of dW and adds to dx in f32: 8 n d v
+// operations, two of them logits over again, and 512 MiB of p. 8192 x 4096 x 131072: MEASURED_BOTH.
 // f32: pieces of rows instead, through the library's f32 products, with the logits of a piece in memory, turned into p in place.
 //
 // Rows without a target (the ignored index) are taken out first: the rows that are left are copied together, and the products run over as
@@ -23,6 +25,7 @@ using namespace group;
 
 constexpr int64_t LIM = int64_t(1) << 30;
 constexpr int64_t PIECE_CELLS = int64_t(1) << 28;  // bf16: p of a piece, 512 MiB
+constexpr int64_t KEPT_CELLS  = int64_t(1) << 30;  // bf16: exponentials that are kept until the sums are known, 2 GiB
 constexpr int64_t PIECE_FLOATS = int64_t(1) << 27; // f32: logits of a piece, 512 MiB
 
 struct Rows {             // per row that is left (all of them without an ignored index)
@@ -150,6 +153,45 @@ __global__ void __launch_bounds__(256) join_kernel(Rows r, int64_t n, int tiles,
     if (loss) finish_loss(r, n, reduction, loss);
 }
 
+// p from the exponentials, in place: exp(l - m) becomes scale exp(l - lse) as bf16, less scale at the target, whose own value comes from its
+// logit; zeros in the rows up to the end of the last 64, which the products over rows read. A warp takes 1024 columns of a row, a lane four times 16
+// bytes. Bound by the bytes: MEASURED_P.
+__global__ void __launch_bounds__(256) probabilities_kernel(Rows r, uint16_t* __restrict__ p, int64_t pitch, int64_t n, int tiles) {
+    const int lane = threadIdx.x & 31;
+    const int left = r.count[0];
+    const int64_t end = min(n, (int64_t(left) + 63) / 64 * 64);
+    const int first   = (int(blockIdx.x) * 8 + int(threadIdx.x >> 5)) * 1024 + lane * 8;
+    for (int64_t j = blockIdx.y; j < end; j += gridDim.y) {
+        const bool there = j < left;
+        const float lse  = there ? r.lse[j] : 0.f, scale = there ? r.scale[j] : 0.f;
+        const int target = there ? r.target[j] : -1;
+        uint4 v[4];
+        float top[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int c = first + i * 256;
+            if (c >= pitch) continue;
+            v[i]   = there ? *reinterpret_cast<const uint4*>(p + j * pitch + c) : make_uint4(0, 0, 0, 0);
+            top[i] = there ? r.part[j * tiles + (c >> 7)].x : 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int c = first + i * 256;
+            if (c >= pitch) continue;
+            const float by = scale * __expf(top[i] - lse);
+            uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                float lo = exp_of(w[e] & 0xffffu) * by, hi = exp_of(w[e] >> 16) * by;
+                if (target - c == 2 * e) lo = scale * (__expf(r.target_logit[j] - lse) - 1.f);
+                if (target - c == 2 * e + 1) hi = scale * (__expf(r.target_logit[j] - lse) - 1.f);
+                w[e] = there ? pack_bf16x2(lo, hi) : 0u;
+            }
+            *reinterpret_cast<uint4*>(p + j * pitch + c) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+    }
+}
+
 // the rows' logarithms from an earlier call, and their scales
 __global__ void recall_kernel(Rows r, const float* __restrict__ lse, const float* dloss, int reduction) {
     const int left = r.count[0];
@@ -247,6 +289,7 @@ struct Plan {
     Staged w, dw;
     int tiles;
     int64_t piece;              // columns (bf16) or rows (f32) of a piece
+    bool kept;                  // bf16: the forward product leaves its exponentials, and all columns are one piece
     void* p;                    // bf16: p of a piece; f32: its logits
     float* dx;                  // partial sums of dx (bf16), or dx of the rows that are left (f32)
     int splits;
@@ -282,11 +325,12 @@ Plan plan(const mimk_linear_ce_desc& d, bool forward, bool backward, Space& spac
     if (taken || !tma_can_read(d.x, d.d)) p.x_pitch = up(d.d, 8), p.x = space.take(n * size_t(p.x_pitch) * 2);
     const bool nk = d.w_layout == MIMK_B_NK;
     p.w           = nk ? stage(space, d.w, d.v, d.d) : stage(space, d.w, d.d, d.v);
-    p.tiles       = int((d.v + 255) / 256);
+    p.tiles       = int((d.v + 255) / 256) * 2;
     if (forward) p.rows.part = static_cast<float2*>(space.take(n * size_t(p.tiles) * 8)), p.rows.target_logit = floats(n);
     if (backward) {
         p.dw    = nk ? stage(space, d.dw, d.v, d.d) : stage(space, d.dw, d.d, d.v);
-        p.piece = std::min(up(d.v, 256), std::max<int64_t>(4096, PIECE_CELLS / d.n / 256 * 256));
+        p.kept  = forward && d.n * up(d.v, 8) <= KEPT_CELLS;
+        p.piece = p.kept ? up(d.v, 8) : std::min(up(d.v, 256), std::max<int64_t>(4096, PIECE_CELLS / d.n / 256 * 256));
         p.p     = space.take(n * size_t(p.piece) * 2);
         p.splits   = pick_splits(d.n, d.d, std::min(d.v, p.piece) / 64 + 1, sm_count);
         p.rows_pad = up(d.n, 32), p.dx_pitch = up(d.d, 4);
@@ -417,25 +461,37 @@ int run_bf16(const mimk_linear_ce_desc& d, const Plan& p, bool forward, bool bac
         args.p[0].dyn_m = count;
         MIMK_TRY(operand_map(&maps.a[0][0], x, false, BM));
         MIMK_TRY(operand_map(&maps.b[0][0], w, !nk, 128));
-        MIMK_TRY(launch_group<CE_STATS>(maps, args, dev, s));
+        if (p.kept) {
+            MIMK_TRY(result_map(&maps.out[0], p.p, false, d.n, d.v, p.piece));
+            MIMK_TRY(launch_group<CE_EXP>(maps, args, dev, s));
+        } else {
+            MIMK_TRY(launch_group<CE_STATS>(maps, args, dev, s));
+        }
         join_kernel<<<grid_for(d.n, 8, 2048), 256, 0, s>>>(p.rows, d.n, p.tiles, d.dloss, d.reduction, loss, d.lse);
     } else {
         recall_kernel<<<grid_for(d.n, 256, 1024), 256, 0, s>>>(p.rows, d.lse, d.dloss, d.reduction);
     }
     MIMK_TRY(launch_status());
     if (!backward) return MIMK_OK;
+    if (p.kept) {
+        const dim3 grid(unsigned((p.piece + 8191) / 8192), grid_for(d.n, 1, 65535));
+        probabilities_kernel<<<grid, 256, 0, s>>>(p.rows, static_cast<uint16_t*>(p.p), p.piece, d.n, p.tiles);
+        MIMK_TRY(launch_status());
+    }
 
     for (int64_t from = 0; from < d.v; from += p.piece) {
         const int64_t cols = std::min(p.piece, d.v - from);
         const Mat wi = part_of(w, from, cols), pi = {p.p, d.n, cols, p.piece};
-        args.count      = 1;
-        args.column0    = int(from);
-        args.p[0]       = problem(d.n, cols, d.d, false, !nk);
-        args.p[0].dyn_m = count;
-        MIMK_TRY(operand_map(&maps.a[0][0], x, false, BM));
-        MIMK_TRY(operand_map(&maps.b[0][0], wi, !nk, 128));
-        MIMK_TRY(result_map(&maps.out[0], p.p, false, d.n, cols, p.piece));
-        MIMK_TRY(launch_group<CE_GRAD>(maps, args, dev, s));
+        if (!p.kept) {
+            args.count      = 1;
+            args.column0    = int(from);
+            args.p[0]       = problem(d.n, cols, d.d, false, !nk);
+            args.p[0].dyn_m = count;
+            MIMK_TRY(operand_map(&maps.a[0][0], x, false, BM));
+            MIMK_TRY(operand_map(&maps.b[0][0], wi, !nk, 128));
+            MIMK_TRY(result_map(&maps.out[0], p.p, false, d.n, cols, p.piece));
+            MIMK_TRY(launch_group<CE_GRAD>(maps, args, dev, s));
+        }
         // dx += p W^T: W stored [v, d] has the result's columns contiguous, [d, v] the classes
         args.count      = 2;
         args.p[0]       = problem(d.n, d.d, cols, false, nk);
