@@ -268,6 +268,147 @@ OP(mlp_gated, 4)
     return result(unlocked([&](void* stream) { return mimk_mlp_gated(&d, stream); }), std::move(out));
 END_OP
 
+// Results as a tuple, or None for a status that is not OK.
+PyObject* results(int status, std::vector<Tensor>&& out) {
+    if (status != MIMK_OK) Py_RETURN_NONE;
+    PyObject* all = PyTuple_New(Py_ssize_t(out.size()));
+    if (!all) return nullptr;
+    for (size_t i = 0; i < out.size(); ++i) {
+        PyObject* o = THPVariable_Wrap(std::move(out[i]));
+        if (!o) {
+            Py_DECREF(all);
+            return nullptr;
+        }
+        PyTuple_SET_ITEM(all, Py_ssize_t(i), o);
+    }
+    return all;
+}
+// A gradient of w's shape, in w's storage layout.
+Tensor like_weight(const Tensor& w, int layout) {
+    return layout == MIMK_B_KN ? empty({w.size(0), w.size(1)}, w.scalar_type(), w) : empty({w.size(1), w.size(0)}, w.scalar_type(), w).t();
+}
+bool mlp_train_desc(PyObject* const* a, mimk_mlp_train_desc& d, const Tensor* (&t)[4]) {
+    t[0] = dense(a[0]);
+    for (int i = 1; i < 4; ++i) t[i] = dense(a[i], true);
+    for (const Tensor* x : t)
+        if (!x || x->dim() != 2 || x->scalar_type() != t[0]->scalar_type()) return false;
+    const int layout = b_layout(*t[1]);
+    if (layout < 0 || b_layout(*t[2]) != layout || b_layout(*t[3]) != layout) return false;
+    if (t[1]->sizes() != t[2]->sizes() || t[0]->size(1) != t[1]->size(0) || t[1]->size(1) != t[3]->size(0)) return false;
+    d = {};
+    d.m = t[0]->size(0), d.k = t[0]->size(1), d.f = t[1]->size(1), d.n = t[3]->size(1);
+    d.x = t[0]->data_ptr(), d.w1 = t[1]->data_ptr(), d.w3 = t[2]->data_ptr(), d.w2 = t[3]->data_ptr();
+    d.dtype = dtype_of(t[0]->scalar_type()), d.b_layout = layout;
+    return true;
+}
+
+// x, w1, w3, w2 -> y, kept
+OP(mlp_gated_fwd, 4)
+    mimk_mlp_train_desc d;
+    const Tensor* t[4];
+    if (!mlp_train_desc(a, d, t)) Py_RETURN_NONE;
+    Tensor y = empty({d.m, d.n}, t[0]->scalar_type(), *t[0]);
+    d.y = y.data_ptr();
+    uint64_t kept = 0;
+    if (mimk_mlp_gated_train_sizes(&d, &kept, &d.workspace_bytes, nullptr) != MIMK_OK) Py_RETURN_NONE;
+    Tensor buffer = empty({int64_t(kept)}, at::kByte, y), scratch = empty({int64_t(d.workspace_bytes)}, at::kByte, y);
+    d.kept = buffer.data_ptr(), d.workspace = scratch.data_ptr();
+    const int status = unlocked([&](void* stream) { return mimk_mlp_gated_fwd(&d, stream); });
+    return results(status, {std::move(y), std::move(buffer)});
+END_OP
+
+// x, w1, w3, w2, dy, the kept buffer, the extents it is for -> dx, dw1, dw3, dw2
+OP(mlp_gated_bwd, 7)
+    mimk_mlp_train_desc d;
+    const Tensor *t[4], *dy = dense(a[4]);
+    if (!mlp_train_desc(a, d, t) || !dy || dy->dim() != 2 || dy->size(0) != d.m || dy->size(1) != d.n || dy->scalar_type() != t[0]->scalar_type()) Py_RETURN_NONE;
+    if (!THPVariable_Check(a[5]) || !PyTuple_CheckExact(a[6]) || PyTuple_GET_SIZE(a[6]) != 4) Py_RETURN_NONE;
+    const int64_t extents[4] = {d.m, d.k, d.f, d.n};
+    for (int i = 0; i < 4; ++i) {
+        int64_t e;
+        if (!is_int(PyTuple_GET_ITEM(a[6], i), e) || e != extents[i]) Py_RETURN_NONE;
+    }
+    std::vector<Tensor> out = {empty({d.m, d.k}, t[0]->scalar_type(), *t[0])};
+    for (int i = 1; i < 4; ++i) out.push_back(like_weight(*t[i], d.b_layout));
+    d.dy = dy->data_ptr(), d.kept = THPVariable_Unpack(a[5]).data_ptr();
+    d.dx = out[0].data_ptr(), d.dw1 = out[1].data_ptr(), d.dw3 = out[2].data_ptr(), d.dw2 = out[3].data_ptr();
+    if (mimk_mlp_gated_train_sizes(&d, nullptr, nullptr, &d.workspace_bytes) != MIMK_OK) Py_RETURN_NONE;
+    Tensor scratch = empty({int64_t(d.workspace_bytes)}, at::kByte, *dy);
+    d.workspace    = scratch.data_ptr();
+    const int status = unlocked([&](void* stream) { return mimk_mlp_gated_bwd(&d, stream); });
+    return results(status, std::move(out));
+END_OP
+
+// x, w, targets, ignored index or None, reduction id, dloss or None, lse or None, forward, backward, lse wanted -> what of loss, lse, dx, dw is asked for
+OP(linear_ce, 10)
+    const Tensor *x = dense(a[0]), *w = dense(a[1], true), *dloss = a[5] == Py_None ? nullptr : dense(a[5]), *lse = a[6] == Py_None ? nullptr : dense(a[6]);
+    if (!x || !w || (!dloss && a[5] != Py_None) || (!lse && a[6] != Py_None) || !THPVariable_CheckExact(a[2])) Py_RETURN_NONE;
+    const Tensor& t = THPVariable_Unpack(a[2]);
+    int64_t reduction, ignore = 0;
+    if (!is_int(a[4], reduction) || (a[3] != Py_None && !is_int(a[3], ignore)) || !PyBool_Check(a[7]) || !PyBool_Check(a[8]) || !PyBool_Check(a[9])) Py_RETURN_NONE;
+    const bool forward = a[7] == Py_True, backward = a[8] == Py_True, want_lse = a[9] == Py_True;
+    const int64_t r = x->dim();
+    const int layout = w->dim() == 2 ? b_layout(*w) : -1;
+    if (r < 1 || layout < 0 || x->size(r - 1) != w->size(0) || x->scalar_type() != w->scalar_type()) Py_RETURN_NONE;
+    if (!t.defined() || !t.is_cuda() || t.layout() != at::kStrided || !t.is_contiguous() || (t.scalar_type() != at::kLong && t.scalar_type() != at::kInt)) Py_RETURN_NONE;
+    const at::IntArrayRef lead = x->sizes().slice(0, size_t(r - 1)), each = reduction == MIMK_REDUCTION_NONE ? lead : at::IntArrayRef();
+    if (t.sizes() != lead) Py_RETURN_NONE;
+    if (dloss && (dloss->scalar_type() != at::kFloat || dloss->sizes() != each)) Py_RETURN_NONE;
+    if (forward == (lse != nullptr) || (lse && (lse->scalar_type() != at::kFloat || lse->sizes() != lead))) Py_RETURN_NONE;
+    mimk_linear_ce_desc d = {};
+    d.d = w->size(0), d.v = w->size(1), d.n = x->numel() / d.d;
+    d.x = x->data_ptr(), d.w = w->data_ptr(), d.targets = t.data_ptr();
+    d.dloss = dloss ? static_cast<const float*>(dloss->data_ptr()) : nullptr, d.lse = lse ? static_cast<float*>(lse->data_ptr()) : nullptr;
+    d.ignore_index = ignore, d.has_ignore = a[3] != Py_None, d.reduction = int(reduction);
+    d.dtype = dtype_of(x->scalar_type()), d.target_dtype = t.scalar_type() == at::kLong ? MIMK_I64 : MIMK_I32, d.w_layout = layout;
+    std::vector<Tensor> out;
+    if (forward) {
+        out.push_back(empty(each, at::kFloat, *x));
+        d.loss = static_cast<float*>(out.back().data_ptr());
+        if (want_lse) out.push_back(empty(lead, at::kFloat, *x)), d.lse = static_cast<float*>(out.back().data_ptr());
+    }
+    if (backward) {
+        out.push_back(empty(x->sizes(), x->scalar_type(), *x)), d.dx = out.back().data_ptr();
+        out.push_back(like_weight(*w, layout)), d.dw = out.back().data_ptr();
+    }
+    if (mimk_linear_ce_workspace(&d, forward, backward, &d.workspace_bytes) != MIMK_OK) Py_RETURN_NONE;
+    Tensor scratch = empty({int64_t(d.workspace_bytes)}, at::kByte, *x);
+    d.workspace    = scratch.data_ptr();
+    const int status = unlocked([&](void* stream) { return forward ? (backward ? mimk_linear_ce_fwd_bwd(&d, stream) : mimk_linear_ce_fwd(&d, stream)) : mimk_linear_ce_bwd(&d, stream); });
+    return results(status, std::move(out));
+END_OP
+
+// a list of gradients, a list of results or None, limit or None (the norm alone), eps -> norm
+OP(clip_grads, 4)
+    if (!PyList_CheckExact(a[0]) || (a[1] != Py_None && !PyList_CheckExact(a[1]))) Py_RETURN_NONE;
+    const Py_ssize_t count = PyList_GET_SIZE(a[0]);
+    const bool clip = a[2] != Py_None;
+    if (!count || (a[1] != Py_None && PyList_GET_SIZE(a[1]) != count) || (clip && (!PyFloat_CheckExact(a[2]) || !PyFloat_CheckExact(a[3])))) Py_RETURN_NONE;
+    std::vector<const void*> in(count);
+    std::vector<void*> out(count);
+    std::vector<int64_t> lengths(count);
+    std::vector<int32_t> dtypes(count);
+    const Tensor* first = nullptr;
+    for (Py_ssize_t i = 0; i < count; ++i) {
+        const Tensor *t = dense(PyList_GET_ITEM(a[0], i), true), *o = a[1] == Py_None ? t : dense(PyList_GET_ITEM(a[1], i), true);
+        if (!t || !o || !t->is_non_overlapping_and_dense()) Py_RETURN_NONE;
+        if (o != t && (o->scalar_type() != t->scalar_type() || o->sizes() != t->sizes() || o->strides() != t->strides())) Py_RETURN_NONE;
+        first = first ? first : t;
+        if (t->device() != first->device() || o->device() != first->device()) Py_RETURN_NONE;
+        in[i] = t->data_ptr(), out[i] = o->data_ptr(), lengths[i] = t->numel(), dtypes[i] = dtype_of(t->scalar_type());
+    }
+    uint64_t bytes = 0;
+    if (mimk_clip_grads_workspace(count, &bytes) != MIMK_OK) Py_RETURN_NONE;
+    Tensor norm = empty({}, at::kFloat, *first), scratch = empty({int64_t(bytes)}, at::kByte, *first);
+    float* to = static_cast<float*>(norm.data_ptr());
+    void* ws  = scratch.data_ptr();
+    return result(unlocked([&](void* stream) {
+                      return clip ? mimk_clip_grads(in.data(), out.data(), lengths.data(), dtypes.data(), count, float(PyFloat_AS_DOUBLE(a[2])), float(PyFloat_AS_DOUBLE(a[3])), to, ws, bytes, stream)
+                                  : mimk_grad_norm(in.data(), lengths.data(), dtypes.data(), count, to, ws, bytes, stream);
+                  }),
+                  std::move(norm));
+END_OP
+
 // x, perm (a tuple of ints): the copy-style map_reduce_post that tensor.py's transpose spells
 OP(transpose, 2)
     const Tensor* x = dense(a[0]);
@@ -293,7 +434,7 @@ END_OP
 PyMethodDef methods[] = {
 #define ENTRY(NAME) {#NAME, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(NAME)), METH_FASTCALL, nullptr}
     ENTRY(product_2d), ENTRY(bmm), ENTRY(reduce), ENTRY(reduce_of_unary), ENTRY(softmax), ENTRY(rmsnorm), ENTRY(unary), ENTRY(binary), ENTRY(binary_ax),
-    ENTRY(attention), ENTRY(mlp_gated), ENTRY(transpose), {nullptr, nullptr, 0, nullptr}};
+    ENTRY(attention), ENTRY(mlp_gated), ENTRY(mlp_gated_fwd), ENTRY(mlp_gated_bwd), ENTRY(linear_ce), ENTRY(clip_grads), ENTRY(transpose), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods};
 
 }  // namespace

@@ -400,6 +400,8 @@ def _mlp_train_desc(x, w1, w3, w2):
 
 def mlp_gated_fwd(x: torch.Tensor, w1: torch.Tensor, w3: torch.Tensor, w2: torch.Tensor):
     """mlp_gated for training, bf16: (y, kept), `kept` being what mlp_gated_bwd needs of this pass (10 bytes per row and hidden column)."""
+    if (out := _native.mlp_gated_fwd(x, w1, w3, w2)) is not None:
+        return out[0], MlpKept(out[1], (*x.shape, *w2.shape))
     d, held = _mlp_train_desc(x, w1, w3, w2)
     y = torch.empty((d.m, d.n), dtype=x.dtype, device=x.device)
     d.y = y.data_ptr()
@@ -414,6 +416,8 @@ def mlp_gated_fwd(x: torch.Tensor, w1: torch.Tensor, w3: torch.Tensor, w2: torch
 def mlp_gated_bwd(dy: torch.Tensor, x: torch.Tensor, w1: torch.Tensor, w3: torch.Tensor, w2: torch.Tensor, kept: MlpKept):
     """The gradients (dx, dw1, dw3, dw2) of the mlp_gated_fwd call that gave `kept`, from its result's gradient; the weights' have the
     weights' storage layout."""
+    if (out := _native.mlp_gated_bwd(x, w1, w3, w2, dy, kept.buffer, kept.extents)) is not None:
+        return out
     d, held = _mlp_train_desc(x, w1, w3, w2)
     _dev(dy)
     if (d.m, d.k, d.f, d.n) != kept.extents:
@@ -437,6 +441,8 @@ _REDUCTION = {"none": L.REDUCTION_NONE, "mean": L.REDUCTION_MEAN, "sum": L.REDUC
 
 
 def _linear_ce(what, x, w, targets, ignore_index, reduction, dloss, lse, forward, backward, want_lse=False):
+    if (out := _native.linear_ce(x, w, targets, ignore_index, _REDUCTION.get(reduction), dloss, lse, forward, backward, want_lse)) is not None:
+        return out
     _dev(x, w, targets, dloss, lse)
     if reduction not in _REDUCTION:
         raise ValueError(f"{what}: reduction is one of {', '.join(_REDUCTION)}")
@@ -546,6 +552,9 @@ def _grad_list(what, grads, out=None):
 
 def grad_norm(grads) -> torch.Tensor:
     """The 2-norm of all values of the tensors (F32 and BF16 ones, of any number) together, as an F32 tensor without axes."""
+    grads = list(grads)
+    if (norm := _native.clip_grads(grads, None, None, None)) is not None:
+        return norm
     ins, _, lengths, dtypes, n, norm, ws, size = _grad_list("grad_norm", grads)
     L.check(L.lib().mimk_grad_norm(ins, lengths, dtypes, n, norm.data_ptr(), ws.data_ptr(), size, _stream()), "grad_norm")
     return norm
@@ -554,9 +563,12 @@ def grad_norm(grads) -> torch.Tensor:
 def clip_grad_norm(grads, limit: float, *, eps: float = 1e-6, out=None) -> torch.Tensor:
     """Scales the tensors by min(1, limit / (norm + eps)), in place or into the tensors `out`, and returns their norm from before
     (grad_norm). A norm of NaN makes every value NaN, an infinite one zeros, and NaN of what was infinite."""
-    ins, outs, lengths, dtypes, n, norm, ws, size = _grad_list("clip_grad_norm", grads, out)
     if not (limit >= 0 and eps >= 0):
         raise ValueError("clip_grad_norm: limit and eps are at least 0")
+    grads, out, limit, eps = list(grads), None if out is None else list(out), float(limit), float(eps)
+    if (norm := _native.clip_grads(grads, out, limit, eps)) is not None:
+        return norm
+    ins, outs, lengths, dtypes, n, norm, ws, size = _grad_list("clip_grad_norm", grads, out)
     L.check(L.lib().mimk_clip_grads(ins, outs, lengths, dtypes, n, limit, eps, norm.data_ptr(), ws.data_ptr(), size, _stream()), "clip_grad_norm")
     return norm
 
