@@ -47,8 +47,8 @@ struct Shape {
     static constexpr int FIRST   = LOSS ? 4 : 3;
     static constexpr int THREADS = (FIRST + WARPS) * 32;
     static constexpr int WIDTH  = GATED ? 128 : 256;                        // result columns of a tile
-    static constexpr int SLOTS  = EPI == GATED_FWD || EPI == GATED_BWD ? 16 : EPI == CE_STATS ? 0 : 8;  // of all epilogue warps
-    static constexpr int STAGES = SLOTS == 16 ? 5 : 6;
+    static constexpr int SLOTS  = EPI == GATED_BWD ? 24 : EPI == GATED_FWD ? 16 : EPI == CE_STATS ? 0 : 8;  // of all epilogue warps
+    static constexpr int STAGES = SLOTS == 24 ? 4 : SLOTS == 16 ? 5 : 6;
     static constexpr int SMEM   = STAGES * STAGE_BYTES + SLOTS * SLOT + 1024 + 256;
 };
 
@@ -82,7 +82,7 @@ static_assert(sizeof(Maps) + sizeof(Args) <= 4096, "too many parameters");
 #ifdef __CUDACC__
 
 struct Bars {
-    uint64_t full[6], empty[6], acc_full[2], acc_empty[2], in[4];
+    uint64_t full[6], empty[6], acc_full[2], acc_empty[2], in[8];
     uint32_t tmem_base;
     int abort_flag;
 };
@@ -190,7 +190,7 @@ group_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args g) 
             mbar_init(smem_u32(&bars->acc_full[b]), 1);
             mbar_init(smem_u32(&bars->acc_empty[b]), 2 * S::WARPS * 32);
         }
-        for (int w = 0; w < 4; ++w) mbar_init(smem_u32(&bars->in[w]), 1);
+        for (int w = 0; w < 8; ++w) mbar_init(smem_u32(&bars->in[w]), 1);
         bars->abort_flag = 0;
         fence_barrier_init();
     }
@@ -203,6 +203,7 @@ group_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args g) 
     cluster_sync();
     tc_fence_after();
     const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(&bars->tmem_base);
+    after_previous();
 
     Tile t;
     if (warp < S::FIRST) {
@@ -290,28 +291,28 @@ group_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args g) 
         // ---------------- epilogue (both CTAs): 32 rows for each warp (for each two of them, where there are eight), one per lane ----------------
         const int quarter = warp & 3;
         const uint32_t slots = tile_base + STAGES * STAGE_BYTES + (warp - S::FIRST) * (S::SLOTS / S::WARPS) * SLOT;
-        const uint32_t in_bar = smem_u32(&bars->in[quarter]);
+        const uint32_t in_bar = smem_u32(&bars->in[quarter * 2]);
         uint32_t acc = 0, acc_phase = 0, turn = 0, in_phase = 0;
         bool ok = true;
         bool have = locate<WIDTH>(g, pair, t);
-        // GATED_BWD: a and b of the 32 columns that come next, requested as soon as the slots are free
+        // GATED_BWD: a and b of 32 columns, two such pairs of slots in turn, requested as soon as a pair is free
         auto request = [&](const Tile& at, int c) {
             if constexpr (EPI == GATED_BWD) {
-                const int row = at.m + int(rank) * BM + quarter * 32;
-                if (lane == 0 && row < at.rows) {
-                    mbar_expect_tx(in_bar, 2 * SLOT);
-                    tma_load_2d(slots, &maps.extra[0], at.n + c, row, in_bar);
-                    tma_load_2d(slots + SLOT, &maps.extra[1], at.n + c, row, in_bar);
+                const int row = at.m + int(rank) * BM + quarter * 32, second = c >> 5 & 1;
+                if (lane == 0 && row < at.rows && c < WIDTH && at.n + c < g.p[at.prob].N) {
+                    mbar_expect_tx(in_bar + second * 8, 2 * SLOT);
+                    tma_load_2d(slots + second * 2 * SLOT, &maps.extra[0], at.n + c, row, in_bar + second * 8);
+                    tma_load_2d(slots + (second * 2 + 1) * SLOT, &maps.extra[1], at.n + c, row, in_bar + second * 8);
                 }
             }
         };
-        if (have) request(t, 0);
+        if (have) request(t, 0), request(t, 32);
         for (int tile = pair; have && ok;) {
             const Problem& p = g.p[t.prob];
             const int row0 = t.m + int(rank) * BM + quarter * 32, row = row0 + lane;
             // (products over rows read whole k-blocks of them: CE_GRAD writes zeros up to the end of the last one)
             const bool empty = t.kb0 == t.kb1, there = row0 < (EPI == CE_GRAD ? (t.rows + BK - 1) / BK * BK : t.rows);
-            const int n0 = t.n;
+            const int n0 = t.n, width = min(WIDTH, p.N - n0);  // (what lies past the last column is not worked on)
             uint32_t t0, acc_empty_even;
             auto next_acc = [&] {
                 const bool full = __all_sync(0xffffffffu, mbar_wait(smem_u32(&bars->acc_full[acc]), acc_phase, abort_flag));
@@ -348,19 +349,19 @@ group_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args g) 
             } else if constexpr (EPI == STORE) {
                 const int step = p.out_f32 ? 32 : 64;
 #pragma unroll 1
-                for (int c0 = 0; c0 < WIDTH; c0 += step, ++turn) {
+                for (int c0 = 0; c0 < width; c0 += step, ++turn) {
                     const uint32_t slot = slots + (turn & 1u) * SLOT;
                     if (lane == 0) bulk_wait_read_1();
                     __syncwarp();
                     float v[32];
                     get_acc(t0 + c0, v, empty);
                     if (p.out_f32) {
-                        if (c0 + 32 >= WIDTH) release();
+                        if (c0 + 32 >= width) release();
                         put_f32(slot, lane, v);
                     } else {
                         put_bf16(slot, lane, 0, v);
                         get_acc(t0 + c0 + 32, v, empty);
-                        if (c0 + 64 >= WIDTH) release();
+                        if (c0 + 64 >= width) release();
                         put_bf16(slot, lane, 4, v);
                     }
                     send(&maps.out[t.prob], slot, n0 + c0, p.add, t.split * p.rows_pad);
@@ -368,12 +369,12 @@ group_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args g) 
             } else if constexpr (EPI == GATED_FWD) {
                 // the accumulator's columns: [a | b] of the even CTA's columns, then [a | b] of the odd one's
 #pragma unroll 1
-                for (int c = 0; c < WIDTH; c += 32) {
+                for (int c = 0; c < width; c += 32) {
                     const int ac = (c / BH) * 2 * BH + c % BH;
                     float a[32], b[32];
                     get_acc(t0 + ac, a, empty);
                     get_acc(t0 + ac + BH, b, empty);
-                    if (c + 32 >= WIDTH) release();
+                    if (c + 32 >= width) release();
                     // slots: a, b, h, h; whichever is next was last sent at least two groups ago
                     if (lane == 0) bulk_wait_read_1();
                     __syncwarp();
@@ -387,38 +388,39 @@ group_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args g) 
                     for (int i = 0; i < 32; ++i) a[i] = a[i] * sigmoid(a[i]) * b[i];
                     const uint32_t slot = slots + (2 + (turn & 1u)) * SLOT;
                     put_bf16(slot, lane, (c & 32) ? 4 : 0, a);
-                    if (c & 32) {
-                        send(&maps.out[t.prob], slot, n0 + c - 32);
+                    if ((c & 32) || c + 32 >= width) {
+                        send(&maps.out[t.prob], slot, n0 + (c & ~63));
                         ++turn;
                     }
                 }
             } else if constexpr (EPI == GATED_BWD) {
 #pragma unroll 1
-                for (int c = 0; c < WIDTH; c += 32) {
+                for (int c = 0; c < width; c += 32) {
                     float a[32], b[32], d[32];
-                    if (!(ok = __all_sync(0xffffffffu, mbar_wait(in_bar, in_phase, abort_flag)))) break;
-                    in_phase ^= 1u;
-                    get_f32(slots, lane, a);
-                    get_f32(slots + SLOT, lane, b);
+                    const uint32_t second = c >> 5 & 1, in = slots + second * 2 * SLOT;
+                    if (!(ok = __all_sync(0xffffffffu, mbar_wait(in_bar + second * 8, in_phase >> second & 1u, abort_flag)))) break;
+                    in_phase ^= 1u << second;
+                    get_f32(in, lane, a);
+                    get_f32(in + SLOT, lane, b);
                     __syncwarp();
-                    if (c + 32 < WIDTH) request(t, c + 32);
+                    request(t, c + 64);
                     get_acc(t0 + c, d, empty);
-                    if (c + 32 >= WIDTH) release();
+                    if (c + 32 >= width) release();
 #pragma unroll
                     for (int i = 0; i < 32; ++i) {
                         const float e = sigmoid(a[i]), gate = a[i] * e, db = d[i] * gate;
                         a[i] = d[i] * b[i] * (e + gate * (1.f - e));
                         b[i] = db;
                     }
-                    if (!(c & 32)) {
+                    if (!second) {
                         if (lane == 0) bulk_wait_read_0();
                         __syncwarp();
                     }
-                    put_bf16(slots + 2 * SLOT, lane, (c & 32) ? 4 : 0, a);
-                    put_bf16(slots + 3 * SLOT, lane, (c & 32) ? 4 : 0, b);
-                    if (c & 32) {
-                        send(&maps.out[0], slots + 2 * SLOT, n0 + c - 32);
-                        send(&maps.out[1], slots + 3 * SLOT, n0 + c - 32);
+                    put_bf16(slots + 4 * SLOT, lane, second * 4, a);
+                    put_bf16(slots + 5 * SLOT, lane, second * 4, b);
+                    if (second || c + 32 >= width) {
+                        send(&maps.out[0], slots + 4 * SLOT, n0 + (c & ~63));
+                        send(&maps.out[1], slots + 5 * SLOT, n0 + (c & ~63));
                     }
                 }
                 if (!ok) break;
@@ -486,7 +488,7 @@ group_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args g) 
                 const int tcol  = mine ? g.target[row] - g.column0 - n0 : -1;
                 const float lse = mine ? g.lse[row] : 0.f, scale = mine ? g.scale[row] : 0.f;
 #pragma unroll 1
-                for (int c = 0; c < WIDTH; c += 32) {
+                for (int c = 0; c < width; c += 32) {
                     const uint32_t slot = slots + (turn & 1u) * SLOT;
                     if (!(c & 32)) {
                         if (lane == 0) bulk_wait_read_1();
@@ -494,20 +496,20 @@ group_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args g) 
                     }
                     float v[32];
                     get_acc(t0 + c, v, empty);
-                    if (c + 32 >= WIDTH) release();
+                    if (c + 32 >= width) release();
                     // rows past the last one are zeros, which the products over rows read
 #pragma unroll
                     for (int i = 0; i < 32; ++i) v[i] = mine ? scale * (__expf(v[i] - lse) - (tcol == c + i ? 1.f : 0.f)) : 0.f;
                     put_bf16(slot, lane, (c & 32) ? 4 : 0, v);
-                    if (c & 32) {
-                        send(&maps.out[0], slot, n0 + c - 32);
+                    if ((c & 32) || c + 32 >= width) {
+                        send(&maps.out[0], slot, n0 + (c & ~63));
                         ++turn;
                     }
                 }
             }
             tile += num_pairs;
             have = locate<WIDTH>(g, tile, t);
-            if (have) request(t, 0);
+            if (have) request(t, 0), request(t, 32);
         }
         if (lane == 0) bulk_wait_all();
     }
@@ -559,8 +561,7 @@ int launch_group(const Maps& maps, const Args& args, const DeviceInfo& dev, cuda
     const int64_t pairs = dev.sm_count / 2;
     const int grid      = int(2 * (tiles < pairs ? tiles : pairs));
     if (!grid) return MIMK_OK;
-    kern<<<grid, Shape<EPI>::THREADS, Shape<EPI>::SMEM, s>>>(maps, args);
-    return launch_status();
+    return launch_after(kern, unsigned(grid), Shape<EPI>::THREADS, Shape<EPI>::SMEM, s, maps, args);
 }
 
 }  // namespace group

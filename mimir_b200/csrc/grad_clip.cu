@@ -125,6 +125,7 @@ __device__ __forceinline__ double block_sum(double v) {
 
 template <int N>
 __global__ void __launch_bounds__(THREADS) squares_kernel(const __grid_constant__ Table<N> t, double* __restrict__ sums) {
+    after_previous();
     double sum      = 0;
     const int total = t.first[t.count];
     for (int at = blockIdx.x; at < total; at += gridDim.x) {
@@ -142,6 +143,7 @@ __device__ __forceinline__ double total_of(const double* sums, int count) {
     return sqrt(block_sum(s));
 }
 __global__ void __launch_bounds__(THREADS) norm_kernel(const double* __restrict__ sums, int count, float* norm) {
+    after_previous();
     const double n = total_of(sums, count);
     if (threadIdx.x == 0) *norm = float(n);
 }
@@ -186,6 +188,7 @@ __device__ __forceinline__ void scale_chunk(const Chunk& c, float by) {
 template <int N>
 __global__ void __launch_bounds__(THREADS) scale_kernel(const __grid_constant__ Table<N> t, const double* __restrict__ sums, int n_sums, double limit, double eps,
                                                        float* norm, bool in_place) {
+    after_previous();
     const double n = total_of(sums, n_sums);
     if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = float(n);
     const double c = limit / (n + eps);
@@ -263,19 +266,17 @@ template <int N>
 int run(const List& l, const DeviceInfo& dev, bool clip, float limit, float eps, float* norm, double* sums, cudaStream_t s) {
     int all = 0;
     MIMK_TRY((each_table<N>(l, dev.sm_count, [&](const Table<N>& t, int first, int ctas) {
-        squares_kernel<N><<<ctas, THREADS, 0, s>>>(t, sums + first);
         all = first + ctas;
-        return launch_status();
+        return launch_after(squares_kernel<N>, unsigned(ctas), THREADS, 0, s, t, sums + first);
     })));
     if (!clip || !all) {
-        norm_kernel<<<1, THREADS, 0, s>>>(sums, all, norm);
-        return launch_status();
+        return launch_after(norm_kernel, 1, THREADS, 0, s, static_cast<const double*>(sums), all, norm);
     }
     bool in_place = true;
     for (int64_t i = 0; i < l.count; ++i) in_place = in_place && (!l.lengths[i] || l.in[i] == l.out[i]);
     return each_table<N>(l, dev.sm_count, [&](const Table<N>& t, int first, int ctas) {
-        scale_kernel<N><<<ctas, THREADS, 0, s>>>(t, sums, all, double(limit), double(eps), first ? nullptr : norm, in_place);
-        return launch_status();
+        return launch_after(scale_kernel<N>, unsigned(ctas), THREADS, 0, s, t, static_cast<const double*>(sums), all, double(limit), double(eps), first ? nullptr : norm,
+                            bool(in_place));
     });
 }
 

@@ -125,25 +125,34 @@ __device__ void finish_loss(const Rows& r, int64_t n, int reduction, float* loss
     }
 }
 
-// A warp per row: the tiles' maxima and sums joined. loss: the reduced one, or null.
-__global__ void __launch_bounds__(256) join_kernel(Rows r, int64_t n, int tiles, const float* dloss, int reduction, float* loss, float* lse_out) {
-    const int lane = threadIdx.x & 31;
+// The maxima and sums of a row's parts joined, a CTA for a row: the largest maximum first, then the sums scaled to it, so that no load waits for another's
+// exponential (one pass by a warp: 14 us for the 1024 parts of one row, MEASURED_JOIN now). loss: the reduced one, or null.
+__global__ void __launch_bounds__(128) join_kernel(Rows r, int64_t n, int parts, const float* dloss, int reduction, float* loss, float* lse_out) {
+    after_previous();
+    __shared__ float warp_top[4], warp_sums[4];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int left = r.count[0];
-    for (int64_t j = int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5); j < left; j += int64_t(gridDim.x) * 8) {
+    for (int64_t j = blockIdx.x; j < left; j += gridDim.x) {
+        const float2* part = r.part + j * parts;
         float top = -INFINITY, sum = 0.f;
-        for (int t = lane; t < tiles; t += 32) {
-            const float2 p  = r.part[j * tiles + t];
-            const float was = top;
-            top = fmaxf(top, p.x);
-            // (a maximum of -inf has a sum of zero, or NaN)
-            sum = (was == -INFINITY ? sum : sum * __expf(was - top)) + (p.x == -INFINITY ? p.y : p.y * __expf(p.x - top));
+#pragma unroll 8
+        for (int t = threadIdx.x; t < parts; t += 128) top = fmaxf(top, part[t].x);
+        top = warp_max(top);
+        if (lane == 0) warp_top[warp] = top;
+        __syncthreads();
+        top = fmaxf(fmaxf(warp_top[0], warp_top[1]), fmaxf(warp_top[2], warp_top[3]));
+#pragma unroll 8
+        for (int t = threadIdx.x; t < parts; t += 128) {
+            const float2 p = part[t];
+            sum += p.x == -INFINITY ? p.y : p.y * __expf(p.x - top);  // (a maximum of -inf has a sum of zero, or NaN)
         }
-        const float all = warp_max(top);
-        sum             = warp_sum(top == -INFINITY ? sum : sum * __expf(top - all));
-        if (lane == 0) {
+        sum = warp_sum(sum);
+        if (lane == 0) warp_sums[warp] = sum;
+        __syncthreads();
+        if (threadIdx.x == 0) {
             const int64_t row = r.index ? r.index[j] : j;
             const int target  = r.target[j];
-            const float lse   = all + logf(sum);
+            const float lse   = top + logf((warp_sums[0] + warp_sums[1]) + (warp_sums[2] + warp_sums[3]));
             r.lse[j]          = lse;
             if (r.scale) r.scale[j] = scale_of(r, row, target, dloss, reduction);
             if (lse_out) lse_out[row] = lse;
@@ -153,10 +162,84 @@ __global__ void __launch_bounds__(256) join_kernel(Rows r, int64_t n, int tiles,
     if (loss) finish_loss(r, n, reduction, loss);
 }
 
+// ---- a few rows ------------------------------------------------------------------------------------------------------------------
+// The forward pass of up to FEW rows with W stored [v, d]: its bytes bound it, and a tile of 256 rows keeps half of shared memory for zeros. A warp takes
+// four classes at a time, a lane 16 bytes of each; the rows of x are in shared memory as f32, split in halves of eight values so that neighbouring
+// lanes read neighbouring 16 bytes. One row of 4096 against 131072 classes: MEASURED_FEW.
+constexpr int FEW = 4, FEW_CTAS = 4;
+template <int N>
+__global__ void __launch_bounds__(256, N == FEW ? 2 : FEW_CTAS) few_rows_kernel(const __nv_bfloat16* __restrict__ x, int64_t x_pitch, const __nv_bfloat16* __restrict__ w, int d, int v,
+                                                                  Rows r) {
+    after_previous();
+    extern __shared__ float4 xs[];  // [N][2][d / 8]
+    const int lane = threadIdx.x & 31, eighths = d / 8, slots = gridDim.x * 8, slot = blockIdx.x * 8 + (threadIdx.x >> 5);
+    const int left = r.count[0];
+    for (int i = threadIdx.x; i < N * eighths; i += 256) {
+        const int j = i / eighths, k = i - j * eighths;
+        uint4 u     = make_uint4(0, 0, 0, 0);
+        if (j < left) u = *reinterpret_cast<const uint4*>(x + int64_t(r.index ? r.index[j] : j) * x_pitch + k * 8);
+        xs[j * 2 * eighths + k] = make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16), __uint_as_float(u.y & 0xffff0000u));
+        xs[(j * 2 + 1) * eighths + k] =
+            make_float4(__uint_as_float(u.z << 16), __uint_as_float(u.z & 0xffff0000u), __uint_as_float(u.w << 16), __uint_as_float(u.w & 0xffff0000u));
+    }
+    __syncthreads();
+    const int target = lane < N && lane < left ? r.target[lane] : -1;  // lane j looks after row j
+    float top = -INFINITY, sum = 0.f;
+    for (int64_t c = int64_t(slot) * 4; c < v; c += int64_t(slots) * 4) {
+        float acc[4][N];
+        const uint4* at[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            at[i] = reinterpret_cast<const uint4*>(w + (c + i < v ? c + i : v - 1) * int64_t(d));
+#pragma unroll
+            for (int j = 0; j < N; ++j) acc[i][j] = 0.f;
+        }
+#pragma unroll 2
+        for (int k = lane; k < eighths; k += 32) {
+            uint4 u[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) u[i] = __ldcs(at[i] + k);
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                const float4 a = xs[j * 2 * eighths + k], b = xs[(j * 2 + 1) * eighths + k];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    acc[i][j] = fmaf(__uint_as_float(u[i].x << 16), a.x, fmaf(__uint_as_float(u[i].x & 0xffff0000u), a.y, acc[i][j]));
+                    acc[i][j] = fmaf(__uint_as_float(u[i].y << 16), a.z, fmaf(__uint_as_float(u[i].y & 0xffff0000u), a.w, acc[i][j]));
+                    acc[i][j] = fmaf(__uint_as_float(u[i].z << 16), b.x, fmaf(__uint_as_float(u[i].z & 0xffff0000u), b.y, acc[i][j]));
+                    acc[i][j] = fmaf(__uint_as_float(u[i].w << 16), b.z, fmaf(__uint_as_float(u[i].w & 0xffff0000u), b.w, acc[i][j]));
+                }
+            }
+        }
+        float l[4] = {};
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float all = warp_sum(acc[i][j]);
+                l[i]            = lane == j ? all : l[i];
+            }
+        if (lane < N) {
+            float most = top;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (c + i >= v) l[i] = -INFINITY;
+                else if (target == c + i) r.target_logit[lane] = l[i];
+                most = fmaxf(most, l[i]);
+            }
+            if (most > top) sum *= top == -INFINITY ? 1.f : __expf(top - most), top = most;  // (an earlier sum at -inf is zero, or NaN)
+            const float base = top == -INFINITY ? 0.f : top;
+            sum += (__expf(l[0] - base) + __expf(l[1] - base)) + (__expf(l[2] - base) + __expf(l[3] - base));
+        }
+    }
+    if (lane < N && lane < left) r.part[int64_t(lane) * slots + slot] = make_float2(top, sum);
+}
+
 // p from the exponentials, in place: exp(l - m) becomes scale exp(l - lse) as bf16, less scale at the target, whose own value comes from its
 // logit; zeros in the rows up to the end of the last 64, which the products over rows read. A warp takes 1024 columns of a row, a lane four times 16
 // bytes. Bound by the bytes: MEASURED_P.
-__global__ void __launch_bounds__(256) probabilities_kernel(Rows r, uint16_t* __restrict__ p, int64_t pitch, int64_t n, int tiles) {
+__global__ void __launch_bounds__(256) probabilities_kernel(Rows r, uint16_t* __restrict__ p, int64_t pitch, int64_t n, int parts) {
+    after_previous();
     const int lane = threadIdx.x & 31;
     const int left = r.count[0];
     const int64_t end = min(n, (int64_t(left) + 63) / 64 * 64);
@@ -172,7 +255,7 @@ __global__ void __launch_bounds__(256) probabilities_kernel(Rows r, uint16_t* __
             const int c = first + i * 256;
             if (c >= pitch) continue;
             v[i]   = there ? *reinterpret_cast<const uint4*>(p + j * pitch + c) : make_uint4(0, 0, 0, 0);
-            top[i] = there ? r.part[j * tiles + (c >> 7)].x : 0.f;
+            top[i] = there ? r.part[j * parts + (c >> 7)].x : 0.f;
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -206,6 +289,7 @@ __global__ void recall_kernel(Rows r, const float* __restrict__ lse, const float
 template <class T>
 __global__ void place_rows_kernel(const float* __restrict__ part, int splits, int64_t stride, int64_t pitch, const int* __restrict__ place, T* __restrict__ dx,
                                   int64_t n, int64_t cols, bool words) {
+    after_previous();
     const int64_t quads = (cols + 3) / 4, all = n * quads;
     for (int64_t i = int64_t(blockIdx.x) * blockDim.x + threadIdx.x; i < all; i += int64_t(gridDim.x) * blockDim.x) {
         const int64_t row = i / quads, c = (i - row * quads) * 4, j = place ? place[row] : row;
@@ -287,7 +371,8 @@ struct Plan {
     void* x;  // the rows that are left, together, or null: the caller's
     int64_t x_pitch;
     Staged w, dw;
-    int tiles;
+    int parts;                  // of a row, whose maxima and sums are joined
+    bool few;
     int64_t piece;              // columns (bf16) or rows (f32) of a piece
     bool kept;                  // bf16: the forward product leaves its exponentials, and all columns are one piece
     void* p;                    // bf16: p of a piece; f32: its logits
@@ -325,8 +410,11 @@ Plan plan(const mimk_linear_ce_desc& d, bool forward, bool backward, Space& spac
     if (taken || !tma_can_read(d.x, d.d)) p.x_pitch = up(d.d, 8), p.x = space.take(n * size_t(p.x_pitch) * 2);
     const bool nk = d.w_layout == MIMK_B_NK;
     p.w           = nk ? stage(space, d.w, d.v, d.d) : stage(space, d.w, d.d, d.v);
-    p.tiles       = int((d.v + 255) / 256) * 2;
-    if (forward) p.rows.part = static_cast<float2*>(space.take(n * size_t(p.tiles) * 8)), p.rows.target_logit = floats(n);
+    // (up to 64 KiB of shared memory: FEW_CTAS CTAs to an SM; with gradients the tensor cores' pass leaves the exponentials, too)
+    p.few   = forward && !backward && nk && d.n <= FEW && (d.n <= 2 ? d.n : FEW) * d.d <= 16384 && !p.w.copied() && tma_can_read(d.x, d.d);
+    p.parts = p.few ? sm_count * FEW_CTAS * 8 : int((d.v + 255) / 256) * 2;
+    if (p.few) p.x = nullptr;
+    if (forward) p.rows.part = static_cast<float2*>(space.take(n * size_t(p.parts) * 8)), p.rows.target_logit = floats(n);
     if (backward) {
         p.dw    = nk ? stage(space, d.dw, d.v, d.d) : stage(space, d.dw, d.d, d.v);
         p.kept  = forward && d.n * up(d.v, 8) <= KEPT_CELLS;
@@ -424,9 +512,8 @@ int run_f32(const mimk_linear_ce_desc& d, const Plan& p, bool forward, bool back
         MIMK_TRY(launch_status());
     }
     if (backward && p.dx) {
-        place_rows_kernel<float><<<grid_for(d.n * ((d.d + 3) / 4), 256, 8192), 256, 0, s>>>(p.dx, 1, 0, d.d, p.rows.place, static_cast<float*>(d.dx), d.n, d.d,
-                                                                                             false);
-        MIMK_TRY(launch_status());
+        MIMK_TRY(launch_after(place_rows_kernel<float>, grid_for(d.n * ((d.d + 3) / 4), 256, 8192), 256, 0, s, static_cast<const float*>(p.dx), 1, int64_t(0), d.d,
+                              static_cast<const int*>(p.rows.place), static_cast<float*>(d.dx), d.n, d.d, false));
     }
     return MIMK_OK;
 }
@@ -436,6 +523,15 @@ Problem problem(int64_t m, int64_t n, int64_t k, bool a_mn, bool b_mn) {
     Problem p{};
     p.M = int(m), p.N = int(n), p.kb[0] = int((k + BK - 1) / BK), p.a_mn = a_mn, p.b_mn = b_mn, p.splits = 1;
     return p;
+}
+
+template <int N>
+int few_rows(const mimk_linear_ce_desc& d, const Plan& p, const DeviceInfo& dev, cudaStream_t s) {
+    const int smem = int(N * d.d * 4);
+    auto kern      = few_rows_kernel<N>;
+    if (smem > 48 * 1024) MIMK_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 65536));
+    return launch_after(kern, unsigned(dev.sm_count * FEW_CTAS), 256, smem, s, static_cast<const __nv_bfloat16*>(d.x), d.d, static_cast<const __nv_bfloat16*>(d.w), int(d.d),
+                        int(d.v), p.rows);
 }
 
 int run_bf16(const mimk_linear_ce_desc& d, const Plan& p, bool forward, bool backward, const DeviceInfo& dev, cudaStream_t s) {
@@ -459,24 +555,27 @@ int run_bf16(const mimk_linear_ce_desc& d, const Plan& p, bool forward, bool bac
         args.count      = 1;
         args.p[0]       = problem(d.n, d.v, d.d, false, !nk);
         args.p[0].dyn_m = count;
-        MIMK_TRY(operand_map(&maps.a[0][0], x, false, BM));
-        MIMK_TRY(operand_map(&maps.b[0][0], w, !nk, 128));
-        if (p.kept) {
+        if (!p.few) {
+            MIMK_TRY(operand_map(&maps.a[0][0], x, false, BM));
+            MIMK_TRY(operand_map(&maps.b[0][0], w, !nk, 128));
+        }
+        if (p.few) {
+            MIMK_TRY((d.n == 1 ? few_rows<1>(d, p, dev, s) : d.n == 2 ? few_rows<2>(d, p, dev, s) : few_rows<FEW>(d, p, dev, s)));
+        } else if (p.kept) {
             MIMK_TRY(result_map(&maps.out[0], p.p, false, d.n, d.v, p.piece));
             MIMK_TRY(launch_group<CE_EXP>(maps, args, dev, s));
         } else {
             MIMK_TRY(launch_group<CE_STATS>(maps, args, dev, s));
         }
-        join_kernel<<<grid_for(d.n, 8, 2048), 256, 0, s>>>(p.rows, d.n, p.tiles, d.dloss, d.reduction, loss, d.lse);
+        MIMK_TRY(launch_after(join_kernel, grid_for(d.n, 1, 4096), 128, 0, s, p.rows, d.n, p.parts, d.dloss, int(d.reduction), loss, d.lse));
     } else {
         recall_kernel<<<grid_for(d.n, 256, 1024), 256, 0, s>>>(p.rows, d.lse, d.dloss, d.reduction);
+        MIMK_TRY(launch_status());
     }
-    MIMK_TRY(launch_status());
     if (!backward) return MIMK_OK;
     if (p.kept) {
         const dim3 grid(unsigned((p.piece + 8191) / 8192), grid_for(d.n, 1, 65535));
-        probabilities_kernel<<<grid, 256, 0, s>>>(p.rows, static_cast<uint16_t*>(p.p), p.piece, d.n, p.tiles);
-        MIMK_TRY(launch_status());
+        MIMK_TRY(launch_after(probabilities_kernel, grid, 256, 0, s, p.rows, static_cast<uint16_t*>(p.p), p.piece, d.n, p.parts));
     }
 
     for (int64_t from = 0; from < d.v; from += p.piece) {
@@ -516,9 +615,8 @@ int run_bf16(const mimk_linear_ce_desc& d, const Plan& p, bool forward, bool bac
     MIMK_TRY(stage_out(p.dw, s));
     if (p.dx) {
         const bool words = d.d % 4 == 0 && reinterpret_cast<uintptr_t>(d.dx) % 8 == 0;
-        place_rows_kernel<__nv_bfloat16><<<grid_for(d.n * ((d.d + 3) / 4), 256, 8192), 256, 0, s>>>(
-            p.dx, p.splits, p.rows_pad * p.dx_pitch, p.dx_pitch, p.rows.place, static_cast<__nv_bfloat16*>(d.dx), d.n, d.d, words);
-        MIMK_TRY(launch_status());
+        MIMK_TRY(launch_after(place_rows_kernel<__nv_bfloat16>, grid_for(d.n * ((d.d + 3) / 4), 256, 8192), 256, 0, s, static_cast<const float*>(p.dx), p.splits,
+                              p.rows_pad * p.dx_pitch, p.dx_pitch, static_cast<const int*>(p.rows.place), static_cast<__nv_bfloat16*>(d.dx), d.n, d.d, words));
     }
     return MIMK_OK;
 }

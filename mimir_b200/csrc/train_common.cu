@@ -15,6 +15,7 @@ __global__ void copy_rows_kernel(const uint16_t* __restrict__ from, int64_t from
 // Four columns a thread (the partial results' rows are whole 16 bytes), the parts in order, so that the sum is the same call after call.
 __global__ void sum_parts_kernel(const float* __restrict__ part, int splits, int64_t stride, int64_t part_pitch, __nv_bfloat16* __restrict__ out,
                                  int64_t out_pitch, int64_t rows, int64_t cols, bool words) {
+    after_previous();
     const int64_t quads = (cols + 3) / 4, all = rows * quads;
     for (int64_t i = int64_t(blockIdx.x) * blockDim.x + threadIdx.x; i < all; i += int64_t(gridDim.x) * blockDim.x) {
         const int64_t r = i / quads, c = (i - r * quads) * 4;
@@ -63,9 +64,8 @@ int sum_parts(const float* part, int splits, int64_t rows_pad, int64_t part_pitc
     const int64_t all = rows * ((cols + 3) / 4), blocks = (all + 255) / 256;
     if (!all) return MIMK_OK;
     const bool words = out_pitch % 4 == 0 && reinterpret_cast<uintptr_t>(out) % 8 == 0;
-    sum_parts_kernel<<<unsigned(blocks < 4096 ? blocks : 4096), 256, 0, s>>>(part, splits, rows_pad * part_pitch, part_pitch, static_cast<__nv_bfloat16*>(out),
-                                                                           out_pitch, rows, cols, words);
-    return launch_status();
+    return launch_after(sum_parts_kernel, unsigned(blocks < 4096 ? blocks : 4096), 256, 0, s, part, splits, rows_pad * part_pitch, part_pitch, static_cast<__nv_bfloat16*>(out),
+                        out_pitch, rows, cols, words);
 }
 
 }  // namespace mimk

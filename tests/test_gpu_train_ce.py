@@ -110,6 +110,26 @@ def test_several_pieces(dtype, shape, nk):
     assert near(dw, total, bound * (1 + shape[0] / 5000))
 
 
+@pytest.mark.parametrize("shape", [(1, 64, 1000), (2, 8, 5), (3, 136, 5001), (4, 4096, 778), (2, 4096, 40000), (1, 16384, 130), (4, 4104, 130)])
+@pytest.mark.parametrize("masked", [0.0, 0.6])
+def test_scoring_a_few_rows(shape, masked):
+    from mimir_b200 import tensor as T
+    x, w, t = inputs(*shape, BF16, True, seed=11, masked=masked)
+    ignore = IGNORED if masked else None
+    want, kept = formulas(x, w, t)
+    losses, lse = T.linear_cross_entropy(x, w, t, ignore_index=ignore, reduction="none", return_lse=True)
+    assert near(losses, *want[0]) and near(lse, *want[1])
+    total = T.linear_cross_entropy(x, w, t, ignore_index=ignore, reduction="sum")
+    assert abs(float(total) - float(want[0][0].sum())) <= float(want[0][1][kept].sum()) + 1e-37 + E * abs(float(total))
+    if masked == 0.0:
+        w = w.clone(memory_format=torch.preserve_format)
+        w[:, shape[2] // 2:] = float("-inf") * torch.sign(x[0]).to(w.dtype)[:, None]      # (row 0's scores of half the classes are -inf)
+        t = t % max(shape[2] // 2, 1)
+        losses = T.linear_cross_entropy(x, w, t, reduction="none")
+        half, _ = formulas(x[:1], w[:, :shape[2] // 2].t().contiguous().t(), t[:1])
+        assert abs(float(losses[0]) - float(half[0][0])) <= float(half[0][1])
+
+
 def test_gradients_that_arrive_and_targets_of_32_bits():
     from mimir_b200 import tensor as T
     x, w, t = inputs(90, 48, 300, BF16, True, masked=0.3)
