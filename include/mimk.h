@@ -375,8 +375,9 @@ int mimk_mlp_gated_bwd(const mimk_mlp_train_desc* desc, void* stream);
  * has_ignore: a row whose target is ignore_index has none: its loss, lse and dX are zeros, nothing of it enters dW, and its X is not read. Any other target
  * outside [0, v) is recorded (mimk_device_status: MIMK_E_SHAPE); the row's loss is NaN, and it enters no gradient.
  * Losses, lse and all sums are f32; bf16 gradients are rounded once from f32 sums of products whose factor p = dloss (softmax - onehot) is
- * rounded to bf16. Equal descriptors give equal bits. Workspace as above, from the query; bf16: 16 bytes per row, 8 per row and 256 classes, and
- * up to 512 MiB of p (8 KiB per row where that is more) and 4 bytes per value of X for gradients. */
+ * rounded to bf16 (in fwd_bwd from exponentials of ten significant bits where n v <= 2^30). Equal descriptors give equal bits. Workspace as above,
+ * from the query; bf16: 16 bytes per row and 8 per row and 128 classes; for gradients also p, 2 n v bytes in fwd_bwd where n v <= 2^30, else at
+ * most 512 MiB (8 KiB per row where that is more), and 4 bytes per value of X where p comes in pieces or rows were taken out. */
 enum { MIMK_REDUCTION_NONE = 0, MIMK_REDUCTION_MEAN = 1, MIMK_REDUCTION_SUM = 2 };
 typedef struct mimk_linear_ce_desc {
     int64_t n, d, v;     /* rows, features, classes */

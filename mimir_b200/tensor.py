@@ -561,7 +561,7 @@ def grad_norm(grads) -> torch.Tensor:
 
 
 def clip_grad_norm(grads, limit: float, *, eps: float = 1e-6, out=None) -> torch.Tensor:
-    """Scales the tensors by min(1, limit / (norm + eps)), in place or into the tensors `out`, and returns their norm from before
+    """Scales the tensors (each listed once) by min(1, limit / (norm + eps)), in place or into the tensors `out`, and returns their norm from before
     (grad_norm). A norm of NaN makes every value NaN, an infinite one zeros, and NaN of what was infinite."""
     if not (limit >= 0 and eps >= 0):
         raise ValueError("clip_grad_norm: limit and eps are at least 0")
