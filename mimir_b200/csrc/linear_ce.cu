@@ -49,10 +49,12 @@ __global__ void __launch_bounds__(1024) prepare_kernel(const I* __restrict__ tar
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t per = (n + 1023) / 1024;
     const int64_t from = threadIdx.x * per < n ? threadIdx.x * per : n, to = from + per < n ? from + per : n;
+    // (the ignored index may be a class, as a padding token's is)
+    const auto has_target = [&](int64_t t) { return t >= 0 && t < v && !(has_ignore && t == ignore); };
     int mine = 0, exist = 0;
     for (int64_t i = from; i < to; ++i) {
         const int64_t t  = targets[i];
-        const bool there = t >= 0 && t < v;
+        const bool there = has_target(t);
         exist += there, mine += r.index ? there : 1;
     }
     int before = mine;
@@ -73,8 +75,8 @@ __global__ void __launch_bounds__(1024) prepare_kernel(const I* __restrict__ tar
     }
     if (threadIdx.x == 0) r.count[0] = all, r.count[1] = exist, r.count[2] = 0;
     for (int64_t i = from; i < to; ++i) {
-        const int64_t t    = targets[i];
-        const bool there   = t >= 0 && t < v, ignored = has_ignore && t == ignore;
+        const int64_t t  = targets[i];
+        const bool there = has_target(t), ignored = has_ignore && t == ignore;
         if (!there && !ignored) *status = MIMK_E_SHAPE;
         if (!r.index) {
             r.target[i] = there ? int(t) : -1;
