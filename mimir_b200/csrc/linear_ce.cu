@@ -320,9 +320,10 @@ __global__ void place_rows_kernel(const float* __restrict__ part, int splits, in
 }
 
 // ---- f32: rows of logits in memory -------------------------------------------------------------------------------------------------
-// A CTA per row of a piece that starts at row `first`: log of the sum and loss, and the row turned into p where the gradient is wanted.
-__global__ void __launch_bounds__(512) logits_kernel(float* __restrict__ logits, int64_t v, int64_t first, Rows r, const float* dloss, int reduction, float* lse_out,
-                                                     bool grad) {
+// A CTA per row of a piece that starts at row `first`: log of the sum and loss, or the logarithm of an earlier call (`earlier`, by place in x), and the row
+// turned into p where the gradient is wanted.
+__global__ void __launch_bounds__(512) logits_kernel(float* __restrict__ logits, int64_t v, int64_t first, Rows r, const float* dloss, int reduction,
+                                                     const float* earlier, float* lse_out, bool grad) {
     __shared__ float warp_top[16], warp_part[16];
     const int64_t j = first + blockIdx.x;
     float* row      = logits + int64_t(blockIdx.x) * v;
@@ -331,30 +332,37 @@ __global__ void __launch_bounds__(512) logits_kernel(float* __restrict__ logits,
             for (int64_t c = threadIdx.x; c < v; c += blockDim.x) row[c] = 0.f;
         return;
     }
-    float top = -INFINITY, sum = 0.f;
-    for (int64_t c = threadIdx.x; c < v; c += blockDim.x) top = fmaxf(top, row[c]);
-    top = warp_max(top);
-    if ((threadIdx.x & 31) == 0) warp_top[threadIdx.x >> 5] = top;
-    __syncthreads();
-    for (unsigned w = 0; w < blockDim.x / 32; ++w) top = fmaxf(top, warp_top[w]);
-    for (int64_t c = threadIdx.x; c < v; c += blockDim.x) sum += expf(row[c] - top);
-    sum = warp_sum(sum);
-    if ((threadIdx.x & 31) == 0) warp_part[threadIdx.x >> 5] = sum;
-    const int target     = r.target[j];
-    const int64_t place  = r.index ? r.index[j] : j;
-    const float at       = target >= 0 ? row[target] : 0.f;
-    __syncthreads();  // (every thread has the target's logit before the row changes)
-    sum = 0.f;
-    for (unsigned w = 0; w < blockDim.x / 32; ++w) sum += warp_part[w];
-    const float lse = top + logf(sum);
-    if (threadIdx.x == 0) {
-        if (lse_out) lse_out[place] = lse;
-        if (r.loss) r.loss[place] = target < 0 ? __int_as_float(0x7fc00000) : lse - at;
+    const int target    = r.target[j];
+    const int64_t place = r.index ? r.index[j] : j;
+    // p = exp(l - base) over
+    float base = 0.f, over = 1.f;
+    if (earlier) {
+        base = earlier[place];
+    } else {
+        float top = -INFINITY, sum = 0.f;
+        for (int64_t c = threadIdx.x; c < v; c += blockDim.x) top = fmaxf(top, row[c]);
+        top = warp_max(top);
+        if ((threadIdx.x & 31) == 0) warp_top[threadIdx.x >> 5] = top;
+        __syncthreads();
+        for (unsigned w = 0; w < blockDim.x / 32; ++w) top = fmaxf(top, warp_top[w]);
+        for (int64_t c = threadIdx.x; c < v; c += blockDim.x) sum += expf(row[c] - top);
+        sum = warp_sum(sum);
+        if ((threadIdx.x & 31) == 0) warp_part[threadIdx.x >> 5] = sum;
+        const float at = target >= 0 ? row[target] : 0.f;
+        __syncthreads();  // (every thread has the target's logit before the row changes)
+        sum = 0.f;
+        for (unsigned w = 0; w < blockDim.x / 32; ++w) sum += warp_part[w];
+        if (threadIdx.x == 0) {
+            const float lse = top + logf(sum);
+            if (lse_out) lse_out[place] = lse;
+            if (r.loss) r.loss[place] = target < 0 ? __int_as_float(0x7fc00000) : lse - at;
+        }
+        base = top, over = 1.f / sum;
     }
     if (grad) {
-        const float scale = scale_of(r, place, target, dloss, reduction), over = 1.f / sum;
+        const float scale = scale_of(r, place, target, dloss, reduction);
         for (int64_t c = threadIdx.x; c < v; c += blockDim.x) {
-            const float p = expf(row[c] - top) * over;
+            const float p = expf(row[c] - base) * over;
             row[c]        = scale * (c == target ? p - 1.f : p);
         }
     }
@@ -495,7 +503,8 @@ int run_f32(const mimk_linear_ce_desc& d, const Plan& p, bool forward, bool back
         const int64_t n = std::min(p.piece, d.n - first);
         const float* xi = x + first * d.d;
         MIMK_TRY(product(n, d.v, d.d, xi, w, d.w_layout, logits, s));
-        logits_kernel<<<unsigned(n), 512, 0, s>>>(logits, d.v, first, rows, d.dloss, d.reduction, forward ? d.lse : nullptr, backward);
+        logits_kernel<<<unsigned(n), 512, 0, s>>>(logits, d.v, first, rows, d.dloss, d.reduction, forward ? nullptr : d.lse, forward ? d.lse : nullptr,
+                                                  backward);
         MIMK_TRY(launch_status());
         if (!backward) continue;
         MIMK_TRY(product(n, d.d, d.v, logits, w, nk ? MIMK_B_KN : MIMK_B_NK, dx + first * d.d, s));
