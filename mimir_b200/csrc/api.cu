@@ -179,20 +179,26 @@ static bool f32_on_tensor_cores() {
     return on;
 }
 
-extern "C" int mimk_gemm(const mimk_gemm_desc* d, void* stream) {
-    MIMK_TRY(check_gemm(d));
+namespace mimk {
+int gemm_any(const mimk_gemm_desc& d, cudaStream_t s, void* scratch) {
+    MIMK_TRY(check_gemm(&d));
     int st = MIMK_OK;
     if (!device_info(&st)) return st;
-    if (d->batch == 0 || d->m == 0 || d->n == 0) return MIMK_OK;
-    if (!d->c || (d->k > 0 && (!d->a || !d->b))) return MIMK_E_ARG;
-    cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (gemm_tc_supported(*d)) return gemm_tc_any(*d, s, 0, nullptr);
-    if (d->in_dtype == MIMK_BF16) {
-        const int r = gemm_tc_ragged(*d, s);
+    if (d.batch == 0 || d.m == 0 || d.n == 0) return MIMK_OK;
+    if (!d.c || (d.k > 0 && (!d.a || !d.b))) return MIMK_E_ARG;
+    if (gemm_tc_supported(d)) return gemm_tc_any(d, s, 0, nullptr);
+    if (d.in_dtype == MIMK_BF16) {
+        const int r = gemm_tc_ragged(d, s);
         if (r != MIMK_E_UNSUPPORTED) return r;
     }
-    if (f32_on_tensor_cores() && gemm_f32_tc_supported(*d) && !gemm_simt_preferred(*d)) return gemm_f32_tc(*d, s);
-    return gemm_simt(*d, s);
+    if (f32_on_tensor_cores() && gemm_f32_tc_supported(d) && !gemm_simt_preferred(d)) return gemm_f32_tc(d, s, scratch);
+    return gemm_simt(d, s);
+}
+}  // namespace mimk
+
+extern "C" int mimk_gemm(const mimk_gemm_desc* d, void* stream) {
+    if (!d) return MIMK_E_ARG;
+    return gemm_any(*d, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int mimk_gemm_gather(const mimk_gemm_desc* d, const void* b2, const mimk_gather_dst* g, void* stream) {

@@ -89,12 +89,17 @@ int gemm_tc2(const mimk_gemm_desc& d, cudaStream_t s, int gated, const void* b2,
 int gemm_tc_any(const mimk_gemm_desc& d, cudaStream_t s, int gated, const void* b2,
                 const mimk_gather_dst* gather = nullptr, int64_t a_panels = 1);  // picks between the two
 int gemm_f32_tc_supported(const mimk_gemm_desc& d);  // f32 operands on the tensor cores (three bf16 pieces each)
-int gemm_f32_tc(const mimk_gemm_desc& d, cudaStream_t s);
+int gemm_f32_tc(const mimk_gemm_desc& d, cudaStream_t s, void* scratch = nullptr);
 double gemm_f32_tc_us(int64_t m, int64_t n, int64_t k, int64_t batch, int sm_count);  // its time estimate
 int gemm_bf16_chunked(const mimk_gemm_desc& d, cudaStream_t s);  // bf16 operands of any extent and alignment, f32 result
 // results with many tiles: the operands cut beforehand, three TF32 products (gemm_tf32.cu)
 int gemm_tf32_preferred(const mimk_gemm_desc& d, int sm_count, double pieces_us);
-int gemm_tf32(const mimk_gemm_desc& d, cudaStream_t s);
+int gemm_tf32(const mimk_gemm_desc& d, cudaStream_t s, void* scratch = nullptr);
+size_t gemm_tf32_scratch(const mimk_gemm_desc& d);  // bytes of the cut operands
+// mimk_gemm, and the same for callers that plan all their memory: with `scratch` (256-byte aligned, what the query says for a descriptor of these extents,
+// wherever its matrices lie) nothing is taken from the cached buffers, and the choice of kernel is the same under capture. F32 operands.
+int gemm_any(const mimk_gemm_desc& d, cudaStream_t s, void* scratch = nullptr);
+size_t gemm_f32_scratch(const mimk_gemm_desc& d, int sm_count);
 double gemm_tf32_us(int64_t m, int64_t n, int64_t k, int64_t batch, int sm_count);
 int conv_tc(const mimk_conv_desc& d, cudaStream_t s);  // the same kernel, its left operand gathered from an image
 int conv_tc_preferred(const mimk_conv_desc& d, int sm_count);  // ... where conv_pieces is not ahead

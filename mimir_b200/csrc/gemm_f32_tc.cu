@@ -707,12 +707,12 @@ static Params product_params(const mimk_gemm_desc& d, const DeviceInfo& dev) {
     return p;
 }
 
-int gemm_f32_tc(const mimk_gemm_desc& d, cudaStream_t s) {
+int gemm_f32_tc(const mimk_gemm_desc& d, cudaStream_t s, void* scratch) {
     int st          = MIMK_OK;
     DeviceInfo* dev = device_info(&st);
     if (!dev) return st;
     if (gemm_tf32_preferred(d, dev->sm_count, gemm_f32_tc_us(d.m, d.n, d.k, d.batch, dev->sm_count))) {
-        const int r = gemm_tf32(d, s);
+        const int r = gemm_tf32(d, s, scratch);
         if (r != MIMK_E_UNSUPPORTED) return r;
     }
     Params p = product_params(d, *dev);

@@ -435,23 +435,34 @@ int gemm_tf32_preferred(const mimk_gemm_desc& d, int sm_count, double pieces_us)
     return gemm_tf32_us(d.m, d.n, d.k, d.batch, sm_count) < pieces_us;
 }
 
-// MIMK_E_UNSUPPORTED, with nothing launched, where the copies' buffer cannot be had: under stream capture (a graph must not
-// hold on to the cached buffer) and when there is no memory for it.
-int gemm_tf32(const mimk_gemm_desc& d, cudaStream_t s) {
+// The operands' hi / lo copies: row pitch a multiple of 16 bytes, each copy on a 256-byte boundary.
+static int64_t copy_pitch(const mimk_gemm_desc& d) { return (d.k + 3) & ~int64_t(3); }
+static size_t copy_bytes(int64_t rows, int64_t pitch) { return (size_t(rows) * size_t(pitch) * 4 + 255) & ~size_t(255); }
+size_t gemm_tf32_scratch(const mimk_gemm_desc& d) { return 2 * copy_bytes(d.m, copy_pitch(d)) + 2 * copy_bytes(d.n, copy_pitch(d)); }
+size_t gemm_f32_scratch(const mimk_gemm_desc& d, int sm_count) {
+    mimk_gemm_desc aligned = d;
+    aligned.a = aligned.b = aligned.post_full = nullptr, aligned.c = nullptr;
+    return gemm_tf32_preferred(aligned, sm_count, gemm_f32_tc_us(d.m, d.n, d.k, d.batch, sm_count)) ? gemm_tf32_scratch(d) : 0;
+}
+
+// The copies go to the caller's `scratch`, or to a cached buffer. MIMK_E_UNSUPPORTED, with nothing launched, where that cannot be had: under
+// stream capture (a graph must not hold on to the cached buffer) and when there is no memory for it.
+int gemm_tf32(const mimk_gemm_desc& d, cudaStream_t s, void* scratch) {
     int st          = MIMK_OK;
     DeviceInfo* dev = device_info(&st);
     if (!dev) return st;
-    const int64_t kp = (d.k + 3) & ~int64_t(3);  // row pitch of the hi / lo copies: 16-byte multiples
+    const int64_t kp = copy_pitch(d);
     const size_t a_elems = size_t(d.m) * kp, b_elems = size_t(d.n) * kp;
-    const size_t a_bytes = (a_elems * 4 + 255) & ~size_t(255), b_bytes = (b_elems * 4 + 255) & ~size_t(255);
-    cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
-    MIMK_CUDA_TRY(cudaStreamIsCapturing(s, &cap));
-    if (cap != cudaStreamCaptureStatusNone) return MIMK_E_UNSUPPORTED;
-    void* scratch = nullptr;
+    const size_t a_bytes = copy_bytes(d.m, kp), b_bytes = copy_bytes(d.n, kp);
     ScratchLease lease;
-    if (lease.take(2 * a_bytes + 2 * b_bytes, &scratch, s) != MIMK_OK) {
-        cudaGetLastError();
-        return MIMK_E_UNSUPPORTED;
+    if (!scratch) {
+        cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+        MIMK_CUDA_TRY(cudaStreamIsCapturing(s, &cap));
+        if (cap != cudaStreamCaptureStatusNone) return MIMK_E_UNSUPPORTED;
+        if (lease.take(gemm_tf32_scratch(d), &scratch, s) != MIMK_OK) {
+            cudaGetLastError();
+            return MIMK_E_UNSUPPORTED;
+        }
     }
     uint8_t* base = static_cast<uint8_t*>(scratch);
     float *a_hi = reinterpret_cast<float*>(base), *a_lo = reinterpret_cast<float*>(base + a_bytes);

@@ -393,7 +393,28 @@ struct Plan {
     int splits;
     int64_t rows_pad, dx_pitch;
     void *turned, *sum;         // f32: x or p transposed; a piece's part of dW
+    void* cut;                  // f32: operands that a product cuts beforehand, or null
 };
+
+// One product of the f32 form.
+mimk_gemm_desc product(int64_t m, int64_t n, int64_t k, const void* a, const void* b, int layout, void* c) {
+    mimk_gemm_desc g = {};
+    g.batch = 1, g.m = m, g.n = n, g.k = k, g.a = a, g.b = b, g.c = c;
+    g.in_dtype = g.out_dtype = MIMK_F32, g.b_layout = layout;
+    return g;
+}
+// What the products of a piece of `rows` rows need for their operands.
+size_t cut_bytes(const mimk_linear_ce_desc& d, int64_t rows, bool backward, int sm_count) {
+    const bool nk     = d.w_layout == MIMK_B_NK;
+    const auto needed = [&](int64_t m, int64_t n, int64_t k, int layout) { return gemm_f32_scratch(product(m, n, k, nullptr, nullptr, layout, nullptr), sm_count); };
+    if (!rows) return 0;
+    size_t bytes = needed(rows, d.v, d.d, d.w_layout);
+    if (backward) {
+        bytes = std::max(bytes, needed(rows, d.d, d.v, nk ? MIMK_B_KN : MIMK_B_NK));
+        bytes = std::max(bytes, nk ? needed(d.v, d.d, rows, MIMK_B_KN) : needed(d.d, d.v, rows, MIMK_B_KN));
+    }
+    return bytes;
+}
 
 Plan plan(const mimk_linear_ce_desc& d, bool forward, bool backward, Space& space, int sm_count) {
     Plan p{};
@@ -417,6 +438,8 @@ Plan plan(const mimk_linear_ce_desc& d, bool forward, bool backward, Space& spac
             p.turned = space.take(size_t(p.piece) * size_t(nk ? d.v : d.d) * 4);
             if (p.piece < d.n) p.sum = space.take(size_t(d.d) * size_t(d.v) * 4);
         }
+        const size_t cut = std::max(cut_bytes(d, p.piece, backward, sm_count), cut_bytes(d, d.n % p.piece, backward, sm_count));
+        if (cut) p.cut = space.take(cut);
         return p;
     }
     p.x_pitch = d.d;
@@ -479,12 +502,6 @@ int begin(const mimk_linear_ce_desc& d, const Plan& p, bool forward, const Devic
 }
 
 // ---- f32 -------------------------------------------------------------------------------------------------------------------------
-int product(int64_t m, int64_t n, int64_t k, const float* a, const float* b, int layout, float* c, cudaStream_t s) {
-    mimk_gemm_desc g = {};
-    g.batch = 1, g.m = m, g.n = n, g.k = k, g.a = a, g.b = b, g.c = c;
-    g.in_dtype = g.out_dtype = MIMK_F32, g.b_layout = layout;
-    return mimk_gemm(&g, s);
-}
 // [rows, cols] -> [cols, rows]
 int turn(const float* from, int64_t rows, int64_t cols, void* to, cudaStream_t s) {
     const int64_t shape[2] = {cols, rows};
@@ -502,19 +519,19 @@ int run_f32(const mimk_linear_ce_desc& d, const Plan& p, bool forward, bool back
     for (int64_t first = 0; first < d.n; first += p.piece) {
         const int64_t n = std::min(p.piece, d.n - first);
         const float* xi = x + first * d.d;
-        MIMK_TRY(product(n, d.v, d.d, xi, w, d.w_layout, logits, s));
+        MIMK_TRY(gemm_any(product(n, d.v, d.d, xi, w, d.w_layout, logits), s, p.cut));
         logits_kernel<<<unsigned(n), 512, 0, s>>>(logits, d.v, first, rows, d.dloss, d.reduction, forward ? nullptr : d.lse, forward ? d.lse : nullptr,
                                                   backward);
         MIMK_TRY(launch_status());
         if (!backward) continue;
-        MIMK_TRY(product(n, d.d, d.v, logits, w, nk ? MIMK_B_KN : MIMK_B_NK, dx + first * d.d, s));
+        MIMK_TRY(gemm_any(product(n, d.d, d.v, logits, w, nk ? MIMK_B_KN : MIMK_B_NK, dx + first * d.d), s, p.cut));
         float* to = first ? static_cast<float*>(p.sum) : dw;
         if (nk) {
             MIMK_TRY(turn(logits, n, d.v, p.turned, s));
-            MIMK_TRY(product(d.v, d.d, n, static_cast<const float*>(p.turned), xi, MIMK_B_KN, to, s));
+            MIMK_TRY(gemm_any(product(d.v, d.d, n, p.turned, xi, MIMK_B_KN, to), s, p.cut));
         } else {
             MIMK_TRY(turn(xi, n, d.d, p.turned, s));
-            MIMK_TRY(product(d.d, d.v, n, static_cast<const float*>(p.turned), logits, MIMK_B_KN, to, s));
+            MIMK_TRY(gemm_any(product(d.d, d.v, n, p.turned, logits, MIMK_B_KN, to), s, p.cut));
         }
         if (first) {
             add_kernel<<<grid_for(d.d * d.v, 1024, 8192), 256, 0, s>>>(dw, to, d.d * d.v);
