@@ -386,6 +386,7 @@ OP(clip_grads, 4)
     if (!count || (a[1] != Py_None && PyList_GET_SIZE(a[1]) != count) || (clip && (!PyFloat_CheckExact(a[2]) || !PyFloat_CheckExact(a[3])))) Py_RETURN_NONE;
     std::vector<const void*> in(count);
     std::vector<void*> out(count);
+    std::vector<const Tensor*> written(count);
     std::vector<int64_t> lengths(count);
     std::vector<int32_t> dtypes(count);
     const Tensor* first = nullptr;
@@ -395,18 +396,22 @@ OP(clip_grads, 4)
         if (o != t && (o->scalar_type() != t->scalar_type() || o->sizes() != t->sizes() || o->strides() != t->strides())) Py_RETURN_NONE;
         first = first ? first : t;
         if (t->device() != first->device() || o->device() != first->device()) Py_RETURN_NONE;
-        in[i] = t->data_ptr(), out[i] = o->data_ptr(), lengths[i] = t->numel(), dtypes[i] = dtype_of(t->scalar_type());
+        in[i] = t->data_ptr(), out[i] = o->data_ptr(), lengths[i] = t->numel(), dtypes[i] = dtype_of(t->scalar_type()), written[i] = o;
     }
     uint64_t bytes = 0;
     if (mimk_clip_grads_workspace(count, &bytes) != MIMK_OK) Py_RETURN_NONE;
     Tensor norm = empty({}, at::kFloat, *first), scratch = empty({int64_t(bytes)}, at::kByte, *first);
     float* to = static_cast<float*>(norm.data_ptr());
     void* ws  = scratch.data_ptr();
-    return result(unlocked([&](void* stream) {
-                      return clip ? mimk_clip_grads(in.data(), out.data(), lengths.data(), dtypes.data(), count, float(PyFloat_AS_DOUBLE(a[2])), float(PyFloat_AS_DOUBLE(a[3])), to, ws, bytes, stream)
-                                  : mimk_grad_norm(in.data(), lengths.data(), dtypes.data(), count, to, ws, bytes, stream);
-                  }),
-                  std::move(norm));
+    const int status = unlocked([&](void* stream) {
+        return clip ? mimk_clip_grads(in.data(), out.data(), lengths.data(), dtypes.data(), count, float(PyFloat_AS_DOUBLE(a[2])), float(PyFloat_AS_DOUBLE(a[3])), to, ws, bytes, stream)
+                    : mimk_grad_norm(in.data(), lengths.data(), dtypes.data(), count, to, ws, bytes, stream);
+    });
+    // a tensor that autograd has saved was changed: its version says so (an inference tensor has none)
+    if (clip && status == MIMK_OK)
+        for (const Tensor* o : written)
+            if (!o->is_inference()) o->unsafeGetTensorImpl()->bump_version();
+    return result(status, std::move(norm));
 END_OP
 
 // x, perm (a tuple of ints): the copy-style map_reduce_post that tensor.py's transpose spells

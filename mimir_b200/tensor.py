@@ -570,6 +570,7 @@ def clip_grad_norm(grads, limit: float, *, eps: float = 1e-6, out=None) -> torch
         return norm
     ins, outs, lengths, dtypes, n, norm, ws, size = _grad_list("clip_grad_norm", grads, out)
     L.check(L.lib().mimk_clip_grads(ins, outs, lengths, dtypes, n, limit, eps, norm.data_ptr(), ws.data_ptr(), size, _stream()), "clip_grad_norm")
+    torch.autograd.graph.increment_version(grads if out is None else out)
     return norm
 
 
