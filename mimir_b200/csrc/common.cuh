@@ -213,7 +213,8 @@ __device__ __forceinline__ void apply_op_n(int op, float (&a)[N], const float (&
     if (composed) apply_op_plain_n((op >> 8) & 0xff, a, b);
 }
 // In a kernel of `launch_after`, by every thread, before anything of the kernels before it is read and before anything is written to global
-// memory: waits until they are done, and lets the next kernel's set-up begin.
+// memory: waits until they are done, and lets the next kernel's set-up begin. What they wrote changes while this kernel is already running, so that
+// it is not for loads of read-only memory: no __ldg, and no `const T* __restrict__`, which lets the compiler choose them.
 __device__ __forceinline__ void after_previous() {
     asm volatile("griddepcontrol.wait;\n\tgriddepcontrol.launch_dependents;" ::: "memory");
 }

@@ -88,7 +88,7 @@ __device__ __forceinline__ double chunk_squares(const Chunk& c) {
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
         const int at = head + (i * THREADS + int(threadIdx.x)) * 16;
-        v[i]         = at < tail ? __ldg(reinterpret_cast<const uint4*>(c.in + at)) : make_uint4(0, 0, 0, 0);
+        v[i]         = at < tail ? *reinterpret_cast<const uint4*>(c.in + at) : make_uint4(0, 0, 0, 0);
     }
 #pragma unroll
     for (int i = 0; i < LOADS; i += F32 ? 4 : 2) {
@@ -142,7 +142,7 @@ __device__ __forceinline__ double total_of(const double* sums, int count) {
     for (int i = threadIdx.x; i < count; i += THREADS) s += sums[i];
     return sqrt(block_sum(s));
 }
-__global__ void __launch_bounds__(THREADS) norm_kernel(const double* __restrict__ sums, int count, float* norm) {
+__global__ void __launch_bounds__(THREADS) norm_kernel(const double* sums, int count, float* norm) {
     after_previous();
     const double n = total_of(sums, count);
     if (threadIdx.x == 0) *norm = float(n);
@@ -186,7 +186,7 @@ __device__ __forceinline__ void scale_chunk(const Chunk& c, float by) {
 }
 
 template <int N>
-__global__ void __launch_bounds__(THREADS) scale_kernel(const __grid_constant__ Table<N> t, const double* __restrict__ sums, int n_sums, double limit, double eps,
+__global__ void __launch_bounds__(THREADS) scale_kernel(const __grid_constant__ Table<N> t, const double* sums, int n_sums, double limit, double eps,
                                                        float* norm, bool in_place) {
     after_previous();
     const double n = total_of(sums, n_sums);

@@ -172,7 +172,7 @@ __global__ void __launch_bounds__(128) join_kernel(Rows r, int64_t n, int parts,
 // 276; five rows and more go there.
 constexpr int FEW = 4, FEW_CTAS = 4;
 template <int N>
-__global__ void __launch_bounds__(256, N == FEW ? 2 : FEW_CTAS) few_rows_kernel(const __nv_bfloat16* __restrict__ x, int64_t x_pitch, const __nv_bfloat16* __restrict__ w, int d, int v,
+__global__ void __launch_bounds__(256, N == FEW ? 2 : FEW_CTAS) few_rows_kernel(const __nv_bfloat16* x, int64_t x_pitch, const __nv_bfloat16* w, int d, int v,
                                                                   Rows r) {
     after_previous();
     extern __shared__ float4 xs[];  // [N][2][d / 8]
@@ -292,7 +292,7 @@ __global__ void recall_kernel(Rows r, const float* __restrict__ lse, const float
 
 // dx from its partial sums, each row to its place; zeros for the rows that were taken out. Four columns a thread.
 template <class T>
-__global__ void place_rows_kernel(const float* __restrict__ part, int splits, int64_t stride, int64_t pitch, const int* __restrict__ place, T* __restrict__ dx,
+__global__ void place_rows_kernel(const float* part, int splits, int64_t stride, int64_t pitch, const int* place, T* dx,
                                   int64_t n, int64_t cols, bool words) {
     after_previous();
     const int64_t quads = (cols + 3) / 4, all = n * quads;

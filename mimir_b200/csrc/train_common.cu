@@ -13,7 +13,7 @@ __global__ void copy_rows_kernel(const uint16_t* __restrict__ from, int64_t from
 }
 
 // Four columns a thread (the partial results' rows are whole 16 bytes), the parts in order, so that the sum is the same call after call.
-__global__ void sum_parts_kernel(const float* __restrict__ part, int splits, int64_t stride, int64_t part_pitch, __nv_bfloat16* __restrict__ out,
+__global__ void sum_parts_kernel(const float* part, int splits, int64_t stride, int64_t part_pitch, __nv_bfloat16* out,
                                  int64_t out_pitch, int64_t rows, int64_t cols, bool words) {
     after_previous();
     const int64_t quads = (cols + 3) / 4, all = rows * quads;
