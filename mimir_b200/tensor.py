@@ -368,11 +368,14 @@ def _bytes(n: int, device) -> torch.Tensor:
 
 
 def _weight_layout(what: str, *ws):
-    """The weights as they lie in memory (copied only where they are neither row-major nor a transposed view of row-major) and their layout."""
-    stored = [_b_layout(w) for w in ws]
-    if any(lay != stored[0][1] for _, lay in stored):
+    """The weights as they lie in memory (copied only where they are neither row-major nor a transposed view of row-major) and the layout that they share. One
+    with an axis of a single value is of either layout, and a copy is made in the others'."""
+    rows, turned = [w.is_contiguous() for w in ws], [w.t().is_contiguous() for w in ws]
+    if all(r or not t for r, t in zip(rows, turned)):
+        return [w.contiguous() for w in ws], L.B_KN
+    if any(r and not t for r, t in zip(rows, turned)):
         raise ValueError(f"{what}: the weights must share one storage layout")
-    return [w for w, _ in stored], stored[0][1]
+    return [w.t().contiguous() for w in ws], L.B_NK
 
 
 def _like_weight(w: torch.Tensor, layout: int) -> torch.Tensor:
