@@ -530,6 +530,11 @@ def _gaps(t: torch.Tensor) -> bool:
     return False
 
 
+def _same_order(t: torch.Tensor, o: torch.Tensor) -> bool:
+    """Whether two tensors of one shape have their values in the same order (strides along axes of one value mean nothing)."""
+    return t.numel() == 0 or all(s == p for s, p, n in zip(t.stride(), o.stride(), t.shape) if n != 1)
+
+
 def _grad_list(what, grads, out=None):
     grads = list(grads)
     out = grads if out is None else list(out)
@@ -542,7 +547,7 @@ def _grad_list(what, grads, out=None):
             raise ValueError(f"{what}: the gradients lie on one device")
         if t.dtype not in (torch.float32, torch.bfloat16) or o.dtype != t.dtype:
             raise TypeError(f"{what}: gradients are F32 or BF16, and results of the same element type")
-        if o.shape != t.shape or (o is not t and o.stride() != t.stride()) or _gaps(t):
+        if o.shape != t.shape or (o is not t and not _same_order(t, o)) or _gaps(t):
             raise ValueError(f"{what}: gradients are dense, and results of the same shape and strides")
     n = len(grads)
     ptrs = lambda ts: (C.c_void_p * n)(*(t.data_ptr() for t in ts))  # noqa: E731
