@@ -481,7 +481,7 @@ def _linear_ce(what, x, w, targets, ignore_index, reduction, dloss, lse, forward
             out.append(torch.empty(lead, **f32))
             d.lse = out[1].data_ptr()
     else:
-        if lse.shape != lead or lse.dtype != torch.float32:
+        if lse is None or lse.shape != lead or lse.dtype != torch.float32:
             raise ValueError(f"{what}: lse is what linear_cross_entropy returned, one F32 for each row")
         lse = lse.contiguous()
         d.lse = lse.data_ptr()

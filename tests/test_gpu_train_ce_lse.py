@@ -37,3 +37,10 @@ def test_the_given_lse_counts(shape, nk, dtype):
         got = T.linear_cross_entropy_grad(x, w, t, lse, ignore_index=IGNORED, reduction="sum")
         assert near(got[0], *want[0]) and near(got[1], *want[1]), shift
     T.device_status()
+
+
+def test_no_lse():
+    from mimir_b200 import tensor as T
+    x, w, t = inputs(16, 32, 50, F32, False)
+    with pytest.raises(ValueError, match="lse"):
+        T.linear_cross_entropy_grad(x, w, t, None)
