@@ -41,7 +41,9 @@ struct Shape {
     // The loss is f32, and the tensor cores cut sums off where f32 rounds: an error of some 2^-25 of the value for each 16 terms, always towards zero
     // (4096 of them: 1.2e-6 of the loss). For the loss k-blocks are therefore summed in runs, which the epilogue adds up in registers: a quarter
     // the error at 4096, and no time, as an accumulator is read while the other one fills. That takes two warps for a row's 256 columns.
-    static constexpr bool LOSS  = EPI == CE_STATS || EPI == CE_EXP;
+    // CE_GRAD sums its logits the same way, to the same bits: exp(l - lse) of an l rounded otherwise than those in lse is off by the difference
+    // (4096 terms, a logit of 30: 3.6e-4, where 1 - p is 1e-10).
+    static constexpr bool LOSS  = EPI == CE_STATS || EPI == CE_EXP || EPI == CE_GRAD;
     static constexpr int RUN    = LOSS ? 16 : 1 << 30;                      // k-blocks in one accumulator
     // of the epilogue: eight where two for a row's columns pay (STORE: results of few
     // k-blocks are bound by it; 64 rows through 4096 x 14336 and back, 318 us with four, 308 with eight)
@@ -433,7 +435,7 @@ group_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args g) 
             } else if constexpr (S::LOSS) {
                 // this warp's 128 of the columns, in registers: the runs of k-blocks added up
                 const int half = (warp - S::FIRST) >> 2 << 7, n1 = n0 + half, left = p.N - n1;
-                const int tcol = row < t.rows ? g.target[row] - n1 : -1;
+                const int tcol = row < t.rows ? g.target[row] - g.column0 - n1 : -1;
                 uint32_t raw[128];
 #pragma unroll
                 for (int c = 0; c < 128; c += 32) tmem_ld_32x32(t0 + half + c, *reinterpret_cast<uint32_t(*)[32]>(raw + c));
@@ -456,60 +458,55 @@ group_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args g) 
                 float v[128];
 #pragma unroll
                 for (int i = 0; i < 128; ++i) v[i] = __uint_as_float(raw[i]);
-                if (left < 128) {
+                if constexpr (EPI == CE_GRAD) {
+                    const bool mine = row < t.rows;
+                    const float lse = mine ? g.lse[row] : 0.f, scale = mine ? g.scale[row] : 0.f;
+                    // rows past the last one are zeros, which the products over rows read
 #pragma unroll
-                    for (int i = 0; i < 128; ++i) v[i] = i < left ? v[i] : -INFINITY;
-                }
-                if (__any_sync(0xffffffffu, tcol >= 0 && tcol < 128)) {
-#pragma unroll
-                    for (int i = 0; i < 128; ++i)
-                        if (tcol == i) g.target_logit[row] = v[i];
-                }
-                float top = -INFINITY, sum = 0.f;
-#pragma unroll
-                for (int i = 0; i < 128; ++i) top = fmaxf(top, v[i]);
-                const float base = top == -INFINITY ? 0.f : top;
-#pragma unroll
-                for (int c = 0; c < 128; c += 32) {
-                    float part = 0.f;
-#pragma unroll
-                    for (int i = c; i < c + 32; ++i) v[i] = __expf(v[i] - base), part += v[i];
-                    sum += part;
-                }
-                if (row < t.rows) g.part[int64_t(row) * ((p.N + 255) / 256 * 2) + (n1 >> 7)] = make_float2(top, sum);
-                if constexpr (EPI == CE_EXP) {
+                    for (int i = 0; i < 128; ++i) v[i] = mine ? scale * (__expf(v[i] - lse) - (tcol == i ? 1.f : 0.f)) : 0.f;
 #pragma unroll
                     for (int c = 0; c < 128; c += 64) {
                         if (lane == 0) bulk_wait_read_0();
                         __syncwarp();
 #pragma unroll
                         for (int i = 0; i < 64; i += 8)
-                            st_shared_v4(slots + lane * 128 + ((uint32_t(i >> 3) ^ uint32_t(lane & 7)) << 4), __byte_perm(exp_code(v[c + i]), exp_code(v[c + i + 1]), 0x5410),
-                                         __byte_perm(exp_code(v[c + i + 2]), exp_code(v[c + i + 3]), 0x5410), __byte_perm(exp_code(v[c + i + 4]), exp_code(v[c + i + 5]), 0x5410), __byte_perm(exp_code(v[c + i + 6]), exp_code(v[c + i + 7]), 0x5410));
+                            st_shared_v4(slots + lane * 128 + ((uint32_t(i >> 3) ^ uint32_t(lane & 7)) << 4), pack_bf16x2(v[c + i], v[c + i + 1]), pack_bf16x2(v[c + i + 2], v[c + i + 3]),
+                                         pack_bf16x2(v[c + i + 4], v[c + i + 5]), pack_bf16x2(v[c + i + 6], v[c + i + 7]));
                         send(&maps.out[0], slots, n1 + c);
                     }
-                }
-            } else {
-                const bool mine = row < t.rows;
-                const int tcol  = mine ? g.target[row] - g.column0 - n0 : -1;
-                const float lse = mine ? g.lse[row] : 0.f, scale = mine ? g.scale[row] : 0.f;
-#pragma unroll 1
-                for (int c = 0; c < width; c += 32) {
-                    const uint32_t slot = slots + (turn & 1u) * SLOT;
-                    if (!(c & 32)) {
-                        if (lane == 0) bulk_wait_read_1();
-                        __syncwarp();
-                    }
-                    float v[32];
-                    get_acc(t0 + c, v, empty);
-                    if (c + 32 >= width) release();
-                    // rows past the last one are zeros, which the products over rows read
+                } else {
+                    if (left < 128) {
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) v[i] = mine ? scale * (__expf(v[i] - lse) - (tcol == c + i ? 1.f : 0.f)) : 0.f;
-                    put_bf16(slot, lane, (c & 32) ? 4 : 0, v);
-                    if ((c & 32) || c + 32 >= width) {
-                        send(&maps.out[0], slot, n0 + (c & ~63));
-                        ++turn;
+                        for (int i = 0; i < 128; ++i) v[i] = i < left ? v[i] : -INFINITY;
+                    }
+                    if (__any_sync(0xffffffffu, tcol >= 0 && tcol < 128)) {
+#pragma unroll
+                        for (int i = 0; i < 128; ++i)
+                            if (tcol == i) g.target_logit[row] = v[i];
+                    }
+                    float top = -INFINITY, sum = 0.f;
+#pragma unroll
+                    for (int i = 0; i < 128; ++i) top = fmaxf(top, v[i]);
+                    const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+                    for (int c = 0; c < 128; c += 32) {
+                        float part = 0.f;
+#pragma unroll
+                        for (int i = c; i < c + 32; ++i) v[i] = __expf(v[i] - base), part += v[i];
+                        sum += part;
+                    }
+                    if (row < t.rows) g.part[int64_t(row) * ((p.N + 255) / 256 * 2) + (n1 >> 7)] = make_float2(top, sum);
+                    if constexpr (EPI == CE_EXP) {
+#pragma unroll
+                        for (int c = 0; c < 128; c += 64) {
+                            if (lane == 0) bulk_wait_read_0();
+                            __syncwarp();
+#pragma unroll
+                            for (int i = 0; i < 64; i += 8)
+                                st_shared_v4(slots + lane * 128 + ((uint32_t(i >> 3) ^ uint32_t(lane & 7)) << 4), __byte_perm(exp_code(v[c + i]), exp_code(v[c + i + 1]), 0x5410),
+                                             __byte_perm(exp_code(v[c + i + 2]), exp_code(v[c + i + 3]), 0x5410), __byte_perm(exp_code(v[c + i + 4]), exp_code(v[c + i + 5]), 0x5410), __byte_perm(exp_code(v[c + i + 6]), exp_code(v[c + i + 7]), 0x5410));
+                            send(&maps.out[0], slots, n1 + c);
+                        }
                     }
                 }
             }

@@ -170,10 +170,12 @@ __global__ void __launch_bounds__(128) join_kernel(Rows r, int64_t n, int parts,
 // four classes at a time, a lane 16 bytes of each; the rows of x are in shared memory as f32, split in halves of eight values so that neighbouring
 // lanes read neighbouring 16 bytes. One row of 4096 against 131072 classes: 166 us, 6.5 TB/s, where the tensor cores' pass takes
 // 276; five rows and more go there.
+// GRAD: gradients from the lse of such a pass take their logits from here, too, to the same bits (those of the tensor cores are 2e-6 of themselves off at
+// 1024 features, which 1 - p of a row that is nearly certain does not bear): p of the `n` rows, zeros for those that were taken out.
 constexpr int FEW = 4, FEW_CTAS = 4;
-template <int N>
+template <int N, bool GRAD>
 __global__ void __launch_bounds__(256, N == FEW ? 2 : FEW_CTAS) few_rows_kernel(const __nv_bfloat16* x, int64_t x_pitch, const __nv_bfloat16* w, int d, int v,
-                                                                  Rows r) {
+                                                                  Rows r, int n, int column0, __nv_bfloat16* p, int64_t pitch) {
     after_previous();
     extern __shared__ float4 xs[];  // [N][2][d / 8]
     const int lane = threadIdx.x & 31, eighths = d / 8, slots = gridDim.x * 8, slot = blockIdx.x * 8 + (threadIdx.x >> 5);
@@ -187,7 +189,9 @@ __global__ void __launch_bounds__(256, N == FEW ? 2 : FEW_CTAS) few_rows_kernel(
             make_float4(__uint_as_float(u.z << 16), __uint_as_float(u.z & 0xffff0000u), __uint_as_float(u.w << 16), __uint_as_float(u.w & 0xffff0000u));
     }
     __syncthreads();
-    const int target = lane < N && lane < left ? r.target[lane] : -1;  // lane j looks after row j
+    const bool mine  = lane < N && lane < left;  // lane j looks after row j
+    const int target = mine ? r.target[lane] - column0 : -1;
+    const float lse = GRAD && mine ? r.lse[lane] : 0.f, scale = GRAD && mine ? r.scale[lane] : 0.f;
     float top = -INFINITY, sum = 0.f;
     for (int64_t c = int64_t(slot) * 4; c < v; c += int64_t(slots) * 4) {
         float acc[4][N];
@@ -223,7 +227,12 @@ __global__ void __launch_bounds__(256, N == FEW ? 2 : FEW_CTAS) few_rows_kernel(
                 const float all = warp_sum(acc[i][j]);
                 l[i]            = lane == j ? all : l[i];
             }
-        if (lane < N) {
+        if constexpr (GRAD) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) l[i] = mine && c + i < v ? scale * (__expf(l[i] - lse) - (target == c + i ? 1.f : 0.f)) : 0.f;
+            // (rows of p are of whole 256 columns)
+            if (lane < n) *reinterpret_cast<uint2*>(p + lane * pitch + c) = make_uint2(pack_bf16x2(l[0], l[1]), pack_bf16x2(l[2], l[3]));
+        } else if (lane < N) {
             float most = top;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -236,7 +245,7 @@ __global__ void __launch_bounds__(256, N == FEW ? 2 : FEW_CTAS) few_rows_kernel(
             sum += (__expf(l[0] - base) + __expf(l[1] - base)) + (__expf(l[2] - base) + __expf(l[3] - base));
         }
     }
-    if (lane < N && lane < left) r.part[int64_t(lane) * slots + slot] = make_float2(top, sum);
+    if (!GRAD && mine) r.part[int64_t(lane) * slots + slot] = make_float2(top, sum);
 }
 
 // p from the exponentials, in place: exp(l - m) becomes scale exp(l - lse) as bf16, less scale at the target, whose own value comes from its
@@ -446,10 +455,10 @@ Plan plan(const mimk_linear_ce_desc& d, bool forward, bool backward, Space& spac
     if (taken || !tma_can_read(d.x, d.d)) p.x_pitch = up(d.d, 8), p.x = space.take(n * size_t(p.x_pitch) * 2);
     const bool nk = d.w_layout == MIMK_B_NK;
     p.w           = nk ? stage(space, d.w, d.v, d.d) : stage(space, d.w, d.d, d.v);
-    // (up to 64 KiB of shared memory: FEW_CTAS CTAs to an SM; with gradients the tensor cores' pass leaves the exponentials, too)
-    p.few   = forward && !backward && nk && d.n <= FEW && (d.n <= 2 ? d.n : FEW) * d.d <= 16384 && !p.w.copied() && tma_can_read(d.x, d.d);
+    // (up to 64 KiB of shared memory: FEW_CTAS CTAs to an SM; loss and gradients at once: the tensor cores' pass leaves the exponentials, too)
+    p.few   = forward != backward && nk && d.n <= FEW && (d.n <= 2 ? d.n : FEW) * d.d <= 16384 && !p.w.copied() && tma_can_read(d.x, d.d);
     p.parts = p.few ? sm_count * FEW_CTAS * 8 : int((d.v + 255) / 256) * 2;
-    if (p.few) p.x = nullptr;
+    if (p.few && forward) p.x = nullptr;
     if (forward) p.rows.part = static_cast<float2*>(space.take(n * size_t(p.parts) * 8)), p.rows.target_logit = floats(n);
     if (backward) {
         p.dw    = nk ? stage(space, d.dw, d.v, d.d) : stage(space, d.dw, d.d, d.v);
@@ -556,13 +565,18 @@ Problem problem(int64_t m, int64_t n, int64_t k, bool a_mn, bool b_mn) {
     return p;
 }
 
-template <int N>
-int few_rows(const mimk_linear_ce_desc& d, const Plan& p, const DeviceInfo& dev, cudaStream_t s) {
+template <int N, bool GRAD>
+int few_rows_of(const mimk_linear_ce_desc& d, const Plan& p, int64_t from, int64_t cols, const DeviceInfo& dev, cudaStream_t s) {
     const int smem = int(N * d.d * 4);
-    auto kern      = few_rows_kernel<N>;
+    auto kern      = few_rows_kernel<N, GRAD>;
     if (smem > 48 * 1024) MIMK_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 65536));
-    return launch_after(kern, unsigned(dev.sm_count * FEW_CTAS), 256, smem, s, static_cast<const __nv_bfloat16*>(d.x), d.d, static_cast<const __nv_bfloat16*>(d.w), int(d.d),
-                        int(d.v), p.rows);
+    return launch_after(kern, unsigned(dev.sm_count * FEW_CTAS), 256, smem, s, static_cast<const __nv_bfloat16*>(d.x), d.d, static_cast<const __nv_bfloat16*>(d.w) + from * d.d,
+                        int(d.d), int(cols), p.rows, int(d.n), int(from), static_cast<__nv_bfloat16*>(p.p), p.piece);
+}
+// classes [from, from + cols)
+template <bool GRAD>
+int few_rows(const mimk_linear_ce_desc& d, const Plan& p, int64_t from, int64_t cols, const DeviceInfo& dev, cudaStream_t s) {
+    return d.n == 1 ? few_rows_of<1, GRAD>(d, p, from, cols, dev, s) : d.n == 2 ? few_rows_of<2, GRAD>(d, p, from, cols, dev, s) : few_rows_of<FEW, GRAD>(d, p, from, cols, dev, s);
 }
 
 int run_bf16(const mimk_linear_ce_desc& d, const Plan& p, bool forward, bool backward, const DeviceInfo& dev, cudaStream_t s) {
@@ -591,7 +605,7 @@ int run_bf16(const mimk_linear_ce_desc& d, const Plan& p, bool forward, bool bac
             MIMK_TRY(operand_map(&maps.b[0][0], w, !nk, 128));
         }
         if (p.few) {
-            MIMK_TRY((d.n == 1 ? few_rows<1>(d, p, dev, s) : d.n == 2 ? few_rows<2>(d, p, dev, s) : few_rows<FEW>(d, p, dev, s)));
+            MIMK_TRY(few_rows<false>(d, p, 0, d.v, dev, s));
         } else if (p.kept) {
             MIMK_TRY(result_map(&maps.out[0], p.p, false, d.n, d.v, p.piece));
             MIMK_TRY(launch_group<CE_EXP>(maps, args, dev, s));
@@ -612,7 +626,9 @@ int run_bf16(const mimk_linear_ce_desc& d, const Plan& p, bool forward, bool bac
     for (int64_t from = 0; from < d.v; from += p.piece) {
         const int64_t cols = std::min(p.piece, d.v - from);
         const Mat wi = part_of(w, from, cols), pi = {p.p, d.n, cols, p.piece};
-        if (!p.kept) {
+        if (p.few) {
+            MIMK_TRY(few_rows<true>(d, p, from, cols, dev, s));
+        } else if (!p.kept) {
             args.count      = 1;
             args.column0    = int(from);
             args.p[0]       = problem(d.n, cols, d.d, false, !nk);
