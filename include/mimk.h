@@ -337,7 +337,7 @@ int mimk_mlp_gated(const mimk_mlp_desc* desc, void* stream);
  * The operators from here to the generic operation are the ends of a training step: they have no counterpart in the reference,
  * whose `tensor` plugin has no gradients. Their scratch is the caller's: a `workspace` of at least the bytes that the operator's size
  * query answers for the same descriptor, aligned to 16 bytes (MIMK_E_ALIGN otherwise, MIMK_E_WORKSPACE if it is missing or too small), of any
- * content, free again once the call's work on `stream` is done. They allocate nothing and may be captured.
+ * content, free again once the call's work on `stream` is done. They allocate nothing, and may be captured: the same kernels run, to the same bits.
  *
  * The gated MLP block with its gradients, bf16:
  *   fwd: a = X W1, b = X W3, h = silu(a) * b, Y = h W2, with a, b (f32) and h (bf16) left in `kept`;
@@ -369,15 +369,22 @@ int mimk_mlp_gated_bwd(const mimk_mlp_train_desc* desc, void* stream);
 
 /* Softmax cross-entropy of a linear layer, logits = X W, without the logits in memory (bf16) or with those of a piece of at most
  * 512 MiB (f32): loss_i = log sum_j exp(l_ij) - l_i,target(i), and its gradients with respect to X and W.
- *   fwd: loss and, unless NULL, lse (log sum exp per row); bwd: dX and dW from lse; fwd_bwd: loss, lse unless NULL, dX and dW.
+ *   fwd: loss and, unless NULL, lse (log sum exp per row); bwd: dX and dW, softmax being exp(l - lse) of the lse that it is given; fwd_bwd: loss,
+ *   lse unless NULL, dX and dW.
  * reduction: one loss per row, their mean over the rows that have a target (0 if none has), or their sum. dloss: the gradient that arrives at the
  * loss, one value or one per row; NULL: ones.
- * has_ignore: a row whose target is ignore_index has none: its loss, lse and dX are zeros, nothing of it enters dW, and its X is not read. Any other target
- * outside [0, v) is recorded (mimk_device_status: MIMK_E_SHAPE); the row's loss is NaN, and it enters no gradient.
+ * has_ignore: a row whose target is ignore_index, a class or not, has none: its loss, lse and dX are zeros, nothing of it enters dW, and its X is not read.
+ * Any other target outside [0, v) is recorded (mimk_device_status: MIMK_E_SHAPE); the row's loss is NaN, and its p below zeros (without has_ignore the
+ * row is still multiplied, so that values of X or logits that are not finite make NaN of dW).
  * Losses, lse and all sums are f32; bf16 gradients are rounded once from f32 sums of products whose factor p = dloss (softmax - onehot) is
- * rounded to bf16 (in fwd_bwd from exponentials of ten significant bits where n v <= 2^30). Equal descriptors give equal bits. Workspace as above,
- * from the query; bf16: 16 bytes per row and 8 per row and 128 classes; for gradients also p, 2 n v bytes in fwd_bwd where n v <= 2^30, else at
- * most 512 MiB (8 KiB per row where that is more), and 4 bytes per value of X where p comes in pieces or rows were taken out. */
+ * rounded to bf16 (in fwd_bwd from exponentials of ten significant bits where n v <= 2^30). The target's softmax - 1 is exp(l - lse) - 1 in
+ * f32: where a row is nearly certain it is off by some units of 2^-24 of lse. bwd's logits are those that fwd's lse of the same operands came from, bit for bit.
+ * Equal descriptors give equal bits. Workspace as above; the query's answer holds
+ *   both types: up to 28 bytes per row; X of the rows that are left, where has_ignore is set;
+ *   bf16: 8 bytes per row and 128 classes (forward); X, W and dW again where their rows are no whole 16 bytes or start elsewhere; p, 2 n v bytes in
+ *     fwd_bwd where n v <= 2^30, else at most 512 MiB (8 KiB per row where that is more); dX in f32, up to 16 times where few rows share many classes;
+ *   F32: logits of a piece, at most 512 MiB or one row; for gradients also one factor transposed, a piece's dW where there are several, dX of the rows that
+ *     are left; and twice the operands of the products that cut them beforehand. */
 enum { MIMK_REDUCTION_NONE = 0, MIMK_REDUCTION_MEAN = 1, MIMK_REDUCTION_SUM = 2 };
 typedef struct mimk_linear_ce_desc {
     int64_t n, d, v;     /* rows, features, classes */
@@ -400,9 +407,9 @@ int mimk_linear_ce_bwd(const mimk_linear_ce_desc* desc, void* stream);
 int mimk_linear_ce_fwd_bwd(const mimk_linear_ce_desc* desc, void* stream);
 
 /* The 2-norm of all values of `count` tensors together (of any length, each dense: tensors[i] has lengths[i] elements of dtypes[i], F32 or BF16), and
- * the tensors scaled so that it is at most `limit`: out[i] = tensors[i] * c, c = min(1, limit / (norm + eps)); out[i] may be tensors[i]. A norm that
- * is NaN makes c NaN, one that is infinite makes it zero. `norm`: one f32 on the device. The arrays are on the
- * host and are read before the call returns. Squares are summed in f32 over 16 values at most and in f64 from there, and over again in
+ * the tensors scaled so that it is at most `limit`: out[i] = tensors[i] * c, c = min(1, limit / (norm + eps)); out[i] may be tensors[i], and overlaps no
+ * tensor otherwise. A norm that is NaN makes c NaN, one that is infinite makes it zero, and 0 / 0 and infinity over infinity make it NaN. `norm`: one f32 on
+ * the device. The arrays are on the host and are read before the call returns. Squares are summed in f32 over 16 values at most and in f64 from there, and over again in
  * f64 where an f32 sum overflows or all but vanishes. Equal calls give equal bits. Workspace as above. */
 int mimk_clip_grads_workspace(int64_t count, uint64_t* bytes); /* of either call */
 int mimk_grad_norm(const void* const* tensors, const int64_t* lengths, const int32_t* dtypes, int64_t count, float* norm, void* workspace,

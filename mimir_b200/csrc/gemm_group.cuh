@@ -1,5 +1,6 @@
 // Products of a training step on paired SMs: the pipeline of gemm_tc2.cu (TMA loads, one issuer of tcgen05.mma.cta_group::2, two accumulators in
-// tensor memory and an epilogue that empties one while the other fills; here a warp for each operand's loads, and four or eight for the epilogue) with what gradients need beyond a forward product:
+// tensor memory and an epilogue that empties one while the other fills; here a warp for each operand's loads, and four or eight for the
+// epilogue) with what gradients need beyond a forward product:
 //   - either operand K-major or MN-major, so that x^T dy reads both matrices where the forward pass left them;
 //   - two operand pairs added in one accumulator (da W1^T + db W3^T);
 //   - several products in one launch (the three weight gradients and the input's), so that the last, half empty round of tiles comes once;
@@ -39,7 +40,7 @@ template <int EPI>
 struct Shape {
     static constexpr bool GATED = EPI == GATED_FWD;
     // The loss is f32, and the tensor cores cut sums off where f32 rounds: an error of some 2^-25 of the value for each 16 terms, always towards zero
-    // (4096 of them: 1.2e-6 of the loss). For the loss k-blocks are therefore summed in runs, which the epilogue adds up in registers: a quarter
+    // (4096 of them: 1.2e-6 of the loss, 1.2e-5 of a logit whose terms have one sign). For the loss k-blocks are therefore summed in runs, which the epilogue adds up in registers: a quarter
     // the error at 4096, and no time, as an accumulator is read while the other one fills. That takes two warps for a row's 256 columns.
     // CE_GRAD sums its logits the same way, to the same bits: exp(l - lse) of an l rounded otherwise than those in lse is off by the difference
     // (4096 terms, a logit of 30: 3.6e-4, where 1 - p is 1e-10).

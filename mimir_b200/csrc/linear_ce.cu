@@ -4,13 +4,17 @@
 //   p_ij = g_i (exp(l_ij - lse_i) - [j = t(i)]),  dx = p W^T,  dW = x^T p        g: the loss's gradient, over the count for a mean
 //
 // bf16: the logits exist as accumulators only. A first product reduces each 128 columns of a row to a maximum and a sum of exponentials
-// (8 bytes for 128 logits); a kernel over rows joins them. Loss and gradients in one call: where n v is at most 2^30, that product also leaves
-// the exponentials themselves in 16 bits (ten of them significant, where p has eight: as bf16 they would round p twice), which a pass over them turns into p once the sums are
-// known (the targets' p from their logits, in f32), and one launch makes dW and dx: 6 n d v operations. Beyond that, and for gradients from an earlier call's lse, by pieces
-// of the classes: a product writes p of the piece as bf16, and one launch makes the piece's rows of dW and adds to dx in f32: 8 n d v
-// operations, two of them logits over again, and 512 MiB of p. 8192 x 4096 x 131072: 24.8 to 26.0 ms
-// at the power limit (1.02 to 1.06 PFLOP/s of the 6 n d v; library products of 8192^3 there: 1.36), by pieces 28.2.
-// f32: pieces of rows instead, through the library's f32 products, with the logits of a piece in memory, turned into p in place.
+// (8 bytes for 128 logits); a kernel over rows joins them: 8192 x 4096 x 131072 in 6.7 to 7.0 ms. Loss and gradients in one call: where n v
+// is at most 2^30, that product also leaves the exponentials themselves in 16 bits (ten of them significant, where p has eight: as bf16
+// they would round p twice), which a pass over them turns into p once the sums are known (the targets' p from their logits, in f32), and
+// one launch makes dW and dx: 6 n d v operations. Beyond that, and for gradients from an earlier call's lse, by pieces of the classes: a
+// product writes p of the piece as bf16, and one launch makes the piece's rows of dW and adds to dx in f32, with the logits over again in the one
+// call: 8 n d v operations, and 512 MiB of p. 8192 rows of that size at once: 24.7 to 26.0 ms at the power limit (1.02 to 1.07 PFLOP/s of
+// the 6 n d v; library products of 8192^3 there: 1.36), 21.5 to 23.4 in a short run; by pieces 26.1 to 27.5 in such a run, the gradients
+// alone 20.2 to 21.4. 2^30 is a limit of memory (2 GiB of exponentials): 8193 rows take 27.3 to 28.6 by pieces and would take 22.2 to 23.4
+// without it, 16384 rows 52.8 to 54.2 and 49.6 to 52.3 (4 GiB).
+// f32: pieces of rows instead, through the library's f32 products, with the logits of a piece in memory, turned into p in place. 512 x 784 x
+// 10007: 398 us, the loss alone 150, the gradients alone 385; 361 of the 398 are the products, whose faster kernel wants rows of whole 16 bytes.
 //
 // Rows without a target (the ignored index) are taken out first: the rows that are left are copied together, and the products run over as
 // many rows as a count in device memory says. What the other rows hold, NaN included, is never read.
@@ -168,10 +172,12 @@ __global__ void __launch_bounds__(128) join_kernel(Rows r, int64_t n, int parts,
 // ---- a few rows ------------------------------------------------------------------------------------------------------------------
 // The forward pass of up to FEW rows with W stored [v, d]: its bytes bound it, and a tile of 256 rows keeps half of shared memory for zeros. A warp takes
 // four classes at a time, a lane 16 bytes of each; the rows of x are in shared memory as f32, split in halves of eight values so that neighbouring
-// lanes read neighbouring 16 bytes. One row of 4096 against 131072 classes: 166 us, 6.5 TB/s, where the tensor cores' pass takes
-// 276; five rows and more go there.
+// lanes read neighbouring 16 bytes. Calls of 1, 2, 3, 4 rows of 4096 against 131072 classes: 169, 185, 211, 210 to 218 us (one row: 6.5 TB/s), by the
+// tensor cores' pass 269, 224, 231, 252. Two rows have a kernel of their own (as two of four: 204), with 92 bytes of spills in its 64 registers.
+// Five rows would be two rounds of this kernel; the tensor cores take 245, and 195 for 16 or 32.
 // GRAD: gradients from the lse of such a pass take their logits from here, too, to the same bits (those of the tensor cores are 2e-6 of themselves off at
-// 1024 features, which 1 - p of a row that is nearly certain does not bear): p of the `n` rows, zeros for those that were taken out.
+// 1024 features, which 1 - p of a row that is nearly certain does not bear): p of the `n` rows, zeros for those that were taken out. Gradients of
+// 1, 2, 4 rows: 650, 672, 695 us; with p from the tensor cores 730 to 800.
 constexpr int FEW = 4, FEW_CTAS = 4;
 template <int N, bool GRAD>
 __global__ void __launch_bounds__(256, N == FEW ? 2 : FEW_CTAS) few_rows_kernel(const __nv_bfloat16* x, int64_t x_pitch, const __nv_bfloat16* w, int d, int v,

@@ -8,8 +8,10 @@
 // y; dh, whose epilogue reads a and b and writes da and db, so that dh is never written; and dx with all three weight gradients. a and b are
 // kept in 32 bits: rounded to bf16 they would put two more roundings into da, beside its own, and the gradients' error from 1.4 to 1.8 times
 // that of the result's rounding; h, da and db are rounded to bf16 because the tensor cores multiply bf16.
-// 8192 rows, 4096 x 14336 x 4096, forward and backward: 7.1 ms at the power limit (1.22 PFLOP/s), 5.9 ms as single launches from idle; 64 rows: 297 us,
-// 2.4 TB/s of weights and gradients, bound by the loads in flight and by two rounds of tiles over 74 pairs of SMs.
+// 8192 rows, 4096 x 14336 x 4096, forward and backward: 7.0 to 7.2 ms at the power limit (1.21 to 1.24 PFLOP/s), 5.9 ms as single launches from idle;
+// 64 rows: 281 to 301 us, 2.4 TB/s of weights and gradients, bound by the loads in flight and by two rounds of tiles over 74 pairs of SMs.
+// Matrices whose rows are no whole 16 bytes are copied, two bytes a thread and turn: 64 rows, 4095 x 14335 x 4095: 2.33 ms; 1777 rows, 1023 x 2815 x 1023: 293 us,
+// where 1024 x 2816 x 1024 takes 122.
 #include "train_common.cuh"
 
 namespace mimk {

@@ -49,7 +49,10 @@ inline int stage_out(const Staged& x, cudaStream_t s) {
 }
 
 // How many tiles share the k-blocks of one: the number that ends first, counting rounds of tiles over the pairs of SMs, 6 k-blocks' time
-// for a tile's ends, the f32 partial results written and read (0.27 us a k-block), and the launch that adds them up.
+// for a tile's ends, the f32 partial results written and read (0.27 us a k-block), and the launch that adds them up. The gated block forward and
+// backward, with this rule and with one number for both products: 64 rows, 4096 x 14336 x 4096: 281 us; 431 (one), 333 (two), 297 (three),
+// 283 (four), 287 (eight), 295 (sixteen). 300 rows, 1000 x 3000 x 1000: 73.5; 110, 91, 82, 78, 74 (eight). 1777 rows, 1024 x 2816 x 1024: 122; 128, 124, 126, 133,
+// 151 (eight).
 int pick_splits(int64_t m, int64_t n, int64_t kblocks, int sm_count);
 // out[r, c] = sum_s part[s][r][c] as bf16; part: `splits` f32 matrices of `rows_pad` rows of `part_pitch`
 int sum_parts(const float* part, int splits, int64_t rows_pad, int64_t part_pitch, void* out, int64_t out_pitch, int64_t rows, int64_t cols, cudaStream_t s);

@@ -501,7 +501,7 @@ def linear_cross_entropy(x: torch.Tensor, w: torch.Tensor, targets: torch.Tensor
                          return_lse: bool = False):
     """The softmax cross-entropy of the logits x w (w: [features, classes] row-major, or a transpose_2d view of [classes, features]) against class
     numbers, F32 or BF16, without the logits in memory. reduction: "mean" over the rows that have a target (0 if none has), "sum", or "none" for one
-    loss per row; losses are F32. A row whose target is `ignore_index` has none: loss and lse 0. return_lse: also each row's log sum exp, which
+    loss per row; losses are F32. A row whose target is `ignore_index`, which may be a class, has none: loss and lse 0. return_lse: also each row's log sum exp, which
     linear_cross_entropy_grad takes. A target that is neither a class nor `ignore_index` gives NaN, and device_status() raises."""
     out = _linear_ce("linear_cross_entropy", x, w, targets, ignore_index, reduction, None, None, True, False, return_lse)
     return tuple(out) if return_lse else out[0]
@@ -509,7 +509,7 @@ def linear_cross_entropy(x: torch.Tensor, w: torch.Tensor, targets: torch.Tensor
 
 def linear_cross_entropy_grad(x: torch.Tensor, w: torch.Tensor, targets: torch.Tensor, lse: torch.Tensor, *, ignore_index: int | None = None,
                               reduction: str = "mean", dloss: torch.Tensor | None = None):
-    """(dx, dw) of linear_cross_entropy with the same arguments, from its lse. dloss: the gradient that arrives at the loss (of its shape; ones if None).
+    """(dx, dw) of linear_cross_entropy with the same arguments, from its lse (softmax: exp(l - lse)). dloss: the gradient that arrives at the loss (of its shape; ones if None).
     dw has w's storage layout."""
     return tuple(_linear_ce("linear_cross_entropy_grad", x, w, targets, ignore_index, reduction, dloss, lse, False, True))
 
@@ -570,7 +570,8 @@ def grad_norm(grads) -> torch.Tensor:
 
 def clip_grad_norm(grads, limit: float, *, eps: float = 1e-6, out=None) -> torch.Tensor:
     """Scales the tensors (each listed once) by min(1, limit / (norm + eps)), in place or into the tensors `out`, and returns their norm from before
-    (grad_norm). A norm of NaN makes every value NaN, an infinite one zeros, and NaN of what was infinite."""
+    (grad_norm). A norm of NaN makes every value NaN, an infinite one zeros, and NaN of what was infinite (0 / 0 and infinity over infinity: NaN). What is
+    written counts as changed in place, for autograd too."""
     if not (limit >= 0 and eps >= 0):
         raise ValueError("clip_grad_norm: limit and eps are at least 0")
     grads, out, limit, eps = list(grads), None if out is None else list(out), float(limit), float(eps)
