@@ -465,6 +465,8 @@ def _linear_ce(what, x, w, targets, ignore_index, reduction, dloss, lse, forward
     d.x, d.w, d.targets = x.data_ptr(), stored.data_ptr(), targets.data_ptr()
     d.dtype, d.target_dtype, d.w_layout, d.reduction = _dt(x), _dt(targets), layout, _REDUCTION[reduction]
     if ignore_index is not None:
+        if not -2 ** 63 <= ignore_index < 2 ** 63:
+            raise ValueError(f"{what}: ignore_index is a number of 64 bits")
         d.has_ignore, d.ignore_index = 1, ignore_index
     each = lead if reduction == "none" else ()
     f32 = dict(dtype=torch.float32, device=x.device)

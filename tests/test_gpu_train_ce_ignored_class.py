@@ -80,3 +80,11 @@ def test_a_class_is_ignored_only_where_it_is_asked_for(dtype):
     loss, dx, dw = T.linear_cross_entropy_with_grad(x, w, t, ignore_index=0)
     assert float(loss) == 0 and not bool(dx.any()) and not bool(dw.any())
     T.device_status()
+
+
+def test_an_index_of_more_than_64_bits():
+    from mimir_b200 import tensor as T
+    x, w, t = inputs(16, 32, 50, BF16, False)
+    for index in (2 ** 64, 2 ** 63, -2 ** 63 - 1):          # (2^64 would be class 0 in the bits that are left)
+        with pytest.raises(ValueError, match="64 bits"):
+            T.linear_cross_entropy(x, w, t, ignore_index=index)
