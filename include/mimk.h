@@ -417,6 +417,86 @@ int mimk_grad_norm(const void* const* tensors, const int64_t* lengths, const int
 int mimk_clip_grads(const void* const* tensors, void* const* out, const int64_t* lengths, const int32_t* dtypes, int64_t count, float limit, float eps,
                     float* norm, void* workspace, uint64_t workspace_bytes, void* stream);
 
+/* Token embedding, F32 or BF16, table and result of either type: out[i] = scale * table[ids[i]], rounded once, and its gradient
+ * dtable[c] = sum over the i with ids[i] = c of scale * dy[i]: all rows written, those of classes that no position names with zeros; with `add` the sums are
+ * added to what dtable holds, and rows of other classes are left alone.
+ * has_ignore: a position whose id is ignore_index, a class or not, has no token: its row of the result is zeros, and its row of dy is not read.
+ * Any other id outside [0, v) is recorded (mimk_device_status: MIMK_E_SHAPE); its row of the result is NaN, and nothing of it enters dtable.
+ * Sums are f32, over positions in rising order in groups that the extents and ids alone decide, rounded once: equal descriptors and ids give equal bits. No
+ * operand overlaps a result. Extents below 2^31 (v d may be more), rows are dense. Workspace as above, of embedding_grad only: 8 bytes per class and position
+ * and what long runs of one class leave between launches. */
+typedef struct mimk_embedding_desc {
+    int64_t n, d, v;   /* positions, features, classes */
+    const void* table; /* [v, d] of dtype */
+    const void* ids;   /* [n] of id_dtype, I32 or I64 */
+    void* out;         /* [n, d] of out_dtype */
+    const void* dy;    /* grad: [n, d] of dtype */
+    void* dtable;      /* grad: [v, d] of out_dtype */
+    void* workspace;
+    uint64_t workspace_bytes;
+    int64_t ignore_index;
+    float scale;
+    int32_t dtype, out_dtype, id_dtype, has_ignore, add;
+} mimk_embedding_desc;
+int mimk_embedding(const mimk_embedding_desc* desc, void* stream);
+int mimk_embedding_grad_workspace(const mimk_embedding_desc* desc, uint64_t* bytes);
+int mimk_embedding_grad(const mimk_embedding_desc* desc, void* stream);
+
+/* From one block of a model to the next, in one pass, and its gradients. With N(v) = v / sqrt(mean(v^2) + eps) over the d features of a row:
+ *   u = N(h) * post_gamma (u = h where post_gamma is NULL);  r_out = residual_scale * r + branch_scale * gate * u;  x = N(r_out) * gamma
+ *   bwd: from dr_out (NULL: zeros) and dx: dr, dh, dgamma, dpost_gamma, dgate of whichever operands there are.
+ * h NULL: no block before, x = N(r) * gamma; gate, post_gamma and r_out are NULL then and both scales 1. gamma NULL: no norm after, x and dx are NULL. gate NULL: ones;
+ * otherwise [ceil(n / gate_rows), d], each row of it for gate_rows rows in turn, as is dgate. r, r_out, dr and dr_out are of stream_dtype, h, x, dh and dx of block_dtype: F32
+ * and F32, F32 and BF16, or BF16 and BF16; gamma, post_gamma, gate and their gradients each F32 or BF16.
+ * x is of r_out before its rounding. kept: fwd leaves what bwd takes of each row's sums, 2 n f32 (NULL: nothing is left); bwd computes r_out over again from r and h.
+ * All sums are f32; gradients of gamma, post_gamma and gate are summed over rows in an order that the extents alone decide: equal descriptors give equal bits.
+ * r_out may be r, and dr may be dr_out; no other result overlaps an operand. d <= 32768, n < 2^31. Workspace as above, of bwd only. */
+typedef struct mimk_residual_rmsnorm_desc {
+    int64_t n, d, gate_rows;
+    const void* r; /* [n, d], so h, r_out, x and their gradients */
+    const void* h;
+    const void* gamma; /* [d], so post_gamma */
+    const void* post_gamma;
+    const void* gate;
+    void* r_out;
+    void* x;
+    float* kept;
+    const void* dr_out;
+    const void* dx;
+    void* dr;
+    void* dh;
+    void* dgamma;
+    void* dpost_gamma;
+    void* dgate;
+    void* workspace;
+    uint64_t workspace_bytes;
+    float eps, residual_scale, branch_scale;
+    int32_t stream_dtype, block_dtype, gamma_dtype, post_gamma_dtype, gate_dtype;
+} mimk_residual_rmsnorm_desc;
+int mimk_residual_rmsnorm_fwd(const mimk_residual_rmsnorm_desc* desc, void* stream);
+int mimk_residual_rmsnorm_workspace(const mimk_residual_rmsnorm_desc* desc, uint64_t* bytes);
+int mimk_residual_rmsnorm_bwd(const mimk_residual_rmsnorm_desc* desc, void* stream);
+
+/* Matrices with their singular values brought near 1 (an optimiser's orthogonalised update) by Newton-Schulz steps: X = x / (|x| + eps), |x| the 2-norm of all
+ * values; for each step (p, q, r): A = X X^T (X^T X where m > n), X <- p X + (q A + r A^2) X (X (q A + r A^2)); out = scale * X as BF16.
+ * x: F32 or BF16. Operands of the products are rounded to 11 significant bits (f16 with powers of two as factors), except the diagonals of A and of q A + r A^2, which
+ * are f32; p X is added in f32 from an X of 22 bits; sums are f32, |x| is f64. What X has below 2^-32 is lost. A matrix with a value that is not finite comes out NaN, one of zeros zeros.
+ * The steps must keep singular values from 0 to 1 within 4 (MIMK_E_UNSUPPORTED otherwise): the largest value of |p s + q s^3 + r s^5| is followed from step to step.
+ * Equal descriptors give equal bits, a matrix the same whatever others are in the batch. The arrays are on the host and are read before the call returns. No result overlaps an operand.
+ * Workspace as above: 8 bytes per value of X, 4 per value of A, of as many matrices as take about 1 GiB. */
+typedef struct mimk_orthogonalize_desc {
+    int64_t batch, m, n;
+    const void* const* x;      /* batch matrices [m, n] of dtype, dense */
+    void* out;                 /* [batch, m, n] BF16 */
+    const float* coefficients; /* [steps][3]: p, q, r */
+    void* workspace;
+    uint64_t workspace_bytes;
+    float eps, scale;
+    int32_t steps, dtype;
+} mimk_orthogonalize_desc;
+int mimk_orthogonalize_workspace(const mimk_orthogonalize_desc* desc, uint64_t* bytes);
+int mimk_orthogonalize(const mimk_orthogonalize_desc* desc, void* stream);
+
 /* ---- the generic operation ------------------------------------------------------------------------------
  * out[map_out(o)] = post(fold_r f(acc, (in_i[maps_i(o, r)])_i), (post_in_j[post_maps_j(map_out(o))])_j)
  * over the loop vector (o..., r...) with bounds `sr`: the leading `ro` loops are the output loops, the trailing

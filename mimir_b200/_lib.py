@@ -26,7 +26,8 @@ SYMBOLS = (
     "mimk_status_str", "mimk_abi_version", "mimk_last_cuda_error", "mimk_device_check", "mimk_device_status", "mimk_selftest_wait_expiry",
     "mimk_gemm", "mimk_gemm_flat", "mimk_gemm_gather", "mimk_gemm_reduce_scatter", "mimk_gemm_kpanels", "mimk_reduce", "mimk_reduce_fused", "mimk_reduce_plan", "mimk_reduce_tiles", "mimk_reduce_static", "mimk_softmax", "mimk_rmsnorm", "mimk_softmax_rmsnorm", "mimk_map", "mimk_map_t",
     "mimk_splat", "mimk_select", "mimk_generate_affine", "mimk_gather", "mimk_scatter", "mimk_attn_fwd", "mimk_conv", "mimk_conv_laid_out", "mimk_mlp_gated", "mimk_mlp_gated_train_sizes", "mimk_mlp_gated_fwd", "mimk_mlp_gated_bwd", "mimk_linear_ce_workspace", "mimk_linear_ce_fwd", "mimk_linear_ce_bwd", "mimk_linear_ce_fwd_bwd",
-    "mimk_clip_grads_workspace", "mimk_grad_norm", "mimk_clip_grads", "mimk_map_reduce_post", "mimk_mrp_classify", "mimk_mrp_cell_kernel", "mimk_program_classify", "mimk_program_run", "mimk_chain_order", "mimk_chain_cost",
+    "mimk_clip_grads_workspace", "mimk_grad_norm", "mimk_clip_grads", "mimk_embedding", "mimk_embedding_grad_workspace", "mimk_embedding_grad",
+    "mimk_residual_rmsnorm_fwd", "mimk_residual_rmsnorm_workspace", "mimk_residual_rmsnorm_bwd", "mimk_orthogonalize_workspace", "mimk_orthogonalize", "mimk_map_reduce_post", "mimk_mrp_classify", "mimk_mrp_cell_kernel", "mimk_program_classify", "mimk_program_run", "mimk_chain_order", "mimk_chain_cost",
     "mimk_host_rows", "mimk_host_rows_pair", "mimk_host_gemm", "mimk_host_attn_fwd", "mimk_host_mlp_gated", "mimk_host_map_reduce_post", "mimk_host_register",
     "mimk_host_unregister", "mimk_host_release",
 )
@@ -101,6 +102,31 @@ class LinearCeDesc(C.Structure):
         ("loss", C.c_void_p), ("lse", C.c_void_p), ("dx", C.c_void_p), ("dw", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64),
         ("ignore_index", C.c_int64), ("dtype", C.c_int32), ("target_dtype", C.c_int32), ("w_layout", C.c_int32), ("reduction", C.c_int32),
         ("has_ignore", C.c_int32),
+    ]
+
+
+class EmbeddingDesc(C.Structure):
+    _fields_ = [
+        ("n", C.c_int64), ("d", C.c_int64), ("v", C.c_int64), ("table", C.c_void_p), ("ids", C.c_void_p), ("out", C.c_void_p), ("dy", C.c_void_p),
+        ("dtable", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64), ("ignore_index", C.c_int64), ("scale", C.c_float),
+        ("dtype", C.c_int32), ("out_dtype", C.c_int32), ("id_dtype", C.c_int32), ("has_ignore", C.c_int32), ("add", C.c_int32),
+    ]
+
+
+class ResidualRmsnormDesc(C.Structure):
+    _fields_ = [
+        ("n", C.c_int64), ("d", C.c_int64), ("gate_rows", C.c_int64), ("r", C.c_void_p), ("h", C.c_void_p), ("gamma", C.c_void_p), ("post_gamma", C.c_void_p),
+        ("gate", C.c_void_p), ("r_out", C.c_void_p), ("x", C.c_void_p), ("kept", C.c_void_p), ("dr_out", C.c_void_p), ("dx", C.c_void_p), ("dr", C.c_void_p),
+        ("dh", C.c_void_p), ("dgamma", C.c_void_p), ("dpost_gamma", C.c_void_p), ("dgate", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64),
+        ("eps", C.c_float), ("residual_scale", C.c_float), ("branch_scale", C.c_float), ("stream_dtype", C.c_int32), ("block_dtype", C.c_int32),
+        ("gamma_dtype", C.c_int32), ("post_gamma_dtype", C.c_int32), ("gate_dtype", C.c_int32),
+    ]
+
+
+class OrthogonalizeDesc(C.Structure):
+    _fields_ = [
+        ("batch", C.c_int64), ("m", C.c_int64), ("n", C.c_int64), ("x", C.POINTER(C.c_void_p)), ("out", C.c_void_p), ("coefficients", C.POINTER(C.c_float)),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64), ("eps", C.c_float), ("scale", C.c_float), ("steps", C.c_int32), ("dtype", C.c_int32),
     ]
 
 
@@ -198,6 +224,12 @@ def lib() -> C.CDLL:
         L.mimk_clip_grads_workspace.argtypes = [i64, u64p]
         L.mimk_grad_norm.argtypes = [vpp, i64p, i32p, i64, vp, vp, C.c_uint64, vp]
         L.mimk_clip_grads.argtypes = [vpp, vpp, i64p, i32p, i64, cf, cf, vp, vp, C.c_uint64, vp]
+        L.mimk_embedding.argtypes = L.mimk_embedding_grad.argtypes = [C.POINTER(EmbeddingDesc), vp]
+        L.mimk_embedding_grad_workspace.argtypes = [C.POINTER(EmbeddingDesc), u64p]
+        L.mimk_residual_rmsnorm_fwd.argtypes = L.mimk_residual_rmsnorm_bwd.argtypes = [C.POINTER(ResidualRmsnormDesc), vp]
+        L.mimk_residual_rmsnorm_workspace.argtypes = [C.POINTER(ResidualRmsnormDesc), u64p]
+        L.mimk_orthogonalize.argtypes = [C.POINTER(OrthogonalizeDesc), vp]
+        L.mimk_orthogonalize_workspace.argtypes = [C.POINTER(OrthogonalizeDesc), u64p]
         L.mimk_map_reduce_post.argtypes = [C.POINTER(MrpDesc), vp]
         L.mimk_mrp_classify.argtypes = [C.POINTER(MrpDesc)]
         L.mimk_mrp_cell_kernel.argtypes = [C.POINTER(MrpDesc), C.POINTER(C.c_int32)]

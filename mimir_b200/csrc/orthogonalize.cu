@@ -1,0 +1,678 @@
+// Orthogonalised updates by Newton-Schulz products. X = x / (|x| + eps); for each step (p, q, r), with k the smaller extent of X and A [k, k]:
+//   A = X X^T (X^T X where X is taller than wide),  B = q A + r A^2,  X <- p X + B X (X B)
+// Three products a step on the tensor cores. A and B are symmetric: the tiles on and below the diagonal are multiplied, and written twice.
+//
+// Rounding. Singular values grow by p a step while they are small, and what is rounded away of X grows with them: with all operands in bf16 the result of
+// a matrix with falling singular values is off by 5e-2 to 3e-1. Here operands are f16 (11 bits, where bf16 has 8) times powers of two that keep
+// their largest possible value below 2^15; p X is added from an X of two f16 (22 bits), so that rounding one operand of B X does not enter X itself;
+// and the diagonals of A and B, near which the values of most matrices lie, are kept in f32 and out of the products:
+//   with A = O + diag(d):  A^2 = O O + (d_i + d_j) O_ij + diag(d_i^2),  B X = (B - diag(e)) X + diag(e) X
+// Against 64 bits the result, before its own rounding to bf16 (1.66e-3), is off by 2e-4 to 1e-3; without the diagonals' part a random matrix by 2.7e-3, without the
+// second f16 of X one with falling values by 6e-3 to 3e-2.
+// What bounds it: the tensor cores; with few rows, three dependent launches a step.
+#include <math.h>
+
+#include <cuda_fp16.h>
+
+#include "elements.cuh"
+#include "sm100_pair.cuh"
+#include "train_common.cuh"
+
+namespace mimk {
+
+namespace {
+
+using namespace sm100;
+
+enum Product {
+    GRAM,    // A from X: its values off the diagonal as f16, the diagonal as f32
+    SQUARE,  // B from A, the same way
+    APPLY,   // the next X from B and X
+};
+constexpr int BM = 128, BK = 64, OPERAND = BM * BK * 2, STAGE = 2 * OPERAND;
+constexpr int FIRST = 3, WARPS = 4, THREADS = (FIRST + WARPS) * 32;  // a warp for each operand's loads and one for the multiplications, then the epilogue's
+constexpr int SLOT = 4096;  // a [32 rows x 128 bytes] tile of an epilogue warp
+constexpr int GROUP_M = 8;
+constexpr float SX = 256.f, LOW = 2048.f;  // factors of X, and of the second f16 of a value against the first
+
+template <int KIND>
+struct Shape {
+    static constexpr int SLOTS  = KIND == APPLY ? 16 : 0;  // per warp: two sets of a first and a second f16
+    static constexpr int STAGES = KIND == APPLY ? 4 : 6;
+    static constexpr int SMEM   = STAGES * STAGE + SLOTS * SLOT + 1024 + 256;
+};
+
+struct Maps {
+    CUtensorMap left, right, hi, lo, out_hi, out_lo;  // the last four: tiles of 32 rows of X, APPLY
+};
+struct Args {
+    int rows, cols, batch;  // of the result
+    int tiles_m, tiles_n, kb;
+    int a_mn, b_mn;  // operand stored with its M (N) axis contiguous
+    int pitch;       // of A and B
+    int last, tall;  // APPLY: the result is BF16; e goes with columns
+    const __half* in;  // SQUARE: A
+    __half* out;       // GRAM: A, SQUARE: B
+    const float* diag_in;  // SQUARE: d, APPLY: e
+    float* diag_out;
+    // GRAM: A = acc * f[0], times f[1] as f16. SQUARE: O O = acc * f[0], A = in * f[1], q = f[2], r = f[3], times f[4] as f16.
+    // APPLY: SX X' = (f[0] + e) SX X + acc * f[1]; the result times f[2]
+    float f[5];
+    int* status;
+};
+
+struct Bars {
+    uint64_t full[6], empty[6], acc_full[2], acc_empty[2], in[2 * WARPS];
+    uint32_t tmem_base;
+    int abort_flag;
+};
+static_assert(sizeof(Bars) <= 256, "barrier block too large");
+
+struct Tile {
+    int z, m, n;
+};
+template <int KIND, int SIDE>
+__device__ __forceinline__ bool tile_at(const Args& g, int index, Tile& t) {
+    const int per = KIND == APPLY ? g.tiles_m * g.tiles_n : g.tiles_m * (g.tiles_m + 1) / 2;
+    t.z = index / per;
+    if (t.z >= g.batch) return false;
+    const int i = index - t.z * per;
+    if (KIND != APPLY) {
+        // row a of the triangle holds tiles a (a + 1) / 2 and on
+        int a = int((sqrtf(8.f * float(i) + 1.f) - 1.f) * 0.5f);
+        while (a * (a + 1) / 2 > i) --a;
+        while ((a + 1) * (a + 2) / 2 <= i) ++a;
+        t.m = a * SIDE, t.n = (i - a * (a + 1) / 2) * SIDE;
+    } else {
+        const int per_group = GROUP_M * g.tiles_n, group = i / per_group, in_group = i - group * per_group;
+        const int size = min(g.tiles_m - group * GROUP_M, GROUP_M), column = in_group / size;
+        t.m = (group * GROUP_M + in_group - column * size) * SIDE, t.n = column * SIDE;
+    }
+    return true;
+}
+
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+    const __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ float2 unpack_f16(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
+// 16-byte piece `piece` of this lane's row of a 128-byte-swizzled slot
+__device__ __forceinline__ uint32_t piece_at(uint32_t slot, int lane, int piece) { return slot + lane * 128 + ((uint32_t(piece) ^ uint32_t(lane & 7)) << 4); }
+__device__ __forceinline__ uint4 ld_shared(uint32_t a) {
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+    return v;
+}
+__device__ __forceinline__ void st_shared(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+
+// SMS: 2, a tile of 256 x 256 on a pair of SMs, or 1, one of 128 x 128 on one. A CTA stages 128 rows of the left operand and 128 columns of the right one.
+template <int KIND, int SMS>
+__device__ __forceinline__ void product(const Maps& maps, const Args& g) {
+    using S = Shape<KIND>;
+    constexpr int STAGES = S::STAGES, SIDE = BM * SMS, COLUMNS = SIDE;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t raw_addr = smem_u32(smem_raw), tile_base = (raw_addr + 1023u) & ~1023u;
+    Bars* bars = reinterpret_cast<Bars*>(smem_raw + (tile_base - raw_addr) + STAGES * STAGE + S::SLOTS * SLOT);
+    volatile int* abort_flag = &bars->abort_flag;
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = SMS == 2 ? cluster_ctarank() : 0;
+    const int first = blockIdx.x / SMS, step = gridDim.x / SMS;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; ++s) {
+            mbar_init(smem_u32(&bars->full[s]), 1);
+            mbar_init(smem_u32(&bars->empty[s]), 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(smem_u32(&bars->acc_full[b]), 1);
+            mbar_init(smem_u32(&bars->acc_empty[b]), SMS * WARPS * 32);
+        }
+        for (int w = 0; w < 2 * WARPS; ++w) mbar_init(smem_u32(&bars->in[w]), 1);
+        bars->abort_flag = 0;
+        fence_barrier_init();
+    }
+    if (warp == 1) {
+        if constexpr (SMS == 2) {
+            tmem_alloc_pair(smem_u32(&bars->tmem_base), 2 * COLUMNS);
+            tmem_relinquish_pair();
+        } else {
+            tmem_alloc(smem_u32(&bars->tmem_base), 2 * COLUMNS);
+            tmem_relinquish();
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if constexpr (SMS == 2) cluster_sync();
+    tc_fence_after();
+    const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(&bars->tmem_base);
+    after_previous();
+
+    Tile t;
+    if (warp == 0 || warp == 2) {
+        // ---------------- loads: warp 0 the left operand, warp 2 the right one ----------------
+        if (lane == 0) {
+            const bool left  = warp == 0;
+            const int mn     = left ? g.a_mn : g.b_mn;
+            const auto* map  = left ? &maps.left : &maps.right;
+            uint32_t stage = 0, phase = 0;
+            bool ok = true;
+            for (int index = first; ok && tile_at<KIND, SIDE>(g, index, t); index += step) {
+                const int at = (left ? t.m : t.n) + int(rank) * BM;
+                for (int kb = 0; kb < g.kb; ++kb) {
+                    if (!(ok = mbar_wait(smem_u32(&bars->empty[stage]), phase ^ 1u, abort_flag))) break;
+                    const uint32_t to = tile_base + stage * STAGE + (left ? 0 : OPERAND), full = smem_u32(&bars->full[stage]);
+                    const int k = kb * BK;
+                    if (left && rank == 0) mbar_expect_tx(full, SMS * STAGE);
+                    if constexpr (SMS == 2) {
+                        const uint32_t full_even = map_to_cta(full, 0);
+                        if (!mn) {
+                            tma_load_3d_pair(to, map, k, at, t.z, full_even);
+                        } else {
+                            tma_load_3d_pair(to, map, at, k, t.z, full_even);
+                            tma_load_3d_pair(to + BK * 128, map, at + 64, k, t.z, full_even);
+                        }
+                    } else {
+                        if (!mn) {
+                            tma_load_3d(to, map, k, at, t.z, full);
+                        } else {
+                            tma_load_3d(to, map, at, k, t.z, full);
+                            tma_load_3d(to + BK * 128, map, at + 64, k, t.z, full);
+                        }
+                    }
+                    if (++stage == STAGES) stage = 0, phase ^= 1u;
+                }
+            }
+        }
+    } else if (warp == 1) {
+        // ---------------- multiplications (of a pair: the even CTA) ----------------
+        if (lane == 0 && rank == 0) {
+            uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0;
+            bool ok = true;
+            const uint64_t high  = smem_desc_sw128(0, 0, 1024);
+            const uint32_t idesc = idesc_f16_f32(SIDE, SIDE, g.a_mn, g.b_mn);
+            // a descriptor's low word is the address >> 4 with the leading offset >> 4 above it, its high word is the same for all
+            const uint32_t a_step = g.a_mn ? 2048 >> 4 : 32 >> 4, b_step = g.b_mn ? 2048 >> 4 : 32 >> 4;
+            const uint32_t a_low = (g.a_mn ? BK * 128 >> 4 : 1) << 16, b_low = ((g.b_mn ? BK * 128 >> 4 : 1) << 16) + (OPERAND >> 4);
+            for (int index = first; ok && tile_at<KIND, SIDE>(g, index, t); index += step) {
+                if (!(ok = mbar_wait(smem_u32(&bars->acc_empty[acc]), acc_phase ^ 1u, abort_flag))) break;
+                tc_fence_after();
+                for (int kb = 0; kb < g.kb; ++kb) {
+                    if (!(ok = mbar_wait(smem_u32(&bars->full[stage]), phase, abort_flag))) break;
+                    tc_fence_after();
+                    const uint32_t at = (tile_base + stage * STAGE) >> 4;
+#pragma unroll
+                    for (int k = 0; k < BK / 16; ++k) {
+                        const uint64_t a = high | (at + a_low + k * a_step), b = high | (at + b_low + k * b_step);
+                        if constexpr (SMS == 2) mma_f16_ss_pair(tmem_base + acc * COLUMNS, a, b, idesc, kb > 0 || k > 0);
+                        else mma_f16_ss(tmem_base + acc * COLUMNS, a, b, idesc, kb > 0 || k > 0);
+                    }
+                    if constexpr (SMS == 2) mma_commit_pair(smem_u32(&bars->empty[stage]));
+                    else mma_commit(smem_u32(&bars->empty[stage]));
+                    if (++stage == STAGES) stage = 0, phase ^= 1u;
+                }
+                if (!ok) break;
+                if constexpr (SMS == 2) mma_commit_pair(smem_u32(&bars->acc_full[acc]));
+                else mma_commit(smem_u32(&bars->acc_full[acc]));
+                if (++acc == 2) acc = 0, acc_phase ^= 1u;
+            }
+        }
+    } else {
+        // ---------------- epilogue: 32 rows for each warp, one per lane ----------------
+        const int quarter = warp & 3;
+        const uint32_t slots = tile_base + STAGES * STAGE + quarter * (S::SLOTS / WARPS) * SLOT, in_bar = smem_u32(&bars->in[quarter * 2]);
+        uint32_t acc = 0, acc_phase = 0, in_phase = 0;
+        bool ok   = true;
+        bool have = tile_at<KIND, SIDE>(g, first, t);
+        // APPLY: 64 columns of X, in two sets of slots in turn
+        auto request = [&](int c) {
+            const int row = t.m + int(rank) * BM + quarter * 32;
+            if (KIND == APPLY && lane == 0 && row < g.rows && c < SIDE && t.n + c < g.cols) {
+                const uint32_t set = c >> 6 & 1, to = slots + set * 2 * SLOT;
+                mbar_expect_tx(in_bar + set * 8, 2 * SLOT);
+                tma_load_3d(to, &maps.hi, t.n + c, row, t.z, in_bar + set * 8);
+                tma_load_3d(to + SLOT, &maps.lo, t.n + c, row, t.z, in_bar + set * 8);
+            }
+        };
+        if (have) request(0), request(64);
+        for (int index = first; have && ok;) {
+            const int row0 = t.m + int(rank) * BM + quarter * 32, row = row0 + lane, width = min(SIDE, g.cols - t.n);
+            if (!(ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&bars->acc_full[acc]), acc_phase, abort_flag)))) break;
+            tc_fence_after();
+            const uint32_t from = tmem_base + acc * COLUMNS + (uint32_t(quarter * 32) << 16);
+            const uint32_t acc_empty = SMS == 2 ? map_to_cta(smem_u32(&bars->acc_empty[acc]), 0) : smem_u32(&bars->acc_empty[acc]);
+            if (++acc == 2) acc = 0, acc_phase ^= 1u;
+            auto release = [&] {
+                tc_fence_before();
+                if constexpr (SMS == 2) mbar_arrive_cluster(acc_empty);
+                else mbar_arrive(acc_empty);
+            };
+            if (row0 >= g.rows) {
+                release();
+            } else if constexpr (KIND != APPLY) {
+                const int64_t matrix = int64_t(t.z) * g.rows;  // (rows of the matrices before this one)
+                const bool there = row < g.rows;
+                const float d    = KIND == SQUARE && there ? g.diag_in[matrix + row] : 0.f;
+#pragma unroll 1
+                for (int c = 0; c < width; c += 32) {
+                    uint32_t raw[32];
+                    tmem_ld_32x32(from + c, raw);
+                    uint16_t a[32];
+                    if constexpr (KIND == SQUARE) {
+                        // A's value (row, column) is also its value (column, row), which lanes read side by side
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) {
+                            const int column = t.n + c + i;
+                            a[i] = there && column < g.cols ? *reinterpret_cast<const uint16_t*>(g.in + (matrix + column) * g.pitch + row) : uint16_t(0);
+                        }
+                    }
+                    tmem_ld_wait();
+                    if (c + 32 >= width) release();
+                    float v[32];
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        const int column = t.n + c + i;
+                        v[i] = __uint_as_float(raw[i]) * g.f[0];
+                        if constexpr (KIND == SQUARE) {
+                            const bool inside = column < g.cols;
+                            const float dj = inside ? g.diag_in[matrix + column] : 0.f, o = __half2float(__ushort_as_half(a[i])) * g.f[1];
+                            v[i] = row == column ? g.f[2] * d + g.f[3] * fmaf(d, d, v[i]) : g.f[2] * o + g.f[3] * fmaf(d + dj, o, v[i]);
+                        }
+                        if (row == column) {
+                            if (there) g.diag_out[matrix + row] = v[i];
+                            v[i] = 0.f;
+                        }
+                        v[i] *= KIND == GRAM ? g.f[1] : g.f[4];
+                    }
+                    __half* out = g.out + matrix * g.pitch;
+                    if (there) {
+#pragma unroll
+                        for (int i = 0; i < 32; i += 8)
+                            if (t.n + c + i < g.cols)
+                                *reinterpret_cast<uint4*>(out + int64_t(row) * g.pitch + t.n + c + i) =
+                                    make_uint4(pack_f16(v[i], v[i + 1]), pack_f16(v[i + 2], v[i + 3]), pack_f16(v[i + 4], v[i + 5]), pack_f16(v[i + 6], v[i + 7]));
+                        if (t.m != t.n) {
+#pragma unroll
+                            for (int i = 0; i < 32; ++i)
+                                if (t.n + c + i < g.cols) out[int64_t(t.n + c + i) * g.pitch + row] = __float2half_rn(v[i]);
+                        }
+                    }
+                }
+            } else {
+                const int64_t matrix = int64_t(t.z) * (g.tall ? g.cols : g.rows);
+                const float e = !g.tall && row < g.rows ? g.diag_in[matrix + row] : 0.f;
+#pragma unroll 1
+                for (int c = 0; c < width; c += 64) {
+                    const uint32_t set = c >> 6 & 1, slot = slots + set * 2 * SLOT;
+                    if (!(ok = __all_sync(0xffffffffu, mbar_wait(in_bar + set * 8, in_phase >> set & 1u, abort_flag)))) break;
+                    in_phase ^= 1u << set;
+#pragma unroll
+                    for (int half = 0; half < 64; half += 32) {
+                        uint32_t raw[32];
+                        tmem_ld_32x32(from + c + half, raw);
+                        float v[32];
+#pragma unroll
+                        for (int i = 0; i < 32; i += 8) {
+                            const uint4 hi = ld_shared(piece_at(slot, lane, (half + i) >> 3)), lo = ld_shared(piece_at(slot + SLOT, lane, (half + i) >> 3));
+                            const uint32_t h[4] = {hi.x, hi.y, hi.z, hi.w}, l[4] = {lo.x, lo.y, lo.z, lo.w};
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                const float2 a = unpack_f16(h[j]), b = unpack_f16(l[j]);
+                                v[i + 2 * j] = fmaf(b.x, 1.f / LOW, a.x), v[i + 2 * j + 1] = fmaf(b.y, 1.f / LOW, a.y);
+                            }
+                        }
+                        tmem_ld_wait();
+                        if (c + 64 >= width && half) release();
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) {
+                            float by = g.f[0] + e;
+                            if (g.tall) by += t.n + c + half + i < g.cols ? g.diag_in[matrix + t.n + c + half + i] : 0.f;
+                            v[i] = fmaf(by, v[i], __uint_as_float(raw[i]) * g.f[1]);
+                        }
+#pragma unroll
+                        for (int i = 0; i < 32; i += 8) {
+                            uint32_t h[4], l[4];
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                const float x = v[i + 2 * j], y = v[i + 2 * j + 1];
+                                if (g.last) {
+                                    h[j] = pack_bf16x2(x * g.f[2], y * g.f[2]);
+                                } else {
+                                    h[j] = pack_f16(x, y);
+                                    const float2 r = unpack_f16(h[j]);
+                                    l[j] = pack_f16((x - r.x) * LOW, (y - r.y) * LOW);
+                                }
+                            }
+                            st_shared(piece_at(slot, lane, (half + i) >> 3), h[0], h[1], h[2], h[3]);
+                            if (!g.last) st_shared(piece_at(slot + SLOT, lane, (half + i) >> 3), l[0], l[1], l[2], l[3]);
+                        }
+                    }
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) {
+                        tma_store_3d(&maps.out_hi, slot, t.n + c, row0, t.z);
+                        if (!g.last) tma_store_3d(&maps.out_lo, slot + SLOT, t.n + c, row0, t.z);
+                        bulk_commit();
+                        bulk_wait_read_0();
+                    }
+                    request(c + 128);
+                }
+                if (!ok) break;
+            }
+            index += step;
+            have = tile_at<KIND, SIDE>(g, index, t);
+            if (have) request(0), request(64);
+        }
+        if (KIND == APPLY && lane == 0) bulk_wait_all();
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    if constexpr (SMS == 2) cluster_sync();  // neither CTA may release shared or tensor memory while the other can still touch it
+    if (warp == 1) {
+        __syncwarp();
+        tc_fence_after();
+        if constexpr (SMS == 2) tmem_dealloc_pair(tmem_base, 2 * COLUMNS);
+        else tmem_dealloc(tmem_base, 2 * COLUMNS);
+    }
+    if (threadIdx.x == 0 && *abort_flag) *g.status = MIMK_E_DEVICE_WAIT;
+}
+template <int KIND>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args g) {
+    product<KIND, 2>(maps, g);
+}
+template <int KIND>
+__global__ void __launch_bounds__(THREADS, 1) single_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args g) {
+    product<KIND, 1>(maps, g);
+}
+
+// ---- x to X ----------------------------------------------------------------------------------------------------------------------
+constexpr int TABLE = 1024;       // matrices of one launch
+constexpr int CHUNK = 1 << 16;    // values that one block squares
+constexpr int PREPARE = 256;
+
+struct Matrices {
+    const void* x[TABLE];
+};
+
+__device__ __forceinline__ double block_total(double v) {
+    __shared__ double part[PREPARE / 32];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = 0;
+#pragma unroll
+    for (int w = 0; w < PREPARE / 32; ++w) v += part[w];
+    return v;
+}
+// Eight squares in f32, or in f64 where they overflow or all but vanish
+template <int VEC>
+__device__ __forceinline__ double squares(const float (&v)[VEC]) {
+    float s = 0.f;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) s = fmaf(v[j], v[j], s);
+    if (s > 1e-25f && s < INFINITY) return double(s);
+    double d = 0;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) d += double(v[j]) * double(v[j]);
+    return d;
+}
+template <class T, int VEC>
+__global__ void __launch_bounds__(PREPARE) squares_kernel(const __grid_constant__ Matrices all, int64_t count, double* sums) {
+    after_previous();
+    const T* x = static_cast<const T*>(all.x[blockIdx.y]);
+    for (int64_t chunk = blockIdx.x; chunk * CHUNK < count; chunk += gridDim.x) {
+        const int64_t end = min(count, (chunk + 1) * CHUNK);
+        double sum        = 0;
+#pragma unroll 4
+        for (int64_t i = chunk * CHUNK + threadIdx.x * VEC; i < end; i += PREPARE * VEC) {
+            Run<T, VEC> run;
+            float v[VEC];
+            run.load(x + i), run.get(v);
+            sum += squares(v);
+        }
+        sum = block_total(sum);
+        if (threadIdx.x == 0) sums[blockIdx.y * ((count + CHUNK - 1) / CHUNK) + chunk] = sum;
+    }
+}
+// X times SX as two f16: rows of `pitch`. Every block adds the chunks' sums up itself, in the same order.
+template <class T, int VEC>
+__global__ void __launch_bounds__(PREPARE) prepare_kernel(const __grid_constant__ Matrices all, int rows, int cols, int pitch, const double* sums, float eps, __half* hi, __half* lo) {
+    after_previous();
+    const int64_t count = int64_t(rows) * cols;
+    const int chunks    = int((count + CHUNK - 1) / CHUNK);
+    double total        = 0;
+    for (int i = threadIdx.x; i < chunks; i += PREPARE) total += sums[blockIdx.y * chunks + i];
+    const double norm = sqrt(block_total(total)), by = isfinite(norm) ? 1.0 / (norm + double(eps)) : double(NAN);
+    // in two factors, as one may be beyond f32
+    int power           = 0;
+    const double lead   = isfinite(by) ? frexp(by, &power) : by;
+    const float first   = ldexpf(1.f, power / 2), second = float(ldexp(lead, power - power / 2)) * SX;
+    const T* x          = static_cast<const T*>(all.x[blockIdx.y]);
+    const int64_t base  = int64_t(blockIdx.y) * rows * pitch;
+    const int units     = (cols + VEC - 1) / VEC;  // of a row
+    for (int row = blockIdx.x; row < rows; row += gridDim.x)
+#pragma unroll 2
+        for (int u = threadIdx.x; u < units; u += PREPARE) {
+            Run<T, VEC> run;
+            float v[VEC];
+            run.load(x + int64_t(row) * cols + u * VEC), run.get(v);
+            __half h[VEC], l[VEC];
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                v[j] = v[j] * first * second;
+                h[j] = __float2half_rn(v[j]), l[j] = __float2half_rn((v[j] - __half2float(h[j])) * LOW);
+            }
+            const int64_t at = base + int64_t(row) * pitch + u * VEC;
+            if constexpr (VEC == 8) {
+                *reinterpret_cast<uint4*>(hi + at) = *reinterpret_cast<const uint4*>(h);
+                *reinterpret_cast<uint4*>(lo + at) = *reinterpret_cast<const uint4*>(l);
+            } else {
+                hi[at] = h[0], lo[at] = l[0];
+            }
+        }
+}
+
+// ---- host ------------------------------------------------------------------------------------------------------------------------
+using Desc = mimk_orthogonalize_desc;
+constexpr int64_t LIM = int64_t(1) << 24, SLICE = int64_t(1) << 30;
+constexpr int MOST_STEPS = 64;
+
+struct Factors {
+    float p, q, r, a, b;  // a step's coefficients, and the factors of A and B
+};
+// Every step's factors: powers of two that keep what A and B can hold below 2^15, from the largest singular value that there can be.
+int factors_of(const Desc& d, Factors (&f)[MOST_STEPS]) {
+    double most = 1;
+    for (int s = 0; s < d.steps; ++s) {
+        const double p = d.coefficients[3 * s], q = d.coefficients[3 * s + 1], r = d.coefficients[3 * s + 2];
+        if (!(fabs(p) <= 1e4 && fabs(q) <= 1e4 && fabs(r) <= 1e4)) return MIMK_E_UNSUPPORTED;
+        const double a = most * most, b = fabs(q) * a + fabs(r) * a * a;
+        const auto power = [](double v) { return float(exp2(floor(log2(32768.0 / (v > 1.0 / 1024 ? v : 1.0 / 1024))))); };
+        f[s] = {float(p), float(q), float(r), power(a), power(b)};
+        double next = 0;
+        for (int i = 0; i <= 4096; ++i) {
+            const double v = most * i / 4096, w = fabs(v * (p + v * v * (q + r * v * v)));
+            next = w > next ? w : next;
+        }
+        most = 1.01 * next;
+        if (!(most <= 4)) return MIMK_E_UNSUPPORTED;
+        if (most < 1e-3) most = 1e-3;
+    }
+    return MIMK_OK;
+}
+
+int check(const Desc* d) {
+    if (!d || d->batch < 0 || d->m < 0 || d->n < 0 || d->steps < 1 || !d->coefficients || (d->batch && !d->x)) return MIMK_E_ARG;
+    if (d->dtype != MIMK_F32 && d->dtype != MIMK_BF16) return MIMK_E_DTYPE;
+    if (!(d->eps >= 0)) return MIMK_E_ARG;
+    if (d->steps > MOST_STEPS || d->m >= LIM || d->n >= LIM || d->batch >= LIM || d->m * d->n >= (int64_t(1) << 40)) return MIMK_E_UNSUPPORTED;
+    return MIMK_OK;
+}
+bool nothing(const Desc& d) { return !d.batch || !d.m || !d.n; }
+
+struct Plan {
+    int64_t k, pitch_x, pitch_a, slice, chunks;
+    __half *x[2][2], *a, *b;
+    float *d, *e;
+    double* sums;
+    __nv_bfloat16* out;  // rows of pitch_x, where the result's are no whole 16 bytes
+};
+Plan plan(const Desc& d, Space& space) {
+    Plan p{};
+    p.k = d.m < d.n ? d.m : d.n, p.pitch_x = up(d.n, 8), p.pitch_a = up(p.k, 8);
+    p.chunks = (d.m * d.n + CHUNK - 1) / CHUNK;
+    const int64_t each = 8 * d.m * p.pitch_x + 4 * p.k * p.pitch_a;
+    p.slice = SLICE / each;
+    if (p.slice > d.batch) p.slice = d.batch;
+    if (p.slice > TABLE) p.slice = TABLE;
+    if (p.slice < 1) p.slice = 1;
+    for (auto& x : p.x)
+        for (__half*& piece : x) piece = static_cast<__half*>(space.take(size_t(p.slice * d.m * p.pitch_x) * 2));
+    p.a = static_cast<__half*>(space.take(size_t(p.slice * p.k * p.pitch_a) * 2)), p.b = static_cast<__half*>(space.take(size_t(p.slice * p.k * p.pitch_a) * 2));
+    p.d = static_cast<float*>(space.take(size_t(p.slice * p.k) * 4)), p.e = static_cast<float*>(space.take(size_t(p.slice * p.k) * 4));
+    p.sums = static_cast<double*>(space.take(size_t(p.slice * p.chunks) * 8));
+    // the same for every address of the result (a size is asked for before there is one)
+    p.out = static_cast<__nv_bfloat16*>(space.take(size_t(p.slice * d.m * p.pitch_x) * 2));
+    return p;
+}
+
+int map_of(CUtensorMap* map, const void* p, int64_t rows, int64_t cols, int64_t pitch, int64_t batch, int box) {
+    return make_tmap_bf16_3d(map, p, uint64_t(cols), uint64_t(rows), uint64_t(batch), uint64_t(pitch) * 2, uint64_t(rows * pitch) * 2, 64, uint32_t(box));
+}
+
+template <int KIND, int SMS>
+int launch_product(const Maps& maps, Args g, const DeviceInfo& dev, cudaStream_t s) {
+    const auto kern = SMS == 2 ? pair_kernel<KIND> : single_kernel<KIND>;
+    static bool configured[64] = {};
+    if (!configured[dev.device & 63]) {
+        MIMK_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<KIND>::SMEM));
+        configured[dev.device & 63] = true;
+    }
+    g.tiles_m = int((g.rows + BM * SMS - 1) / (BM * SMS)), g.tiles_n = int((g.cols + BM * SMS - 1) / (BM * SMS));
+    const int64_t per   = KIND == APPLY ? int64_t(g.tiles_m) * g.tiles_n : int64_t(g.tiles_m) * (g.tiles_m + 1) / 2, tiles = per * g.batch;
+    if (tiles >= (int64_t(1) << 30)) return MIMK_E_UNSUPPORTED;
+    const int64_t most = dev.sm_count / SMS;
+    return launch_after(kern, unsigned(SMS * (tiles < most ? tiles : most)), THREADS, Shape<KIND>::SMEM, s, maps, g);
+}
+// On pairs of SMs or on single ones: whichever ends first, counting rounds of tiles, 512 or 256 cycles a k-block and some 6 k-blocks' for a tile's ends.
+template <int KIND>
+int launch(const Maps& maps, const Args& g, const DeviceInfo& dev, cudaStream_t s) {
+    double time[3];
+    for (int sms = 1; sms <= 2; ++sms) {
+        const int64_t m = (g.rows + BM * sms - 1) / (BM * sms), n = (g.cols + BM * sms - 1) / (BM * sms), tiles = (KIND == APPLY ? m * n : m * (m + 1) / 2) * g.batch;
+        time[sms] = double((tiles + dev.sm_count / sms - 1) / (dev.sm_count / sms)) * (double(g.kb) + 6) * (sms == 2 ? 512 : 270);
+    }
+    return time[2] <= time[1] ? launch_product<KIND, 2>(maps, g, dev, s) : launch_product<KIND, 1>(maps, g, dev, s);
+}
+
+template <class T>
+int prepare(const Desc& d, const Plan& p, int64_t first, int64_t count, cudaStream_t s) {
+    static thread_local Matrices all;
+    bool vec = d.n % 8 == 0;
+    for (int64_t i = 0; i < count; ++i) {
+        all.x[i] = d.x[first + i];
+        vec      = vec && aligned16(d.x[first + i]);
+    }
+    const int64_t values = d.m * d.n;
+    const dim3 squares(unsigned(p.chunks < 4096 ? p.chunks : 4096), unsigned(count)), rows(unsigned(d.m < 4096 ? d.m : 4096), unsigned(count));
+    if (vec) {
+        MIMK_TRY(launch_after(squares_kernel<T, 8>, squares, PREPARE, 0, s, all, values, p.sums));
+        return launch_after(prepare_kernel<T, 8>, rows, PREPARE, 0, s, all, int(d.m), int(d.n), int(p.pitch_x), static_cast<const double*>(p.sums), d.eps, p.x[0][0], p.x[0][1]);
+    }
+    MIMK_TRY(launch_after(squares_kernel<T, 1>, squares, PREPARE, 0, s, all, values, p.sums));
+    return launch_after(prepare_kernel<T, 1>, rows, PREPARE, 0, s, all, int(d.m), int(d.n), int(p.pitch_x), static_cast<const double*>(p.sums), d.eps, p.x[0][0], p.x[0][1]);
+}
+
+int slice(const Desc& d, const Plan& p, const Factors* f, int64_t first, int64_t count, const DeviceInfo& dev, cudaStream_t s) {
+    MIMK_TRY(d.dtype == MIMK_F32 ? prepare<float>(d, p, first, count, s) : prepare<__nv_bfloat16>(d, p, first, count, s));
+    const bool tall = d.m > d.n;
+    __nv_bfloat16* out = static_cast<__nv_bfloat16*>(d.out) + first * d.m * d.n;
+    const bool staged  = !group::tma_can_read(out, d.n);
+    Maps maps;
+    CUtensorMap a_map, b_map;
+    MIMK_TRY(map_of(&a_map, p.a, p.k, p.k, p.pitch_a, count, BM));
+    MIMK_TRY(map_of(&b_map, p.b, p.k, p.k, p.pitch_a, count, BM));
+    const auto blocks = [](int64_t v) { return int((v + BK - 1) / BK); };
+    for (int step = 0; step < d.steps; ++step) {
+        const Factors& c   = f[step];
+        __half* const* now = p.x[step & 1];
+        __half* const* next = p.x[~step & 1];
+        Args g{};
+        g.batch = int(count), g.pitch = int(p.pitch_a), g.status = dev.status_dev;
+        // A
+        g.rows = g.cols = int(p.k), g.kb = blocks(tall ? d.m : d.n), g.a_mn = g.b_mn = tall, g.out = p.a, g.diag_out = p.d;
+        g.f[0] = 1.f / (SX * SX), g.f[1] = c.a;
+        MIMK_TRY(map_of(&maps.left, now[0], d.m, d.n, p.pitch_x, count, tall ? 64 : BM));
+        maps.right = maps.left;
+        MIMK_TRY(launch<GRAM>(maps, g, dev, s));
+        // B
+        g.kb = blocks(p.k), g.a_mn = g.b_mn = 0, g.in = p.a, g.out = p.b, g.diag_in = p.d, g.diag_out = p.e;
+        g.f[0] = 1.f / (c.a * c.a), g.f[1] = 1.f / c.a, g.f[2] = c.q, g.f[3] = c.r, g.f[4] = c.b;
+        maps.left = maps.right = a_map;
+        MIMK_TRY(launch<SQUARE>(maps, g, dev, s));
+        // X
+        g.rows = int(d.m), g.cols = int(d.n), g.b_mn = !tall, g.tall = tall, g.last = step + 1 == d.steps, g.diag_in = p.e;
+        g.f[0] = c.p, g.f[1] = 1.f / c.b, g.f[2] = d.scale / SX;
+        if (tall) {
+            MIMK_TRY(map_of(&maps.left, now[0], d.m, d.n, p.pitch_x, count, BM));
+            maps.right = b_map;
+        } else {
+            maps.left = b_map;
+            MIMK_TRY(map_of(&maps.right, now[0], d.m, d.n, p.pitch_x, count, 64));
+        }
+        MIMK_TRY(map_of(&maps.hi, now[0], d.m, d.n, p.pitch_x, count, 32));
+        MIMK_TRY(map_of(&maps.lo, now[1], d.m, d.n, p.pitch_x, count, 32));
+        if (g.last) {
+            MIMK_TRY(staged ? map_of(&maps.out_hi, p.out, d.m, d.n, p.pitch_x, count, 32) : map_of(&maps.out_hi, out, d.m, d.n, d.n, count, 32));
+            maps.out_lo = maps.out_hi;
+        } else {
+            MIMK_TRY(map_of(&maps.out_hi, next[0], d.m, d.n, p.pitch_x, count, 32));
+            MIMK_TRY(map_of(&maps.out_lo, next[1], d.m, d.n, p.pitch_x, count, 32));
+        }
+        MIMK_TRY(launch<APPLY>(maps, g, dev, s));
+    }
+    return staged ? copy_rows(p.out, p.pitch_x, out, d.n, count * d.m, d.n, s) : MIMK_OK;
+}
+
+}  // namespace
+}  // namespace mimk
+
+using namespace mimk;
+
+extern "C" int mimk_orthogonalize_workspace(const mimk_orthogonalize_desc* d, uint64_t* bytes) {
+    MIMK_TRY(check(d));
+    if (!bytes) return MIMK_E_ARG;
+    Space space(nullptr);
+    if (!nothing(*d)) plan(*d, space);
+    *bytes = space.used();
+    return MIMK_OK;
+}
+
+extern "C" int mimk_orthogonalize(const mimk_orthogonalize_desc* d, void* stream) {
+    MIMK_TRY(check(d));
+    Factors f[MOST_STEPS];
+    MIMK_TRY(factors_of(*d, f));
+    int st                = MIMK_OK;
+    const DeviceInfo* dev = device_info(&st);
+    if (!dev) return st;
+    if (nothing(*d)) return MIMK_OK;
+    if (!d->out) return MIMK_E_ARG;
+    const size_t size = dtype_size(d->dtype);
+    if (reinterpret_cast<uintptr_t>(d->out) % 2) return MIMK_E_ALIGN;
+    for (int64_t i = 0; i < d->batch; ++i) {
+        if (!d->x[i]) return MIMK_E_ARG;
+        if (reinterpret_cast<uintptr_t>(d->x[i]) % size) return MIMK_E_ALIGN;
+    }
+    Space space(d->workspace);
+    const Plan p = plan(*d, space);
+    if (!d->workspace || space.used() > d->workspace_bytes) return MIMK_E_WORKSPACE;
+    if (!aligned16(d->workspace)) return MIMK_E_ALIGN;
+    for (int64_t first = 0; first < d->batch; first += p.slice)
+        MIMK_TRY(slice(*d, p, f, first, d->batch - first < p.slice ? d->batch - first : p.slice, *dev, static_cast<cudaStream_t>(stream)));
+    return MIMK_OK;
+}

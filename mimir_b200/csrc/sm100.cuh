@@ -218,6 +218,11 @@ __host__ __device__ __forceinline__ uint32_t idesc_bf16_f32(int m, int n, int a_
     return d;
 }
 
+// The same with f16 A and B (format 0).
+__host__ __device__ __forceinline__ uint32_t idesc_f16_f32(int m, int n, int a_mn_major, int b_mn_major) {
+    return idesc_bf16_f32(m, n, a_mn_major, b_mn_major) & ~(1u << 7 | 1u << 10);
+}
+
 }  // namespace sm100
 
 // ---- host: tensor maps ------------------------------------------------------------------------------

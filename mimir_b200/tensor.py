@@ -585,6 +585,257 @@ def clip_grad_norm(grads, limit: float, *, eps: float = 1e-6, out=None) -> torch
     return norm
 
 
+def _float_types(what: str, *ts):
+    for t in ts:
+        if t is not None and t.dtype not in (torch.float32, torch.bfloat16):
+            raise TypeError(f"{what}: operands are F32 or BF16")
+
+
+def _device_of(what: str, *ts) -> torch.device:
+    """The one device that the operands lie on; a call is made with that one current, on its current stream."""
+    _dev(*ts)
+    devices = {t.device for t in ts if t is not None}
+    if len(devices) != 1:
+        raise ValueError(f"{what}: the operands lie on one device")
+    return devices.pop()
+
+
+def _embedding_desc(what: str, ids, rows, classes, features, scale, ignore_index, out_dtype):
+    if ids.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"{what}: ids are I32 or I64")
+    _float_types(what, rows)
+    d = L.EmbeddingDesc()
+    d.n, d.d, d.v = ids.numel(), features, classes
+    d.ids, d.scale, d.dtype, d.id_dtype = ids.data_ptr(), float(scale), _dt(rows), _dt(ids)
+    if out_dtype not in (torch.float32, torch.bfloat16):
+        raise TypeError(f"{what}: the result is F32 or BF16")
+    d.out_dtype = L.F32 if out_dtype == torch.float32 else L.BF16
+    if ignore_index is not None:
+        if not -2 ** 63 <= ignore_index < 2 ** 63:
+            raise ValueError(f"{what}: ignore_index is a number of 64 bits")
+        d.has_ignore, d.ignore_index = 1, ignore_index
+    return d
+
+
+def embedding(table: torch.Tensor, ids: torch.Tensor, *, scale: float = 1.0, ignore_index: int | None = None, out_dtype=None) -> torch.Tensor:
+    """scale * table[ids], table [classes, features] F32 or BF16, ids I32 or I64 of any shape: [*ids.shape, features]. A position whose id is `ignore_index`, which may be a
+    class, has no token: its row is zeros. Any other id that is no class gives a row of NaN, and device_status() raises."""
+    device = _device_of("embedding", table, ids)
+    if table.dim() != 2:
+        raise ValueError("embedding: the table is of rank 2")
+    table, ids = table.contiguous(), ids.contiguous()
+    v, features = table.shape
+    d = _embedding_desc("embedding", ids, table, v, features, scale, ignore_index, out_dtype or table.dtype)
+    out = torch.empty((*ids.shape, features), dtype=out_dtype or table.dtype, device=device)
+    d.table, d.out = table.data_ptr(), out.data_ptr()
+    with torch.cuda.device(device):
+        L.check(L.lib().mimk_embedding(C.byref(d), _stream()), "embedding")
+    return out
+
+
+def embedding_grad(dy: torch.Tensor, ids: torch.Tensor, classes: int, *, scale: float = 1.0, ignore_index: int | None = None, out_dtype=None,
+                   add_to: torch.Tensor | None = None) -> torch.Tensor:
+    """The gradient of embedding's table [classes, features] from its result's gradient dy [*ids.shape, features]: row c is scale times the sum of dy's rows whose id is c,
+    in f32, the same call after call. Positions without a token and ids that are no class add nothing; the latter make device_status() raise. add_to: a gradient of the table's
+    (of a tied output layer, or of an earlier part of the batch) that the sums are added to, in place, and which is returned; rows of classes that do not occur are not touched."""
+    device = _device_of("embedding_grad", dy, ids, add_to)
+    if dy.dim() < 1 or dy.shape[:-1] != ids.shape:
+        raise ValueError("embedding_grad: one row of dy for each id")
+    if classes < 0:
+        raise ValueError("embedding_grad: the number of classes is at least 0")
+    features = dy.shape[-1]
+    dy, ids = dy.contiguous(), ids.contiguous()
+    if add_to is None:
+        out = torch.empty((classes, features), dtype=out_dtype or dy.dtype, device=device)
+    else:
+        out = add_to
+        if tuple(out.shape) != (classes, features) or not out.is_contiguous():
+            raise ValueError("embedding_grad: add_to is a row-major [classes, features]")
+        if out_dtype not in (None, out.dtype):
+            raise TypeError("embedding_grad: the result has add_to's element type")
+    d = _embedding_desc("embedding_grad", ids, dy, classes, features, scale, ignore_index, out.dtype)
+    d.dy, d.dtable, d.add = dy.data_ptr(), out.data_ptr(), int(add_to is not None)
+    scratch, lib = C.c_uint64(), L.lib()
+    L.check(lib.mimk_embedding_grad_workspace(C.byref(d), C.byref(scratch)), "embedding_grad")
+    with torch.cuda.device(device):
+        ws = _bytes(scratch.value, device)
+        d.workspace, d.workspace_bytes = ws.data_ptr(), scratch.value
+        L.check(lib.mimk_embedding_grad(C.byref(d), _stream()), "embedding_grad")
+    if add_to is not None:
+        torch.autograd.graph.increment_version(add_to)
+    return out
+
+
+class ResidualKept:
+    """What residual_rmsnorm_fwd keeps for residual_rmsnorm_bwd: two F32 values per row, and what the call was."""
+    __slots__ = ("buffer", "call")
+
+    def __init__(self, buffer: torch.Tensor, call):
+        self.buffer, self.call = buffer, call
+
+
+def _gate_rows(what: str, gate: torch.Tensor, shape) -> int:
+    """How many rows in turn share a row of the gate: [features], or the operands' leading axes up to one of them, ones for those behind it, and the features."""
+    lead, own = tuple(shape[:-1]), tuple(gate.shape[:-1])
+    own = (1,) * (len(lead) - len(own)) + own
+    same = 0
+    while same < len(lead) and own[same:same + 1] == lead[same:same + 1]:
+        same += 1
+    if gate.dim() < 1 or gate.shape[-1] != shape[-1] or len(own) != len(lead) or any(n != 1 for n in own[same:]):
+        raise ValueError(f"{what}: the gate is [features], or has the operands' shape with ones for its last axes before the features")
+    return math.prod(lead[same:])
+
+
+def _residual_desc(what, r, h, gamma, post_gamma, gate, eps, residual_scale, branch_scale):
+    device = _device_of(what, r, h, gamma, post_gamma, gate)
+    _float_types(what, r, h, gamma, post_gamma, gate)
+    if r.dim() < 1 or (h is not None and h.shape != r.shape):
+        raise ValueError(f"{what}: r and h have one shape, of rank 1 at least")
+    if h is not None and h.dtype != r.dtype and r.dtype != torch.float32:
+        raise TypeError(f"{what}: h has r's element type, or is BF16 beside an F32 r")
+    if h is None and (gamma is None or post_gamma is not None or gate is not None or residual_scale != 1 or branch_scale != 1):
+        raise ValueError(f"{what}: without h there is the norm of r alone")
+    features = r.shape[-1]
+    for g in (gamma, post_gamma):
+        if g is not None and tuple(g.shape) != (features,):
+            raise ValueError(f"{what}: gamma extent must equal the last extent of r")
+    if not eps >= 0:
+        raise ValueError(f"{what}: eps is at least 0")
+    d = L.ResidualRmsnormDesc()
+    d.n, d.d, d.gate_rows = math.prod(r.shape[:-1]), features, 1
+    d.eps, d.residual_scale, d.branch_scale = eps, residual_scale, branch_scale
+    held = []
+
+    def put(name, t, kind=None):
+        if t is not None:
+            held.append(t.contiguous())
+            setattr(d, name, held[-1].data_ptr())
+            if kind:
+                setattr(d, kind, _dt(t))
+    put("r", r, "stream_dtype"), put("h", h), put("gamma", gamma, "gamma_dtype"), put("post_gamma", post_gamma, "post_gamma_dtype")
+    d.block_dtype = _dt(r if h is None else h)
+    if gate is not None:
+        d.gate_rows = max(1, _gate_rows(what, gate, r.shape))
+        put("gate", gate, "gate_dtype")
+    return d, held, device, put
+
+
+def _residual_fwd(what, r, h, gamma, eps, post_gamma, gate, residual_scale, branch_scale, keep):
+    eps, residual_scale, branch_scale = float(eps), float(residual_scale), float(branch_scale)
+    d, held, device, put = _residual_desc(what, r, h, gamma, post_gamma, gate, eps, residual_scale, branch_scale)
+    new, x, kept = r, None, None
+    if h is not None:
+        new = torch.empty(r.shape, dtype=r.dtype, device=device)
+        d.r_out = new.data_ptr()
+    if gamma is not None:
+        x = torch.empty(r.shape, dtype=(r if h is None else h).dtype, device=device)
+        d.x = x.data_ptr()
+    if keep:
+        kept = torch.empty((2, d.n), dtype=torch.float32, device=device)
+        d.kept = kept.data_ptr()
+    with torch.cuda.device(device):
+        L.check(L.lib().mimk_residual_rmsnorm_fwd(C.byref(d), _stream()), what)
+    return new, x, None if kept is None else ResidualKept(kept, ((d.n, d.d), h is not None, gamma is not None, post_gamma is not None, gate is not None, eps, residual_scale, branch_scale))
+
+
+def residual_rmsnorm(r: torch.Tensor, h: torch.Tensor | None, gamma: torch.Tensor | None, eps: float, *, post_gamma: torch.Tensor | None = None,
+                     gate: torch.Tensor | None = None, residual_scale: float = 1.0, branch_scale: float = 1.0):
+    """From one block to the next in one pass over memory: (r', x) with r' = residual_scale * r + branch_scale * gate * u, u = rmsnorm(h, post_gamma, eps) (h itself without
+    post_gamma), and x = rmsnorm(r', gamma, eps), the next block's input (None without gamma), of r' before its rounding. r: the residual stream, h: the block's result, of one shape; r' has
+    r's element type, x has h's: F32 and F32, F32 and BF16, or BF16 and BF16. gate: [features], or the operands' shape with ones for its last axes before the features (a
+    row of it for each sample, or for each row). h None: the norm before the first block, r' is r."""
+    return _residual_fwd("residual_rmsnorm", r, h, gamma, eps, post_gamma, gate, residual_scale, branch_scale, False)[:2]
+
+
+def residual_rmsnorm_fwd(r: torch.Tensor, h: torch.Tensor | None, gamma: torch.Tensor | None, eps: float, *, post_gamma: torch.Tensor | None = None,
+                         gate: torch.Tensor | None = None, residual_scale: float = 1.0, branch_scale: float = 1.0):
+    """residual_rmsnorm for training: (r', x, kept), `kept` being what residual_rmsnorm_bwd needs of this pass beside the operands (8 bytes per row)."""
+    return _residual_fwd("residual_rmsnorm_fwd", r, h, gamma, eps, post_gamma, gate, residual_scale, branch_scale, True)
+
+
+def residual_rmsnorm_bwd(dr: torch.Tensor | None, dx: torch.Tensor | None, r: torch.Tensor, h: torch.Tensor | None, gamma: torch.Tensor | None, kept: ResidualKept, *,
+                         post_gamma: torch.Tensor | None = None, gate: torch.Tensor | None = None):
+    """The gradients (of r, h, gamma, post_gamma, gate; None for what there is not) of the residual_rmsnorm_fwd call that gave `kept`, from those of its results r' (dr, None:
+    nothing arrives there) and x (dx, None without gamma). Each has its operand's shape and element type; a gate's row gets the sum over the rows that share it."""
+    what = "residual_rmsnorm_bwd"
+    d, held, device, put = _residual_desc(what, r, h, gamma, post_gamma, gate, *kept.call[5:])
+    if ((d.n, d.d), h is not None, gamma is not None, post_gamma is not None, gate is not None) != kept.call[:5]:
+        raise ValueError(f"{what}: `kept` is of a call with other operands")
+    if (dx is None) != (gamma is None):
+        raise ValueError(f"{what}: dx is the gradient of x, which there is with gamma")
+    if _device_of(what, r, dr, dx, kept.buffer) != device or any(t is not None and t.shape != r.shape for t in (dr, dx)):
+        raise ValueError(f"{what}: dr and dx must have the results' shape")
+    if (dr is not None and dr.dtype != r.dtype) or (dx is not None and dx.dtype != (r if h is None else h).dtype):
+        raise TypeError(f"{what}: dr and dx have the results' element types")
+    put("dr_out", dr), put("dx", dx)
+    out = [t if t is None else torch.empty(t.shape, dtype=t.dtype, device=device) for t in (r, h, gamma, post_gamma, gate)]
+    if gate is not None and not d.n:
+        out[4].zero_()
+    d.dr, d.dh, d.dgamma, d.dpost_gamma, d.dgate = (t if t is None else t.data_ptr() for t in out)
+    d.kept = kept.buffer.data_ptr()
+    scratch, lib = C.c_uint64(), L.lib()
+    with torch.cuda.device(device):
+        L.check(lib.mimk_residual_rmsnorm_workspace(C.byref(d), C.byref(scratch)), what)
+        ws = _bytes(scratch.value, device)
+        d.workspace, d.workspace_bytes = ws.data_ptr(), scratch.value
+        L.check(lib.mimk_residual_rmsnorm_bwd(C.byref(d), _stream()), what)
+    return tuple(out)
+
+
+NEWTON_SCHULZ = (3.4445, -4.7750, 2.0315)  # brings singular values from 1e-3 on to between 0.7 and 1.2 in five steps
+
+
+def _orthogonalize(what, xs, steps, coefficients, eps, scale):
+    """The results for matrices of one shape, element type and device, each dense and row-major, as one [len(xs), m, n]."""
+    device, (m, n) = xs[0].device, xs[0].shape
+    out = torch.empty((len(xs), m, n), dtype=torch.bfloat16, device=device)
+    d = L.OrthogonalizeDesc()
+    d.batch, d.m, d.n = len(xs), m, n
+    d.x, d.out, d.coefficients = (C.c_void_p * len(xs))(*(x.data_ptr() for x in xs)), out.data_ptr(), (C.c_float * len(coefficients))(*coefficients)
+    d.eps, d.scale, d.steps, d.dtype = eps, scale, steps, _dt(xs[0])
+    scratch, lib = C.c_uint64(), L.lib()
+    with torch.cuda.device(device):
+        L.check(lib.mimk_orthogonalize_workspace(C.byref(d), C.byref(scratch)), what)
+        ws = _bytes(scratch.value, device)
+        d.workspace, d.workspace_bytes = ws.data_ptr(), scratch.value
+        L.check(lib.mimk_orthogonalize(C.byref(d), _stream()), what)
+    return out
+
+
+def orthogonalize(x, *, steps: int = 5, coefficients=NEWTON_SCHULZ, eps: float = 1e-7, scale: float = 1.0):
+    """Matrices F32 or BF16 with their singular values brought near 1, as BF16: an optimiser's orthogonalised update. X = x / (|x| + eps), |x| the 2-norm of all values of a
+    matrix, then `steps` times X <- p X + (q A + r A^2) X, A = X X^T (by X^T X where x is taller than wide), (p, q, r) = coefficients, or coefficients[step] where there are `steps` of them; the result is
+    scale * X. x: a matrix, a stack of them (leading axes), or a list of either, for which the result is a list; those of one shape are multiplied together. Transposed views give transposed results.
+    The products' operands are rounded to 11 bits; the result is off by up to 1e-3 of its 2-norm before it is rounded to BF16, several times that for matrices of a few rows and hardly any rank."""
+    what = "orthogonalize"
+    matrices = [x] if isinstance(x, torch.Tensor) else list(x)
+    p = [float(v) for c in coefficients for v in (c if isinstance(c, (tuple, list)) else (c,))]
+    p = p * steps if len(p) == 3 and not isinstance(coefficients[0], (tuple, list)) else p
+    if steps < 1 or len(p) != 3 * steps:
+        raise ValueError(f"{what}: one or more steps, of three coefficients each")
+    if not eps >= 0:
+        raise ValueError(f"{what}: eps is at least 0")
+    alike = {}
+    for i, t in enumerate(matrices):
+        _dev(t)
+        _float_types(what, t)
+        if t.dim() < 2:
+            raise ValueError(f"{what}: matrices, or stacks of them")
+        turned = not t.is_contiguous() and t.mT.is_contiguous()
+        t = (t.mT if turned else t).contiguous()
+        alike.setdefault((t.shape[-2:], t.dtype, t.device), []).append((i, turned, t))
+    results = [None] * len(matrices)
+    for (shape, _, device), group in alike.items():
+        flat = [s for _, _, t in group for s in t.reshape(-1, *shape).unbind(0)] if 0 not in shape else []
+        out = _orthogonalize(what, flat, steps, p, float(eps), float(scale)) if flat else torch.empty((0, *shape), dtype=torch.bfloat16, device=device)
+        at = 0
+        for i, turned, t in group:
+            count = math.prod(t.shape[:-2]) if flat else 0
+            o = out[at:at + count].reshape(t.shape) if flat else torch.empty(t.shape, dtype=torch.bfloat16, device=device)
+            results[i], at = o.mT if turned else o, at + count
+    return results[0] if isinstance(x, torch.Tensor) else results
+
+
 # ------------------------------------------------------------------------------------------------ the generic op
 def proj_map(n_loops: int, subs):
     """`proj_map subs`: result j reads loop variable subs[j] (tensor.mim:196-203), as a coefficient matrix."""
