@@ -10,6 +10,7 @@
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
+#include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
@@ -414,6 +415,156 @@ OP(clip_grads, 4)
     return result(status, std::move(norm));
 END_OP
 
+// On the device that is current, whose stream the call is made on.
+bool here(const Tensor* t) { return t && t->device().index() == c10::cuda::current_device(); }
+// A dense I32 or I64 tensor on the current device, or null.
+const Tensor* index_tensor(PyObject* o) {
+    if (!THPVariable_CheckExact(o)) return nullptr;
+    const Tensor& t = THPVariable_Unpack(o);
+    if (!t.defined() || !t.is_cuda() || t.layout() != at::kStrided || !t.is_contiguous() || t.numel() == 0 || (t.scalar_type() != at::kLong && t.scalar_type() != at::kInt)) return nullptr;
+    return here(&t) ? &t : nullptr;
+}
+bool embedding_desc(mimk_embedding_desc& d, const Tensor& rows, const Tensor& ids, PyObject* scale, PyObject* ignore) {
+    d = {};
+    if (!PyFloat_CheckExact(scale) || (ignore != Py_None && !is_int(ignore, d.ignore_index))) return false;
+    d.n = ids.numel(), d.ids = ids.data_ptr(), d.scale = float(PyFloat_AS_DOUBLE(scale)), d.has_ignore = ignore != Py_None;
+    d.dtype = dtype_of(rows.scalar_type()), d.id_dtype = ids.scalar_type() == at::kLong ? MIMK_I64 : MIMK_I32;
+    return true;
+}
+
+// table, ids, scale, ignored index or None, out dtype
+OP(embedding, 5)
+    const Tensor *table = dense(a[0]), *ids = index_tensor(a[1]);
+    mimk_embedding_desc d;
+    at::ScalarType t;
+    if (!here(table) || !ids || table->dim() != 2 || !embedding_desc(d, *table, *ids, a[2], a[3]) || !out_type(a[4], table->scalar_type(), t)) Py_RETURN_NONE;
+    std::vector<int64_t> shape(ids->sizes().begin(), ids->sizes().end());
+    shape.push_back(table->size(1));
+    Tensor out = empty(shape, t, *table);
+    d.v = table->size(0), d.d = table->size(1), d.table = table->data_ptr(), d.out = out.data_ptr(), d.out_dtype = dtype_of(t);
+    return result(unlocked([&](void* stream) { return mimk_embedding(&d, stream); }), std::move(out));
+END_OP
+
+// dy, ids, classes, scale, ignored index or None, out dtype
+OP(embedding_grad, 6)
+    const Tensor *dy = dense(a[0]), *ids = index_tensor(a[1]);
+    mimk_embedding_desc d;
+    at::ScalarType t;
+    int64_t classes;
+    if (!here(dy) || !ids || dy->dim() < 1 || !is_int(a[2], classes) || classes < 1 || !embedding_desc(d, *dy, *ids, a[3], a[4]) || !out_type(a[5], dy->scalar_type(), t)) Py_RETURN_NONE;
+    if (dy->sizes().slice(0, size_t(dy->dim() - 1)) != ids->sizes()) Py_RETURN_NONE;
+    d.v = classes, d.d = dy->size(dy->dim() - 1), d.dy = dy->data_ptr(), d.out_dtype = dtype_of(t);
+    if (mimk_embedding_grad_workspace(&d, &d.workspace_bytes) != MIMK_OK) Py_RETURN_NONE;
+    Tensor out = empty({classes, d.d}, t, *dy), scratch = empty({int64_t(d.workspace_bytes)}, at::kByte, *dy);
+    d.dtable = out.data_ptr(), d.workspace = scratch.data_ptr();
+    return result(unlocked([&](void* stream) { return mimk_embedding_grad(&d, stream); }), std::move(out));
+END_OP
+
+// The operands of residual_rmsnorm, r, h, gamma, post_gamma and gate, of which all but r may be None.
+bool residual_desc(mimk_residual_rmsnorm_desc& d, PyObject* const (&o)[5], const Tensor* (&t)[5]) {
+    d = {};
+    for (int i = 0; i < 5; ++i) {
+        t[i] = o[i] == Py_None ? nullptr : dense(o[i]);
+        if ((!t[i] && (o[i] != Py_None || i == 0)) || (t[i] && !here(t[i]))) return false;
+    }
+    const Tensor &r = *t[0], *h = t[1], *gate = t[4];
+    if (r.dim() < 1 || (h && h->sizes() != r.sizes())) return false;
+    const int64_t features = r.size(r.dim() - 1);
+    for (const Tensor* g : {t[2], t[3]})
+        if (g && (g->dim() != 1 || g->size(0) != features)) return false;
+    d.n = r.numel() / features, d.d = features, d.gate_rows = 1;
+    d.r = r.data_ptr(), d.stream_dtype = d.block_dtype = dtype_of(r.scalar_type());
+    if (h) d.h = h->data_ptr(), d.block_dtype = dtype_of(h->scalar_type());
+    if (t[2]) d.gamma = t[2]->data_ptr(), d.gamma_dtype = dtype_of(t[2]->scalar_type());
+    if (t[3]) d.post_gamma = t[3]->data_ptr(), d.post_gamma_dtype = dtype_of(t[3]->scalar_type());
+    if (gate) {
+        // the operands' leading axes up to one of them, and ones
+        const int64_t lead = r.dim() - 1, own = gate->dim() - 1, missing = lead - own;
+        if (own < 0 || missing < 0 || gate->size(own) != features) return false;
+        int64_t same = 0;
+        while (same < lead && (same < missing ? 1 : gate->size(same - missing)) == r.size(same)) ++same;
+        for (int64_t i = same; i < lead; ++i) {
+            if (i >= missing && gate->size(i - missing) != 1) return false;
+            d.gate_rows *= r.size(i);
+        }
+        d.gate = gate->data_ptr(), d.gate_dtype = dtype_of(gate->scalar_type());
+    }
+    return true;
+}
+
+// r, h, gamma, post_gamma, gate, eps, residual scale, branch scale, whether bwd follows -> r' (None without h), x (None without gamma), kept
+OP(residual_rmsnorm, 9)
+    mimk_residual_rmsnorm_desc d;
+    const Tensor* t[5];
+    PyObject* const o[5] = {a[0], a[1], a[2], a[3], a[4]};
+    if (!PyFloat_CheckExact(a[5]) || !PyFloat_CheckExact(a[6]) || !PyFloat_CheckExact(a[7]) || !PyBool_Check(a[8]) || !residual_desc(d, o, t)) Py_RETURN_NONE;
+    d.eps = float(PyFloat_AS_DOUBLE(a[5])), d.residual_scale = float(PyFloat_AS_DOUBLE(a[6])), d.branch_scale = float(PyFloat_AS_DOUBLE(a[7]));
+    std::vector<Tensor> out(3);
+    if (t[1]) out[0] = empty(t[0]->sizes(), t[0]->scalar_type(), *t[0]), d.r_out = out[0].data_ptr();
+    if (t[2]) out[1] = empty(t[0]->sizes(), (t[1] ? t[1] : t[0])->scalar_type(), *t[0]), d.x = out[1].data_ptr();
+    if (a[8] == Py_True) out[2] = empty({2, d.n}, at::kFloat, *t[0]), d.kept = static_cast<float*>(out[2].data_ptr());
+    const int status = unlocked([&](void* stream) { return mimk_residual_rmsnorm_fwd(&d, stream); });
+    return results(status, std::move(out));
+END_OP
+
+// dr or None, dx or None, r, h, gamma, post_gamma, gate, the kept buffer, what the forward call was (a tuple) -> the gradients of r, h, gamma, post_gamma, gate, None for what there is not
+OP(residual_rmsnorm_bwd, 9)
+    mimk_residual_rmsnorm_desc d;
+    const Tensor *t[5], *dr = a[0] == Py_None ? nullptr : dense(a[0]), *dx = a[1] == Py_None ? nullptr : dense(a[1]);
+    PyObject* const o[5] = {a[2], a[3], a[4], a[5], a[6]};
+    if ((!dr && a[0] != Py_None) || (!dx && a[1] != Py_None) || !residual_desc(d, o, t)) Py_RETURN_NONE;
+    const Tensor* block = t[1] ? t[1] : t[0];
+    if ((dx != nullptr) != (t[2] != nullptr) || (dr && (!here(dr) || dr->sizes() != t[0]->sizes() || dr->scalar_type() != t[0]->scalar_type()))) Py_RETURN_NONE;
+    if (dx && (!here(dx) || dx->sizes() != block->sizes() || dx->scalar_type() != block->scalar_type())) Py_RETURN_NONE;
+    const Tensor* kept = dense(a[7]);
+    if (!here(kept) || kept->scalar_type() != at::kFloat || !PyTuple_CheckExact(a[8]) || PyTuple_GET_SIZE(a[8]) != 9) Py_RETURN_NONE;
+    int64_t v;
+    for (int i = 0; i < 2; ++i)
+        if (!is_int(PyTuple_GET_ITEM(a[8], i), v) || v != (i ? d.d : d.n)) Py_RETURN_NONE;
+    for (int i = 1; i < 5; ++i)
+        if (PyTuple_GET_ITEM(a[8], 1 + i) != (t[i] ? Py_True : Py_False)) Py_RETURN_NONE;
+    float f[3];
+    for (int i = 0; i < 3; ++i) {
+        if (!PyFloat_CheckExact(PyTuple_GET_ITEM(a[8], 6 + i))) Py_RETURN_NONE;
+        f[i] = float(PyFloat_AS_DOUBLE(PyTuple_GET_ITEM(a[8], 6 + i)));
+    }
+    d.eps = f[0], d.residual_scale = f[1], d.branch_scale = f[2];
+    if (mimk_residual_rmsnorm_workspace(&d, &d.workspace_bytes) != MIMK_OK) Py_RETURN_NONE;
+    std::vector<Tensor> out(5);
+    void* to[5] = {};
+    for (int i = 0; i < 5; ++i)
+        if (t[i]) out[i] = empty(t[i]->sizes(), t[i]->scalar_type(), *t[i]), to[i] = out[i].data_ptr();
+    Tensor scratch = empty({int64_t(d.workspace_bytes)}, at::kByte, *t[0]);
+    d.dr = to[0], d.dh = to[1], d.dgamma = to[2], d.dpost_gamma = to[3], d.dgate = to[4];
+    d.dr_out = dr ? dr->data_ptr() : nullptr, d.dx = dx ? dx->data_ptr() : nullptr, d.kept = static_cast<float*>(kept->data_ptr()), d.workspace = scratch.data_ptr();
+    const int status = unlocked([&](void* stream) { return mimk_residual_rmsnorm_bwd(&d, stream); });
+    return results(status, std::move(out));
+END_OP
+
+// one tensor of matrices, steps, three coefficients (a tuple), eps, scale
+OP(orthogonalize, 5)
+    const Tensor* x = dense(a[0]);
+    int64_t steps;
+    if (!here(x) || x->dim() < 2 || !is_int(a[1], steps) || steps < 1 || steps > 64 || !PyTuple_CheckExact(a[2]) || PyTuple_GET_SIZE(a[2]) != 3) Py_RETURN_NONE;
+    if (!PyFloat_CheckExact(a[3]) || !PyFloat_CheckExact(a[4])) Py_RETURN_NONE;
+    float one[3], all[3 * 64];
+    for (int i = 0; i < 3; ++i) {
+        if (!PyFloat_CheckExact(PyTuple_GET_ITEM(a[2], i))) Py_RETURN_NONE;
+        one[i] = float(PyFloat_AS_DOUBLE(PyTuple_GET_ITEM(a[2], i)));
+    }
+    for (int64_t i = 0; i < 3 * steps; ++i) all[i] = one[i % 3];
+    mimk_orthogonalize_desc d = {};
+    d.m = x->size(x->dim() - 2), d.n = x->size(x->dim() - 1), d.batch = x->numel() / (d.m * d.n);
+    std::vector<const void*> each(d.batch);
+    for (int64_t i = 0; i < d.batch; ++i) each[i] = static_cast<const char*>(x->data_ptr()) + i * d.m * d.n * x->element_size();
+    d.x = each.data(), d.coefficients = all, d.steps = int(steps), d.dtype = dtype_of(x->scalar_type());
+    d.eps = float(PyFloat_AS_DOUBLE(a[3])), d.scale = float(PyFloat_AS_DOUBLE(a[4]));
+    if (mimk_orthogonalize_workspace(&d, &d.workspace_bytes) != MIMK_OK) Py_RETURN_NONE;
+    Tensor out = empty(x->sizes(), at::kBFloat16, *x), scratch = empty({int64_t(d.workspace_bytes)}, at::kByte, *x);
+    d.out = out.data_ptr(), d.workspace = scratch.data_ptr();
+    return result(unlocked([&](void* stream) { return mimk_orthogonalize(&d, stream); }), std::move(out));
+END_OP
+
 // x, perm (a tuple of ints): the copy-style map_reduce_post that tensor.py's transpose spells
 OP(transpose, 2)
     const Tensor* x = dense(a[0]);
@@ -439,7 +590,8 @@ END_OP
 PyMethodDef methods[] = {
 #define ENTRY(NAME) {#NAME, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(NAME)), METH_FASTCALL, nullptr}
     ENTRY(product_2d), ENTRY(bmm), ENTRY(reduce), ENTRY(reduce_of_unary), ENTRY(softmax), ENTRY(rmsnorm), ENTRY(unary), ENTRY(binary), ENTRY(binary_ax),
-    ENTRY(attention), ENTRY(mlp_gated), ENTRY(mlp_gated_fwd), ENTRY(mlp_gated_bwd), ENTRY(linear_ce), ENTRY(clip_grads), ENTRY(transpose), {nullptr, nullptr, 0, nullptr}};
+    ENTRY(attention), ENTRY(mlp_gated), ENTRY(mlp_gated_fwd), ENTRY(mlp_gated_bwd), ENTRY(linear_ce), ENTRY(clip_grads), ENTRY(embedding), ENTRY(embedding_grad), ENTRY(residual_rmsnorm), ENTRY(residual_rmsnorm_bwd), ENTRY(orthogonalize),
+    ENTRY(transpose), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods};
 
 }  // namespace

@@ -620,6 +620,8 @@ def _embedding_desc(what: str, ids, rows, classes, features, scale, ignore_index
 def embedding(table: torch.Tensor, ids: torch.Tensor, *, scale: float = 1.0, ignore_index: int | None = None, out_dtype=None) -> torch.Tensor:
     """scale * table[ids], table [classes, features] F32 or BF16, ids I32 or I64 of any shape: [*ids.shape, features]. A position whose id is `ignore_index`, which may be a
     class, has no token: its row is zeros. Any other id that is no class gives a row of NaN, and device_status() raises."""
+    if (out := _native.embedding(table, ids, scale, ignore_index, out_dtype)) is not None:
+        return out
     device = _device_of("embedding", table, ids)
     if table.dim() != 2:
         raise ValueError("embedding: the table is of rank 2")
@@ -638,6 +640,8 @@ def embedding_grad(dy: torch.Tensor, ids: torch.Tensor, classes: int, *, scale: 
     """The gradient of embedding's table [classes, features] from its result's gradient dy [*ids.shape, features]: row c is scale times the sum of dy's rows whose id is c,
     in f32, the same call after call. Positions without a token and ids that are no class add nothing; the latter make device_status() raise. add_to: a gradient of the table's
     (of a tied output layer, or of an earlier part of the batch) that the sums are added to, in place, and which is returned; rows of classes that do not occur are not touched."""
+    if add_to is None and (out := _native.embedding_grad(dy, ids, classes, scale, ignore_index, out_dtype)) is not None:
+        return out
     device = _device_of("embedding_grad", dy, ids, add_to)
     if dy.dim() < 1 or dy.shape[:-1] != ids.shape:
         raise ValueError("embedding_grad: one row of dy for each id")
@@ -722,6 +726,10 @@ def _residual_desc(what, r, h, gamma, post_gamma, gate, eps, residual_scale, bra
 
 def _residual_fwd(what, r, h, gamma, eps, post_gamma, gate, residual_scale, branch_scale, keep):
     eps, residual_scale, branch_scale = float(eps), float(residual_scale), float(branch_scale)
+    kinds = h is not None, gamma is not None, post_gamma is not None, gate is not None, eps, residual_scale, branch_scale
+    if (out := _native.residual_rmsnorm(r, h, gamma, post_gamma, gate, eps, residual_scale, branch_scale, keep)) is not None:
+        new, x, kept = out
+        return r if h is None else new, x, ResidualKept(kept, (kept.shape[1], r.shape[-1], *kinds)) if keep else None
     d, held, device, put = _residual_desc(what, r, h, gamma, post_gamma, gate, eps, residual_scale, branch_scale)
     new, x, kept = r, None, None
     if h is not None:
@@ -735,7 +743,7 @@ def _residual_fwd(what, r, h, gamma, eps, post_gamma, gate, residual_scale, bran
         d.kept = kept.data_ptr()
     with torch.cuda.device(device):
         L.check(L.lib().mimk_residual_rmsnorm_fwd(C.byref(d), _stream()), what)
-    return new, x, None if kept is None else ResidualKept(kept, ((d.n, d.d), h is not None, gamma is not None, post_gamma is not None, gate is not None, eps, residual_scale, branch_scale))
+    return new, x, ResidualKept(kept, (d.n, d.d, *kinds)) if keep else None
 
 
 def residual_rmsnorm(r: torch.Tensor, h: torch.Tensor | None, gamma: torch.Tensor | None, eps: float, *, post_gamma: torch.Tensor | None = None,
@@ -757,9 +765,11 @@ def residual_rmsnorm_bwd(dr: torch.Tensor | None, dx: torch.Tensor | None, r: to
                          post_gamma: torch.Tensor | None = None, gate: torch.Tensor | None = None):
     """The gradients (of r, h, gamma, post_gamma, gate; None for what there is not) of the residual_rmsnorm_fwd call that gave `kept`, from those of its results r' (dr, None:
     nothing arrives there) and x (dx, None without gamma). Each has its operand's shape and element type; a gate's row gets the sum over the rows that share it."""
+    if (out := _native.residual_rmsnorm_bwd(dr, dx, r, h, gamma, post_gamma, gate, kept.buffer, kept.call)) is not None:
+        return out
     what = "residual_rmsnorm_bwd"
-    d, held, device, put = _residual_desc(what, r, h, gamma, post_gamma, gate, *kept.call[5:])
-    if ((d.n, d.d), h is not None, gamma is not None, post_gamma is not None, gate is not None) != kept.call[:5]:
+    d, held, device, put = _residual_desc(what, r, h, gamma, post_gamma, gate, *kept.call[6:])
+    if (d.n, d.d, h is not None, gamma is not None, post_gamma is not None, gate is not None) != kept.call[:6]:
         raise ValueError(f"{what}: `kept` is of a call with other operands")
     if (dx is None) != (gamma is None):
         raise ValueError(f"{what}: dx is the gradient of x, which there is with gamma")
@@ -807,6 +817,8 @@ def orthogonalize(x, *, steps: int = 5, coefficients=NEWTON_SCHULZ, eps: float =
     matrix, then `steps` times X <- p X + (q A + r A^2) X, A = X X^T (by X^T X where x is taller than wide), (p, q, r) = coefficients, or coefficients[step] where there are `steps` of them; the result is
     scale * X. x: a matrix, a stack of them (leading axes), or a list of either, for which the result is a list; those of one shape are multiplied together. Transposed views give transposed results.
     The products' operands are rounded to 11 bits; the result is off by up to 1e-3 of its 2-norm before it is rounded to BF16, several times that for matrices of a few rows and hardly any rank."""
+    if (out := _native.orthogonalize(x, steps, coefficients, eps, scale)) is not None:
+        return out
     what = "orthogonalize"
     matrices = [x] if isinstance(x, torch.Tensor) else list(x)
     p = [float(v) for c in coefficients for v in (c if isinstance(c, (tuple, list)) else (c,))]
