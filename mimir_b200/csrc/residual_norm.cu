@@ -226,12 +226,410 @@ __global__ void __launch_bounds__(MAXT, 1) backward_kernel(const __grid_constant
     }
 }
 
-// out[group, c] = the sum of `count` rows of partial sums; 32 columns and 32 runs of rows a block
+// ---- the same with rows on their way in shared memory --------------------------------------------------------------------------------
+// Each thread copies the columns that are its own, some rows ahead, into places of its own (cp.async), so that what is on its way takes no registers and no barrier.
+// Columns are taken in chunks of eight that start on 16-byte boundaries: of a row that begins `lead` elements past one, the first chunk has the end of the row
+// before it and the last one the beginning of the next, which are left out when values are read. With 8 / gcd(d, 8) classes of rows, a row's number modulo that count
+// decides its lead: a team's rows are all of one class, so that its columns are the same in every row.
+template <class T>
+constexpr int PLANES = sizeof(T) * 8 / 16;  // 16-byte pieces of a chunk
+
+__device__ __forceinline__ void copy_async(uint32_t to, const void* from, int bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copies_end() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// at most n groups of copies of this thread still on their way
+__device__ __forceinline__ void copies_wait(int n) {
+    switch (n) {
+        case 0: asm volatile("cp.async.wait_group 0;" ::: "memory"); break;
+        case 1: asm volatile("cp.async.wait_group 1;" ::: "memory"); break;
+        case 2: asm volatile("cp.async.wait_group 2;" ::: "memory"); break;
+        case 3: asm volatile("cp.async.wait_group 3;" ::: "memory"); break;
+        case 4: asm volatile("cp.async.wait_group 4;" ::: "memory"); break;
+        case 5: asm volatile("cp.async.wait_group 5;" ::: "memory"); break;
+        case 6: asm volatile("cp.async.wait_group 6;" ::: "memory"); break;
+        default: asm volatile("cp.async.wait_group 7;" ::: "memory"); break;
+    }
+}
+__device__ __forceinline__ uint4 take16(uint32_t at) {
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ void leave16(uint32_t at, float a, float b, float c, float d) {
+    asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(at), "f"(a), "f"(b), "f"(c), "f"(d) : "memory");
+}
+
+struct Ring {
+    int team, teams;      // threads of a team, teams in the whole grid (a multiple of the classes)
+    int classes, stages;
+};
+// Which rows a team takes: units of rows (group, piece, piece + pieces, ...), of its class.
+struct Walk {
+    int64_t unit, row, end, group;
+    int64_t w, step, per, n, run, pieces, units;
+    int cls, classes;
+    template <class A>
+    __device__ __forceinline__ Walk(const A& g, const Ring& k, int64_t team)
+        : w(team / k.classes - k.teams / k.classes), step(k.teams / k.classes), n(g.n), run(g.gate_rows), pieces(g.pieces), units(g.groups * g.pieces), cls(int(team % k.classes)), classes(k.classes) {
+        per = pieces % classes ? 0 : pieces / classes;
+        row = end = 0;
+    }
+    // the next row of the unit, or the first of the team's next one; false: there is none
+    __device__ __forceinline__ bool next() {
+        row += pieces;
+        while (row >= end) {
+            w += step;
+            int64_t piece;
+            if (per) {
+                group = w / per, piece = (w - group * per) * classes;
+                if (group * pieces >= units) return false;
+                int shift = int((cls - (group * run + piece)) % classes);
+                piece += shift < 0 ? shift + classes : shift;
+            } else {  // units of one row
+                const int64_t u = w * classes + cls;
+                if (u >= units) return false;
+                group = u / run, piece = u - group * run;
+            }
+            unit = group * pieces + piece, row = group * run + piece, end = min(n, (group + 1) * run);
+        }
+        return true;
+    }
+};
+
+template <class T>
+struct Chunks {  // a tensor's chunks in a team's shared memory
+    const T* p;
+    int64_t count;  // of its elements
+    // chunk at element `at`, a multiple of eight
+    __device__ __forceinline__ void copy(uint32_t to, uint32_t plane, int64_t at) const {
+#pragma unroll
+        for (int q = 0; q < PLANES<T>; ++q) {
+            const int64_t left = (count - at) * int64_t(sizeof(T)) - q * 16;
+            copy_async(to + q * plane, p + (left > 0 ? at + q * (16 / int(sizeof(T))) : 0), left >= 16 ? 16 : left > 0 ? int(left) : 0);
+        }
+    }
+    static __device__ __forceinline__ void get(uint32_t from, uint32_t plane, float (&v)[8]) {
+        Run<T, 8> r;
+        r.a = take16(from);
+        if constexpr (PLANES<T> == 2) r.b = take16(from + plane);
+        r.get(v);
+    }
+};
+// Columns [lo, hi) of a chunk belong to the row.
+__device__ __forceinline__ void only(float (&v)[8], int lo, int hi) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = j >= lo && j < hi ? v[j] : 0.f;
+}
+template <class T>
+__device__ __forceinline__ void put_part(T* p, const float (&v)[8], int lo, int hi) {
+    if (lo == 0 && hi == 8) {
+        put(p, v);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (j >= lo && j < hi) put(p + j, *reinterpret_cast<const float(*)[1]>(v + j));
+    }
+}
+// the same where rows are not laid out by chunks (partial sums, a gate's gradient)
+template <class T>
+__device__ __forceinline__ void put_anywhere(T* p, const float (&v)[8], int lo, int hi) {
+    if (lo == 0 && hi == 8 && reinterpret_cast<uintptr_t>(p) % 16 == 0) {
+        put(p, v);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (j >= lo && j < hi) put(p + j, *reinterpret_cast<const float(*)[1]>(v + j));
+    }
+}
+// eight factors from column `at` on, of which those in [lo, hi) are there; zeros for the others
+__device__ __forceinline__ void factors_part(const Factors& f, int64_t at, int lo, int hi, float (&v)[8]) {
+    if (lo == 0 && hi == 8 && (reinterpret_cast<uintptr_t>(f.p) + uintptr_t(at) * (f.bf16 ? 2 : 4)) % 16 == 0) {
+        factors_at(f, at, v);
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        float one[1] = {0.f};
+        if (j >= lo && j < hi) factors_at(f, at + j, one);
+        v[j] = one[0];
+    }
+}
+
+// Sums over a team of k.team threads, which is of whole warps: one barrier, places in turn.
+template <int N>
+__device__ __forceinline__ void ring_sum(float (&v)[N], float (*part)[32][N], int& turn, int team, int in_block) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = warp_sum(v[i]);
+    if (team == 32) return;
+    const int warps = team >> 5, first = in_block * warps, warp = (threadIdx.x >> 5) - first, lane = threadIdx.x & 31;
+    if (lane == 0)
+#pragma unroll
+        for (int i = 0; i < N; ++i) part[turn][first + warp][i] = v[i];
+    asm volatile("bar.sync %0, %1;" ::"r"(in_block + 1), "r"(team) : "memory");
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = warp_sum(lane < warps ? part[turn][first + lane][i] : 0.f);
+    turn ^= 1;
+}
+
+constexpr int MOST_STAGES = 8;
+
+template <class RT, class HT, int CH>
+__global__ void __launch_bounds__(512, 2) forward_ring_kernel(const __grid_constant__ Args<RT, HT> g, const __grid_constant__ Ring k) {
+    extern __shared__ __align__(16) uint8_t smem[];
+    __shared__ float part[2][32][1];
+    after_previous();
+    const int in_block = threadIdx.x / k.team, t = threadIdx.x - in_block * k.team;
+    const int64_t team = int64_t(blockIdx.x) * (blockDim.x / k.team) + in_block;
+    if (team >= k.teams) return;  // (whole teams: their barriers are their own)
+    const uint32_t plane = blockDim.x * 16, mine = uint32_t(__cvta_generic_to_shared(smem)) + threadIdx.x * 16;
+    constexpr int ROW = CH * (PLANES<RT> + PLANES<HT>);
+    const uint32_t factors = mine, ring = mine + 4 * CH * plane;  // q and gamma, f32
+    Walk cur(g, k, team), ahead = cur;
+    const int lead  = int((team % k.classes) * g.d & 7);
+    const float per = 1.f / float(g.d);
+    const Chunks<RT> r{g.r, g.n * g.d};
+    const Chunks<HT> h{g.h, g.n * g.d};
+    int lo[CH], hi[CH], at[CH];  // this thread's chunks, from the row's first on
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+        at[c] = (c * k.team + t) * 8 - lead;
+        lo[c] = max(0, -at[c]), hi[c] = int(min(int64_t(8), g.d - at[c]));  // (none: hi <= lo)
+    }
+    bool more = true;
+    auto request = [&](uint32_t stage) {
+        if (more && (more = ahead.next())) {
+#pragma unroll
+            for (int c = 0; c < CH; ++c) {
+                if (hi[c] <= lo[c]) continue;
+                const uint32_t to = ring + (stage * ROW + c * (PLANES<RT> + PLANES<HT>)) * plane;
+                r.copy(to, plane, ahead.row * g.d + at[c]);
+                if (g.h) h.copy(to + PLANES<RT> * plane, plane, ahead.row * g.d + at[c]);
+            }
+        }
+        copies_end();
+    };
+    for (int stage = 0; stage < k.stages; ++stage) request(stage);
+    int64_t group = -1;
+    uint32_t stage = 0;
+    int turn = 0;
+    while (cur.next()) {
+        if (cur.group != group) {
+            group = cur.group;
+#pragma unroll
+            for (int c = 0; c < CH; ++c) {
+                if (hi[c] <= lo[c]) continue;
+                float q[8], w[8];
+                factors_part(g.post_gamma, at[c], lo[c], hi[c], q), factors_part(g.gate, (g.gate.p ? group * g.d : 0) + at[c], lo[c], hi[c], w);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) q[j] *= g.b * w[j];
+                const uint32_t to = factors + c * 4 * plane;
+                leave16(to, q[0], q[1], q[2], q[3]), leave16(to + plane, q[4], q[5], q[6], q[7]);
+                factors_part(g.gamma, at[c], lo[c], hi[c], w);
+                leave16(to + 2 * plane, w[0], w[1], w[2], w[3]), leave16(to + 3 * plane, w[4], w[5], w[6], w[7]);
+            }
+        }
+        copies_wait(k.stages - 1);
+        float v[CH][8], hv[CH][8];
+        const uint32_t from = ring + stage * ROW * plane;
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            const uint32_t p = from + c * (PLANES<RT> + PLANES<HT>) * plane;
+            const int l = hi[c] > lo[c] ? lo[c] : 8;
+            Chunks<RT>::get(p, plane, v[c]), Chunks<HT>::get(p + PLANES<RT> * plane, plane, hv[c]);
+            if (l > 0 || hi[c] < 8) only(v[c], l, hi[c]), only(hv[c], l, hi[c]);
+        }
+        request(stage);
+        if (++stage == uint32_t(k.stages)) stage = 0;
+        float e = 1.f, s = 1.f, sum[1] = {0.f};
+        if (g.post_gamma.p) {
+#pragma unroll
+            for (int c = 0; c < CH; ++c)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) sum[0] = fmaf(hv[c][j], hv[c][j], sum[0]);
+            ring_sum(sum, part, turn, k.team, in_block);
+            e = 1.f / sqrtf(sum[0] * per + g.eps);
+        }
+        sum[0] = 0.f;
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            if (hi[c] <= lo[c]) continue;
+            if (g.h) {
+                float q[8];
+                Chunks<float>::get(factors + c * 4 * plane, plane, q);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[c][j] = fmaf(g.a, v[c][j], q[j] * (hv[c][j] * e));
+                put_part(g.r_out + cur.row * g.d + at[c], v[c], lo[c], hi[c]);
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) sum[0] = fmaf(v[c][j], v[c][j], sum[0]);
+        }
+        if (g.gamma.p) {
+            ring_sum(sum, part, turn, k.team, in_block);
+            s = 1.f / sqrtf(sum[0] * per + g.eps);
+#pragma unroll
+            for (int c = 0; c < CH; ++c) {
+                if (hi[c] <= lo[c]) continue;
+                float w[8];
+                Chunks<float>::get(factors + (c * 4 + 2) * plane, plane, w);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[c][j] *= s * w[j];
+                put_part(g.x + cur.row * g.d + at[c], v[c], lo[c], hi[c]);
+            }
+        }
+        if (g.kept && t == 0) g.kept[cur.row] = e, g.kept[g.n + cur.row] = s;
+    }
+}
+
+// GROUPS: the gate has several rows, so that sum D h^ is needed for each unit of rows; else one for all rows will do, from which both dpost_gamma and dgate follow.
+template <class RT, class HT, int CH, bool GROUPS>
+__global__ void __launch_bounds__(512, 1) backward_ring_kernel(const __grid_constant__ Args<RT, HT> g, const __grid_constant__ Ring k) {
+    extern __shared__ __align__(16) uint8_t smem[];
+    __shared__ float part[2][32][3];
+    after_previous();
+    const int in_block = threadIdx.x / k.team, t = threadIdx.x - in_block * k.team;
+    const int64_t team = int64_t(blockIdx.x) * (blockDim.x / k.team) + in_block;
+    if (team >= k.teams) return;
+    const uint32_t plane = blockDim.x * 16, mine = uint32_t(__cvta_generic_to_shared(smem)) + threadIdx.x * 16;
+    constexpr int PAIR = PLANES<RT> + PLANES<HT>, ROW = CH * 2 * PAIR;
+    const uint32_t factors = mine, ring = mine + 4 * CH * plane;
+    Walk cur(g, k, team), ahead = cur;
+    const int lead  = int((team % k.classes) * g.d & 7);
+    const float per = 1.f / float(g.d);
+    const Chunks<RT> r{g.r, g.n * g.d}, dr{g.dr_out, g.n * g.d};
+    const Chunks<HT> h{g.h, g.n * g.d}, dx{g.dx, g.n * g.d};
+    int lo[CH], hi[CH], at[CH];
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+        at[c] = (c * k.team + t) * 8 - lead;
+        lo[c] = max(0, -at[c]), hi[c] = int(min(int64_t(8), g.d - at[c]));
+        // what there is no tensor for stays zero
+        for (int stage = 0; stage < k.stages; ++stage)
+            for (int q = 0; q < 2 * PAIR; ++q) leave16(ring + (stage * ROW + c * 2 * PAIR + q) * plane, 0.f, 0.f, 0.f, 0.f);
+    }
+    bool more = true;
+    auto request = [&](uint32_t stage) {
+        if (more && (more = ahead.next())) {
+#pragma unroll
+            for (int c = 0; c < CH; ++c) {
+                if (hi[c] <= lo[c]) continue;
+                const uint32_t to = ring + (stage * ROW + c * 2 * PAIR) * plane;
+                const int64_t p   = ahead.row * g.d + at[c];
+                r.copy(to, plane, p);
+                if (g.h) h.copy(to + PLANES<RT> * plane, plane, p);
+                if (g.dr_out) dr.copy(to + PAIR * plane, plane, p);
+                if (g.dx) dx.copy(to + (PAIR + PLANES<RT>) * plane, plane, p);
+            }
+        }
+        copies_end();
+    };
+    for (int stage = 0; stage < k.stages; ++stage) request(stage);
+    float dgamma[CH][8] = {}, z[CH][8] = {}, dpost[GROUPS ? CH : 1][8] = {};
+    // the sums of a unit of rows: dgate's, and (as the gate changes) dpost_gamma's
+    auto finish = [&](int64_t unit, int64_t group) {
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            if (hi[c] <= lo[c]) continue;
+            float f[8], w[8];
+            factors_part(g.post_gamma, at[c], lo[c], hi[c], f), factors_part(g.gate, group * g.d + at[c], lo[c], hi[c], w);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) dpost[c][j] = fmaf(g.b * w[j], z[c][j], dpost[c][j]), f[j] *= g.b * z[c][j], z[c][j] = 0.f;
+            if (g.pieces > 1) put_anywhere(g.part_gate + unit * g.d + at[c], f, lo[c], hi[c]);
+            else if (g.gate.bf16) put_anywhere(static_cast<__nv_bfloat16*>(g.dgate) + group * g.d + at[c], f, lo[c], hi[c]);
+            else put_anywhere(static_cast<float*>(g.dgate) + group * g.d + at[c], f, lo[c], hi[c]);
+        }
+    };
+    int64_t group = -1, unit = -1;
+    uint32_t stage = 0;
+    int turn = 0;
+    while (cur.next()) {
+        if constexpr (GROUPS) {
+            if (cur.unit != unit && unit >= 0) finish(unit, group);
+            unit = cur.unit;
+        }
+        if (cur.group != group) {
+            group = cur.group;
+#pragma unroll
+            for (int c = 0; c < CH; ++c) {
+                if (hi[c] <= lo[c]) continue;
+                float q[8], w[8];
+                factors_part(g.post_gamma, at[c], lo[c], hi[c], q), factors_part(g.gate, (g.gate.p ? group * g.d : 0) + at[c], lo[c], hi[c], w);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) q[j] *= g.b * w[j];
+                const uint32_t to = factors + c * 4 * plane;
+                leave16(to, q[0], q[1], q[2], q[3]), leave16(to + plane, q[4], q[5], q[6], q[7]);
+                factors_part(g.gamma, at[c], lo[c], hi[c], w);
+                leave16(to + 2 * plane, w[0], w[1], w[2], w[3]), leave16(to + 3 * plane, w[4], w[5], w[6], w[7]);
+            }
+        }
+        const float e = g.post_gamma.p ? g.kept[cur.row] : 1.f, s = g.gamma.p ? g.kept[g.n + cur.row] : 1.f;
+        copies_wait(k.stages - 1);
+        float hat[CH][8], rhat[CH][8], before[CH][8], q[CH][8], sum[3] = {};
+        const uint32_t from = ring + stage * ROW * plane;
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            const uint32_t p = from + c * 2 * PAIR * plane;
+            const int l      = hi[c] > lo[c] ? lo[c] : 8;
+            float w[8], d[8];
+            Chunks<RT>::get(p, plane, rhat[c]), Chunks<HT>::get(p + PLANES<RT> * plane, plane, hat[c]);
+            Chunks<RT>::get(p + PAIR * plane, plane, before[c]), Chunks<HT>::get(p + (PAIR + PLANES<RT>) * plane, plane, d);
+            Chunks<float>::get(factors + c * 4 * plane, plane, q[c]), Chunks<float>::get(factors + (c * 4 + 2) * plane, plane, w);
+            if (l > 0 || hi[c] < 8) only(rhat[c], l, hi[c]), only(hat[c], l, hi[c]), only(before[c], l, hi[c]), only(d, l, hi[c]), only(q[c], l, hi[c]), only(w, l, hi[c]);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                hat[c][j] *= e;
+                const float qh = q[c][j] * hat[c][j], t = d[j] * w[j];
+                rhat[c][j]   = s * fmaf(g.a, rhat[c][j], qh);
+                before[c][j] = fmaf(s, t, before[c][j]);
+                dgamma[c][j] = fmaf(d[j], rhat[c][j], dgamma[c][j]);
+                sum[0] = fmaf(t, rhat[c][j], sum[0]), sum[1] = fmaf(qh, before[c][j], sum[1]), sum[2] = fmaf(qh, rhat[c][j], sum[2]);
+            }
+        }
+        request(stage);
+        if (++stage == uint32_t(k.stages)) stage = 0;
+        ring_sum(sum, part, turn, k.team, in_block);
+        const float m0 = g.gamma.p ? s * sum[0] * per : 0.f, m = g.post_gamma.p ? (sum[1] - m0 * sum[2]) * per : 0.f;
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            if (hi[c] <= lo[c]) continue;
+            float out[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float D = fmaf(-m0, rhat[c][j], before[c][j]);
+                out[j]        = g.a * D;
+                z[c][j]       = fmaf(D, hat[c][j], z[c][j]);
+                q[c][j]       = e * fmaf(q[c][j], D, -hat[c][j] * m);
+            }
+            put_part(g.dr + cur.row * g.d + at[c], out, lo[c], hi[c]);
+            if (g.dh) put_part(g.dh + cur.row * g.d + at[c], q[c], lo[c], hi[c]);
+        }
+    }
+    if constexpr (GROUPS) {
+        if (unit >= 0) finish(unit, group);
+    }
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+        if (hi[c] <= lo[c]) continue;
+        if (g.part_gamma) put_anywhere(g.part_gamma + team * g.d + at[c], dgamma[c], lo[c], hi[c]);
+        if constexpr (GROUPS) {
+            if (g.part_post) put_anywhere(g.part_post + team * g.d + at[c], dpost[c], lo[c], hi[c]);
+        } else {
+            if (g.part_post) put_anywhere(g.part_post + team * g.d + at[c], z[c], lo[c], hi[c]);
+        }
+    }
+}
+
+// out[group, c] = factor[c] times the sum of `count` rows of partial sums, into up to two results; 32 columns and 32 runs of rows a block
+struct Result {
+    void* out;
+    int bf16, times;  // times: by `by` and the factors
+    float by;
+    Factors factors;
+};
 struct Join {
     const float* part;
-    void* out;
-    int64_t groups, count;
-    int bf16;
+    int64_t groups, count, rows, run;  // a group's units: `count`, or its rows (`run` of them, of `rows` in all), one each
+    Result to[2];
 };
 struct Joins {
     Join j[3];
@@ -242,19 +640,23 @@ __global__ void __launch_bounds__(1024) join_kernel(const __grid_constant__ Join
     const Join& j   = all.j[blockIdx.z];
     const int64_t c = int64_t(blockIdx.x) * 32 + threadIdx.x;
     for (int64_t group = blockIdx.y; group < j.groups; group += gridDim.y) {
-        const float* p = j.part + group * j.count * d + c;
-        float v        = 0.f;
+        const float* p      = j.part + group * j.count * d + c;
+        const int64_t count = min(j.count, j.rows - group * j.run);
+        float v             = 0.f;
         if (c < d)
 #pragma unroll 8
-            for (int64_t k = threadIdx.y; k < j.count; k += 32) v += p[k * d];
+            for (int64_t k = threadIdx.y; k < count; k += 32) v += p[k * d];
         __syncthreads();
         sums[threadIdx.y][threadIdx.x] = v;
         __syncthreads();
         v                = warp_sum(sums[threadIdx.x][threadIdx.y]);  // a warp for each column
         const int64_t to = int64_t(blockIdx.x) * 32 + threadIdx.y;
-        if (threadIdx.x == 0 && to < d) {
-            if (j.bf16) static_cast<__nv_bfloat16*>(j.out)[group * d + to] = __float2bfloat16(v);
-            else static_cast<float*>(j.out)[group * d + to] = v;
+        if (threadIdx.x < 2 && to < d && j.to[threadIdx.x].out) {
+            const Result& r = j.to[threadIdx.x];
+            float one[1]    = {1.f};
+            if (r.times) factors_at(r.factors, to, one), v *= r.by * one[0];
+            if (r.bf16) static_cast<__nv_bfloat16*>(r.out)[group * d + to] = __float2bfloat16(v);
+            else static_cast<float*>(r.out)[group * d + to] = v;
         }
     }
 }
@@ -284,36 +686,63 @@ int misplaced(const Desc& d) {
     if (off(d.gate, d.gate_dtype) || off(d.dgate, d.gate_dtype) || off(d.kept, MIMK_F32)) return MIMK_E_ALIGN;
     return MIMK_OK;
 }
-bool vectors(const Desc& d) {
-    bool all = d.d % 8 == 0;
+// whether all tensors start on 16 bytes
+bool aligned(const Desc& d) {
+    bool all = true;
     for (const void* p : {d.r, d.h, d.gamma, d.post_gamma, d.gate, static_cast<const void*>(d.r_out), static_cast<const void*>(d.x), d.dr_out, d.dx, static_cast<const void*>(d.dr),
                           static_cast<const void*>(d.dh), static_cast<const void*>(d.dgate)})
         all = all && aligned16(p);
     return all;
 }
 
-// How rows are dealt out: threads and rows of a block, and for the backward pass blocks and units of rows.
+// How rows are dealt out: threads and rows of a block, blocks, and units of rows; and what the backward pass leaves for the second launch.
 struct Plan {
-    int threads, rows, blocks;
-    int64_t groups, pieces;
+    bool ring;
+    int threads, rows, blocks, columns;  // columns: eights of them that a thread holds (ring)
+    Ring k;
+    size_t smem;
+    int64_t teams, groups, pieces;
     float *gamma, *post, *gate;
 };
-Plan plan(const Desc& d, bool vec, Space& space, int sm_count) {
+constexpr size_t MOST_SMEM = 200 << 10;
+Plan plan(const Desc& d, bool backward, bool aligned, Space& space, int sm_count) {
     Plan p{};
-    const int64_t each = d.d <= 2048 ? 8 : d.d <= 8192 ? 16 : 32, lanes = up((d.d + each - 1) / each, 32);
-    (void)vec;
-    p.threads = int(lanes), p.rows = lanes == 32 ? 4 : 1;
-    // (registers for 512 threads or so of 16 columns with their three sums on an SM)
-    const int64_t most = int64_t(sm_count) * (lanes <= 128 ? 4 : lanes <= 256 ? 2 : 1), need = (d.n + p.rows - 1) / p.rows;
-    p.blocks = int(need < most ? (need < 1 ? 1 : need) : most);
-    const int64_t teams = int64_t(p.blocks) * p.rows, run = d.gate ? d.gate_rows : (d.n > 0 ? d.n : 1);
-    p.groups = (d.n + run - 1) / run;
-    p.pieces = p.groups ? (teams + p.groups - 1) / p.groups : 1;
+    const size_t pair = dtype_size(d.stream_dtype) + dtype_size(d.block_dtype);
+    const int64_t run = d.gate ? d.gate_rows : (d.n > 0 ? d.n : 1);
+    p.groups          = (d.n + run - 1) / run;
+    int classes       = 8;
+    while (classes > 1 && d.d % (16 / classes) == 0) classes /= 2;
+    // a team's threads hold eight columns each, sixteen from 4096 on
+    const int64_t chunks = (d.d + (classes > 1 ? 7 : 0) + 7) / 8;
+    p.columns            = chunks <= 512 ? 1 : 2;
+    const int64_t team = up((chunks + p.columns - 1) / p.columns, 32), in_block = team >= 512 ? 1 : 512 / team, threads = team * in_block;
+    // factors, and rows on their way: as many as there is room for
+    const size_t fixed = size_t(threads) * size_t(p.columns) * 64, row = size_t(threads) * size_t(p.columns) * 8 * pair * (backward ? 2 : 1);
+    const size_t room  = backward ? MOST_SMEM : MOST_SMEM / 2;
+    p.ring             = aligned && chunks <= 1024 && fixed + row <= room;
+    if (p.ring) {
+        const size_t stages = (room - fixed) / row;
+        p.k.team = int(team), p.k.classes = classes, p.k.stages = int(stages < MOST_STAGES ? stages : MOST_STAGES);
+        p.threads = int(threads), p.rows = int(in_block), p.smem = fixed + size_t(p.k.stages) * row;
+        const int64_t most = int64_t(sm_count) * (backward ? 1 : 2) * in_block, need = up(d.n, classes);
+        p.k.teams = int((need < most ? need : most) / classes * classes);
+        p.teams   = p.k.teams;
+        p.blocks  = int((p.teams + in_block - 1) / in_block);
+        p.pieces  = up((p.teams + p.groups - 1) / (p.groups ? p.groups : 1), classes);
+    } else {
+        const int64_t each = d.d <= 2048 ? 8 : d.d <= 8192 ? 16 : 32, lanes = up((d.d + each - 1) / each, 32);
+        p.threads = int(lanes), p.rows = lanes == 32 ? 4 : 1;
+        const int64_t most = int64_t(sm_count) * (lanes <= 128 ? 4 : lanes <= 256 ? 2 : 1), need = (d.n + p.rows - 1) / p.rows;
+        p.blocks = int(need < most ? (need < 1 ? 1 : need) : most);
+        p.teams  = int64_t(p.blocks) * p.rows;
+        p.pieces = p.groups ? (p.teams + p.groups - 1) / p.groups : 1;
+    }
     if (p.pieces > run) p.pieces = run;
+    if (!backward) return p;
     auto part = [&](int64_t rows) { return static_cast<float*>(space.take(size_t(rows) * size_t(d.d) * 4)); };
-    if (d.gamma) p.gamma = part(teams);
-    if (d.post_gamma) p.post = part(teams);
-    if (d.gate && p.pieces > 1) p.gate = part(p.groups * p.pieces);
+    if (d.gamma) p.gamma = part(p.teams);
+    if (d.post_gamma || (d.gate && p.ring && p.groups == 1)) p.post = part(p.teams);
+    if (d.gate && p.pieces > 1 && !(p.ring && p.groups == 1)) p.gate = part(p.groups * p.pieces);
     return p;
 }
 
@@ -329,37 +758,58 @@ Args<RT, HT> args_of(const Desc& d) {
     return g;
 }
 
-template <class RT, class HT, int VEC>
-int forward(const Desc& d, const Plan& p, const DeviceInfo& dev, cudaStream_t s) {
-    const Args<RT, HT> g = args_of<RT, HT>(d);
-    const auto kern = d.d <= 2048 ? forward_kernel<RT, HT, VEC, 8 / VEC, 256> : d.d <= 8192 ? forward_kernel<RT, HT, VEC, 16 / VEC, 512> : forward_kernel<RT, HT, VEC, 32 / VEC, 1024>;
-    const int64_t blocks = (d.n + p.rows - 1) / p.rows;
+template <auto KERN, class A>
+int launch_ring(const Plan& p, const A& g, const DeviceInfo& dev, cudaStream_t s) {
+    static bool configured[64] = {};
+    if (!configured[dev.device & 63]) {
+        MIMK_CUDA_TRY(cudaFuncSetAttribute(KERN, cudaFuncAttributeMaxDynamicSharedMemorySize, int(MOST_SMEM)));
+        configured[dev.device & 63] = true;
+    }
+    return launch_after(KERN, unsigned(p.blocks), unsigned(p.threads), p.smem, s, g, p.k);
+}
+template <class... P, class... A>
+int launch(void (*kern)(P...), dim3 grid, dim3 block, cudaStream_t s, A&&... args) {
     cudaLaunchAttribute early = {};
     early.id = cudaLaunchAttributeProgrammaticStreamSerialization, early.val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t config = {};
-    config.gridDim = dim3(unsigned(blocks < (1 << 20) ? blocks : 1 << 20)), config.blockDim = dim3(p.threads, p.rows), config.stream = s, config.attrs = &early, config.numAttrs = 1;
-    return note_cuda_error(cudaLaunchKernelEx(&config, kern, g));
+    config.gridDim = grid, config.blockDim = block, config.stream = s, config.attrs = &early, config.numAttrs = 1;
+    return note_cuda_error(cudaLaunchKernelEx(&config, kern, static_cast<A&&>(args)...));
+}
+
+template <class RT, class HT, int VEC>
+int forward(const Desc& d, const Plan& p, const DeviceInfo& dev, cudaStream_t s) {
+    Args<RT, HT> g = args_of<RT, HT>(d);
+    g.groups = p.groups, g.pieces = p.pieces;
+    if (p.ring) return p.columns == 1 ? launch_ring<forward_ring_kernel<RT, HT, 1>>(p, g, dev, s) : launch_ring<forward_ring_kernel<RT, HT, 2>>(p, g, dev, s);
+    const auto kern = d.d <= 2048 ? forward_kernel<RT, HT, VEC, 8 / VEC, 256> : d.d <= 8192 ? forward_kernel<RT, HT, VEC, 16 / VEC, 512> : forward_kernel<RT, HT, VEC, 32 / VEC, 1024>;
+    const int64_t blocks = (d.n + p.rows - 1) / p.rows;
+    return launch(kern, dim3(unsigned(blocks < (1 << 20) ? blocks : 1 << 20)), dim3(p.threads, p.rows), s, g);
 }
 template <class RT, class HT, int VEC>
 int backward(const Desc& d, const Plan& p, const DeviceInfo& dev, cudaStream_t s) {
     Args<RT, HT> g = args_of<RT, HT>(d);
     g.part_gamma = p.gamma, g.part_post = p.post, g.part_gate = p.gate, g.groups = p.groups, g.pieces = p.pieces;
-    const auto kern = d.d <= 2048 ? backward_kernel<RT, HT, VEC, 8 / VEC, 256> : d.d <= 8192 ? backward_kernel<RT, HT, VEC, 16 / VEC, 512> : backward_kernel<RT, HT, VEC, 32 / VEC, 1024>;
-    cudaLaunchAttribute early = {};
-    early.id = cudaLaunchAttributeProgrammaticStreamSerialization, early.val.programmaticStreamSerializationAllowed = 1;
-    cudaLaunchConfig_t config = {};
-    config.gridDim = dim3(unsigned(p.blocks)), config.blockDim = dim3(p.threads, p.rows), config.stream = s, config.attrs = &early, config.numAttrs = 1;
-    MIMK_TRY(note_cuda_error(cudaLaunchKernelEx(&config, kern, g)));
+    const bool several = p.groups > 1;
+    if (p.ring && p.columns == 1) {
+        MIMK_TRY((several ? launch_ring<backward_ring_kernel<RT, HT, 1, true>>(p, g, dev, s) : launch_ring<backward_ring_kernel<RT, HT, 1, false>>(p, g, dev, s)));
+    } else if (p.ring) {
+        MIMK_TRY((several ? launch_ring<backward_ring_kernel<RT, HT, 2, true>>(p, g, dev, s) : launch_ring<backward_ring_kernel<RT, HT, 2, false>>(p, g, dev, s)));
+    } else {
+        const auto kern = d.d <= 2048 ? backward_kernel<RT, HT, VEC, 8 / VEC, 256> : d.d <= 8192 ? backward_kernel<RT, HT, VEC, 16 / VEC, 512> : backward_kernel<RT, HT, VEC, 32 / VEC, 1024>;
+        MIMK_TRY(launch(kern, dim3(unsigned(p.blocks)), dim3(p.threads, p.rows), s, g));
+    }
     Joins all{};
-    int count           = 0;
-    int64_t most        = 1;
-    const int64_t teams = int64_t(p.blocks) * p.rows;
-    if (p.gamma) all.j[count++] = {p.gamma, d.dgamma, 1, teams, d.gamma_dtype == MIMK_BF16};
-    if (p.post) all.j[count++] = {p.post, d.dpost_gamma, 1, teams, d.post_gamma_dtype == MIMK_BF16};
-    if (p.gate) all.j[count++] = {p.gate, d.dgate, p.groups, p.pieces, d.gate_dtype == MIMK_BF16}, most = p.groups;
+    int count    = 0;
+    int64_t most = 1;
+    if (p.gamma) all.j[count++] = {p.gamma, 1, p.teams, p.teams, 0, {{d.dgamma, d.gamma_dtype == MIMK_BF16}}};
+    if (p.post && p.ring && !several) {
+        all.j[count++] = {p.post, 1, p.teams, p.teams, 0, {{d.post_gamma ? d.dpost_gamma : nullptr, d.post_gamma_dtype == MIMK_BF16, 1, g.b, g.gate}, {d.gate ? d.dgate : nullptr, d.gate_dtype == MIMK_BF16, 1, g.b, g.post_gamma}}};
+    } else if (p.post) {
+        all.j[count++] = {p.post, 1, p.teams, p.teams, 0, {{d.dpost_gamma, d.post_gamma_dtype == MIMK_BF16}}};
+    }
+    if (p.gate) all.j[count++] = {p.gate, p.groups, p.pieces, d.n, g.gate_rows, {{d.dgate, d.gate_dtype == MIMK_BF16}}}, most = p.groups;
     if (!count) return MIMK_OK;
-    config.gridDim = dim3(unsigned((d.d + 31) / 32), unsigned(most < 65535 ? most : 65535), unsigned(count)), config.blockDim = dim3(32, 32);
-    return note_cuda_error(cudaLaunchKernelEx(&config, join_kernel, all, d.d));
+    return launch(join_kernel, dim3(unsigned((d.d + 31) / 32), unsigned(most < 65535 ? most : 65535), unsigned(count)), dim3(32, 32), s, all, d.d);
 }
 
 #define MIMK_BY_TYPES(F, VEC, ...)                                                                        \
@@ -387,9 +837,9 @@ extern "C" int mimk_residual_rmsnorm_fwd(const mimk_residual_rmsnorm_desc* d, vo
     MIMK_TRY(misplaced(*d));
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     Space space(nullptr);
-    const bool vec = vectors(*d);
-    const Plan p   = plan(*d, vec, space, dev->sm_count);
-    return vec ? MIMK_BY_TYPES(forward, 8, *d, p, *dev, s) : MIMK_BY_TYPES(forward, 1, *d, p, *dev, s);
+    const bool whole = aligned(*d);
+    const Plan p     = plan(*d, false, whole, space, dev->sm_count);
+    return whole && d->d % 8 == 0 ? MIMK_BY_TYPES(forward, 8, *d, p, *dev, s) : MIMK_BY_TYPES(forward, 1, *d, p, *dev, s);
 }
 
 extern "C" int mimk_residual_rmsnorm_workspace(const mimk_residual_rmsnorm_desc* d, uint64_t* bytes) {
@@ -399,8 +849,13 @@ extern "C" int mimk_residual_rmsnorm_workspace(const mimk_residual_rmsnorm_desc*
     const DeviceInfo* dev = device_info(&st);
     if (!dev) return st;
     Space space(nullptr);
-    plan(*d, false, space, dev->sm_count);
-    *bytes = space.used();
+    *bytes = 0;
+    if (!d->n || !d->d) return MIMK_OK;
+    // (whatever the tensors' addresses turn out to be)
+    plan(*d, true, true, space, dev->sm_count);
+    Space other(nullptr);
+    plan(*d, true, false, other, dev->sm_count);
+    *bytes = space.used() > other.used() ? space.used() : other.used();
     return MIMK_OK;
 }
 
@@ -420,9 +875,9 @@ extern "C" int mimk_residual_rmsnorm_bwd(const mimk_residual_rmsnorm_desc* d, vo
     if ((d->gamma || d->post_gamma) && !d->kept) return MIMK_E_ARG;
     MIMK_TRY(misplaced(*d));
     Space space(d->workspace);
-    const bool vec = vectors(*d);
-    const Plan p   = plan(*d, vec, space, dev->sm_count);
+    const bool whole = aligned(*d);
+    const Plan p     = plan(*d, true, whole, space, dev->sm_count);
     if (space.used() > d->workspace_bytes || (space.used() && !d->workspace)) return MIMK_E_WORKSPACE;
     if (space.used() && !aligned16(d->workspace)) return MIMK_E_ALIGN;
-    return vec ? MIMK_BY_TYPES(backward, 8, *d, p, *dev, s) : MIMK_BY_TYPES(backward, 1, *d, p, *dev, s);
+    return whole && d->d % 8 == 0 ? MIMK_BY_TYPES(backward, 8, *d, p, *dev, s) : MIMK_BY_TYPES(backward, 1, *d, p, *dev, s);
 }
