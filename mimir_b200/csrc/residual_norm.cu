@@ -7,6 +7,7 @@
 // computed over again from r and h, the same bytes as reading it, so that a stream kept in bf16 is not rounded on the way into the gradients.
 // Gradients over rows are summed by each block over its rows, in registers, and over the blocks by a second launch.
 // What bounds it: the bytes.
+#include "attn_common.cuh"
 #include "elements.cuh"
 #include "train_common.cuh"
 
@@ -100,7 +101,7 @@ __global__ void __launch_bounds__(MAXT, 1) forward_kernel(const __grid_constant_
                 for (int j = 0; j < VEC; ++j) sum[0] = fmaf(h[j], h[j], sum[0]);
             }
             team_sum(sum);
-            e = 1.f / sqrtf(sum[0] * per + g.eps);
+            e = rsqrtf(fmaf(sum[0], per, g.eps));
         }
         const int64_t group = g.gate.p ? row / g.gate_rows : 0;
         float v[CH][VEC];
@@ -123,7 +124,7 @@ __global__ void __launch_bounds__(MAXT, 1) forward_kernel(const __grid_constant_
         float s = 1.f;
         if (g.gamma.p) {
             team_sum(sum);
-            s = 1.f / sqrtf(sum[0] * per + g.eps);
+            s = rsqrtf(fmaf(sum[0], per, g.eps));
 #pragma unroll
             for (int c = 0; c < CH; ++c) {
                 const int64_t at = (c * int(blockDim.x) + int(threadIdx.x)) * VEC;
@@ -238,18 +239,10 @@ __device__ __forceinline__ void copy_async(uint32_t to, const void* from, int by
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ void copies_end() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-// at most n groups of copies of this thread still on their way
-__device__ __forceinline__ void copies_wait(int n) {
-    switch (n) {
-        case 0: asm volatile("cp.async.wait_group 0;" ::: "memory"); break;
-        case 1: asm volatile("cp.async.wait_group 1;" ::: "memory"); break;
-        case 2: asm volatile("cp.async.wait_group 2;" ::: "memory"); break;
-        case 3: asm volatile("cp.async.wait_group 3;" ::: "memory"); break;
-        case 4: asm volatile("cp.async.wait_group 4;" ::: "memory"); break;
-        case 5: asm volatile("cp.async.wait_group 5;" ::: "memory"); break;
-        case 6: asm volatile("cp.async.wait_group 6;" ::: "memory"); break;
-        default: asm volatile("cp.async.wait_group 7;" ::: "memory"); break;
-    }
+// at most N groups of copies of this thread still on their way
+template <int N>
+__device__ __forceinline__ void copies_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 __device__ __forceinline__ uint4 take16(uint32_t at) {
     uint4 v;
@@ -260,31 +253,69 @@ __device__ __forceinline__ void leave16(uint32_t at, float a, float b, float c, 
     asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(at), "f"(a), "f"(b), "f"(c), "f"(d) : "memory");
 }
 
+constexpr int THREADS = 512;                // of a block: one team of all of them, or several
+constexpr uint32_t PLANE = THREADS * 16;    // 16 bytes for each
+constexpr int MOST_SMEM = 200 << 10;
+template <int ROW>                          // planes of a row
+constexpr int STAGES = MOST_SMEM / (ROW * int(PLANE)) < 6 ? MOST_SMEM / (ROW * int(PLANE)) : 6;
+
+// Two f32 values to an instruction.
+struct F2 {
+    uint64_t v;
+    __device__ __forceinline__ F2() {}
+    __device__ __forceinline__ F2(float a, float b) : v(attn::pack2(a, b)) {}
+    __device__ __forceinline__ explicit F2(float a) : v(attn::pack2(a, a)) {}
+    __device__ __forceinline__ float sum() const {
+        float a, b;
+        attn::unpack2(v, a, b);
+        return a + b;
+    }
+};
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+    a.v = attn::fma2(a.v, b.v, c.v);
+    return a;
+}
+__device__ __forceinline__ F2 operator*(F2 a, F2 b) {
+    asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(a.v) : "l"(b.v));
+    return a;
+}
+__device__ __forceinline__ void pairs(const float (&v)[8], F2 (&p)[4]) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) p[j] = F2(v[2 * j], v[2 * j + 1]);
+}
+__device__ __forceinline__ void singles(const F2 (&p)[4], float (&v)[8]) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) attn::unpack2(p[j].v, v[2 * j], v[2 * j + 1]);
+}
+
 struct Ring {
-    int team, teams;      // threads of a team, teams in the whole grid (a multiple of the classes)
-    int classes, stages;
+    int team, teams;  // threads of a team, teams in the whole grid (a multiple of the classes)
+    int classes;
 };
 // Which rows a team takes: units of rows (group, piece, piece + pieces, ...), of its class.
 struct Walk {
-    int64_t unit, row, end, group;
-    int64_t w, step, per, n, run, pieces, units;
+    int64_t row, end, offset, unit, group;  // offset: of the row's first element
+    int64_t w, step, per, n, d, run, pieces, units;
     int cls, classes;
     template <class A>
-    __device__ __forceinline__ Walk(const A& g, const Ring& k, int64_t team)
-        : w(team / k.classes - k.teams / k.classes), step(k.teams / k.classes), n(g.n), run(g.gate_rows), pieces(g.pieces), units(g.groups * g.pieces), cls(int(team % k.classes)), classes(k.classes) {
+    __device__ __forceinline__ Walk(const A& g, const Ring& k, int team)
+        : row(0), end(0), offset(0), w(team / k.classes - k.teams / k.classes), step(k.teams / k.classes), n(g.n), d(g.d), run(g.gate_rows), pieces(g.pieces), units(g.groups * g.pieces),
+          cls(team % k.classes), classes(k.classes) {
         per = pieces % classes ? 0 : pieces / classes;
-        row = end = 0;
     }
     // the next row of the unit, or the first of the team's next one; false: there is none
     __device__ __forceinline__ bool next() {
-        row += pieces;
-        while (row >= end) {
+        row += pieces, offset += pieces * d;
+        return row < end || next_unit();
+    }
+    __device__ __forceinline__ bool next_unit() {
+        do {
             w += step;
             int64_t piece;
             if (per) {
                 group = w / per, piece = (w - group * per) * classes;
                 if (group * pieces >= units) return false;
-                int shift = int((cls - (group * run + piece)) % classes);
+                const int shift = int((cls - (group * run + piece)) % classes);
                 piece += shift < 0 ? shift + classes : shift;
             } else {  // units of one row
                 const int64_t u = w * classes + cls;
@@ -292,35 +323,44 @@ struct Walk {
                 group = u / run, piece = u - group * run;
             }
             unit = group * pieces + piece, row = group * run + piece, end = min(n, (group + 1) * run);
-        }
+        } while (row >= end);
+        offset = row * d;
         return true;
     }
 };
 
-template <class T>
-struct Chunks {  // a tensor's chunks in a team's shared memory
-    const T* p;
-    int64_t count;  // of its elements
-    // chunk at element `at`, a multiple of eight
-    __device__ __forceinline__ void copy(uint32_t to, uint32_t plane, int64_t at) const {
-#pragma unroll
-        for (int q = 0; q < PLANES<T>; ++q) {
-            const int64_t left = (count - at) * int64_t(sizeof(T)) - q * 16;
-            copy_async(to + q * plane, p + (left > 0 ? at + q * (16 / int(sizeof(T))) : 0), left >= 16 ? 16 : left > 0 ? int(left) : 0);
-        }
-    }
-    static __device__ __forceinline__ void get(uint32_t from, uint32_t plane, float (&v)[8]) {
-        Run<T, 8> r;
-        r.a = take16(from);
-        if constexpr (PLANES<T> == 2) r.b = take16(from + plane);
-        r.get(v);
-    }
-};
 // Columns [lo, hi) of a chunk belong to the row.
 __device__ __forceinline__ void only(float (&v)[8], int lo, int hi) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = j >= lo && j < hi ? v[j] : 0.f;
 }
+template <class T>
+struct Chunks {  // a tensor's chunks
+    // the chunk that begins with element `at`, a multiple of eight; `left` elements of the tensor are from there on
+    static __device__ __forceinline__ void copy(uint32_t to, const T* p, int64_t at, int left) {
+#pragma unroll
+        for (int q = 0; q < PLANES<T>; ++q) {
+            constexpr int EACH = 16 / int(sizeof(T));
+            const int here     = max(0, min(EACH, left - q * EACH));
+            copy_async(to + q * PLANE, p + at + (here ? q * EACH : 0), here * int(sizeof(T)));
+        }
+    }
+    static __device__ __forceinline__ void copy(uint32_t to, const T* p, int64_t at) {
+#pragma unroll
+        for (int q = 0; q < PLANES<T>; ++q) copy_async(to + q * PLANE, p + at + q * (16 / int(sizeof(T))), 16);
+    }
+    // a row's columns of a chunk, zeros for the others
+    template <class M>
+    static __device__ __forceinline__ void get(uint32_t from, F2 (&p)[4], const M& m, int c) {
+        Run<T, 8> r;
+        float v[8];
+        r.a = take16(from);
+        if constexpr (PLANES<T> == 2) r.b = take16(from + PLANE);
+        r.get(v);
+        if (m.part[c]) only(v, m.lo[c], m.hi[c]);
+        pairs(v, p);
+    }
+};
 template <class T>
 __device__ __forceinline__ void put_part(T* p, const float (&v)[8], int lo, int hi) {
     if (lo == 0 && hi == 8) {
@@ -356,252 +396,299 @@ __device__ __forceinline__ void factors_part(const Factors& f, int64_t at, int l
     }
 }
 
-// Sums over a team of k.team threads, which is of whole warps: one barrier, places in turn.
-template <int N>
-__device__ __forceinline__ void ring_sum(float (&v)[N], float (*part)[32][N], int& turn, int team, int in_block) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = warp_sum(v[i]);
+// Sums over a team of whole warps, in every thread: one barrier, places in turn.
+struct Sums {
+    float v[2][32][4];
+};
+__device__ __forceinline__ void meet(int team, int in_block) { asm volatile("bar.sync %0, %1;" ::"r"(in_block + 1), "r"(team) : "memory"); }
+__device__ __forceinline__ void ring_sum(float& v, Sums& part, int& turn, int team, int in_block) {
+    v = warp_sum(v);
     if (team == 32) return;
-    const int warps = team >> 5, first = in_block * warps, warp = (threadIdx.x >> 5) - first, lane = threadIdx.x & 31;
-    if (lane == 0)
+    const int warps = team >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (lane == 0) part.v[turn][warp][0] = v;
+    meet(team, in_block);
+    v = (lane & 15) < warps ? part.v[turn][in_block * warps + (lane & 15)][0] : 0.f;
 #pragma unroll
-        for (int i = 0; i < N; ++i) part[turn][first + warp][i] = v[i];
-    asm volatile("bar.sync %0, %1;" ::"r"(in_block + 1), "r"(team) : "memory");
-#pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = warp_sum(lane < warps ? part[turn][first + lane][i] : 0.f);
+    for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     turn ^= 1;
 }
+// Three sums at once. The lanes of a half keep two of four values (the fourth is nothing), those of a quarter one: six exchanges in place of fifteen.
+__device__ __forceinline__ void ring_sum(float (&v)[3], Sums& part, int& turn, int team, int in_block) {
+    const int lane = threadIdx.x & 31;
+    const bool high = lane & 16, odd = lane & 8;
+    float a = high ? v[2] : v[0], b = high ? 0.f : v[1];
+    a += __shfl_xor_sync(0xffffffffu, high ? v[0] : v[2], 16), b += __shfl_xor_sync(0xffffffffu, high ? v[1] : 0.f, 16);
+    float s = odd ? b : a;
+    s += __shfl_xor_sync(0xffffffffu, odd ? a : b, 8);
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);  // lanes 0, 8, 16: the warp's three sums
+    if (team != 32) {
+        const int warps = team >> 5, warp = threadIdx.x >> 5, at = lane & 15;
+        if ((lane & 7) == 0) part.v[turn][warp][lane >> 3] = s;
+        meet(team, in_block);
+        const float2 two = at < warps ? *reinterpret_cast<const float2*>(&part.v[turn][in_block * warps + at][high ? 2 : 0]) : make_float2(0.f, 0.f);
+        s = (odd ? two.y : two.x) + __shfl_xor_sync(0xffffffffu, odd ? two.x : two.y, 8);
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+        turn ^= 1;
+    }
+#pragma unroll
+    for (int i = 0; i < 3; ++i) v[i] = __shfl_sync(0xffffffffu, s, i * 8);
+}
 
-constexpr int MOST_STAGES = 8;
+// A thread's place: its team, and the chunks of a row that are its own.
+template <int CH>
+struct Mine {
+    int team, in_block, t;
+    int at[CH], lo[CH], hi[CH];  // first column; of the chunk's eight those that belong to the row, [lo, hi) (none: hi <= lo)
+    bool any[CH], part[CH];
+    uint32_t place;
+    __device__ __forceinline__ Mine(const Ring& k, int64_t d, const uint8_t* smem) {
+        in_block = threadIdx.x / k.team, t = threadIdx.x - in_block * k.team;
+        const int teams = THREADS / k.team;
+        team  = in_block < teams ? int(blockIdx.x) * teams + in_block : k.teams;  // (threads behind the last team: none)
+        place = uint32_t(__cvta_generic_to_shared(smem)) + threadIdx.x * 16;
+        const int lead = int((team % k.classes) * d & 7);
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            at[c] = (c * k.team + t) * 8 - lead;
+            lo[c] = max(0, -at[c]), hi[c] = int(min(int64_t(8), d - at[c]));
+            any[c] = hi[c] > lo[c], part[c] = lo[c] > 0 || hi[c] < 8;
+            if (!any[c]) lo[c] = hi[c] = 0;
+        }
+    }
+};
+// The factors of a thread's columns: q = b gate post_gamma, and gamma.
+template <int CH>
+struct Weights {
+    F2 q[CH][4], w[CH][4];
+    template <class A>
+    __device__ __forceinline__ void load(const A& g, const Mine<CH>& m, int64_t group) {
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            float post[8], gate[8], gamma[8];
+            factors_part(g.post_gamma, m.at[c], m.lo[c], m.hi[c], post), factors_part(g.gate, (g.gate.p ? group * g.d : 0) + m.at[c], m.lo[c], m.hi[c], gate);
+            factors_part(g.gamma, m.at[c], m.lo[c], m.hi[c], gamma);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) post[j] *= g.b * gate[j];
+            pairs(post, q[c]), pairs(gamma, w[c]);
+        }
+    }
+};
 
 template <class RT, class HT, int CH>
-__global__ void __launch_bounds__(512, 2) forward_ring_kernel(const __grid_constant__ Args<RT, HT> g, const __grid_constant__ Ring k) {
+__global__ void __launch_bounds__(THREADS, 1) forward_ring_kernel(const __grid_constant__ Args<RT, HT> g, const __grid_constant__ Ring k) {
     extern __shared__ __align__(16) uint8_t smem[];
-    __shared__ float part[2][32][1];
+    __shared__ Sums sums;
     after_previous();
-    const int in_block = threadIdx.x / k.team, t = threadIdx.x - in_block * k.team;
-    const int64_t team = int64_t(blockIdx.x) * (blockDim.x / k.team) + in_block;
-    if (team >= k.teams) return;  // (whole teams: their barriers are their own)
-    const uint32_t plane = blockDim.x * 16, mine = uint32_t(__cvta_generic_to_shared(smem)) + threadIdx.x * 16;
-    constexpr int ROW = CH * (PLANES<RT> + PLANES<HT>);
-    const uint32_t factors = mine, ring = mine + 4 * CH * plane;  // q and gamma, f32
-    Walk cur(g, k, team), ahead = cur;
-    const int lead  = int((team % k.classes) * g.d & 7);
-    const float per = 1.f / float(g.d);
-    const Chunks<RT> r{g.r, g.n * g.d};
-    const Chunks<HT> h{g.h, g.n * g.d};
-    int lo[CH], hi[CH], at[CH];  // this thread's chunks, from the row's first on
-#pragma unroll
-    for (int c = 0; c < CH; ++c) {
-        at[c] = (c * k.team + t) * 8 - lead;
-        lo[c] = max(0, -at[c]), hi[c] = int(min(int64_t(8), g.d - at[c]));  // (none: hi <= lo)
-    }
-    bool more = true;
+    const Mine<CH> m(k, g.d, smem);
+    if (m.team >= k.teams) return;  // (whole teams: their barriers are their own)
+    constexpr int PAIR = PLANES<RT> + PLANES<HT>, ROW = CH * PAIR;
+    Walk cur(g, k, m.team), ahead = cur;
+    const int64_t total = g.n * g.d;
+    const float per     = 1.f / float(g.d);
+    bool more           = true;
     auto request = [&](uint32_t stage) {
         if (more && (more = ahead.next())) {
+            const bool last = ahead.offset + g.d + 8 > total;  // (a chunk may end behind the tensor)
 #pragma unroll
             for (int c = 0; c < CH; ++c) {
-                if (hi[c] <= lo[c]) continue;
-                const uint32_t to = ring + (stage * ROW + c * (PLANES<RT> + PLANES<HT>)) * plane;
-                r.copy(to, plane, ahead.row * g.d + at[c]);
-                if (g.h) h.copy(to + PLANES<RT> * plane, plane, ahead.row * g.d + at[c]);
+                if (!m.any[c]) continue;
+                const uint32_t to = m.place + stage + c * PAIR * PLANE;
+                const int64_t p   = ahead.offset + m.at[c];
+                if (last) {
+                    const int left = int(min(int64_t(8), total - p));
+                    Chunks<RT>::copy(to, g.r, p, left);
+                    if (g.h) Chunks<HT>::copy(to + PLANES<RT> * PLANE, g.h, p, left);
+                } else {
+                    Chunks<RT>::copy(to, g.r, p);
+                    if (g.h) Chunks<HT>::copy(to + PLANES<RT> * PLANE, g.h, p);
+                }
             }
         }
         copies_end();
     };
-    for (int stage = 0; stage < k.stages; ++stage) request(stage);
-    int64_t group = -1;
+    for (int stage = 0; stage < STAGES<ROW>; ++stage) request(stage * ROW * PLANE);
+    Weights<CH> f;
+    int64_t group  = -1;
     uint32_t stage = 0;
-    int turn = 0;
+    int turn       = 0;
     while (cur.next()) {
-        if (cur.group != group) {
-            group = cur.group;
-#pragma unroll
-            for (int c = 0; c < CH; ++c) {
-                if (hi[c] <= lo[c]) continue;
-                float q[8], w[8];
-                factors_part(g.post_gamma, at[c], lo[c], hi[c], q), factors_part(g.gate, (g.gate.p ? group * g.d : 0) + at[c], lo[c], hi[c], w);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) q[j] *= g.b * w[j];
-                const uint32_t to = factors + c * 4 * plane;
-                leave16(to, q[0], q[1], q[2], q[3]), leave16(to + plane, q[4], q[5], q[6], q[7]);
-                factors_part(g.gamma, at[c], lo[c], hi[c], w);
-                leave16(to + 2 * plane, w[0], w[1], w[2], w[3]), leave16(to + 3 * plane, w[4], w[5], w[6], w[7]);
-            }
-        }
-        copies_wait(k.stages - 1);
-        float v[CH][8], hv[CH][8];
-        const uint32_t from = ring + stage * ROW * plane;
+        if (cur.group != group) f.load(g, m, group = cur.group);
+        copies_wait<STAGES<ROW> - 1>();
+        F2 v[CH][4], h[CH][4], squares(0.f);
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
-            const uint32_t p = from + c * (PLANES<RT> + PLANES<HT>) * plane;
-            const int l = hi[c] > lo[c] ? lo[c] : 8;
-            Chunks<RT>::get(p, plane, v[c]), Chunks<HT>::get(p + PLANES<RT> * plane, plane, hv[c]);
-            if (l > 0 || hi[c] < 8) only(v[c], l, hi[c]), only(hv[c], l, hi[c]);
+            const uint32_t p = m.place + stage + c * PAIR * PLANE;
+            Chunks<RT>::get(p, v[c], m, c), Chunks<HT>::get(p + PLANES<RT> * PLANE, h[c], m, c);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) squares = fma2(h[c][j], h[c][j], squares);
+        }
+        float e = 1.f, s = 1.f, sum = squares.sum();
+        if (g.post_gamma.p) {
+            ring_sum(sum, sums, turn, k.team, m.in_block);
+            e = rsqrtf(fmaf(sum, per, g.eps));
         }
         request(stage);
-        if (++stage == uint32_t(k.stages)) stage = 0;
-        float e = 1.f, s = 1.f, sum[1] = {0.f};
-        if (g.post_gamma.p) {
-#pragma unroll
-            for (int c = 0; c < CH; ++c)
-#pragma unroll
-                for (int j = 0; j < 8; ++j) sum[0] = fmaf(hv[c][j], hv[c][j], sum[0]);
-            ring_sum(sum, part, turn, k.team, in_block);
-            e = 1.f / sqrtf(sum[0] * per + g.eps);
-        }
-        sum[0] = 0.f;
+        stage   = stage == (STAGES<ROW> - 1) * ROW * PLANE ? 0 : stage + ROW * PLANE;
+        squares = F2(0.f);
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
-            if (hi[c] <= lo[c]) continue;
             if (g.h) {
-                float q[8];
-                Chunks<float>::get(factors + c * 4 * plane, plane, q);
+                float out[8];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) v[c][j] = fmaf(g.a, v[c][j], q[j] * (hv[c][j] * e));
-                put_part(g.r_out + cur.row * g.d + at[c], v[c], lo[c], hi[c]);
+                for (int j = 0; j < 4; ++j) v[c][j] = fma2(F2(g.a), v[c][j], f.q[c][j] * (h[c][j] * F2(e)));
+                singles(v[c], out);
+                if (m.any[c]) put_part(g.r_out + cur.offset + m.at[c], out, m.lo[c], m.hi[c]);
             }
 #pragma unroll
-            for (int j = 0; j < 8; ++j) sum[0] = fmaf(v[c][j], v[c][j], sum[0]);
+            for (int j = 0; j < 4; ++j) squares = fma2(v[c][j], v[c][j], squares);
         }
         if (g.gamma.p) {
-            ring_sum(sum, part, turn, k.team, in_block);
-            s = 1.f / sqrtf(sum[0] * per + g.eps);
+            sum = squares.sum();
+            ring_sum(sum, sums, turn, k.team, m.in_block);
+            s = rsqrtf(fmaf(sum, per, g.eps));
 #pragma unroll
             for (int c = 0; c < CH; ++c) {
-                if (hi[c] <= lo[c]) continue;
-                float w[8];
-                Chunks<float>::get(factors + (c * 4 + 2) * plane, plane, w);
+                float out[8];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) v[c][j] *= s * w[j];
-                put_part(g.x + cur.row * g.d + at[c], v[c], lo[c], hi[c]);
+                for (int j = 0; j < 4; ++j) v[c][j] = v[c][j] * (F2(s) * f.w[c][j]);
+                singles(v[c], out);
+                if (m.any[c]) put_part(g.x + cur.offset + m.at[c], out, m.lo[c], m.hi[c]);
             }
         }
-        if (g.kept && t == 0) g.kept[cur.row] = e, g.kept[g.n + cur.row] = s;
+        if (g.kept && m.t == 0) g.kept[cur.row] = e, g.kept[g.n + cur.row] = s;
     }
 }
 
 // GROUPS: the gate has several rows, so that sum D h^ is needed for each unit of rows; else one for all rows will do, from which both dpost_gamma and dgate follow.
 template <class RT, class HT, int CH, bool GROUPS>
-__global__ void __launch_bounds__(512, 1) backward_ring_kernel(const __grid_constant__ Args<RT, HT> g, const __grid_constant__ Ring k) {
+__global__ void __launch_bounds__(THREADS, 1) backward_ring_kernel(const __grid_constant__ Args<RT, HT> g, const __grid_constant__ Ring k) {
     extern __shared__ __align__(16) uint8_t smem[];
-    __shared__ float part[2][32][3];
+    __shared__ Sums sums;
     after_previous();
-    const int in_block = threadIdx.x / k.team, t = threadIdx.x - in_block * k.team;
-    const int64_t team = int64_t(blockIdx.x) * (blockDim.x / k.team) + in_block;
-    if (team >= k.teams) return;
-    const uint32_t plane = blockDim.x * 16, mine = uint32_t(__cvta_generic_to_shared(smem)) + threadIdx.x * 16;
+    const Mine<CH> m(k, g.d, smem);
+    if (m.team >= k.teams) return;
     constexpr int PAIR = PLANES<RT> + PLANES<HT>, ROW = CH * 2 * PAIR;
-    const uint32_t factors = mine, ring = mine + 4 * CH * plane;
-    Walk cur(g, k, team), ahead = cur;
-    const int lead  = int((team % k.classes) * g.d & 7);
-    const float per = 1.f / float(g.d);
-    const Chunks<RT> r{g.r, g.n * g.d}, dr{g.dr_out, g.n * g.d};
-    const Chunks<HT> h{g.h, g.n * g.d}, dx{g.dx, g.n * g.d};
-    int lo[CH], hi[CH], at[CH];
-#pragma unroll
-    for (int c = 0; c < CH; ++c) {
-        at[c] = (c * k.team + t) * 8 - lead;
-        lo[c] = max(0, -at[c]), hi[c] = int(min(int64_t(8), g.d - at[c]));
-        // what there is no tensor for stays zero
-        for (int stage = 0; stage < k.stages; ++stage)
-            for (int q = 0; q < 2 * PAIR; ++q) leave16(ring + (stage * ROW + c * 2 * PAIR + q) * plane, 0.f, 0.f, 0.f, 0.f);
-    }
+    Walk cur(g, k, m.team), ahead = cur;
+    const int64_t total = g.n * g.d;
+    const float per     = 1.f / float(g.d);
+    // what there is no tensor for stays zero
+#pragma unroll 1
+    for (int q = 0; q < STAGES<ROW> * ROW; ++q) leave16(m.place + q * PLANE, 0.f, 0.f, 0.f, 0.f);
     bool more = true;
     auto request = [&](uint32_t stage) {
         if (more && (more = ahead.next())) {
+            const bool last = ahead.offset + g.d + 8 > total;  // (a chunk may end behind the tensor)
 #pragma unroll
             for (int c = 0; c < CH; ++c) {
-                if (hi[c] <= lo[c]) continue;
-                const uint32_t to = ring + (stage * ROW + c * 2 * PAIR) * plane;
-                const int64_t p   = ahead.row * g.d + at[c];
-                r.copy(to, plane, p);
-                if (g.h) h.copy(to + PLANES<RT> * plane, plane, p);
-                if (g.dr_out) dr.copy(to + PAIR * plane, plane, p);
-                if (g.dx) dx.copy(to + (PAIR + PLANES<RT>) * plane, plane, p);
+                if (!m.any[c]) continue;
+                const uint32_t to = m.place + stage + c * 2 * PAIR * PLANE;
+                const int64_t p   = ahead.offset + m.at[c];
+                if (last) {
+                    const int left = int(min(int64_t(8), total - p));
+                    Chunks<RT>::copy(to, g.r, p, left);
+                    if (g.h) Chunks<HT>::copy(to + PLANES<RT> * PLANE, g.h, p, left);
+                    if (g.dr_out) Chunks<RT>::copy(to + PAIR * PLANE, g.dr_out, p, left);
+                    if (g.dx) Chunks<HT>::copy(to + (PAIR + PLANES<RT>) * PLANE, g.dx, p, left);
+                } else {
+                    Chunks<RT>::copy(to, g.r, p);
+                    if (g.h) Chunks<HT>::copy(to + PLANES<RT> * PLANE, g.h, p);
+                    if (g.dr_out) Chunks<RT>::copy(to + PAIR * PLANE, g.dr_out, p);
+                    if (g.dx) Chunks<HT>::copy(to + (PAIR + PLANES<RT>) * PLANE, g.dx, p);
+                }
             }
         }
         copies_end();
     };
-    for (int stage = 0; stage < k.stages; ++stage) request(stage);
-    float dgamma[CH][8] = {}, z[CH][8] = {}, dpost[GROUPS ? CH : 1][8] = {};
+    for (int stage = 0; stage < STAGES<ROW>; ++stage) request(stage * ROW * PLANE);
+    F2 dgamma[CH][4], z[CH][4];
+    float dpost[GROUPS ? CH : 1][8] = {};
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) dgamma[c][j] = z[c][j] = F2(0.f);
     // the sums of a unit of rows: dgate's, and (as the gate changes) dpost_gamma's
     auto finish = [&](int64_t unit, int64_t group) {
+        if constexpr (GROUPS) {
 #pragma unroll
-        for (int c = 0; c < CH; ++c) {
-            if (hi[c] <= lo[c]) continue;
-            float f[8], w[8];
-            factors_part(g.post_gamma, at[c], lo[c], hi[c], f), factors_part(g.gate, group * g.d + at[c], lo[c], hi[c], w);
+            for (int c = 0; c < CH; ++c) {
+                float f[8], w[8], sum[8];
+                factors_part(g.post_gamma, m.at[c], m.lo[c], m.hi[c], f), factors_part(g.gate, group * g.d + m.at[c], m.lo[c], m.hi[c], w);
+                singles(z[c], sum);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) dpost[c][j] = fmaf(g.b * w[j], z[c][j], dpost[c][j]), f[j] *= g.b * z[c][j], z[c][j] = 0.f;
-            if (g.pieces > 1) put_anywhere(g.part_gate + unit * g.d + at[c], f, lo[c], hi[c]);
-            else if (g.gate.bf16) put_anywhere(static_cast<__nv_bfloat16*>(g.dgate) + group * g.d + at[c], f, lo[c], hi[c]);
-            else put_anywhere(static_cast<float*>(g.dgate) + group * g.d + at[c], f, lo[c], hi[c]);
+                for (int j = 0; j < 8; ++j) dpost[c][j] = fmaf(g.b * w[j], sum[j], dpost[c][j]), f[j] *= g.b * sum[j];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) z[c][j] = F2(0.f);
+                if (!m.any[c]) continue;
+                if (g.pieces > 1) put_anywhere(g.part_gate + unit * g.d + m.at[c], f, m.lo[c], m.hi[c]);
+                else if (g.gate.bf16) put_anywhere(static_cast<__nv_bfloat16*>(g.dgate) + group * g.d + m.at[c], f, m.lo[c], m.hi[c]);
+                else put_anywhere(static_cast<float*>(g.dgate) + group * g.d + m.at[c], f, m.lo[c], m.hi[c]);
+            }
         }
     };
+    Weights<CH> f;
     int64_t group = -1, unit = -1;
     uint32_t stage = 0;
-    int turn = 0;
-    while (cur.next()) {
+    int turn       = 0;
+    // (a row's e and s are asked for a row ahead)
+    float e = 1.f, s = 1.f;
+    auto advance = [&] {
+        const bool there = cur.next();
+        if (there && g.post_gamma.p) e = g.kept[cur.row];
+        if (there && g.gamma.p) s = g.kept[g.n + cur.row];
+        return there;
+    };
+    for (bool there = advance(); there;) {
         if constexpr (GROUPS) {
             if (cur.unit != unit && unit >= 0) finish(unit, group);
             unit = cur.unit;
         }
-        if (cur.group != group) {
-            group = cur.group;
-#pragma unroll
-            for (int c = 0; c < CH; ++c) {
-                if (hi[c] <= lo[c]) continue;
-                float q[8], w[8];
-                factors_part(g.post_gamma, at[c], lo[c], hi[c], q), factors_part(g.gate, (g.gate.p ? group * g.d : 0) + at[c], lo[c], hi[c], w);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) q[j] *= g.b * w[j];
-                const uint32_t to = factors + c * 4 * plane;
-                leave16(to, q[0], q[1], q[2], q[3]), leave16(to + plane, q[4], q[5], q[6], q[7]);
-                factors_part(g.gamma, at[c], lo[c], hi[c], w);
-                leave16(to + 2 * plane, w[0], w[1], w[2], w[3]), leave16(to + 3 * plane, w[4], w[5], w[6], w[7]);
-            }
-        }
-        const float e = g.post_gamma.p ? g.kept[cur.row] : 1.f, s = g.gamma.p ? g.kept[g.n + cur.row] : 1.f;
-        copies_wait(k.stages - 1);
-        float hat[CH][8], rhat[CH][8], before[CH][8], q[CH][8], sum[3] = {};
-        const uint32_t from = ring + stage * ROW * plane;
+        if (cur.group != group) f.load(g, m, group = cur.group);
+        const int64_t offset = cur.offset;
+        const F2 e2(e), s2(s);
+        const float s1 = s, e1 = e;
+        copies_wait<STAGES<ROW> - 1>();
+        F2 hat[CH][4], rhat[CH][4], before[CH][4], all[3] = {F2(0.f), F2(0.f), F2(0.f)};
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
-            const uint32_t p = from + c * 2 * PAIR * plane;
-            const int l      = hi[c] > lo[c] ? lo[c] : 8;
-            float w[8], d[8];
-            Chunks<RT>::get(p, plane, rhat[c]), Chunks<HT>::get(p + PLANES<RT> * plane, plane, hat[c]);
-            Chunks<RT>::get(p + PAIR * plane, plane, before[c]), Chunks<HT>::get(p + (PAIR + PLANES<RT>) * plane, plane, d);
-            Chunks<float>::get(factors + c * 4 * plane, plane, q[c]), Chunks<float>::get(factors + (c * 4 + 2) * plane, plane, w);
-            if (l > 0 || hi[c] < 8) only(rhat[c], l, hi[c]), only(hat[c], l, hi[c]), only(before[c], l, hi[c]), only(d, l, hi[c]), only(q[c], l, hi[c]), only(w, l, hi[c]);
+            const uint32_t p = m.place + stage + c * 2 * PAIR * PLANE;
+            F2 d[4];
+            Chunks<RT>::get(p, rhat[c], m, c), Chunks<HT>::get(p + PLANES<RT> * PLANE, hat[c], m, c);
+            Chunks<RT>::get(p + PAIR * PLANE, before[c], m, c), Chunks<HT>::get(p + (PAIR + PLANES<RT>) * PLANE, d, m, c);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                hat[c][j] *= e;
-                const float qh = q[c][j] * hat[c][j], t = d[j] * w[j];
-                rhat[c][j]   = s * fmaf(g.a, rhat[c][j], qh);
-                before[c][j] = fmaf(s, t, before[c][j]);
-                dgamma[c][j] = fmaf(d[j], rhat[c][j], dgamma[c][j]);
-                sum[0] = fmaf(t, rhat[c][j], sum[0]), sum[1] = fmaf(qh, before[c][j], sum[1]), sum[2] = fmaf(qh, rhat[c][j], sum[2]);
+            for (int j = 0; j < 4; ++j) {
+                hat[c][j]   = hat[c][j] * e2;
+                const F2 qh = f.q[c][j] * hat[c][j], t = d[j] * f.w[c][j];
+                rhat[c][j]   = s2 * fma2(F2(g.a), rhat[c][j], qh);
+                before[c][j] = fma2(s2, t, before[c][j]);
+                dgamma[c][j] = fma2(d[j], rhat[c][j], dgamma[c][j]);
+                all[0] = fma2(t, rhat[c][j], all[0]), all[1] = fma2(qh, before[c][j], all[1]), all[2] = fma2(qh, rhat[c][j], all[2]);
             }
         }
+        there        = advance();
+        float sum[3] = {all[0].sum(), all[1].sum(), all[2].sum()};
+        ring_sum(sum, sums, turn, k.team, m.in_block);
         request(stage);
-        if (++stage == uint32_t(k.stages)) stage = 0;
-        ring_sum(sum, part, turn, k.team, in_block);
-        const float m0 = g.gamma.p ? s * sum[0] * per : 0.f, m = g.post_gamma.p ? (sum[1] - m0 * sum[2]) * per : 0.f;
+        stage = stage == (STAGES<ROW> - 1) * ROW * PLANE ? 0 : stage + ROW * PLANE;
+        const float m0 = g.gamma.p ? s1 * sum[0] * per : 0.f, m1 = g.post_gamma.p ? (sum[1] - m0 * sum[2]) * per : 0.f;
+        const F2 less(-m0), f1(-m1 * e1);
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
-            if (hi[c] <= lo[c]) continue;
-            float out[8];
+            F2 dr[4], dh[4];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float D = fmaf(-m0, rhat[c][j], before[c][j]);
-                out[j]        = g.a * D;
-                z[c][j]       = fmaf(D, hat[c][j], z[c][j]);
-                q[c][j]       = e * fmaf(q[c][j], D, -hat[c][j] * m);
+            for (int j = 0; j < 4; ++j) {
+                const F2 D = fma2(less, rhat[c][j], before[c][j]);
+                dr[j]   = F2(g.a) * D;
+                z[c][j] = fma2(D, hat[c][j], z[c][j]);
+                dh[j]   = fma2(f.q[c][j], D * e2, hat[c][j] * f1);
             }
-            put_part(g.dr + cur.row * g.d + at[c], out, lo[c], hi[c]);
-            if (g.dh) put_part(g.dh + cur.row * g.d + at[c], q[c], lo[c], hi[c]);
+            if (!m.any[c]) continue;
+            float out[8];
+            singles(dr, out);
+            put_part(g.dr + offset + m.at[c], out, m.lo[c], m.hi[c]);
+            singles(dh, out);
+            if (g.dh) put_part(g.dh + offset + m.at[c], out, m.lo[c], m.hi[c]);
         }
     }
     if constexpr (GROUPS) {
@@ -609,12 +696,15 @@ __global__ void __launch_bounds__(512, 1) backward_ring_kernel(const __grid_cons
     }
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-        if (hi[c] <= lo[c]) continue;
-        if (g.part_gamma) put_anywhere(g.part_gamma + team * g.d + at[c], dgamma[c], lo[c], hi[c]);
+        if (!m.any[c]) continue;
+        float out[8];
+        singles(dgamma[c], out);
+        if (g.part_gamma) put_anywhere(g.part_gamma + int64_t(m.team) * g.d + m.at[c], out, m.lo[c], m.hi[c]);
         if constexpr (GROUPS) {
-            if (g.part_post) put_anywhere(g.part_post + team * g.d + at[c], dpost[c], lo[c], hi[c]);
+            if (g.part_post) put_anywhere(g.part_post + int64_t(m.team) * g.d + m.at[c], dpost[c], m.lo[c], m.hi[c]);
         } else {
-            if (g.part_post) put_anywhere(g.part_post + team * g.d + at[c], z[c], lo[c], hi[c]);
+            singles(z[c], out);
+            if (g.part_post) put_anywhere(g.part_post + int64_t(m.team) * g.d + m.at[c], out, m.lo[c], m.hi[c]);
         }
     }
 }
@@ -704,7 +794,6 @@ struct Plan {
     int64_t teams, groups, pieces;
     float *gamma, *post, *gate;
 };
-constexpr size_t MOST_SMEM = 200 << 10;
 Plan plan(const Desc& d, bool backward, bool aligned, Space& space, int sm_count) {
     Plan p{};
     const size_t pair = dtype_size(d.stream_dtype) + dtype_size(d.block_dtype);
@@ -712,19 +801,17 @@ Plan plan(const Desc& d, bool backward, bool aligned, Space& space, int sm_count
     p.groups          = (d.n + run - 1) / run;
     int classes       = 8;
     while (classes > 1 && d.d % (16 / classes) == 0) classes /= 2;
-    // a team's threads hold eight columns each, sixteen from 4096 on
+    // A team's threads hold eight columns each, sixteen where those are too many threads for one team, or (forward, whose columns cost less than what each
+    // row costs a thread) for two on an SM.
     const int64_t chunks = (d.d + (classes > 1 ? 7 : 0) + 7) / 8;
-    p.columns            = chunks <= 512 ? 1 : 2;
-    const int64_t team = up((chunks + p.columns - 1) / p.columns, 32), in_block = team >= 512 ? 1 : 512 / team, threads = team * in_block;
-    // factors, and rows on their way: as many as there is room for
-    const size_t fixed = size_t(threads) * size_t(p.columns) * 64, row = size_t(threads) * size_t(p.columns) * 8 * pair * (backward ? 2 : 1);
-    const size_t room  = backward ? MOST_SMEM : MOST_SMEM / 2;
-    p.ring             = aligned && chunks <= 1024 && fixed + row <= room;
+    p.columns            = chunks <= (backward ? 512 : 256) ? 1 : 2;
+    const int64_t team = up((chunks + p.columns - 1) / p.columns, 32), in_block = team <= THREADS ? THREADS / team : 0;
+    const int64_t row  = p.columns * int64_t(PLANE) * int64_t(pair) / 2 * (backward ? 2 : 1);
+    p.ring             = aligned && in_block > 0 && row <= MOST_SMEM;
     if (p.ring) {
-        const size_t stages = (room - fixed) / row;
-        p.k.team = int(team), p.k.classes = classes, p.k.stages = int(stages < MOST_STAGES ? stages : MOST_STAGES);
-        p.threads = int(threads), p.rows = int(in_block), p.smem = fixed + size_t(p.k.stages) * row;
-        const int64_t most = int64_t(sm_count) * (backward ? 1 : 2) * in_block, need = up(d.n, classes);
+        p.k.team = int(team), p.k.classes = classes;
+        p.threads = THREADS, p.smem = size_t(row * (MOST_SMEM / row < 6 ? MOST_SMEM / row : 6));
+        const int64_t most = int64_t(sm_count) * in_block, need = up(d.n, classes);
         p.k.teams = int((need < most ? need : most) / classes * classes);
         p.teams   = p.k.teams;
         p.blocks  = int((p.teams + in_block - 1) / in_block);
@@ -762,7 +849,7 @@ template <auto KERN, class A>
 int launch_ring(const Plan& p, const A& g, const DeviceInfo& dev, cudaStream_t s) {
     static bool configured[64] = {};
     if (!configured[dev.device & 63]) {
-        MIMK_CUDA_TRY(cudaFuncSetAttribute(KERN, cudaFuncAttributeMaxDynamicSharedMemorySize, int(MOST_SMEM)));
+        MIMK_CUDA_TRY(cudaFuncSetAttribute(KERN, cudaFuncAttributeMaxDynamicSharedMemorySize, MOST_SMEM));
         configured[dev.device & 63] = true;
     }
     return launch_after(KERN, unsigned(p.blocks), unsigned(p.threads), p.smem, s, g, p.k);
