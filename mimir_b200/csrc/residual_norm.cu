@@ -292,8 +292,25 @@ struct Ring {
     int team, teams;  // threads of a team, teams in the whole grid (a multiple of the classes)
     int classes;
 };
-// Which rows a team takes: units of rows (group, piece, piece + pieces, ...), of its class.
-struct Walk {
+// Which rows a team takes: with one group every k.teams-th; else units of rows (group, piece, piece + pieces, ...), of its class.
+template <bool GROUPS>
+struct Walk;
+template <>
+struct Walk<false> {
+    int64_t offset, d;  // of the row's first element
+    int row, n, teams;
+    static constexpr int unit = 0, group = 0;
+    template <class A>
+    __device__ __forceinline__ Walk(const A& g, const Ring& k, int team)
+        : offset((int64_t(team) - k.teams) * g.d), d(int64_t(k.teams) * g.d), row(team - k.teams), n(int(g.n)), teams(k.teams) {}
+    __device__ __forceinline__ bool next() {
+        if (n - row <= teams) return false;
+        row += teams, offset += d;
+        return true;
+    }
+};
+template <>
+struct Walk<true> {
     int64_t row, end, offset, unit, group;  // offset: of the row's first element
     int64_t w, step, per, n, d, run, pieces, units;
     int cls, classes;
@@ -335,7 +352,7 @@ __device__ __forceinline__ void only(float (&v)[8], int lo, int hi) {
     for (int j = 0; j < 8; ++j) v[j] = j >= lo && j < hi ? v[j] : 0.f;
 }
 template <class T>
-struct Chunks {  // a tensor's chunks
+struct Chunks {  // a tensor's chunks (RAGGED: rows that are no whole ones)
     // the chunk that begins with element `at`, a multiple of eight; `left` elements of the tensor are from there on
     static __device__ __forceinline__ void copy(uint32_t to, const T* p, int64_t at, int left) {
 #pragma unroll
@@ -350,20 +367,20 @@ struct Chunks {  // a tensor's chunks
         for (int q = 0; q < PLANES<T>; ++q) copy_async(to + q * PLANE, p + at + q * (16 / int(sizeof(T))), 16);
     }
     // a row's columns of a chunk, zeros for the others
-    template <class M>
+    template <bool RAGGED, class M>
     static __device__ __forceinline__ void get(uint32_t from, F2 (&p)[4], const M& m, int c) {
         Run<T, 8> r;
         float v[8];
         r.a = take16(from);
         if constexpr (PLANES<T> == 2) r.b = take16(from + PLANE);
         r.get(v);
-        if (m.part[c]) only(v, m.lo[c], m.hi[c]);
+        if (RAGGED ? m.part[c] : !m.any[c]) only(v, m.lo[c], m.hi[c]);
         pairs(v, p);
     }
 };
-template <class T>
+template <bool RAGGED, class T>
 __device__ __forceinline__ void put_part(T* p, const float (&v)[8], int lo, int hi) {
-    if (lo == 0 && hi == 8) {
+    if (!RAGGED || (lo == 0 && hi == 8)) {
         put(p, v);
     } else {
 #pragma unroll
@@ -476,7 +493,7 @@ struct Weights {
     }
 };
 
-template <class RT, class HT, int CH>
+template <class RT, class HT, int CH, bool RAGGED, bool GROUPS>
 __global__ void __launch_bounds__(THREADS, 1) forward_ring_kernel(const __grid_constant__ Args<RT, HT> g, const __grid_constant__ Ring k) {
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ Sums sums;
@@ -484,7 +501,7 @@ __global__ void __launch_bounds__(THREADS, 1) forward_ring_kernel(const __grid_c
     const Mine<CH> m(k, g.d, smem);
     if (m.team >= k.teams) return;  // (whole teams: their barriers are their own)
     constexpr int PAIR = PLANES<RT> + PLANES<HT>, ROW = CH * PAIR;
-    Walk cur(g, k, m.team), ahead = cur;
+    Walk<GROUPS> cur(g, k, m.team), ahead = cur;
     const int64_t total = g.n * g.d;
     const float per     = 1.f / float(g.d);
     bool more           = true;
@@ -496,7 +513,7 @@ __global__ void __launch_bounds__(THREADS, 1) forward_ring_kernel(const __grid_c
                 if (!m.any[c]) continue;
                 const uint32_t to = m.place + stage + c * PAIR * PLANE;
                 const int64_t p   = ahead.offset + m.at[c];
-                if (last) {
+                if (RAGGED && last) {
                     const int left = int(min(int64_t(8), total - p));
                     Chunks<RT>::copy(to, g.r, p, left);
                     if (g.h) Chunks<HT>::copy(to + PLANES<RT> * PLANE, g.h, p, left);
@@ -520,7 +537,7 @@ __global__ void __launch_bounds__(THREADS, 1) forward_ring_kernel(const __grid_c
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
             const uint32_t p = m.place + stage + c * PAIR * PLANE;
-            Chunks<RT>::get(p, v[c], m, c), Chunks<HT>::get(p + PLANES<RT> * PLANE, h[c], m, c);
+            Chunks<RT>::template get<RAGGED>(p, v[c], m, c), Chunks<HT>::template get<RAGGED>(p + PLANES<RT> * PLANE, h[c], m, c);
 #pragma unroll
             for (int j = 0; j < 4; ++j) squares = fma2(h[c][j], h[c][j], squares);
         }
@@ -539,7 +556,7 @@ __global__ void __launch_bounds__(THREADS, 1) forward_ring_kernel(const __grid_c
 #pragma unroll
                 for (int j = 0; j < 4; ++j) v[c][j] = fma2(F2(g.a), v[c][j], f.q[c][j] * (h[c][j] * F2(e)));
                 singles(v[c], out);
-                if (m.any[c]) put_part(g.r_out + cur.offset + m.at[c], out, m.lo[c], m.hi[c]);
+                if (m.any[c]) put_part<RAGGED>(g.r_out + cur.offset + m.at[c], out, m.lo[c], m.hi[c]);
             }
 #pragma unroll
             for (int j = 0; j < 4; ++j) squares = fma2(v[c][j], v[c][j], squares);
@@ -554,7 +571,7 @@ __global__ void __launch_bounds__(THREADS, 1) forward_ring_kernel(const __grid_c
 #pragma unroll
                 for (int j = 0; j < 4; ++j) v[c][j] = v[c][j] * (F2(s) * f.w[c][j]);
                 singles(v[c], out);
-                if (m.any[c]) put_part(g.x + cur.offset + m.at[c], out, m.lo[c], m.hi[c]);
+                if (m.any[c]) put_part<RAGGED>(g.x + cur.offset + m.at[c], out, m.lo[c], m.hi[c]);
             }
         }
         if (g.kept && m.t == 0) g.kept[cur.row] = e, g.kept[g.n + cur.row] = s;
@@ -562,7 +579,7 @@ __global__ void __launch_bounds__(THREADS, 1) forward_ring_kernel(const __grid_c
 }
 
 // GROUPS: the gate has several rows, so that sum D h^ is needed for each unit of rows; else one for all rows will do, from which both dpost_gamma and dgate follow.
-template <class RT, class HT, int CH, bool GROUPS>
+template <class RT, class HT, int CH, bool RAGGED, bool GROUPS>
 __global__ void __launch_bounds__(THREADS, 1) backward_ring_kernel(const __grid_constant__ Args<RT, HT> g, const __grid_constant__ Ring k) {
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ Sums sums;
@@ -570,7 +587,7 @@ __global__ void __launch_bounds__(THREADS, 1) backward_ring_kernel(const __grid_
     const Mine<CH> m(k, g.d, smem);
     if (m.team >= k.teams) return;
     constexpr int PAIR = PLANES<RT> + PLANES<HT>, ROW = CH * 2 * PAIR;
-    Walk cur(g, k, m.team), ahead = cur;
+    Walk<GROUPS> cur(g, k, m.team), ahead = cur;
     const int64_t total = g.n * g.d;
     const float per     = 1.f / float(g.d);
     // what there is no tensor for stays zero
@@ -585,7 +602,7 @@ __global__ void __launch_bounds__(THREADS, 1) backward_ring_kernel(const __grid_
                 if (!m.any[c]) continue;
                 const uint32_t to = m.place + stage + c * 2 * PAIR * PLANE;
                 const int64_t p   = ahead.offset + m.at[c];
-                if (last) {
+                if (RAGGED && last) {
                     const int left = int(min(int64_t(8), total - p));
                     Chunks<RT>::copy(to, g.r, p, left);
                     if (g.h) Chunks<HT>::copy(to + PLANES<RT> * PLANE, g.h, p, left);
@@ -654,8 +671,8 @@ __global__ void __launch_bounds__(THREADS, 1) backward_ring_kernel(const __grid_
         for (int c = 0; c < CH; ++c) {
             const uint32_t p = m.place + stage + c * 2 * PAIR * PLANE;
             F2 d[4];
-            Chunks<RT>::get(p, rhat[c], m, c), Chunks<HT>::get(p + PLANES<RT> * PLANE, hat[c], m, c);
-            Chunks<RT>::get(p + PAIR * PLANE, before[c], m, c), Chunks<HT>::get(p + (PAIR + PLANES<RT>) * PLANE, d, m, c);
+            Chunks<RT>::template get<RAGGED>(p, rhat[c], m, c), Chunks<HT>::template get<RAGGED>(p + PLANES<RT> * PLANE, hat[c], m, c);
+            Chunks<RT>::template get<RAGGED>(p + PAIR * PLANE, before[c], m, c), Chunks<HT>::template get<RAGGED>(p + (PAIR + PLANES<RT>) * PLANE, d, m, c);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 hat[c][j]   = hat[c][j] * e2;
@@ -686,9 +703,9 @@ __global__ void __launch_bounds__(THREADS, 1) backward_ring_kernel(const __grid_
             if (!m.any[c]) continue;
             float out[8];
             singles(dr, out);
-            put_part(g.dr + offset + m.at[c], out, m.lo[c], m.hi[c]);
+            put_part<RAGGED>(g.dr + offset + m.at[c], out, m.lo[c], m.hi[c]);
             singles(dh, out);
-            if (g.dh) put_part(g.dh + offset + m.at[c], out, m.lo[c], m.hi[c]);
+            if (g.dh) put_part<RAGGED>(g.dh + offset + m.at[c], out, m.lo[c], m.hi[c]);
         }
     }
     if constexpr (GROUPS) {
@@ -709,7 +726,7 @@ __global__ void __launch_bounds__(THREADS, 1) backward_ring_kernel(const __grid_
     }
 }
 
-// out[group, c] = factor[c] times the sum of `count` rows of partial sums, into up to two results; 32 columns and 32 runs of rows a block
+// out[group, c] = factor[c] times the sum of `count` rows of partial sums, into up to two results; 32 columns a block, a run of the rows for each warp
 struct Result {
     void* out;
     int bf16, times;  // times: by `by` and the factors
@@ -724,29 +741,39 @@ struct Join {
 struct Joins {
     Join j[3];
 };
-__global__ void __launch_bounds__(1024) join_kernel(const __grid_constant__ Joins all, int64_t d) {
-    __shared__ float sums[32][33];
+constexpr int JOINED = 256, AT_ONCE = 8;  // threads; rows that each has on their way
+__global__ void __launch_bounds__(JOINED) join_kernel(const __grid_constant__ Joins all, int64_t d) {
+    __shared__ float sums[JOINED / 32][32];
     after_previous();
     const Join& j   = all.j[blockIdx.z];
-    const int64_t c = int64_t(blockIdx.x) * 32 + threadIdx.x;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t c = int64_t(blockIdx.x) * 32 + lane;
     for (int64_t group = blockIdx.y; group < j.groups; group += gridDim.y) {
         const float* p      = j.part + group * j.count * d + c;
         const int64_t count = min(j.count, j.rows - group * j.run);
         float v             = 0.f;
-        if (c < d)
-#pragma unroll 8
-            for (int64_t k = threadIdx.y; k < count; k += 32) v += p[k * d];
+        for (int64_t first = warp; first < count; first += AT_ONCE * JOINED / 32) {
+            float each[AT_ONCE];
+#pragma unroll
+            for (int i = 0; i < AT_ONCE; ++i) {
+                const int64_t row = first + i * (JOINED / 32);
+                each[i]           = c < d && row < count ? p[row * d] : 0.f;
+            }
+#pragma unroll
+            for (int i = 0; i < AT_ONCE; ++i) v += each[i];
+        }
         __syncthreads();
-        sums[threadIdx.y][threadIdx.x] = v;
+        sums[warp][lane] = v;
         __syncthreads();
-        v                = warp_sum(sums[threadIdx.x][threadIdx.y]);  // a warp for each column
-        const int64_t to = int64_t(blockIdx.x) * 32 + threadIdx.y;
-        if (threadIdx.x < 2 && to < d && j.to[threadIdx.x].out) {
-            const Result& r = j.to[threadIdx.x];
-            float one[1]    = {1.f};
-            if (r.times) factors_at(r.factors, to, one), v *= r.by * one[0];
-            if (r.bf16) static_cast<__nv_bfloat16*>(r.out)[group * d + to] = __float2bfloat16(v);
-            else static_cast<float*>(r.out)[group * d + to] = v;
+        if (warp < 2 && c < d && j.to[warp].out) {
+            const Result& r = j.to[warp];
+            v               = 0.f;
+#pragma unroll
+            for (int w = 0; w < JOINED / 32; ++w) v += sums[w][lane];
+            float one[1] = {1.f};
+            if (r.times) factors_at(r.factors, c, one), v *= r.by * one[0];
+            if (r.bf16) static_cast<__nv_bfloat16*>(r.out)[group * d + c] = __float2bfloat16(v);
+            else static_cast<float*>(r.out)[group * d + c] = v;
         }
     }
 }
@@ -854,6 +881,19 @@ int launch_ring(const Plan& p, const A& g, const DeviceInfo& dev, cudaStream_t s
     }
     return launch_after(KERN, unsigned(p.blocks), unsigned(p.threads), p.smem, s, g, p.k);
 }
+template <int V>
+struct Number {
+    static constexpr int value = V;
+};
+// f(columns, whether rows are no whole chunks, whether the gate has several rows)
+template <class F>
+int with_columns(const Plan& p, F&& f) {
+    const auto rest = [&](auto columns) {
+        if (p.k.classes > 1) return p.groups > 1 ? f(columns, Number<1>(), Number<1>()) : f(columns, Number<1>(), Number<0>());
+        return p.groups > 1 ? f(columns, Number<0>(), Number<1>()) : f(columns, Number<0>(), Number<0>());
+    };
+    return p.columns == 1 ? rest(Number<1>()) : rest(Number<2>());
+}
 template <class... P, class... A>
 int launch(void (*kern)(P...), dim3 grid, dim3 block, cudaStream_t s, A&&... args) {
     cudaLaunchAttribute early = {};
@@ -867,7 +907,7 @@ template <class RT, class HT, int VEC>
 int forward(const Desc& d, const Plan& p, const DeviceInfo& dev, cudaStream_t s) {
     Args<RT, HT> g = args_of<RT, HT>(d);
     g.groups = p.groups, g.pieces = p.pieces;
-    if (p.ring) return p.columns == 1 ? launch_ring<forward_ring_kernel<RT, HT, 1>>(p, g, dev, s) : launch_ring<forward_ring_kernel<RT, HT, 2>>(p, g, dev, s);
+    if (p.ring) return with_columns(p, [&](auto columns, auto ragged, auto several) { return launch_ring<forward_ring_kernel<RT, HT, columns.value, ragged.value, several.value>>(p, g, dev, s); });
     const auto kern = d.d <= 2048 ? forward_kernel<RT, HT, VEC, 8 / VEC, 256> : d.d <= 8192 ? forward_kernel<RT, HT, VEC, 16 / VEC, 512> : forward_kernel<RT, HT, VEC, 32 / VEC, 1024>;
     const int64_t blocks = (d.n + p.rows - 1) / p.rows;
     return launch(kern, dim3(unsigned(blocks < (1 << 20) ? blocks : 1 << 20)), dim3(p.threads, p.rows), s, g);
@@ -877,10 +917,8 @@ int backward(const Desc& d, const Plan& p, const DeviceInfo& dev, cudaStream_t s
     Args<RT, HT> g = args_of<RT, HT>(d);
     g.part_gamma = p.gamma, g.part_post = p.post, g.part_gate = p.gate, g.groups = p.groups, g.pieces = p.pieces;
     const bool several = p.groups > 1;
-    if (p.ring && p.columns == 1) {
-        MIMK_TRY((several ? launch_ring<backward_ring_kernel<RT, HT, 1, true>>(p, g, dev, s) : launch_ring<backward_ring_kernel<RT, HT, 1, false>>(p, g, dev, s)));
-    } else if (p.ring) {
-        MIMK_TRY((several ? launch_ring<backward_ring_kernel<RT, HT, 2, true>>(p, g, dev, s) : launch_ring<backward_ring_kernel<RT, HT, 2, false>>(p, g, dev, s)));
+    if (p.ring) {
+        MIMK_TRY(with_columns(p, [&](auto columns, auto ragged, auto several) { return launch_ring<backward_ring_kernel<RT, HT, columns.value, ragged.value, several.value>>(p, g, dev, s); }));
     } else {
         const auto kern = d.d <= 2048 ? backward_kernel<RT, HT, VEC, 8 / VEC, 256> : d.d <= 8192 ? backward_kernel<RT, HT, VEC, 16 / VEC, 512> : backward_kernel<RT, HT, VEC, 32 / VEC, 1024>;
         MIMK_TRY(launch(kern, dim3(unsigned(p.blocks)), dim3(p.threads, p.rows), s, g));
@@ -896,7 +934,7 @@ int backward(const Desc& d, const Plan& p, const DeviceInfo& dev, cudaStream_t s
     }
     if (p.gate) all.j[count++] = {p.gate, p.groups, p.pieces, d.n, g.gate_rows, {{d.dgate, d.gate_dtype == MIMK_BF16}}}, most = p.groups;
     if (!count) return MIMK_OK;
-    return launch(join_kernel, dim3(unsigned((d.d + 31) / 32), unsigned(most < 65535 ? most : 65535), unsigned(count)), dim3(32, 32), s, all, d.d);
+    return launch(join_kernel, dim3(unsigned((d.d + 31) / 32), unsigned(most < 65535 ? most : 65535), unsigned(count)), dim3(JOINED), s, all, d.d);
 }
 
 #define MIMK_BY_TYPES(F, VEC, ...)                                                                        \
