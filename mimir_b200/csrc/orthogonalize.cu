@@ -30,14 +30,14 @@ enum Product {
     APPLY,   // the next X from B and X
 };
 constexpr int BM = 128, BK = 64, OPERAND = BM * BK * 2, STAGE = 2 * OPERAND;
-constexpr int FIRST = 3, WARPS = 4, THREADS = (FIRST + WARPS) * 32;  // a warp for each operand's loads and one for the multiplications, then the epilogue's
+constexpr int FIRST = 3, WARPS = 8, THREADS = (FIRST + WARPS) * 32;  // a warp for each operand's loads and one for the multiplications, then the epilogue's: two for 32 rows
 constexpr int SLOT = 4096;  // a [32 rows x 128 bytes] tile of an epilogue warp
 constexpr int GROUP_M = 8;
 constexpr float SX = 256.f, LOW = 2048.f;  // factors of X, and of the second f16 of a value against the first
 
 template <int KIND>
 struct Shape {
-    static constexpr int SLOTS  = KIND == APPLY ? 16 : 0;  // per warp: two sets of a first and a second f16
+    static constexpr int SLOTS  = KIND == APPLY ? 2 * WARPS : 0;  // per warp: a first and a second f16 of 64 columns
     static constexpr int STAGES = KIND == APPLY ? 4 : 6;
     static constexpr int SMEM   = STAGES * STAGE + SLOTS * SLOT + 1024 + 256;
 };
@@ -49,20 +49,20 @@ struct Args {
     int rows, cols, batch;  // of the result
     int tiles_m, tiles_n, kb;
     int a_mn, b_mn;  // operand stored with its M (N) axis contiguous
-    int pitch;       // of A and B
+    int pitch, diag_pitch;  // of A and B; of the diagonals
     int last, tall;  // APPLY: the result is BF16; e goes with columns
     const __half* in;  // SQUARE: A
     __half* out;       // GRAM: A, SQUARE: B
     const float* diag_in;  // SQUARE: d, APPLY: e
     float* diag_out;
-    // GRAM: A = acc * f[0], times f[1] as f16. SQUARE: O O = acc * f[0], A = in * f[1], q = f[2], r = f[3], times f[4] as f16.
+    // GRAM: A = acc * f[0], times f[4] as f16. SQUARE: O O = acc * f[0], A = in * f[1], q = f[2], r = f[3], times f[4] as f16.
     // APPLY: SX X' = (f[0] + e) SX X + acc * f[1]; the result times f[2]
     float f[5];
     int* status;
 };
 
 struct Bars {
-    uint64_t full[6], empty[6], acc_full[2], acc_empty[2], in[2 * WARPS];
+    uint64_t full[6], empty[6], acc_full[2], acc_empty[2], in[WARPS];
     uint32_t tmem_base;
     int abort_flag;
 };
@@ -130,7 +130,7 @@ __device__ __forceinline__ void product(const Maps& maps, const Args& g) {
             mbar_init(smem_u32(&bars->acc_full[b]), 1);
             mbar_init(smem_u32(&bars->acc_empty[b]), SMS * WARPS * 32);
         }
-        for (int w = 0; w < 2 * WARPS; ++w) mbar_init(smem_u32(&bars->in[w]), 1);
+        for (int w = 0; w < WARPS; ++w) mbar_init(smem_u32(&bars->in[w]), 1);
         bars->abort_flag = 0;
         fence_barrier_init();
     }
@@ -220,25 +220,44 @@ __device__ __forceinline__ void product(const Maps& maps, const Args& g) {
             }
         }
     } else {
-        // ---------------- epilogue: 32 rows for each warp, one per lane ----------------
-        const int quarter = warp & 3;
-        const uint32_t slots = tile_base + STAGES * STAGE + quarter * (S::SLOTS / WARPS) * SLOT, in_bar = smem_u32(&bars->in[quarter * 2]);
+        // ---------------- epilogue: 32 rows and half of the columns for each warp, a row per lane ----------------
+        constexpr int HALF = SIDE / 2;
+        const int quarter = warp & 3, half = (warp - FIRST) >> 2, side = half * HALF;
+        const uint32_t slot = tile_base + STAGES * STAGE + (warp - FIRST) * 2 * SLOT, in_bar = smem_u32(&bars->in[warp - FIRST]);
         uint32_t acc = 0, acc_phase = 0, in_phase = 0;
         bool ok   = true;
         bool have = tile_at<KIND, SIDE>(g, first, t);
-        // APPLY: 64 columns of X, in two sets of slots in turn
+        // APPLY: 64 columns of X
         auto request = [&](int c) {
             const int row = t.m + int(rank) * BM + quarter * 32;
-            if (KIND == APPLY && lane == 0 && row < g.rows && c < SIDE && t.n + c < g.cols) {
-                const uint32_t set = c >> 6 & 1, to = slots + set * 2 * SLOT;
-                mbar_expect_tx(in_bar + set * 8, 2 * SLOT);
-                tma_load_3d(to, &maps.hi, t.n + c, row, t.z, in_bar + set * 8);
-                tma_load_3d(to + SLOT, &maps.lo, t.n + c, row, t.z, in_bar + set * 8);
+            if (KIND == APPLY && lane == 0 && row < g.rows && c < side + HALF && t.n + c < g.cols) {
+                mbar_expect_tx(in_bar, 2 * SLOT);
+                tma_load_3d(slot, &maps.hi, t.n + c, row, t.z, in_bar);
+                tma_load_3d(slot + SLOT, &maps.lo, t.n + c, row, t.z, in_bar);
             }
         };
-        if (have) request(0), request(64);
+        if (have) request(side);
         for (int index = first; have && ok;) {
-            const int row0 = t.m + int(rank) * BM + quarter * 32, row = row0 + lane, width = min(SIDE, g.cols - t.n);
+            const int row0 = t.m + int(rank) * BM + quarter * 32, row = row0 + lane, end = min(side + HALF, g.cols - t.n);
+            const bool there = row < g.rows;
+            // SQUARE: A's value (row, column) is also its value (column, row), which lanes read side by side; 32 columns, asked for ahead
+            const int64_t matrix = int64_t(t.z) * g.rows;  // (rows of the matrices before this one)
+            const float* diag    = g.diag_in + int64_t(t.z) * g.diag_pitch;
+            uint16_t a[32];
+            float4 dj[8];
+            auto ask = [&](int c) {
+                if constexpr (KIND == SQUARE) {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        const int column = t.n + c + i;
+                        a[i] = there && column < g.cols ? *reinterpret_cast<const uint16_t*>(g.in + (matrix + column) * g.pitch + row) : uint16_t(0);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) dj[i] = t.n + c + 4 * i < g.cols ? *reinterpret_cast<const float4*>(diag + t.n + c + 4 * i) : make_float4(0.f, 0.f, 0.f, 0.f);
+                }
+            };
+            if (row0 < g.rows && side < end) ask(side);
+            const float d = KIND == SQUARE && there ? diag[row] : 0.f;
             if (!(ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&bars->acc_full[acc]), acc_phase, abort_flag)))) break;
             tc_fence_after();
             const uint32_t from = tmem_base + acc * COLUMNS + (uint32_t(quarter * 32) << 16);
@@ -249,73 +268,80 @@ __device__ __forceinline__ void product(const Maps& maps, const Args& g) {
                 if constexpr (SMS == 2) mbar_arrive_cluster(acc_empty);
                 else mbar_arrive(acc_empty);
             };
-            if (row0 >= g.rows) {
+            if (row0 >= g.rows || side >= end) {
                 release();
             } else if constexpr (KIND != APPLY) {
-                const int64_t matrix = int64_t(t.z) * g.rows;  // (rows of the matrices before this one)
-                const bool there = row < g.rows;
-                const float d    = KIND == SQUARE && there ? g.diag_in[matrix + row] : 0.f;
+                __half* out = g.out + matrix * g.pitch;
 #pragma unroll 1
-                for (int c = 0; c < width; c += 32) {
+                for (int c = side; c < end; c += 32) {
                     uint32_t raw[32];
                     tmem_ld_32x32(from + c, raw);
-                    uint16_t a[32];
-                    if constexpr (KIND == SQUARE) {
-                        // A's value (row, column) is also its value (column, row), which lanes read side by side
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) {
-                            const int column = t.n + c + i;
-                            a[i] = there && column < g.cols ? *reinterpret_cast<const uint16_t*>(g.in + (matrix + column) * g.pitch + row) : uint16_t(0);
-                        }
-                    }
                     tmem_ld_wait();
-                    if (c + 32 >= width) release();
+                    if (c + 32 >= end) release();
                     float v[32];
 #pragma unroll
                     for (int i = 0; i < 32; ++i) {
-                        const int column = t.n + c + i;
                         v[i] = __uint_as_float(raw[i]) * g.f[0];
                         if constexpr (KIND == SQUARE) {
-                            const bool inside = column < g.cols;
-                            const float dj = inside ? g.diag_in[matrix + column] : 0.f, o = __half2float(__ushort_as_half(a[i])) * g.f[1];
-                            v[i] = row == column ? g.f[2] * d + g.f[3] * fmaf(d, d, v[i]) : g.f[2] * o + g.f[3] * fmaf(d + dj, o, v[i]);
+                            const float o = __half2float(__ushort_as_half(a[i])) * g.f[1], other = (&dj[i >> 2].x)[i & 3];
+                            v[i] = fmaf(fmaf(g.f[3], d + other, g.f[2]), o, g.f[3] * v[i]);
                         }
-                        if (row == column) {
-                            if (there) g.diag_out[matrix + row] = v[i];
-                            v[i] = 0.f;
-                        }
-                        v[i] *= KIND == GRAM ? g.f[1] : g.f[4];
                     }
-                    __half* out = g.out + matrix * g.pitch;
+                    if (row0 == t.n + c) {  // the diagonal: lane i has it in column i
+                        float on = 0.f;
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) on = i == lane ? __uint_as_float(raw[i]) * g.f[0] : on, v[i] = i == lane ? 0.f : v[i];
+                        if (KIND == SQUARE) on = g.f[2] * d + g.f[3] * fmaf(d, d, on);
+                        if (there) g.diag_out[int64_t(t.z) * g.diag_pitch + row] = on;
+                    }
+                    if (c + 32 < end) ask(c + 32);
+                    uint32_t two[16];
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) two[i] = pack_f16(v[2 * i] * g.f[4], v[2 * i + 1] * g.f[4]);
                     if (there) {
 #pragma unroll
-                        for (int i = 0; i < 32; i += 8)
-                            if (t.n + c + i < g.cols)
-                                *reinterpret_cast<uint4*>(out + int64_t(row) * g.pitch + t.n + c + i) =
-                                    make_uint4(pack_f16(v[i], v[i + 1]), pack_f16(v[i + 2], v[i + 3]), pack_f16(v[i + 4], v[i + 5]), pack_f16(v[i + 6], v[i + 7]));
-                        if (t.m != t.n) {
+                        for (int i = 0; i < 4; ++i)
+                            if (t.n + c + 8 * i < g.cols)
+                                *reinterpret_cast<uint4*>(out + int64_t(row) * g.pitch + t.n + c + 8 * i) = make_uint4(two[4 * i], two[4 * i + 1], two[4 * i + 2], two[4 * i + 3]);
+                    }
+                    if (t.m != t.n) {
+                        // the other triangle: an even lane stores its row's and the next one's value of an even column, an odd lane those of the odd column
+                        const bool odd = lane & 1;
 #pragma unroll
-                            for (int i = 0; i < 32; ++i)
-                                if (t.n + c + i < g.cols) out[int64_t(t.n + c + i) * g.pitch + row] = __float2half_rn(v[i]);
+                        for (int i = 0; i < 16; ++i) {
+                            const uint32_t other = __shfl_xor_sync(0xffffffffu, two[i], 1);
+                            const uint32_t both  = odd ? __byte_perm(other, two[i], 0x7632) : __byte_perm(two[i], other, 0x5410);
+                            const int column = t.n + c + 2 * i + odd, pair = row & ~1;
+                            if (column < g.cols && pair < g.rows) {
+                                __half* to = out + int64_t(column) * g.pitch + pair;
+                                *reinterpret_cast<uint32_t*>(to) = both;  // (a last odd row's neighbour lies in the rows' padding)
+                            }
                         }
                     }
                 }
             } else {
-                const int64_t matrix = int64_t(t.z) * (g.tall ? g.cols : g.rows);
-                const float e = !g.tall && row < g.rows ? g.diag_in[matrix + row] : 0.f;
+                const float e = !g.tall && there ? diag[row] : 0.f;
 #pragma unroll 1
-                for (int c = 0; c < width; c += 64) {
-                    const uint32_t set = c >> 6 & 1, slot = slots + set * 2 * SLOT;
-                    if (!(ok = __all_sync(0xffffffffu, mbar_wait(in_bar + set * 8, in_phase >> set & 1u, abort_flag)))) break;
-                    in_phase ^= 1u << set;
+                for (int c = side; c < end; c += 64) {
+                    if (!(ok = __all_sync(0xffffffffu, mbar_wait(in_bar, in_phase, abort_flag)))) break;
+                    in_phase ^= 1u;
 #pragma unroll
-                    for (int half = 0; half < 64; half += 32) {
+                    for (int part = 0; part < 64; part += 32) {
                         uint32_t raw[32];
-                        tmem_ld_32x32(from + c + half, raw);
+                        tmem_ld_32x32(from + c + part, raw);
+                        float4 ej[8];
+                        if (g.tall) {
+#pragma unroll
+                            for (int i = 0; i < 8; ++i)
+                                ej[i] = t.n + c + part + 4 * i < g.cols ? *reinterpret_cast<const float4*>(diag + t.n + c + part + 4 * i) : make_float4(0.f, 0.f, 0.f, 0.f);
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) ej[i] = make_float4(e, e, e, e);
+                        }
                         float v[32];
 #pragma unroll
                         for (int i = 0; i < 32; i += 8) {
-                            const uint4 hi = ld_shared(piece_at(slot, lane, (half + i) >> 3)), lo = ld_shared(piece_at(slot + SLOT, lane, (half + i) >> 3));
+                            const uint4 hi = ld_shared(piece_at(slot, lane, (part + i) >> 3)), lo = ld_shared(piece_at(slot + SLOT, lane, (part + i) >> 3));
                             const uint32_t h[4] = {hi.x, hi.y, hi.z, hi.w}, l[4] = {lo.x, lo.y, lo.z, lo.w};
 #pragma unroll
                             for (int j = 0; j < 4; ++j) {
@@ -324,13 +350,9 @@ __device__ __forceinline__ void product(const Maps& maps, const Args& g) {
                             }
                         }
                         tmem_ld_wait();
-                        if (c + 64 >= width && half) release();
+                        if (c + 64 >= end && part) release();
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) {
-                            float by = g.f[0] + e;
-                            if (g.tall) by += t.n + c + half + i < g.cols ? g.diag_in[matrix + t.n + c + half + i] : 0.f;
-                            v[i] = fmaf(by, v[i], __uint_as_float(raw[i]) * g.f[1]);
-                        }
+                        for (int i = 0; i < 32; ++i) v[i] = fmaf(g.f[0] + (&ej[i >> 2].x)[i & 3], v[i], __uint_as_float(raw[i]) * g.f[1]);
 #pragma unroll
                         for (int i = 0; i < 32; i += 8) {
                             uint32_t h[4], l[4];
@@ -345,8 +367,8 @@ __device__ __forceinline__ void product(const Maps& maps, const Args& g) {
                                     l[j] = pack_f16((x - r.x) * LOW, (y - r.y) * LOW);
                                 }
                             }
-                            st_shared(piece_at(slot, lane, (half + i) >> 3), h[0], h[1], h[2], h[3]);
-                            if (!g.last) st_shared(piece_at(slot + SLOT, lane, (half + i) >> 3), l[0], l[1], l[2], l[3]);
+                            st_shared(piece_at(slot, lane, (part + i) >> 3), h[0], h[1], h[2], h[3]);
+                            if (!g.last) st_shared(piece_at(slot + SLOT, lane, (part + i) >> 3), l[0], l[1], l[2], l[3]);
                         }
                     }
                     fence_proxy_async_smem();
@@ -357,13 +379,13 @@ __device__ __forceinline__ void product(const Maps& maps, const Args& g) {
                         bulk_commit();
                         bulk_wait_read_0();
                     }
-                    request(c + 128);
+                    request(c + 64);
                 }
                 if (!ok) break;
             }
             index += step;
             have = tile_at<KIND, SIDE>(g, index, t);
-            if (have) request(0), request(64);
+            if (have) request(side);
         }
         if (KIND == APPLY && lane == 0) bulk_wait_all();
     }
@@ -516,7 +538,7 @@ int check(const Desc* d) {
 bool nothing(const Desc& d) { return !d.batch || !d.m || !d.n; }
 
 struct Plan {
-    int64_t k, pitch_x, pitch_a, slice, chunks;
+    int64_t k, pitch_x, pitch_a, pitch_d, slice, chunks;
     __half *x[2][2], *a, *b;
     float *d, *e;
     double* sums;
@@ -524,7 +546,7 @@ struct Plan {
 };
 Plan plan(const Desc& d, Space& space) {
     Plan p{};
-    p.k = d.m < d.n ? d.m : d.n, p.pitch_x = up(d.n, 8), p.pitch_a = up(p.k, 8);
+    p.k = d.m < d.n ? d.m : d.n, p.pitch_x = up(d.n, 8), p.pitch_a = up(p.k, 8), p.pitch_d = up(p.k, 4);
     p.chunks = (d.m * d.n + CHUNK - 1) / CHUNK;
     const int64_t each = 8 * d.m * p.pitch_x + 4 * p.k * p.pitch_a;
     p.slice = SLICE / each;
@@ -534,7 +556,7 @@ Plan plan(const Desc& d, Space& space) {
     for (auto& x : p.x)
         for (__half*& piece : x) piece = static_cast<__half*>(space.take(size_t(p.slice * d.m * p.pitch_x) * 2));
     p.a = static_cast<__half*>(space.take(size_t(p.slice * p.k * p.pitch_a) * 2)), p.b = static_cast<__half*>(space.take(size_t(p.slice * p.k * p.pitch_a) * 2));
-    p.d = static_cast<float*>(space.take(size_t(p.slice * p.k) * 4)), p.e = static_cast<float*>(space.take(size_t(p.slice * p.k) * 4));
+    p.d = static_cast<float*>(space.take(size_t(p.slice * p.pitch_d) * 4)), p.e = static_cast<float*>(space.take(size_t(p.slice * p.pitch_d) * 4));
     p.sums = static_cast<double*>(space.take(size_t(p.slice * p.chunks) * 8));
     // the same for every address of the result (a size is asked for before there is one)
     p.out = static_cast<__nv_bfloat16*>(space.take(size_t(p.slice * d.m * p.pitch_x) * 2));
@@ -603,10 +625,10 @@ int slice(const Desc& d, const Plan& p, const Factors* f, int64_t first, int64_t
         __half* const* now = p.x[step & 1];
         __half* const* next = p.x[~step & 1];
         Args g{};
-        g.batch = int(count), g.pitch = int(p.pitch_a), g.status = dev.status_dev;
+        g.batch = int(count), g.pitch = int(p.pitch_a), g.diag_pitch = int(p.pitch_d), g.status = dev.status_dev;
         // A
         g.rows = g.cols = int(p.k), g.kb = blocks(tall ? d.m : d.n), g.a_mn = g.b_mn = tall, g.out = p.a, g.diag_out = p.d;
-        g.f[0] = 1.f / (SX * SX), g.f[1] = c.a;
+        g.f[0] = 1.f / (SX * SX), g.f[4] = c.a;
         MIMK_TRY(map_of(&maps.left, now[0], d.m, d.n, p.pitch_x, count, tall ? 64 : BM));
         maps.right = maps.left;
         MIMK_TRY(launch<GRAM>(maps, g, dev, s));
