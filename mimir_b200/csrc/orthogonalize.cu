@@ -31,15 +31,15 @@ enum Product {
 };
 constexpr int BM = 128, BK = 64, OPERAND = BM * BK * 2, STAGE = 2 * OPERAND;
 constexpr int FIRST = 3, WARPS = 8, THREADS = (FIRST + WARPS) * 32;  // a warp for each operand's loads and one for the multiplications, then the epilogue's: two for 32 rows
-constexpr int SLOT = 4096;  // a [32 rows x 128 bytes] tile of an epilogue warp
+constexpr int SLOT = 4096;  // 32 columns of 32 rows of X, a first and a second f16: two tiles of [32 rows x 64 bytes]
 constexpr int GROUP_M = 8;
 constexpr float SX = 256.f, LOW = 2048.f;  // factors of X, and of the second f16 of a value against the first
 
 template <int KIND>
 struct Shape {
-    static constexpr int SLOTS  = KIND == APPLY ? 2 * WARPS : 0;  // per warp: a first and a second f16 of 64 columns
+    static constexpr int SLOTS  = KIND == APPLY ? 2 * WARPS : 0;  // two for each warp
     static constexpr int STAGES = KIND == APPLY ? 4 : 6;
-    static constexpr int SMEM   = STAGES * STAGE + SLOTS * SLOT + 1024 + 256;
+    static constexpr int SMEM   = STAGES * STAGE + SLOTS * SLOT + 1024 + 512;
 };
 
 struct Maps {
@@ -48,11 +48,13 @@ struct Maps {
 struct Args {
     int rows, cols, batch;  // of the result
     int tiles_m, tiles_n, kb;
+    int splits, per;  // GRAM: the k-blocks dealt out over that many tiles, `per` each, whose sums are f32 partial results
     int a_mn, b_mn;  // operand stored with its M (N) axis contiguous
     int pitch, diag_pitch;  // of A and B; of the diagonals
     int last, tall;  // APPLY: the result is BF16; e goes with columns
     const __half* in;  // SQUARE: A
     __half* out;       // GRAM: A, SQUARE: B
+    float* part;       // [splits][batch][rows][pitch], tiles on and below the diagonal
     const float* diag_in;  // SQUARE: d, APPLY: e
     float* diag_out;
     // GRAM: A = acc * f[0], times f[4] as f16. SQUARE: O O = acc * f[0], A = in * f[1], q = f[2], r = f[3], times f[4] as f16.
@@ -62,18 +64,23 @@ struct Args {
 };
 
 struct Bars {
-    uint64_t full[6], empty[6], acc_full[2], acc_empty[2], in[WARPS];
+    uint64_t full[6], empty[6], acc_full[2], acc_empty[2], in[2 * WARPS];
     uint32_t tmem_base;
     int abort_flag;
 };
-static_assert(sizeof(Bars) <= 256, "barrier block too large");
+static_assert(sizeof(Bars) <= 512, "barrier block too large");
 
 struct Tile {
-    int z, m, n;
+    int z, m, n, split;
 };
 template <int KIND, int SIDE>
 __device__ __forceinline__ bool tile_at(const Args& g, int index, Tile& t) {
     const int per = KIND == APPLY ? g.tiles_m * g.tiles_n : g.tiles_m * (g.tiles_m + 1) / 2;
+    t.split = 0;
+    if (KIND == GRAM && g.splits > 1) {
+        t.split = index / (per * g.batch), index -= t.split * per * g.batch;
+        if (t.split >= g.splits) return false;
+    }
     t.z = index / per;
     if (t.z >= g.batch) return false;
     const int i = index - t.z * per;
@@ -96,8 +103,8 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
     return *reinterpret_cast<const uint32_t*>(&v);
 }
 __device__ __forceinline__ float2 unpack_f16(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
-// 16-byte piece `piece` of this lane's row of a 128-byte-swizzled slot
-__device__ __forceinline__ uint32_t piece_at(uint32_t slot, int lane, int piece) { return slot + lane * 128 + ((uint32_t(piece) ^ uint32_t(lane & 7)) << 4); }
+// 16-byte piece `piece` of this lane's row of a 64-byte-swizzled tile
+__device__ __forceinline__ uint32_t piece_at(uint32_t tile, int lane, int piece) { return tile + lane * 64 + ((uint32_t(piece) ^ uint32_t(lane >> 1 & 3)) << 4); }
 __device__ __forceinline__ uint4 ld_shared(uint32_t a) {
     uint4 v;
     asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
@@ -121,6 +128,10 @@ __device__ __forceinline__ void product(const Maps& maps, const Args& g) {
     const uint32_t rank = SMS == 2 ? cluster_ctarank() : 0;
     const int first = blockIdx.x / SMS, step = gridDim.x / SMS;
 
+    if (threadIdx.x == 32) {
+        tma_prefetch_desc(&maps.left), tma_prefetch_desc(&maps.right);
+        if (KIND == APPLY) tma_prefetch_desc(&maps.hi), tma_prefetch_desc(&maps.lo), tma_prefetch_desc(&maps.out_hi), tma_prefetch_desc(&maps.out_lo);
+    }
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; ++s) {
             mbar_init(smem_u32(&bars->full[s]), 1);
@@ -130,7 +141,7 @@ __device__ __forceinline__ void product(const Maps& maps, const Args& g) {
             mbar_init(smem_u32(&bars->acc_full[b]), 1);
             mbar_init(smem_u32(&bars->acc_empty[b]), SMS * WARPS * 32);
         }
-        for (int w = 0; w < WARPS; ++w) mbar_init(smem_u32(&bars->in[w]), 1);
+        for (int w = 0; w < 2 * WARPS; ++w) mbar_init(smem_u32(&bars->in[w]), 1);
         bars->abort_flag = 0;
         fence_barrier_init();
     }
@@ -161,7 +172,8 @@ __device__ __forceinline__ void product(const Maps& maps, const Args& g) {
             bool ok = true;
             for (int index = first; ok && tile_at<KIND, SIDE>(g, index, t); index += step) {
                 const int at = (left ? t.m : t.n) + int(rank) * BM;
-                for (int kb = 0; kb < g.kb; ++kb) {
+                const int end = KIND == GRAM ? min(g.kb, (t.split + 1) * g.per) : g.kb;
+                for (int kb = KIND == GRAM ? t.split * g.per : 0; kb < end; ++kb) {
                     if (!(ok = mbar_wait(smem_u32(&bars->empty[stage]), phase ^ 1u, abort_flag))) break;
                     const uint32_t to = tile_base + stage * STAGE + (left ? 0 : OPERAND), full = smem_u32(&bars->full[stage]);
                     const int k = kb * BK;
@@ -199,15 +211,16 @@ __device__ __forceinline__ void product(const Maps& maps, const Args& g) {
             for (int index = first; ok && tile_at<KIND, SIDE>(g, index, t); index += step) {
                 if (!(ok = mbar_wait(smem_u32(&bars->acc_empty[acc]), acc_phase ^ 1u, abort_flag))) break;
                 tc_fence_after();
-                for (int kb = 0; kb < g.kb; ++kb) {
+                const int begin = KIND == GRAM ? t.split * g.per : 0, end = KIND == GRAM ? min(g.kb, begin + g.per) : g.kb;
+                for (int kb = begin; kb < end; ++kb) {
                     if (!(ok = mbar_wait(smem_u32(&bars->full[stage]), phase, abort_flag))) break;
                     tc_fence_after();
                     const uint32_t at = (tile_base + stage * STAGE) >> 4;
 #pragma unroll
                     for (int k = 0; k < BK / 16; ++k) {
                         const uint64_t a = high | (at + a_low + k * a_step), b = high | (at + b_low + k * b_step);
-                        if constexpr (SMS == 2) mma_f16_ss_pair(tmem_base + acc * COLUMNS, a, b, idesc, kb > 0 || k > 0);
-                        else mma_f16_ss(tmem_base + acc * COLUMNS, a, b, idesc, kb > 0 || k > 0);
+                        if constexpr (SMS == 2) mma_f16_ss_pair(tmem_base + acc * COLUMNS, a, b, idesc, kb > begin || k > 0);
+                        else mma_f16_ss(tmem_base + acc * COLUMNS, a, b, idesc, kb > begin || k > 0);
                     }
                     if constexpr (SMS == 2) mma_commit_pair(smem_u32(&bars->empty[stage]));
                     else mma_commit(smem_u32(&bars->empty[stage]));
@@ -223,35 +236,34 @@ __device__ __forceinline__ void product(const Maps& maps, const Args& g) {
         // ---------------- epilogue: 32 rows and half of the columns for each warp, a row per lane ----------------
         constexpr int HALF = SIDE / 2;
         const int quarter = warp & 3, half = (warp - FIRST) >> 2, side = half * HALF;
-        const uint32_t slot = tile_base + STAGES * STAGE + (warp - FIRST) * 2 * SLOT, in_bar = smem_u32(&bars->in[warp - FIRST]);
+        const uint32_t slot = tile_base + STAGES * STAGE + (warp - FIRST) * 2 * SLOT, in_bar = smem_u32(&bars->in[(warp - FIRST) * 2]);
         uint32_t acc = 0, acc_phase = 0, in_phase = 0;
         bool ok   = true;
         bool have = tile_at<KIND, SIDE>(g, first, t);
-        // APPLY: 64 columns of X
+        // APPLY: 32 columns of X, in two sets of slots in turn
         auto request = [&](int c) {
             const int row = t.m + int(rank) * BM + quarter * 32;
             if (KIND == APPLY && lane == 0 && row < g.rows && c < side + HALF && t.n + c < g.cols) {
-                mbar_expect_tx(in_bar, 2 * SLOT);
-                tma_load_3d(slot, &maps.hi, t.n + c, row, t.z, in_bar);
-                tma_load_3d(slot + SLOT, &maps.lo, t.n + c, row, t.z, in_bar);
+                const uint32_t set = c >> 5 & 1, to = slot + set * SLOT, bar = in_bar + set * 8;
+                mbar_expect_tx(bar, SLOT);
+                tma_load_3d(to, &maps.hi, t.n + c, row, t.z, bar);
+                tma_load_3d(to + SLOT / 2, &maps.lo, t.n + c, row, t.z, bar);
             }
         };
-        if (have) request(side);
+        if (have) request(side), request(side + 32);
         for (int index = first; have && ok;) {
             const int row0 = t.m + int(rank) * BM + quarter * 32, row = row0 + lane, end = min(side + HALF, g.cols - t.n);
             const bool there = row < g.rows;
-            // SQUARE: A's value (row, column) is also its value (column, row), which lanes read side by side; 32 columns, asked for ahead
+            // SQUARE: A's values, and the diagonal's of their columns, 32 columns asked for ahead
             const int64_t matrix = int64_t(t.z) * g.rows;  // (rows of the matrices before this one)
             const float* diag    = g.diag_in + int64_t(t.z) * g.diag_pitch;
-            uint16_t a[32];
+            uint4 a[4];
             float4 dj[8];
             auto ask = [&](int c) {
                 if constexpr (KIND == SQUARE) {
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) {
-                        const int column = t.n + c + i;
-                        a[i] = there && column < g.cols ? *reinterpret_cast<const uint16_t*>(g.in + (matrix + column) * g.pitch + row) : uint16_t(0);
-                    }
+                    for (int i = 0; i < 4; ++i)
+                        a[i] = there && t.n + c + 8 * i < g.cols ? *reinterpret_cast<const uint4*>(g.in + (matrix + row) * g.pitch + t.n + c + 8 * i) : make_uint4(0, 0, 0, 0);
 #pragma unroll
                     for (int i = 0; i < 8; ++i) dj[i] = t.n + c + 4 * i < g.cols ? *reinterpret_cast<const float4*>(diag + t.n + c + 4 * i) : make_float4(0.f, 0.f, 0.f, 0.f);
                 }
@@ -272,19 +284,29 @@ __device__ __forceinline__ void product(const Maps& maps, const Args& g) {
                 release();
             } else if constexpr (KIND != APPLY) {
                 __half* out = g.out + matrix * g.pitch;
+                float* part = g.part + (int64_t(t.split) * g.batch * g.rows + matrix + row) * g.pitch + t.n;
 #pragma unroll 1
                 for (int c = side; c < end; c += 32) {
                     uint32_t raw[32];
                     tmem_ld_32x32(from + c, raw);
                     tmem_ld_wait();
                     if (c + 32 >= end) release();
+                    if (KIND == GRAM && g.splits > 1) {
+#pragma unroll
+                        for (int i = 0; i < 32; i += 4)
+                            if (there && t.n + c + i < g.cols) *reinterpret_cast<uint4*>(part + c + i) = make_uint4(raw[i], raw[i + 1], raw[i + 2], raw[i + 3]);
+                        continue;
+                    }
                     float v[32];
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) {
-                        v[i] = __uint_as_float(raw[i]) * g.f[0];
-                        if constexpr (KIND == SQUARE) {
-                            const float o = __half2float(__ushort_as_half(a[i])) * g.f[1], other = (&dj[i >> 2].x)[i & 3];
-                            v[i] = fmaf(fmaf(g.f[3], d + other, g.f[2]), o, g.f[3] * v[i]);
+                    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(raw[i]) * g.f[0];
+                    if constexpr (KIND == SQUARE) {
+#pragma unroll
+                        for (int i = 0; i < 32; i += 2) {
+                            const float2 o = unpack_f16((&a[i >> 3].x)[i >> 1 & 3]);
+                            const float d0 = (&dj[i >> 2].x)[i & 3], d1 = (&dj[i >> 2].x)[(i & 3) + 1];
+                            v[i]     = fmaf(fmaf(g.f[3], d + d0, g.f[2]), o.x * g.f[1], g.f[3] * v[i]);
+                            v[i + 1] = fmaf(fmaf(g.f[3], d + d1, g.f[2]), o.y * g.f[1], g.f[3] * v[i + 1]);
                         }
                     }
                     if (row0 == t.n + c) {  // the diagonal: lane i has it in column i
@@ -322,70 +344,61 @@ __device__ __forceinline__ void product(const Maps& maps, const Args& g) {
             } else {
                 const float e = !g.tall && there ? diag[row] : 0.f;
 #pragma unroll 1
-                for (int c = side; c < end; c += 64) {
-                    if (!(ok = __all_sync(0xffffffffu, mbar_wait(in_bar, in_phase, abort_flag)))) break;
-                    in_phase ^= 1u;
+                for (int c = side; c < end; c += 32) {
+                    const uint32_t set = c >> 5 & 1, at = slot + set * SLOT;
+                    if (!(ok = __all_sync(0xffffffffu, mbar_wait(in_bar + set * 8, in_phase >> set & 1u, abort_flag)))) break;
+                    in_phase ^= 1u << set;
+                    uint32_t raw[32];
+                    tmem_ld_32x32(from + c, raw);
+                    float4 ej[8];
+                    if (g.tall) {
 #pragma unroll
-                    for (int part = 0; part < 64; part += 32) {
-                        uint32_t raw[32];
-                        tmem_ld_32x32(from + c + part, raw);
-                        float4 ej[8];
-                        if (g.tall) {
+                        for (int i = 0; i < 8; ++i) ej[i] = t.n + c + 4 * i < g.cols ? *reinterpret_cast<const float4*>(diag + t.n + c + 4 * i) : make_float4(0.f, 0.f, 0.f, 0.f);
+                    } else {
 #pragma unroll
-                            for (int i = 0; i < 8; ++i)
-                                ej[i] = t.n + c + part + 4 * i < g.cols ? *reinterpret_cast<const float4*>(diag + t.n + c + part + 4 * i) : make_float4(0.f, 0.f, 0.f, 0.f);
-                        } else {
+                        for (int i = 0; i < 8; ++i) ej[i] = make_float4(e, e, e, e);
+                    }
+                    uint4 hi[4], lo[4];
 #pragma unroll
-                            for (int i = 0; i < 8; ++i) ej[i] = make_float4(e, e, e, e);
-                        }
-                        float v[32];
+                    for (int i = 0; i < 4; ++i) hi[i] = ld_shared(piece_at(at, lane, i)), lo[i] = ld_shared(piece_at(at + SLOT / 2, lane, i));
+                    tmem_ld_wait();
+                    if (c + 32 >= end) release();
 #pragma unroll
-                        for (int i = 0; i < 32; i += 8) {
-                            const uint4 hi = ld_shared(piece_at(slot, lane, (part + i) >> 3)), lo = ld_shared(piece_at(slot + SLOT, lane, (part + i) >> 3));
-                            const uint32_t h[4] = {hi.x, hi.y, hi.z, hi.w}, l[4] = {lo.x, lo.y, lo.z, lo.w};
+                    for (int i = 0; i < 4; ++i) {
+                        uint32_t h[4] = {hi[i].x, hi[i].y, hi[i].z, hi[i].w}, l[4] = {lo[i].x, lo[i].y, lo[i].z, lo[i].w};
 #pragma unroll
-                            for (int j = 0; j < 4; ++j) {
-                                const float2 a = unpack_f16(h[j]), b = unpack_f16(l[j]);
-                                v[i + 2 * j] = fmaf(b.x, 1.f / LOW, a.x), v[i + 2 * j + 1] = fmaf(b.y, 1.f / LOW, a.y);
+                        for (int j = 0; j < 4; ++j) {
+                            const int k    = 8 * i + 2 * j;
+                            const float2 a = unpack_f16(h[j]), b = unpack_f16(l[j]);
+                            const float x = fmaf(g.f[0] + (&ej[k >> 2].x)[k & 3], fmaf(b.x, 1.f / LOW, a.x), __uint_as_float(raw[k]) * g.f[1]);
+                            const float y = fmaf(g.f[0] + (&ej[k >> 2].x)[(k & 3) + 1], fmaf(b.y, 1.f / LOW, a.y), __uint_as_float(raw[k + 1]) * g.f[1]);
+                            if (g.last) {
+                                h[j] = pack_bf16x2(x * g.f[2], y * g.f[2]);
+                            } else {
+                                h[j] = pack_f16(x, y);
+                                const float2 r = unpack_f16(h[j]);
+                                l[j] = pack_f16((x - r.x) * LOW, (y - r.y) * LOW);
                             }
                         }
-                        tmem_ld_wait();
-                        if (c + 64 >= end && part) release();
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) v[i] = fmaf(g.f[0] + (&ej[i >> 2].x)[i & 3], v[i], __uint_as_float(raw[i]) * g.f[1]);
-#pragma unroll
-                        for (int i = 0; i < 32; i += 8) {
-                            uint32_t h[4], l[4];
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) {
-                                const float x = v[i + 2 * j], y = v[i + 2 * j + 1];
-                                if (g.last) {
-                                    h[j] = pack_bf16x2(x * g.f[2], y * g.f[2]);
-                                } else {
-                                    h[j] = pack_f16(x, y);
-                                    const float2 r = unpack_f16(h[j]);
-                                    l[j] = pack_f16((x - r.x) * LOW, (y - r.y) * LOW);
-                                }
-                            }
-                            st_shared(piece_at(slot, lane, (part + i) >> 3), h[0], h[1], h[2], h[3]);
-                            if (!g.last) st_shared(piece_at(slot + SLOT, lane, (part + i) >> 3), l[0], l[1], l[2], l[3]);
-                        }
+                        st_shared(piece_at(at, lane, i), h[0], h[1], h[2], h[3]);
+                        if (!g.last) st_shared(piece_at(at + SLOT / 2, lane, i), l[0], l[1], l[2], l[3]);
                     }
                     fence_proxy_async_smem();
                     __syncwarp();
                     if (lane == 0) {
-                        tma_store_3d(&maps.out_hi, slot, t.n + c, row0, t.z);
-                        if (!g.last) tma_store_3d(&maps.out_lo, slot + SLOT, t.n + c, row0, t.z);
+                        tma_store_3d(&maps.out_hi, at, t.n + c, row0, t.z);
+                        if (!g.last) tma_store_3d(&maps.out_lo, at + SLOT / 2, t.n + c, row0, t.z);
                         bulk_commit();
-                        bulk_wait_read_0();
+                        if (c > side) bulk_wait_read_1();
                     }
-                    request(c + 64);
+                    if (c > side) request(c + 32);  // (into the set of the columns before these, whose store has been read)
                 }
+                if (lane == 0) bulk_wait_read_0();
                 if (!ok) break;
             }
             index += step;
             have = tile_at<KIND, SIDE>(g, index, t);
-            if (have) request(side);
+            if (have) request(side), request(side + 32);
         }
         if (KIND == APPLY && lane == 0) bulk_wait_all();
     }
@@ -408,6 +421,35 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
 template <int KIND>
 __global__ void __launch_bounds__(THREADS, 1) single_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args g) {
     product<KIND, 1>(maps, g);
+}
+
+// A from partial results: 32 x 32 of its values a block, of a triangle of such tiles; its own and the other triangle's.
+__global__ void __launch_bounds__(256) sum_kernel(const __grid_constant__ Args g, int splits) {
+    __shared__ float tile[32][33];
+    after_previous();
+    Tile t;
+    if (!tile_at<SQUARE, 32>(g, blockIdx.x, t)) return;
+    const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
+    const int64_t matrix = int64_t(t.z) * g.rows, stride = int64_t(g.batch) * g.rows * g.pitch;
+    for (int i = y; i < 32; i += 8) {
+        const int row = t.m + i, column = t.n + x;
+        float v       = 0.f;
+        if (row < g.rows && column < g.cols) {
+            const float* p = g.part + (matrix + row) * g.pitch + column;
+#pragma unroll 4
+            for (int s = 0; s < splits; ++s) v += p[s * stride];
+            v *= g.f[0];
+            if (row == column) g.diag_out[int64_t(t.z) * g.diag_pitch + row] = v, v = 0.f;
+            g.out[(matrix + row) * g.pitch + column] = __float2half_rn(v * g.f[4]);
+        }
+        tile[i][x] = v;
+    }
+    __syncthreads();
+    if (t.m == t.n) return;
+    for (int i = y; i < 32; i += 8) {
+        const int row = t.n + i, column = t.m + x;
+        if (row < g.rows && column < g.cols) g.out[(matrix + row) * g.pitch + column] = __float2half_rn(tile[x][i] * g.f[4]);
+    }
 }
 
 // ---- x to X ----------------------------------------------------------------------------------------------------------------------
@@ -542,13 +584,19 @@ struct Plan {
     __half *x[2][2], *a, *b;
     float *d, *e;
     double* sums;
+    int splits;          // partial results of A that there is room for
+    float* part;
     __nv_bfloat16* out;  // rows of pitch_x, where the result's are no whole 16 bytes
 };
 Plan plan(const Desc& d, Space& space) {
     Plan p{};
     p.k = d.m < d.n ? d.m : d.n, p.pitch_x = up(d.n, 8), p.pitch_a = up(p.k, 8), p.pitch_d = up(p.k, 4);
     p.chunks = (d.m * d.n + CHUNK - 1) / CHUNK;
-    const int64_t each = 8 * d.m * p.pitch_x + 4 * p.k * p.pitch_a;
+    // Partial results where A has few tiles and they are long: no more bytes than X has.
+    const int64_t l = d.m < d.n ? d.n : d.m, part = 4 * p.k * p.pitch_a;
+    p.splits = 1;
+    while (p.splits < 64 && p.splits * 2 * part <= 8 * d.m * p.pitch_x && p.splits * 2 * BK * 4 <= l) p.splits *= 2;
+    const int64_t each = 8 * d.m * p.pitch_x + 4 * p.k * p.pitch_a + (p.splits > 1 ? p.splits * part : 0);
     p.slice = SLICE / each;
     if (p.slice > d.batch) p.slice = d.batch;
     if (p.slice > TABLE) p.slice = TABLE;
@@ -557,6 +605,7 @@ Plan plan(const Desc& d, Space& space) {
         for (__half*& piece : x) piece = static_cast<__half*>(space.take(size_t(p.slice * d.m * p.pitch_x) * 2));
     p.a = static_cast<__half*>(space.take(size_t(p.slice * p.k * p.pitch_a) * 2)), p.b = static_cast<__half*>(space.take(size_t(p.slice * p.k * p.pitch_a) * 2));
     p.d = static_cast<float*>(space.take(size_t(p.slice * p.pitch_d) * 4)), p.e = static_cast<float*>(space.take(size_t(p.slice * p.pitch_d) * 4));
+    if (p.splits > 1) p.part = static_cast<float*>(space.take(size_t(p.slice) * size_t(p.splits) * size_t(part)));
     p.sums = static_cast<double*>(space.take(size_t(p.slice * p.chunks) * 8));
     // the same for every address of the result (a size is asked for before there is one)
     p.out = static_cast<__nv_bfloat16*>(space.take(size_t(p.slice * d.m * p.pitch_x) * 2));
@@ -565,6 +614,12 @@ Plan plan(const Desc& d, Space& space) {
 
 int map_of(CUtensorMap* map, const void* p, int64_t rows, int64_t cols, int64_t pitch, int64_t batch, int box) {
     return make_tmap_bf16_3d(map, p, uint64_t(cols), uint64_t(rows), uint64_t(batch), uint64_t(pitch) * 2, uint64_t(rows * pitch) * 2, 64, uint32_t(box));
+}
+
+int tile_map(CUtensorMap* map, const void* p, int64_t rows, int64_t cols, int64_t pitch, int64_t batch) {
+    const cuuint64_t dims[3] = {cuuint64_t(cols), cuuint64_t(rows), cuuint64_t(batch)}, strides[2] = {cuuint64_t(pitch) * 2, cuuint64_t(rows * pitch) * 2};
+    const cuuint32_t box[3] = {32, 32, 1};
+    return encode_tmap_bf16(map, p, 3, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_64B);
 }
 
 template <int KIND, int SMS>
@@ -576,20 +631,38 @@ int launch_product(const Maps& maps, Args g, const DeviceInfo& dev, cudaStream_t
         configured[dev.device & 63] = true;
     }
     g.tiles_m = int((g.rows + BM * SMS - 1) / (BM * SMS)), g.tiles_n = int((g.cols + BM * SMS - 1) / (BM * SMS));
-    const int64_t per   = KIND == APPLY ? int64_t(g.tiles_m) * g.tiles_n : int64_t(g.tiles_m) * (g.tiles_m + 1) / 2, tiles = per * g.batch;
+    const int64_t per   = KIND == APPLY ? int64_t(g.tiles_m) * g.tiles_n : int64_t(g.tiles_m) * (g.tiles_m + 1) / 2, tiles = per * g.batch * g.splits;
     if (tiles >= (int64_t(1) << 30)) return MIMK_E_UNSUPPORTED;
     const int64_t most = dev.sm_count / SMS;
     return launch_after(kern, unsigned(SMS * (tiles < most ? tiles : most)), THREADS, Shape<KIND>::SMEM, s, maps, g);
 }
-// On pairs of SMs or on single ones: whichever ends first, counting rounds of tiles, 512 or 256 cycles a k-block and some 6 k-blocks' for a tile's ends.
-template <int KIND>
-int launch(const Maps& maps, const Args& g, const DeviceInfo& dev, cudaStream_t s) {
-    double time[3];
+// How a product runs: a tile on pairs of SMs or on single ones, and over how many tiles the k-blocks of one are dealt out; whichever ends first, in cycles. A
+// k-block takes 540 cycles on either, the single ones' 128 x 128 as the 64 bytes a cycle that an SM gets from the L2 cache carry its operands no faster (measured 500, pairs 542);
+// a tile's ends some 6000; adding up partial results another launch of 6000 and their bytes.
+struct How {
+    int sms, splits, per, asked;
+};
+How how(int kind, int64_t rows, int64_t cols, int64_t batch, int64_t kb, int sm_count, int least_splits, int most_splits) {
+    How best{1, 1, int(kb), 1};
+    double least = 1e300;
     for (int sms = 1; sms <= 2; ++sms) {
-        const int64_t m = (g.rows + BM * sms - 1) / (BM * sms), n = (g.cols + BM * sms - 1) / (BM * sms), tiles = (KIND == APPLY ? m * n : m * (m + 1) / 2) * g.batch;
-        time[sms] = double((tiles + dev.sm_count / sms - 1) / (dev.sm_count / sms)) * (double(g.kb) + 6) * (sms == 2 ? 512 : 270);
+        const int64_t m = (rows + BM * sms - 1) / (BM * sms), n = (cols + BM * sms - 1) / (BM * sms), tiles = (kind == APPLY ? m * n : m * (m + 1) / 2) * batch;
+        for (int64_t splits = least_splits; splits <= most_splits; splits *= 2) {
+            const int64_t per = (kb + splits - 1) / splits, rounds = (tiles * splits + sm_count / sms - 1) / (sm_count / sms);
+            double time = double(rounds) * double(per) * (sms == 2 ? 540 : 500) + 6000.0 * double(rounds < 2 ? rounds : 2);
+            if (splits > 1) time += 6000 + double(splits) * double(rows) * double(rows) * double(batch) * 4 / 3000;
+            if (time < least) least = time, best = {sms, int((kb + per - 1) / per), int(per), int(splits)};
+        }
     }
-    return time[2] <= time[1] ? launch_product<KIND, 2>(maps, g, dev, s) : launch_product<KIND, 1>(maps, g, dev, s);
+    return best;
+}
+template <int KIND>
+int launch(const Maps& maps, Args g, const How& h, const DeviceInfo& dev, cudaStream_t s) {
+    g.splits = h.splits, g.per = h.per;
+    MIMK_TRY((h.sms == 2 ? launch_product<KIND, 2>(maps, g, dev, s) : launch_product<KIND, 1>(maps, g, dev, s)));
+    if (h.splits == 1) return MIMK_OK;
+    g.tiles_m = g.tiles_n = (g.rows + 31) / 32;
+    return launch_after(sum_kernel, unsigned(g.tiles_m * (g.tiles_m + 1) / 2 * g.batch), 256, 0, s, g, h.splits);
 }
 
 template <class T>
@@ -615,48 +688,44 @@ int slice(const Desc& d, const Plan& p, const Factors* f, int64_t first, int64_t
     const bool tall = d.m > d.n;
     __nv_bfloat16* out = static_cast<__nv_bfloat16*>(d.out) + first * d.m * d.n;
     const bool staged  = !group::tma_can_read(out, d.n);
-    Maps maps;
-    CUtensorMap a_map, b_map;
+    // every map once: X as an operand of each product and as tiles of 32 rows and columns, A, B, and the result's tiles
+    CUtensorMap gram[2], apply[2], x_hi[2], x_lo[2], a_map, b_map, result;
+    for (int i = 0; i < 2; ++i) {
+        MIMK_TRY(map_of(&gram[i], p.x[i][0], d.m, d.n, p.pitch_x, count, tall ? 64 : BM));
+        MIMK_TRY(map_of(&apply[i], p.x[i][0], d.m, d.n, p.pitch_x, count, tall ? BM : 64));
+        MIMK_TRY(tile_map(&x_hi[i], p.x[i][0], d.m, d.n, p.pitch_x, count));
+        MIMK_TRY(tile_map(&x_lo[i], p.x[i][1], d.m, d.n, p.pitch_x, count));
+    }
     MIMK_TRY(map_of(&a_map, p.a, p.k, p.k, p.pitch_a, count, BM));
     MIMK_TRY(map_of(&b_map, p.b, p.k, p.k, p.pitch_a, count, BM));
-    const auto blocks = [](int64_t v) { return int((v + BK - 1) / BK); };
+    MIMK_TRY(staged ? tile_map(&result, p.out, d.m, d.n, p.pitch_x, count) : tile_map(&result, out, d.m, d.n, d.n, count));
+    const int64_t kb_gram = ((tall ? d.m : d.n) + BK - 1) / BK, kb = (p.k + BK - 1) / BK;
+    // (sums are split as for one matrix alone, so that it comes out the same in any batch)
+    const int splits  = how(GRAM, p.k, p.k, 1, kb_gram, dev.sm_count, 1, p.splits).asked;
+    const How hows[3] = {how(GRAM, p.k, p.k, count, kb_gram, dev.sm_count, splits, splits), how(SQUARE, p.k, p.k, count, kb, dev.sm_count, 1, 1), how(APPLY, d.m, d.n, count, kb, dev.sm_count, 1, 1)};
+    Maps maps;
     for (int step = 0; step < d.steps; ++step) {
-        const Factors& c   = f[step];
-        __half* const* now = p.x[step & 1];
-        __half* const* next = p.x[~step & 1];
+        const Factors& c = f[step];
+        const int now = step & 1, next = now ^ 1;
         Args g{};
         g.batch = int(count), g.pitch = int(p.pitch_a), g.diag_pitch = int(p.pitch_d), g.status = dev.status_dev;
         // A
-        g.rows = g.cols = int(p.k), g.kb = blocks(tall ? d.m : d.n), g.a_mn = g.b_mn = tall, g.out = p.a, g.diag_out = p.d;
+        g.rows = g.cols = int(p.k), g.kb = int(kb_gram), g.a_mn = g.b_mn = tall, g.out = p.a, g.diag_out = p.d, g.part = p.part;
         g.f[0] = 1.f / (SX * SX), g.f[4] = c.a;
-        MIMK_TRY(map_of(&maps.left, now[0], d.m, d.n, p.pitch_x, count, tall ? 64 : BM));
-        maps.right = maps.left;
-        MIMK_TRY(launch<GRAM>(maps, g, dev, s));
+        maps.left = maps.right = gram[now];
+        MIMK_TRY(launch<GRAM>(maps, g, hows[0], dev, s));
         // B
-        g.kb = blocks(p.k), g.a_mn = g.b_mn = 0, g.in = p.a, g.out = p.b, g.diag_in = p.d, g.diag_out = p.e;
+        g.kb = int(kb), g.a_mn = g.b_mn = 0, g.in = p.a, g.out = p.b, g.diag_in = p.d, g.diag_out = p.e;
         g.f[0] = 1.f / (c.a * c.a), g.f[1] = 1.f / c.a, g.f[2] = c.q, g.f[3] = c.r, g.f[4] = c.b;
         maps.left = maps.right = a_map;
-        MIMK_TRY(launch<SQUARE>(maps, g, dev, s));
+        MIMK_TRY(launch<SQUARE>(maps, g, hows[1], dev, s));
         // X
         g.rows = int(d.m), g.cols = int(d.n), g.b_mn = !tall, g.tall = tall, g.last = step + 1 == d.steps, g.diag_in = p.e;
         g.f[0] = c.p, g.f[1] = 1.f / c.b, g.f[2] = d.scale / SX;
-        if (tall) {
-            MIMK_TRY(map_of(&maps.left, now[0], d.m, d.n, p.pitch_x, count, BM));
-            maps.right = b_map;
-        } else {
-            maps.left = b_map;
-            MIMK_TRY(map_of(&maps.right, now[0], d.m, d.n, p.pitch_x, count, 64));
-        }
-        MIMK_TRY(map_of(&maps.hi, now[0], d.m, d.n, p.pitch_x, count, 32));
-        MIMK_TRY(map_of(&maps.lo, now[1], d.m, d.n, p.pitch_x, count, 32));
-        if (g.last) {
-            MIMK_TRY(staged ? map_of(&maps.out_hi, p.out, d.m, d.n, p.pitch_x, count, 32) : map_of(&maps.out_hi, out, d.m, d.n, d.n, count, 32));
-            maps.out_lo = maps.out_hi;
-        } else {
-            MIMK_TRY(map_of(&maps.out_hi, next[0], d.m, d.n, p.pitch_x, count, 32));
-            MIMK_TRY(map_of(&maps.out_lo, next[1], d.m, d.n, p.pitch_x, count, 32));
-        }
-        MIMK_TRY(launch<APPLY>(maps, g, dev, s));
+        maps.left = tall ? apply[now] : b_map, maps.right = tall ? b_map : apply[now];
+        maps.hi = x_hi[now], maps.lo = x_lo[now];
+        maps.out_hi = g.last ? result : x_hi[next], maps.out_lo = g.last ? result : x_lo[next];
+        MIMK_TRY(launch<APPLY>(maps, g, hows[2], dev, s));
     }
     return staged ? copy_rows(p.out, p.pitch_x, out, d.n, count * d.m, d.n, s) : MIMK_OK;
 }
