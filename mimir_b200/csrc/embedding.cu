@@ -4,7 +4,8 @@
 // for each class's group taken from a cursor, each position written to its group. Atomics leave a group's positions in any order, but their
 // set is known, so each group is put in rising order before it is summed (32 positions by a warp, in registers; more of them by a block, as a map of
 // bits), and results are the same call after call. A warp then owns 32 x VEC x COLS columns of a class: it adds up to 32 rows of dy, or writes zeros;
-// classes of more rows are taken by whole blocks, a run of the rows for each warp, joined in shared memory.
+// classes of more rows are taken by whole blocks, a run of the rows for each warp, joined in shared memory. All of it is one launch whose blocks meet between
+// its phases (and one that clears the counts). Up to 2048 positions: a launch of blocks that each look through all of them for the classes that are their own.
 // What bounds it: the bytes, most of all the table's gradient.
 #include "elements.cuh"
 #include "train_common.cuh"
@@ -14,7 +15,10 @@ namespace mimk {
 namespace {
 
 constexpr int THREADS = 256, WARPS = THREADS / 32;
+constexpr int WORKERS = 512, BLOCK = WORKERS + 32;  // of the launch whose blocks meet (the fewer of them, the sooner), and a warp that writes zeros
+constexpr int ZEROS = 4096;          // bytes of one bulk store
 constexpr int LIGHT = 32;            // positions of a class that one warp adds up
+constexpr int PIECE = 512;           // and that one block does
 constexpr int WINDOW = 1 << 17;      // positions in one map of bits
 constexpr int64_t LIM = int64_t(1) << 31;
 
@@ -33,13 +37,13 @@ __device__ __forceinline__ int class_at(const Ids& ids, int64_t i) {
 
 // COLS loads of VEC elements, 32 lanes side by side, are a part of a row: one warp's work.
 template <class T, class O, int VEC, int COLS>
-__global__ void __launch_bounds__(THREADS) rows_kernel(const T* table, Ids ids, O* out, int64_t n, int64_t d, int parts, float scale, int* status) {
+__global__ void __launch_bounds__(THREADS) rows_kernel(const T* table, Ids ids, O* out, int64_t n, int64_t d, int shift, float scale, int* status) {
     after_previous();
     const int lane = threadIdx.x & 31;
-    const int64_t units = n * parts;
+    const int64_t units = n << shift;  // (as many parts to a row as the next power of two)
     for (int64_t u = int64_t(blockIdx.x) * WARPS + (threadIdx.x >> 5); u < units; u += int64_t(gridDim.x) * WARPS) {
-        const int64_t i = parts == 1 ? u : u / parts;
-        const int64_t from = (u - i * parts) * (32 * VEC * COLS) + lane * VEC;
+        const int64_t i = u >> shift, from = (u - (i << shift)) * (32 * VEC * COLS) + lane * VEC;
+        if (from - lane * VEC >= d) continue;
         const int c = class_at(ids, i);
         if (c == BAD && lane == 0) *status = MIMK_E_SHAPE;
         Run<T, VEC> run[COLS];
@@ -62,6 +66,42 @@ __global__ void __launch_bounds__(THREADS) rows_kernel(const T* table, Ids ids, 
     }
 }
 
+template <int N>
+__device__ __forceinline__ void workers_meet() {
+    asm volatile("bar.sync 1, %0;" ::"n"(N) : "memory");
+}
+template <int N>
+__device__ __forceinline__ void with_writer() {
+    asm volatile("bar.sync 2, %0;" ::"n"(N) : "memory");
+}
+
+// ---- zeros -----------------------------------------------------------------------------------------------------------------------
+// Bulk stores from a piece of shared memory that holds zeros, OUTSTANDING of them on their way. By themselves 32 KiB or so for each SM write 1.07 GB in 150 to 176 us, as stores by
+// all threads do at best; beside the sums of 8192 rows stores of 2 KiB took 248 us (130 cycles each), of 4 KiB 208.
+template <int OUTSTANDING>
+__device__ __forceinline__ void zero_span(uint8_t* p, int64_t bytes, uint32_t zeros) {
+    const int lane = threadIdx.x & 31;
+    const int64_t head = min(bytes, int64_t(-reinterpret_cast<uintptr_t>(p) & 15)), body = (bytes - head) & ~int64_t(15), tail = bytes - head - body;
+    // (elements are two or four bytes, on such boundaries)
+    if (lane * 2 < head) *reinterpret_cast<uint16_t*>(p + lane * 2) = 0;
+    if (lane * 2 < tail) *reinterpret_cast<uint16_t*>(p + head + body + lane * 2) = 0;
+    if (lane == 0)
+        for (int64_t at = 0; at < body; at += ZEROS) {
+            asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(p + head + at), "r"(zeros), "r"(int(min(body - at, int64_t(ZEROS)))) : "memory");
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+            asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(OUTSTANDING - 1) : "memory");
+        }
+}
+__device__ __forceinline__ uint32_t make_zeros(uint4* room) {
+    for (int i = threadIdx.x & 31; i < ZEROS / 16; i += 32) room[i] = make_uint4(0, 0, 0, 0);
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncwarp();
+    return uint32_t(__cvta_generic_to_shared(room));
+}
+__device__ __forceinline__ void zeros_written() {
+    if ((threadIdx.x & 31) == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+}
+
 // ---- groups ------------------------------------------------------------------------------------------------------------------------
 struct Groups {
     int* count;   // [v] positions of a class
@@ -69,19 +109,48 @@ struct Groups {
     int* slot;    // [n] place in the group, in any order
     int* order;   // [n] positions by group
     int* sorted;  // [n] the same, groups of more than LIGHT positions in rising order
-    int* heavy;   // [n / LIGHT] classes of such groups
-    int* cursor;  // places taken; heavy classes
+    int4* heavy;  // pieces of such groups: class, which piece, of how many, place of the partial sums where there are several
+    int* light;   // [n] the other classes that occur
+    float* part;  // rows of partial sums
+    int* cursor;  // places taken; pieces; blocks that have met; whether one gave up; the other classes; rows of partial sums
+    int64_t part_pitch;
 };
 
 __global__ void __launch_bounds__(THREADS) clear_kernel(Groups g, int64_t v) {
     after_previous();
-    if (blockIdx.x == 0 && threadIdx.x < 2) g.cursor[threadIdx.x] = 0;
+    if (blockIdx.x == 0 && threadIdx.x < 6) g.cursor[threadIdx.x] = 0;
     for (int64_t i = int64_t(blockIdx.x) * THREADS + threadIdx.x; i < v; i += int64_t(gridDim.x) * THREADS) g.count[i] = 0;
 }
 
-__global__ void __launch_bounds__(THREADS) count_kernel(Ids ids, Groups g, int64_t n, int* status) {
-    after_previous();
-    for (int64_t base = int64_t(blockIdx.x) * THREADS; base < n; base += int64_t(gridDim.x) * THREADS) {
+// All blocks of the launch (which are resident at once) have come here. False: one of them has not come in a second or so, the status word says so, and the kernel is
+// left by all.
+__device__ __forceinline__ bool all_blocks_meet(const Groups& g, int nth, int* status) {
+    __shared__ int met;
+    workers_meet<WORKERS>();
+    if (threadIdx.x == 0) {
+        int* arrived = g.cursor + 2;
+        volatile int* given_up = g.cursor + 3;
+        __threadfence();
+        atomicAdd(arrived, 1);
+        const int all      = nth * int(gridDim.x);
+        const long long t0 = clock64();
+        met = 1;
+        for (;;) {
+            int now;
+            asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(now) : "l"(arrived) : "memory");
+            if (now >= all) break;
+            if (*given_up || clock64() - t0 > 2000000000LL) {
+                *given_up = 1, *status = MIMK_E_DEVICE_WAIT, met = 0;
+                break;
+            }
+        }
+    }
+    workers_meet<WORKERS>();
+    return met;
+}
+
+__device__ __forceinline__ void count_positions(const Ids& ids, const Groups& g, int64_t n, int* status) {
+    for (int64_t base = int64_t(blockIdx.x) * WORKERS; base < n; base += int64_t(gridDim.x) * WORKERS) {
         const int64_t i = base + threadIdx.x;
         const int c     = i < n ? class_at(ids, i) : NO_TOKEN;
         if (c == BAD) *status = MIMK_E_SHAPE;
@@ -96,7 +165,7 @@ __global__ void __launch_bounds__(THREADS) count_kernel(Ids ids, Groups g, int64
 
 // the sum of a value over the threads of the block before this one, and over all
 __device__ __forceinline__ int block_before(int v, int* total) {
-    __shared__ int part[WARPS];
+    __shared__ int part[WORKERS / 32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     int sum = v;
 #pragma unroll
@@ -104,12 +173,12 @@ __device__ __forceinline__ int block_before(int v, int* total) {
         const int w = __shfl_up_sync(0xffffffffu, sum, o);
         if (lane >= o) sum += w;
     }
-    __syncthreads();  // (of an earlier call's reads)
+    workers_meet<WORKERS>();  // (of an earlier call's reads)
     if (lane == 31) part[warp] = sum;
-    __syncthreads();
+    workers_meet<WORKERS>();
     int before = 0, all = 0;
 #pragma unroll
-    for (int w = 0; w < WARPS; ++w) {
+    for (int w = 0; w < WORKERS / 32; ++w) {
         before += w < warp ? part[w] : 0;
         all += part[w];
     }
@@ -117,49 +186,52 @@ __device__ __forceinline__ int block_before(int v, int* total) {
     return before + sum - v;
 }
 
-__global__ void __launch_bounds__(THREADS) start_kernel(Groups g, int64_t v) {
-    __shared__ int first[2];
-    after_previous();
-    for (int64_t base = int64_t(blockIdx.x) * THREADS; base < v; base += int64_t(gridDim.x) * THREADS) {
+__device__ __forceinline__ void take_places(const Groups& g, int64_t v) {
+    __shared__ int first[4];
+    for (int64_t base = int64_t(blockIdx.x) * WORKERS; base < v; base += int64_t(gridDim.x) * WORKERS) {
         const int64_t c = base + threadIdx.x;
         const int count = c < v ? g.count[c] : 0;
-        int all, heavies;
-        const int before = block_before(count, &all), nth = block_before(count > LIGHT, &heavies);
+        const int pieces = count > LIGHT ? (count + PIECE - 1) / PIECE : 0, parts = pieces > 1 ? pieces : 0;
+        int all, heavies, lights, partials;
+        const int before = block_before(count, &all);
         if (!all) continue;
-        if (threadIdx.x == 0) first[0] = atomicAdd(g.cursor, all), first[1] = heavies ? atomicAdd(g.cursor + 1, heavies) : 0;
-        __syncthreads();
+        const int nth = block_before(pieces, &heavies), other = block_before(count > 0 && !pieces, &lights), row = block_before(parts, &partials);
+        if (threadIdx.x == 0) first[0] = atomicAdd(g.cursor, all);
+        if (threadIdx.x == 32 && heavies) first[1] = atomicAdd(g.cursor + 1, heavies);
+        if (threadIdx.x == 64 && lights) first[2] = atomicAdd(g.cursor + 4, lights);
+        if (threadIdx.x == 96 && partials) first[3] = atomicAdd(g.cursor + 5, partials);
+        workers_meet<WORKERS>();
         if (count) g.start[c] = first[0] + before;
-        if (count > LIGHT) g.heavy[first[1] + nth] = int(c);
-        __syncthreads();
+        for (int k = 0; k < pieces; ++k) g.heavy[first[1] + nth + k] = make_int4(int(c), k, pieces, first[3] + row);
+        if (count && !pieces) g.light[first[2] + other] = int(c);
+        workers_meet<WORKERS>();
     }
 }
 
-__global__ void __launch_bounds__(THREADS) place_kernel(Ids ids, Groups g, int64_t n) {
-    after_previous();
-    for (int64_t i = int64_t(blockIdx.x) * THREADS + threadIdx.x; i < n; i += int64_t(gridDim.x) * THREADS) {
+__device__ __forceinline__ void fill_groups(const Ids& ids, const Groups& g, int64_t n) {
+    for (int64_t i = int64_t(blockIdx.x) * WORKERS + threadIdx.x; i < n; i += int64_t(gridDim.x) * WORKERS) {
         const int slot = g.slot[i];
         if (slot >= 0) g.order[g.start[class_at(ids, i)] + slot] = int(i);
     }
 }
 
 // A block for a heavy class: its positions as bits of a map, read off in order.
-__global__ void __launch_bounds__(THREADS) sort_kernel(Groups g, int64_t n) {
-    __shared__ uint32_t bits[WINDOW / 32];
-    after_previous();
+__device__ __forceinline__ void sort_heavies(const Groups& g, int64_t n, uint32_t* bits) {
     const int heavies = g.cursor[1];
     for (int h = blockIdx.x; h < heavies; h += gridDim.x) {
-        const int c = g.heavy[h], count = g.count[c], start = g.start[c];
+        if (g.heavy[h].y) continue;
+        const int c = g.heavy[h].x, count = g.count[c], start = g.start[c];
         int done = 0;
         for (int64_t window = 0; window < n && done < count; window += WINDOW) {
             const int words = int(n - window < WINDOW ? (n - window + 31) / 32 : WINDOW / 32);
-            const int each  = (words + THREADS - 1) / THREADS;
-            for (int w = threadIdx.x; w < words; w += THREADS) bits[w] = 0;
-            __syncthreads();
-            for (int k = threadIdx.x; k < count; k += THREADS) {
+            const int each  = (words + WORKERS - 1) / WORKERS;
+            for (int w = threadIdx.x; w < words; w += WORKERS) bits[w] = 0;
+            workers_meet<WORKERS>();
+            for (int k = threadIdx.x; k < count; k += WORKERS) {
                 const int64_t at = g.order[start + k] - window;
                 if (at >= 0 && at < WINDOW) atomicOr(bits + (at >> 5), 1u << (at & 31));
             }
-            __syncthreads();
+            workers_meet<WORKERS>();
             const int lo = min(words, int(threadIdx.x) * each), hi = min(words, lo + each);
             int mine = 0, all;
             for (int w = lo; w < hi; ++w) mine += __popc(bits[w]);
@@ -167,7 +239,7 @@ __global__ void __launch_bounds__(THREADS) sort_kernel(Groups g, int64_t n) {
             for (int w = lo; w < hi; ++w)
                 for (uint32_t b = bits[w]; b; b &= b - 1) g.sorted[to++] = int(window) + w * 32 + __ffs(b) - 1;
             done += all;
-            __syncthreads();
+            workers_meet<WORKERS>();
         }
     }
 }
@@ -214,69 +286,238 @@ __device__ __forceinline__ void add_rows(float (&acc)[COLS][VEC], const T* dy, i
             }
     }
 }
+template <class O, int VEC>
+__device__ __forceinline__ void store_one(const float (&acc)[VEC], O* to, float scale, bool add) {
+    float v[VEC], old[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) old[j] = 0.f;
+    if (add) {
+        Run<O, VEC> r;
+        r.load(to), r.get(old);
+    }
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) v[j] = add ? fmaf(acc[j], scale, old[j]) : acc[j] * scale;
+    put(to, v);
+}
 template <class O, int VEC, int COLS>
 __device__ __forceinline__ void store_row(const float (&acc)[COLS][VEC], O* row, int64_t d, int64_t from, float scale, bool add) {
 #pragma unroll
     for (int q = 0; q < COLS; ++q) {
         const int64_t at = from + q * 32 * VEC;
-        if (at >= d) break;
-        float v[VEC], old[VEC];
+        if (at < d) store_one<O, VEC>(acc[q], row + at, scale, add);
+    }
+}
+
+// What the N workers' warps of a block have summed of one row's part, joined in their order and stored, 32 x VEC columns to a warp.
+template <int N, class O, int VEC, int COLS>
+__device__ __forceinline__ void join_warps(float (&acc)[COLS][VEC], float (*joined)[32 * VEC], O* row, int64_t d, int64_t from, float scale, bool add) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) old[j] = 0.f;
-        if (add) {
-            Run<O, VEC> r;
-            r.load(row + at), r.get(old);
+    for (int q = 0; q < COLS; ++q) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) joined[warp][j * 32 + lane] = acc[q][j];
+        workers_meet<N * 32>();
+        const int64_t at = from + q * 32 * VEC;
+        if (warp == q % N && at < d) {
+            float all[VEC];
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                all[j] = 0.f;
+#pragma unroll 8
+                for (int w = 0; w < N; ++w) all[j] += joined[w][j * 32 + lane];
+            }
+            store_one<O, VEC>(all, row + at, scale, add);
         }
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) v[j] = add ? fmaf(acc[q][j], scale, old[j]) : acc[q][j] * scale;
-        put(row + at, v);
+        workers_meet<N * 32>();
     }
 }
 
 template <class T, class O, int VEC, int COLS>
-__global__ void __launch_bounds__(THREADS) sum_kernel(const T* dy, Groups g, O* dtable, int64_t d, int64_t v, int parts, float scale, bool add) {
+__global__ void __launch_bounds__(BLOCK, 1) grad_kernel(const T* dy, Ids ids, Groups g, O* dtable, int64_t n, int64_t d, int64_t v, int shift, float scale, bool add, int* status) {
     constexpr int PART = 32 * VEC * COLS;
-    __shared__ float joined[WARPS][PART];
-    after_previous();
+    __shared__ union {
+        float joined[WORKERS / 32][32 * VEC];
+        uint32_t bits[WINDOW / 32];
+    } room;
+    __shared__ alignas(16) uint4 nothing[ZEROS / 16];
+    __shared__ int counted;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int64_t heavy_units = int64_t(g.cursor[1]) * parts;
+    if (threadIdx.x >= WORKERS) {
+        // the rows of classes that no position names, as soon as those are known: every gridDim.x-th 32 classes, neighbours among them together
+        const uint32_t zeros = make_zeros(nothing);
+        with_writer<BLOCK>();
+        if (!counted || add) return;
+        const int64_t row = d * int64_t(sizeof(O)), step = int64_t(gridDim.x) * 32, first = int64_t(blockIdx.x) * 32;
+        int next = first + lane < v ? g.count[first + lane] : -1;
+        for (int64_t base = first; base < v; base += step) {
+            unsigned left = __ballot_sync(0xffffffffu, next == 0);
+            next          = base + step + lane < v ? g.count[base + step + lane] : -1;
+            while (left) {
+                const int from = __ffs(left) - 1, to = min(32, from + (~(left >> from) ? __ffs(~(left >> from)) - 1 : 32));
+                zero_span<8>(reinterpret_cast<uint8_t*>(dtable) + (base + from) * row, (to - from) * row, zeros);
+                left = to == 32 ? 0u : left >> to << to;
+            }
+        }
+        zeros_written();
+        return;
+    }
+    // (launched together: the blocks meet)
+    count_positions(ids, g, n, status);
+    const bool met = all_blocks_meet(g, 1, status);
+    if (threadIdx.x == 0) counted = met;
+    with_writer<BLOCK>();
+    if (!met) return;
+    take_places(g, v);
+    if (!all_blocks_meet(g, 2, status)) return;
+    fill_groups(ids, g, n);
+    if (!all_blocks_meet(g, 3, status)) return;
+    if (g.cursor[1]) {
+        sort_heavies(g, n, room.bits);
+        if (!all_blocks_meet(g, 4, status)) return;
+    }
+    const int64_t heavy_units = int64_t(g.cursor[1]) << shift;
     for (int64_t u = blockIdx.x; u < heavy_units; u += gridDim.x) {
-        const int64_t h    = u / parts;
-        const int64_t from = (u - h * parts) * PART + lane * VEC;
-        const int c = g.heavy[h], count = g.count[c], start = g.start[c];
-        const int each = (count + WARPS - 1) / WARPS, lo = min(count, warp * each), hi = min(count, lo + each);
+        const int64_t h = u >> shift, first = (u - (h << shift)) * PART, from = first + lane * VEC;
+        if (first >= d) continue;
+        const int4 piece = g.heavy[h];
+        const int c = piece.x, start = g.start[c] + piece.y * PIECE, count = min(PIECE, g.count[c] - piece.y * PIECE);
+        const int each = (count + WORKERS / 32 - 1) / (WORKERS / 32), lo = min(count, warp * each), hi = min(count, lo + each);
         float acc[COLS][VEC] = {};
         for (int k = lo; k < hi; k += 32) add_rows<T, VEC, COLS>(acc, dy, d, from, k + lane < hi ? g.sorted[start + k + lane] : 0, min(32, hi - k));
-#pragma unroll
-        for (int q = 0; q < COLS; ++q)
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) joined[warp][(q * VEC + j) * 32 + lane] = acc[q][j];
-        __syncthreads();
-        if (warp == 0) {
-#pragma unroll
-            for (int q = 0; q < COLS; ++q)
-#pragma unroll
-                for (int j = 0; j < VEC; ++j)
-                    for (int w = 1; w < WARPS; ++w) acc[q][j] += joined[w][(q * VEC + j) * 32 + lane];
+        if (piece.z == 1) join_warps<WORKERS / 32, O, VEC, COLS>(acc, room.joined, dtable + int64_t(c) * d, d, from, scale, add);
+        else join_warps<WORKERS / 32, float, VEC, COLS>(acc, room.joined, g.part + int64_t(piece.w + piece.y) * g.part_pitch, d, from, 1.f, false);
+    }
+    // The other classes that occur: units warp, warp + warps, ...; what 32 of them need to know comes in one load each, the positions of one while the rows of the one before
+    // are on their way (a read takes several microseconds while zeros are written).
+    const int64_t units = int64_t(g.cursor[4]) << shift, warps = int64_t(gridDim.x) * (WORKERS / 32);
+    for (int64_t first = int64_t(warp) * gridDim.x + blockIdx.x; first < units; first += 32 * warps) {
+        const int64_t mine = first + lane * warps;
+        const int its      = mine < units ? g.light[mine >> shift] : 0;
+        const int count = mine < units ? g.count[its] : 0, start = mine < units ? g.start[its] : 0;
+        const int here  = int(min(int64_t(32), (units - first + warps - 1) / warps));
+        const auto ask  = [&](int k) {
+            const int positions = __shfl_sync(0xffffffffu, count, k & 31), begin = __shfl_sync(0xffffffffu, start, k & 31);
+            return k < here && lane < positions ? g.order[begin + lane] : INT_MAX;
+        };
+        int next = ask(0);
+        for (int k = 0; k < here; ++k) {
+            const int position  = sorted_lanes(next), positions = __shfl_sync(0xffffffffu, count, k), c = __shfl_sync(0xffffffffu, its, k);
+            const int64_t begin = ((first + k * warps) & ((int64_t(1) << shift) - 1)) * PART, from = begin + lane * VEC;
+            next                = ask(k + 1);
+            if (begin >= d) continue;
+            float acc[COLS][VEC] = {};
+            add_rows<T, VEC, COLS>(acc, dy, d, from, position, positions);
             store_row<O, VEC, COLS>(acc, dtable + int64_t(c) * d, d, from, scale, add);
         }
-        __syncthreads();
     }
-    // the other classes: units warp, warp + warps, ...; what 32 of them need to know comes in one load each
-    const int64_t units = v * parts, warps = int64_t(gridDim.x) * WARPS;
-    for (int64_t first = int64_t(blockIdx.x) * WARPS + warp; first < units; first += 32 * warps) {
-        const int64_t mine = first + lane * warps;
-        const int count    = mine < units ? g.count[mine / parts] : -1;
-        const int start    = count > 0 && count <= LIGHT ? g.start[mine / parts] : 0;
-        for (unsigned left = __ballot_sync(0xffffffffu, count >= 0 && count <= LIGHT && !(add && count == 0)); left; left &= left - 1) {
-            const int k        = __ffs(left) - 1;
-            const int64_t u    = first + k * warps, c = u / parts;
-            const int64_t from = (u - c * parts) * PART + lane * VEC;
-            const int positions = __shfl_sync(0xffffffffu, count, k), begin = __shfl_sync(0xffffffffu, start, k);
-            float acc[COLS][VEC] = {};
-            if (positions) add_rows<T, VEC, COLS>(acc, dy, d, from, sorted_lanes(lane < positions ? g.order[begin + lane] : INT_MAX), positions);
-            store_row<O, VEC, COLS>(acc, dtable + c * d, d, from, positions ? scale : 0.f, add);
+    if (!g.cursor[5]) return;
+    // what pieces of one class left, in their order
+    if (!all_blocks_meet(g, 5, status)) return;
+    for (int64_t u = int64_t(blockIdx.x) * (WORKERS / 32) + warp; u < heavy_units; u += warps) {
+        const int64_t h = u >> shift, begin = (u - (h << shift)) * PART, from = begin + lane * VEC;
+        const int4 piece = g.heavy[h];
+        if (begin >= d || piece.y || piece.z == 1) continue;
+        float acc[COLS][VEC] = {};
+#pragma unroll
+        for (int q = 0; q < COLS; ++q) {
+            const int64_t at = from + q * 32 * VEC;
+            if (at >= d) break;
+            for (int k = 0; k < piece.z; ++k) {
+                Run<float, VEC> run;
+                float v[VEC];
+                run.load(g.part + int64_t(piece.w + k) * g.part_pitch + at), run.get(v);
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) acc[q][j] += v[j];
+            }
         }
+        store_row<O, VEC, COLS>(acc, dtable + int64_t(piece.x) * d, d, from, scale, add);
+    }
+}
+
+// ---- few positions ---------------------------------------------------------------------------------------------------------------
+// A block has every `group`-th class (blockIdx.x, blockIdx.x + groups, ...) and a part of the columns. Its warps look through a run of the positions each and
+// list what belongs to those classes, in order; the classes that there are then take their positions off the lists.
+constexpr int FEW = 2048, RUN = FEW / WARPS, OWN = 2048, AT_ONCE = 4;  // positions, of them a warp's, classes that a block counts at a time, positions that one warp adds up
+template <class T, class O, int VEC, int COLS>
+__global__ void __launch_bounds__(THREADS) few_kernel(const T* dy, Ids ids, O* dtable, int n, int64_t d, int v, int log_groups, float scale, bool add, int* status) {
+    constexpr int PART = 32 * VEC * COLS;
+    __shared__ int list[WARPS][RUN];          // position | local class << 11
+    __shared__ int length[WARPS];
+    __shared__ uint16_t counts[OWN];
+    __shared__ uint16_t heavy[FEW / 5];       // local classes of more than AT_ONCE positions
+    __shared__ int heavies;
+    __shared__ float joined[WARPS][32 * VEC];
+    after_previous();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, groups = 1 << log_groups, own = (v - int(blockIdx.x) + groups - 1) >> log_groups;
+    const int64_t from = int64_t(blockIdx.y) * PART + lane * VEC;
+    // (a window of the block's classes: all of them, unless there are more than 2048)
+    for (int window = 0; window < own; window += OWN) {
+        const int here = min(OWN, own - window);
+        for (int i = threadIdx.x; i < here; i += THREADS) counts[i] = 0;
+        if (threadIdx.x == 0) heavies = 0;
+        const int each = (n + WARPS - 1) / WARPS, begin = min(n, warp * each), end = min(n, begin + each);
+        int found = 0;
+        for (int base = begin; base < end; base += 32) {
+            const int i = base + lane;
+            const int c = i < end ? class_at(ids, i) : NO_TOKEN;
+            if (c == BAD) *status = MIMK_E_SHAPE;
+            const int local = (c >> log_groups) - window;
+            const bool mine = c >= 0 && (c & (groups - 1)) == int(blockIdx.x) && local >= 0 && local < here;
+            const unsigned all = __ballot_sync(0xffffffffu, mine);
+            if (mine) list[warp][found + __popc(all & ((1u << lane) - 1))] = i | local << 11;
+            found += __popc(all);
+        }
+        if (lane == 0) length[warp] = found;
+        workers_meet<THREADS>();
+        // how many each class has: a class's first position in its warp's list adds all of that list's
+        for (int w = 0; w < WARPS; ++w) {
+            if (warp == w)
+                for (int base = 0; base < found; base += 32) {
+                    const int local = base + lane < found ? list[w][base + lane] >> 11 : -1;
+                    const unsigned same = __match_any_sync(0xffffffffu, local);
+                    if (local >= 0 && __ffs(same) - 1 == lane) {
+                        const int before = counts[local], now = before + __popc(same);
+                        counts[local] = uint16_t(now);
+                        if (before <= AT_ONCE && now > AT_ONCE) heavy[atomicAdd(&heavies, 1)] = uint16_t(local);
+                    }
+                    __syncwarp();
+                }
+            workers_meet<THREADS>();
+        }
+        // A class's positions in list w, behind the `held` that lanes hold: lane k takes the (k - held)-th of them.
+        const auto take = [&](int w, int base, int local, int& position, int held) {
+            const int entry    = base + lane < length[w] ? list[w][base + lane] : -1;
+            const unsigned all = __ballot_sync(0xffffffffu, entry >= 0 && entry >> 11 == local);
+            if (!all) return 0;
+            const int nth = lane - held, source = nth >= 0 && nth < __popc(all) ? int(__fns(all, 0, nth + 1)) : 0;
+            const int its = __shfl_sync(0xffffffffu, entry, source);
+            if (nth >= 0 && nth < __popc(all)) position = its & (FEW - 1);
+            return __popc(all);
+        };
+        // classes of several positions (each by itself: in whichever order): by the block, a list to a warp
+        for (int h = 0; h < heavies; ++h) {
+            const int local = heavy[h];
+            float acc[COLS][VEC] = {};
+            for (int base = 0; base < length[warp]; base += 32) {
+                int position = 0;
+                if (const int count = take(warp, base, local, position, 0)) add_rows<T, VEC, COLS>(acc, dy, d, from, position, count);
+            }
+            join_warps<WARPS, O, VEC, COLS>(acc, joined, dtable + ((int64_t(window + local) << log_groups) + blockIdx.x) * d, d, from, scale, add);
+        }
+        // the others, and zeros for those that do not occur (after them it took 17% longer: 206 us in place of 176 for 1.07 GB)
+        for (int local = warp; local < here; local += WARPS) {
+            const int positions = counts[local];
+            if (positions > AT_ONCE || (add && !positions)) continue;
+            float acc[COLS][VEC] = {};
+            if (positions) {
+                int position = 0, held = 0;
+                for (int w = 0; w < WARPS && held < positions; ++w)
+                    for (int base = 0; base < length[w]; base += 32) held += take(w, base, local, position, held);
+                add_rows<T, VEC, COLS>(acc, dy, d, from, position, positions);
+            }
+            store_row<O, VEC, COLS>(acc, dtable + ((int64_t(window + local) << log_groups) + blockIdx.x) * d, d, from, positions ? scale : 0.f, add);
+        }
+        workers_meet<THREADS>();
     }
 }
 
@@ -285,8 +526,12 @@ Groups groups_in(Space& space, const mimk_embedding_desc& d) {
     Groups g;
     g.count = static_cast<int*>(space.take(size_t(d.v) * 4)), g.start = static_cast<int*>(space.take(size_t(d.v) * 4));
     g.slot = static_cast<int*>(space.take(size_t(d.n) * 4)), g.order = static_cast<int*>(space.take(size_t(d.n) * 4));
-    g.sorted = static_cast<int*>(space.take(size_t(d.n) * 4)), g.heavy = static_cast<int*>(space.take(size_t(d.n) / LIGHT * 4));
-    g.cursor = static_cast<int*>(space.take(8));
+    g.sorted = static_cast<int*>(space.take(size_t(d.n) * 4));
+    // (a class of more than PIECE positions has less than twice as many pieces as it has whole ones)
+    g.heavy = static_cast<int4*>(space.take((size_t(d.n) / LIGHT + size_t(d.n) / PIECE) * 16));
+    g.part_pitch = up(d.d, 8), g.part = static_cast<float*>(space.take(size_t(d.n) / PIECE * 2 * size_t(g.part_pitch) * 4));
+    g.light = static_cast<int*>(space.take(size_t(d.n) * 4));
+    g.cursor = static_cast<int*>(space.take(24));
     return g;
 }
 
@@ -304,19 +549,43 @@ unsigned blocks_for(int64_t units, int64_t each, int64_t most) {
     return unsigned(b < 1 ? 1 : b < most ? b : most);
 }
 
-constexpr int WIDE = 2, NARROW = 8;  // loads a lane: of 8 elements, or of one
+constexpr int WIDE = 2, NARROW = 8;  // loads a lane for a gradient's part of a row: of 8 elements, or of one
 
-template <class T, class O, int VEC, int COLS>
-int rows(const mimk_embedding_desc& d, const DeviceInfo& dev, cudaStream_t s) {
-    const int parts = int((d.d + 32 * VEC * COLS - 1) / (32 * VEC * COLS));
-    return launch_after(rows_kernel<T, O, VEC, COLS>, blocks_for(d.n * parts, WARPS, 1 << 20), THREADS, 0, s, static_cast<const T*>(d.table), ids_of(d),
-                        static_cast<O*>(d.out), d.n, d.d, parts, d.scale, dev.status_dev);
+template <int VEC, int COLS>
+int parts_of(int64_t d) {
+    return int((d + 32 * VEC * COLS - 1) / (32 * VEC * COLS));
+}
+int log_up(int64_t v) {
+    int log = 0;
+    while ((int64_t(1) << log) < v) ++log;
+    return log;
 }
 template <class T, class O, int VEC, int COLS>
-int sums(const mimk_embedding_desc& d, const Groups& g, const DeviceInfo& dev, cudaStream_t s) {
-    const int parts = int((d.d + 32 * VEC * COLS - 1) / (32 * VEC * COLS));
-    return launch_after(sum_kernel<T, O, VEC, COLS>, blocks_for(d.v * parts, WARPS, int64_t(dev.sm_count) * 4), THREADS, 0, s, static_cast<const T*>(d.dy), g,
-                        static_cast<O*>(d.dtable), d.d, d.v, parts, d.scale, d.add != 0);
+int rows(const mimk_embedding_desc& d, const DeviceInfo& dev, cudaStream_t s) {
+    constexpr int LOADS = VEC == 1 ? COLS : 2 * COLS;
+    const int shift     = log_up(parts_of<VEC, LOADS>(d.d));
+    return launch_after(rows_kernel<T, O, VEC, LOADS>, blocks_for(d.n << shift, WARPS, 1 << 20), THREADS, 0, s, static_cast<const T*>(d.table), ids_of(d), static_cast<O*>(d.out), d.n,
+                        d.d, shift, d.scale, dev.status_dev);
+}
+template <class T, class O, int VEC, int COLS>
+int grad(const mimk_embedding_desc& d, const Groups& g, const DeviceInfo& dev, cudaStream_t s) {
+    const int parts = parts_of<VEC, COLS>(d.d);
+    if (d.n <= FEW && parts <= 65535) {
+        // Eight blocks to an SM, but no more groups than classes. 2048 positions here and 3000 the other way: 131072 x 4096 bf16 191 and 185 us, 50021 x 2048 54 and 62,
+        // 10007 x 777 f32 28 and 62, 1000 x 4096 25 and 36, 131072 x 64 28 and 32.
+        int log = 0;
+        while ((int64_t(1) << (log + 1)) * parts <= int64_t(dev.sm_count) * 8 && (int64_t(1) << (log + 1)) <= d.v) ++log;
+        return launch_after(few_kernel<T, O, VEC, COLS>, dim3(1u << log, unsigned(parts)), THREADS, 0, s, static_cast<const T*>(d.dy), ids_of(d), static_cast<O*>(d.dtable), int(d.n), d.d,
+                            int(d.v), log, d.scale, d.add != 0, dev.status_dev);
+    }
+    MIMK_TRY(launch_after(clear_kernel, blocks_for(d.v, THREADS, int64_t(dev.sm_count) * 8), THREADS, 0, s, g, d.v));
+    cudaLaunchAttribute together = {};
+    together.id = cudaLaunchAttributeCooperative, together.val.cooperative = 1;
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(unsigned(dev.sm_count)), config.blockDim = dim3(BLOCK),  // (one to an SM)
+    config.stream = s, config.attrs = &together, config.numAttrs = 1;
+    return note_cuda_error(cudaLaunchKernelEx(&config, grad_kernel<T, O, VEC, COLS>, static_cast<const T*>(d.dy), ids_of(d), g, static_cast<O*>(d.dtable), d.n, d.d, d.v,
+                                              log_up(parts), d.scale, d.add != 0, dev.status_dev));
 }
 // f<T, O, VEC, COLS>: by the element types, and whether rows are whole 16 bytes that start on such
 #define MIMK_BY_TYPES(F, ALIGNED, ...)                                                                                                        \
@@ -368,15 +637,6 @@ extern "C" int mimk_embedding_grad(const mimk_embedding_desc* d, void* stream) {
     const Groups g = groups_in(space, *d);
     if (!d->workspace || space.used() > d->workspace_bytes) return MIMK_E_WORKSPACE;
     if (!aligned16(d->workspace)) return MIMK_E_ALIGN;
-    cudaStream_t s     = static_cast<cudaStream_t>(stream);
-    const int64_t most = int64_t(dev->sm_count) * 8;
-    const Ids ids      = ids_of(*d);
-    MIMK_TRY(launch_after(clear_kernel, blocks_for(d->v, THREADS, most), THREADS, 0, s, g, d->v));
-    if (d->n) {
-        MIMK_TRY(launch_after(count_kernel, blocks_for(d->n, THREADS, most), THREADS, 0, s, ids, g, d->n, dev->status_dev));
-        MIMK_TRY(launch_after(start_kernel, blocks_for(d->v, THREADS, most), THREADS, 0, s, g, d->v));
-        MIMK_TRY(launch_after(place_kernel, blocks_for(d->n, THREADS, most), THREADS, 0, s, ids, g, d->n));
-        if (d->n > LIGHT) MIMK_TRY(launch_after(sort_kernel, blocks_for(d->n, LIGHT + 1, most / 2), THREADS, 0, s, g, d->n));
-    }
-    MIMK_BY_TYPES(sums, d->d % 8 == 0 && aligned16(d->dy) && aligned16(d->dtable), *d, g, *dev, s);
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    MIMK_BY_TYPES(grad, d->d % 8 == 0 && aligned16(d->dy) && aligned16(d->dtable), *d, g, *dev, s);
 }
