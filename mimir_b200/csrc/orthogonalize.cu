@@ -485,6 +485,17 @@ __device__ __forceinline__ double squares(const float (&v)[VEC]) {
     for (int j = 0; j < VEC; ++j) d += double(v[j]) * double(v[j]);
     return d;
 }
+// SX / (norm + eps), in two factors, as one may be beyond f32; NaN of a norm that is not finite
+struct Inverse {
+    float first, second;
+    __device__ __forceinline__ Inverse(double norm, float eps) {
+        const double by = isfinite(norm) ? 1.0 / (norm + double(eps)) : double(NAN);
+        int power         = 0;
+        const double lead = isfinite(by) ? frexp(by, &power) : by;
+        first = ldexpf(1.f, power / 2), second = float(ldexp(lead, power - power / 2)) * SX;
+    }
+    __device__ __forceinline__ float times(float v) const { return v * first * second; }
+};
 template <class T, int VEC>
 __global__ void __launch_bounds__(PREPARE) squares_kernel(const __grid_constant__ Matrices all, int64_t count, double* sums) {
     after_previous();
@@ -511,11 +522,7 @@ __global__ void __launch_bounds__(PREPARE) prepare_kernel(const __grid_constant_
     const int chunks    = int((count + CHUNK - 1) / CHUNK);
     double total        = 0;
     for (int i = threadIdx.x; i < chunks; i += PREPARE) total += sums[blockIdx.y * chunks + i];
-    const double norm = sqrt(block_total(total)), by = isfinite(norm) ? 1.0 / (norm + double(eps)) : double(NAN);
-    // in two factors, as one may be beyond f32
-    int power           = 0;
-    const double lead   = isfinite(by) ? frexp(by, &power) : by;
-    const float first   = ldexpf(1.f, power / 2), second = float(ldexp(lead, power - power / 2)) * SX;
+    const Inverse by(sqrt(block_total(total)), eps);
     const T* x          = static_cast<const T*>(all.x[blockIdx.y]);
     const int64_t base  = int64_t(blockIdx.y) * rows * pitch;
     const int units     = (cols + VEC - 1) / VEC;  // of a row
@@ -528,7 +535,7 @@ __global__ void __launch_bounds__(PREPARE) prepare_kernel(const __grid_constant_
             __half h[VEC], l[VEC];
 #pragma unroll
             for (int j = 0; j < VEC; ++j) {
-                v[j] = v[j] * first * second;
+                v[j] = by.times(v[j]);
                 h[j] = __float2half_rn(v[j]), l[j] = __float2half_rn((v[j] - __half2float(h[j])) * LOW);
             }
             const int64_t at = base + int64_t(row) * pitch + u * VEC;
@@ -541,14 +548,247 @@ __global__ void __launch_bounds__(PREPARE) prepare_kernel(const __grid_constant_
         }
 }
 
-// ---- host ------------------------------------------------------------------------------------------------------------------------
-using Desc = mimk_orthogonalize_desc;
-constexpr int64_t LIM = int64_t(1) << 24, SLICE = int64_t(1) << 30;
+// ---- small matrices --------------------------------------------------------------------------------------------------------------
+// All steps of a matrix with up to 128 rows and 256 columns (or turned: 256 and 128) in one CTA: X as f32 in tensor memory and as f16 in shared memory, 64 columns to a
+// 128-byte row, which serves as the operand of X X^T and as the right one of B X; A, then B, as f16 in another such matrix. Eight warps: 32 rows, one to a lane, and half of
+// the columns each. A step's three products take some 512 cycles each, what is between them 600 to 1500. [128, 128]: 
+constexpr int SMALL_K = 128, SMALL_L = 256, SMALL_THREADS = 256, CHUNK64 = 128 * 128;  // bytes of 128 rows of 64 columns
 constexpr int MOST_STEPS = 64;
-
 struct Factors {
     float p, q, r, a, b;  // a step's coefficients, and the factors of A and B
 };
+struct SmallArgs {
+    int k, l, chunks, steps;  // rows and columns of X (turned where x is taller than wide), its chunks of 64 columns
+    int vec;                  // rows of x and of the result are whole 16 bytes
+    float eps, scale;
+    __nv_bfloat16* out;
+    int* status;
+    Factors f[MOST_STEPS];
+};
+struct SmallShared {
+    uint64_t done;
+    uint32_t tmem_base;
+    int abort_flag;
+    float d[SMALL_K], e[SMALL_K];
+    double part[SMALL_THREADS / 32];
+};
+// 16-byte piece of row `row` of a 128-byte-swizzled matrix of 64-column chunks
+__device__ __forceinline__ uint32_t at64(uint32_t base, int row, int column) {
+    return base + (column >> 6) * CHUNK64 + row * 128 + ((uint32_t(column >> 3 & 7) ^ uint32_t(row & 7)) << 4);
+}
+__device__ __forceinline__ void put_tmem(uint32_t to, const float (&v)[32]) {
+#pragma unroll
+    for (int h = 0; h < 32; h += 16) {
+        uint32_t r[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) r[i] = __float_as_uint(v[h + i]);
+        tmem_st_32x32_x16(to + h, r);
+    }
+}
+// 32 values of a row as f16
+__device__ __forceinline__ void put_row(uint32_t base, int row, int column, const float (&v)[32], float by) {
+#pragma unroll
+    for (int i = 0; i < 32; i += 8)
+        st_shared(at64(base, row, column + i), pack_f16(v[i] * by, v[i + 1] * by), pack_f16(v[i + 2] * by, v[i + 3] * by), pack_f16(v[i + 4] * by, v[i + 5] * by), pack_f16(v[i + 6] * by, v[i + 7] * by));
+}
+
+template <class T, bool TALL>
+__global__ void __launch_bounds__(SMALL_THREADS) small_kernel(const __grid_constant__ Matrices all, const __grid_constant__ SmallArgs g) {
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ SmallShared sh;
+    const uint32_t raw = smem_u32(smem_raw), x16 = (raw + 1023u) & ~1023u, a16 = x16 + g.chunks * CHUNK64;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row = (warp & 3) * 32 + lane, half = warp >> 2;
+    const int width = g.chunks * 64, columns = g.chunks > 2 ? 512 : 256;  // of tensor memory: X, and the products behind it
+    if (threadIdx.x == 0) mbar_init(smem_u32(&sh.done), 1), sh.abort_flag = 0, fence_barrier_init();
+    if (warp == 0) {
+        tmem_alloc(smem_u32(&sh.tmem_base), columns);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&sh.tmem_base) + (uint32_t((warp & 3) * 32) << 16), acc = tmem + columns / 2;
+    const uint32_t mma_acc = *reinterpret_cast<volatile uint32_t*>(&sh.tmem_base) + columns / 2;
+    after_previous();
+
+    // x, its columns from `half` of them on
+    const T* x       = static_cast<const T*>(all.x[blockIdx.x]);
+    const bool there = row < g.k;
+    double total     = 0;
+#pragma unroll 1
+    for (int c = half * width / 2; c < (half + 1) * width / 2; c += 32) {
+        float v[32];
+        if (!TALL && g.vec) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 8) {
+                Run<T, 8> run;
+                run.clear();
+                if (there && c + i < g.l) run.load(x + int64_t(row) * g.l + c + i);
+                run.get(*reinterpret_cast<float(*)[8]>(v + i));
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+                Run<T, 1> run;
+                run.clear();
+                if (there && c + i < g.l) run.load(TALL ? x + int64_t(c + i) * g.k + row : x + int64_t(row) * g.l + c + i);
+                run.get(*reinterpret_cast<float(*)[1]>(v + i));
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 32; i += 8) total += squares(*reinterpret_cast<const float(*)[8]>(v + i));
+        put_tmem(tmem + c, v);
+    }
+    tmem_st_wait();
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    if (lane == 0) sh.part[warp] = total;
+    __syncthreads();
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < SMALL_THREADS / 32; ++w) total += sh.part[w];
+    const Inverse by(sqrt(total), g.eps);
+#pragma unroll 1
+    for (int c = half * width / 2; c < (half + 1) * width / 2; c += 32) {
+        uint32_t r[32];
+        float v[32];
+        tmem_ld_32x32(tmem + c, r);
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] = by.times(__uint_as_float(r[i]));
+        put_tmem(tmem + c, v);
+        put_row(x16, row, c, v, 1.f);
+    }
+    tmem_st_wait();
+
+    uint32_t phase = 0;
+    bool ok        = true;
+    // What is in shared memory is multiplied by one thread, `issue`, and all wait for the result.
+    auto multiply = [&](auto&& issue) {
+        fence_proxy_async_smem();
+        tc_fence_before();
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            tc_fence_after();
+            issue();
+            mma_commit(smem_u32(&sh.done));
+        }
+        ok = mbar_wait(smem_u32(&sh.done), phase, &sh.abort_flag);
+        phase ^= 1u;
+        __syncwarp();
+        tc_fence_after();
+    };
+    const uint64_t high  = smem_desc_sw128(0, 0, 1024);
+    const int kblocks    = (g.k + 63) / 64;
+    const uint32_t square = idesc_f16_f32(128, 128, 0, 0), wide = idesc_f16_f32(128, width, 0, 1);
+    for (int step = 0; step < g.steps; ++step) {
+        const Factors f = g.f[step];
+        const bool last = step + 1 == g.steps;
+        // A
+        multiply([&] {
+            for (int c = 0; c < g.chunks; ++c)
+                for (int i = 0; i < 4; ++i) {
+                    const uint64_t d = high | (((x16 + c * CHUNK64 + i * 32) >> 4) | 1u << 16);
+                    mma_f16_ss(mma_acc, d, d, square, c > 0 || i > 0);
+                }
+        });
+#pragma unroll 1
+        for (int c = half * 64; c < half * 64 + 64; c += 32) {
+            uint32_t r[32];
+            float v[32];
+            tmem_ld_32x32(acc + c, r);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]) * (1.f / (SX * SX));
+            if (c == (warp & 3) * 32) {  // the diagonal: lane i has it in column i
+#pragma unroll
+                for (int i = 0; i < 32; ++i)
+                    if (i == lane) sh.d[row] = v[i], v[i] = 0.f;
+            }
+            put_row(a16, row, c, v, f.a);
+        }
+        // B
+        multiply([&] {
+            for (int c = 0; c < kblocks; ++c)
+                for (int i = 0; i < 4; ++i) {
+                    const uint64_t d = high | (((a16 + c * CHUNK64 + i * 32) >> 4) | 1u << 16);
+                    mma_f16_ss(mma_acc, d, d, square, c > 0 || i > 0);
+                }
+        });
+        const float di = sh.d[row], less = 1.f / f.a;
+#pragma unroll 1
+        for (int c = half * 64; c < half * 64 + 64; c += 32) {
+            uint32_t r[32];
+            float v[32];
+            tmem_ld_32x32(acc + c, r);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 32; i += 8) {
+                const uint4 w = ld_shared(at64(a16, row, c + i));
+#pragma unroll
+                for (int j = 0; j < 8; j += 2) {
+                    const float2 o = unpack_f16((&w.x)[j >> 1]);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+                        v[i + j + h] = fmaf(fmaf(f.r, di + sh.d[c + i + j + h], f.q), (h ? o.y : o.x) * less, f.r * (__uint_as_float(r[i + j + h]) * less * less));
+                }
+            }
+            if (c == (warp & 3) * 32) {
+#pragma unroll
+                for (int i = 0; i < 32; ++i)
+                    if (i == lane) sh.e[row] = f.q * di + f.r * fmaf(di, di, __uint_as_float(r[i]) * less * less), v[i] = 0.f;
+            }
+            put_row(a16, row, c, v, f.b);
+        }
+        // X
+        multiply([&] {
+            for (int c = 0; c < kblocks; ++c)
+                for (int i = 0; i < 4; ++i)
+                    mma_f16_ss(mma_acc, high | (((a16 + c * CHUNK64 + i * 32) >> 4) | 1u << 16), high | (((x16 + (c * 64 + i * 16) * 128) >> 4) | uint32_t(CHUNK64 >> 4) << 16), wide, c > 0 || i > 0);
+        });
+        const float plus = f.p + sh.e[row], back = 1.f / f.b;
+        __nv_bfloat16* out = g.out + int64_t(blockIdx.x) * g.k * g.l;
+#pragma unroll 1
+        for (int c = half * width / 2; c < (half + 1) * width / 2; c += 32) {
+            uint32_t r[32], was[32];
+            float v[32];
+            tmem_ld_32x32(acc + c, r);
+            tmem_ld_32x32(tmem + c, was);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = fmaf(plus, __uint_as_float(was[i]), __uint_as_float(r[i]) * back);
+            if (!last) {
+                put_tmem(tmem + c, v);
+                put_row(x16, row, c, v, 1.f);
+                continue;
+            }
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] *= g.scale * (1.f / SX);
+            if (!there) continue;
+            if (!TALL && g.vec) {
+#pragma unroll
+                for (int i = 0; i < 32; i += 8)
+                    if (c + i < g.l) put(out + int64_t(row) * g.l + c + i, *reinterpret_cast<const float(*)[8]>(v + i));
+            } else {
+#pragma unroll
+                for (int i = 0; i < 32; ++i)
+                    if (c + i < g.l) out[TALL ? int64_t(c + i) * g.k + row : int64_t(row) * g.l + c + i] = __float2bfloat16(v[i]);
+            }
+        }
+        tmem_st_wait();
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 0) {
+        tc_fence_after();
+        tmem_dealloc(*reinterpret_cast<volatile uint32_t*>(&sh.tmem_base), columns);
+    }
+    if (threadIdx.x == 0 && !ok) *g.status = MIMK_E_DEVICE_WAIT;
+}
+
+// ---- host ------------------------------------------------------------------------------------------------------------------------
+using Desc = mimk_orthogonalize_desc;
+constexpr int64_t LIM = int64_t(1) << 24, SLICE = int64_t(1) << 30;
 // Every step's factors: powers of two that keep what A and B can hold below 2^15, from the largest singular value that there can be.
 int factors_of(const Desc& d, Factors (&f)[MOST_STEPS]) {
     double most = 1;
@@ -683,6 +923,35 @@ int prepare(const Desc& d, const Plan& p, int64_t first, int64_t count, cudaStre
     return launch_after(prepare_kernel<T, 1>, rows, PREPARE, 0, s, all, int(d.m), int(d.n), int(p.pitch_x), static_cast<const double*>(p.sums), d.eps, p.x[0][0], p.x[0][1]);
 }
 
+// Matrices that a CTA takes whole. Against three launches a step: 64 of [128, 128] 141 us, here ; one of [255, 120] , here .
+bool small(const Desc& d) { return (d.m < d.n ? d.m : d.n) <= SMALL_K && (d.m < d.n ? d.n : d.m) <= SMALL_L; }
+template <class T, bool TALL>
+int small_launch(const Matrices& all, const SmallArgs& g, int64_t count, const DeviceInfo& dev, cudaStream_t s) {
+    const auto kern = small_kernel<T, TALL>;
+    static bool configured[64] = {};
+    if (!configured[dev.device & 63]) {
+        MIMK_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (SMALL_L / 64 + 2) * CHUNK64 + 1024));
+        configured[dev.device & 63] = true;
+    }
+    return launch_after(kern, unsigned(count), SMALL_THREADS, size_t(g.chunks + 2) * CHUNK64 + 1024, s, all, g);
+}
+int small_all(const Desc& d, const Factors* f, const DeviceInfo& dev, cudaStream_t s) {
+    static thread_local Matrices all;
+    const bool tall = d.m > d.n;
+    SmallArgs g;
+    g.k = int(tall ? d.n : d.m), g.l = int(tall ? d.m : d.n), g.chunks = (g.l + 63) / 64, g.steps = d.steps, g.eps = d.eps, g.scale = d.scale, g.status = dev.status_dev;
+    for (int i = 0; i < d.steps; ++i) g.f[i] = f[i];
+    for (int64_t first = 0; first < d.batch; first += TABLE) {
+        const int64_t count = d.batch - first < TABLE ? d.batch - first : TABLE;
+        g.out = static_cast<__nv_bfloat16*>(d.out) + first * d.m * d.n;
+        g.vec = d.n % 8 == 0 && aligned16(g.out);
+        for (int64_t i = 0; i < count; ++i) all.x[i] = d.x[first + i], g.vec = g.vec && aligned16(d.x[first + i]);
+        if (d.dtype == MIMK_F32) MIMK_TRY((tall ? small_launch<float, true>(all, g, count, dev, s) : small_launch<float, false>(all, g, count, dev, s)));
+        else MIMK_TRY((tall ? small_launch<__nv_bfloat16, true>(all, g, count, dev, s) : small_launch<__nv_bfloat16, false>(all, g, count, dev, s)));
+    }
+    return MIMK_OK;
+}
+
 int slice(const Desc& d, const Plan& p, const Factors* f, int64_t first, int64_t count, const DeviceInfo& dev, cudaStream_t s) {
     MIMK_TRY(d.dtype == MIMK_F32 ? prepare<float>(d, p, first, count, s) : prepare<__nv_bfloat16>(d, p, first, count, s));
     const bool tall = d.m > d.n;
@@ -739,7 +1008,7 @@ extern "C" int mimk_orthogonalize_workspace(const mimk_orthogonalize_desc* d, ui
     MIMK_TRY(check(d));
     if (!bytes) return MIMK_E_ARG;
     Space space(nullptr);
-    if (!nothing(*d)) plan(*d, space);
+    if (!nothing(*d) && !small(*d)) plan(*d, space);
     *bytes = space.used();
     return MIMK_OK;
 }
@@ -759,6 +1028,7 @@ extern "C" int mimk_orthogonalize(const mimk_orthogonalize_desc* d, void* stream
         if (!d->x[i]) return MIMK_E_ARG;
         if (reinterpret_cast<uintptr_t>(d->x[i]) % size) return MIMK_E_ALIGN;
     }
+    if (small(*d)) return small_all(*d, f, *dev, static_cast<cudaStream_t>(stream));
     Space space(d->workspace);
     const Plan p = plan(*d, space);
     if (!d->workspace || space.used() > d->workspace_bytes) return MIMK_E_WORKSPACE;

@@ -234,9 +234,10 @@ def test_refusals():
             T.orthogonalize(x, **bad)
         assert e.value.status == 8
     # the C entry point: addresses, and a workspace that is missing, too small or unaligned
-    lib, need, out = _lib.lib(), C.c_uint64(), torch.empty((16, 24), dtype=BF16, device="cuda")
+    x = matrix("random", (16, 300))
+    lib, need, out = _lib.lib(), C.c_uint64(), torch.empty((16, 300), dtype=BF16, device="cuda")
     d = _lib.OrthogonalizeDesc()
-    d.batch, d.m, d.n, d.x, d.coefficients, d.eps, d.scale, d.steps, d.dtype = 1, 16, 24, (C.c_void_p * 1)(x.data_ptr()), (C.c_float * 3)(1.5, -0.5, 0.0), 1e-7, 1.0, 1, _lib.F32
+    d.batch, d.m, d.n, d.x, d.coefficients, d.eps, d.scale, d.steps, d.dtype = 1, 16, 300, (C.c_void_p * 1)(x.data_ptr()), (C.c_float * 3)(1.5, -0.5, 0.0), 1e-7, 1.0, 1, _lib.F32
     assert lib.mimk_orthogonalize_workspace(C.byref(d), C.byref(need)) == 0
     assert lib.mimk_orthogonalize(C.byref(d), None) == 1
     d.out = out.data_ptr()

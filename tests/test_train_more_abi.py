@@ -70,7 +70,8 @@ def test_orthogonalize(lib):
     # singular values that grow without limit: 6 s, and a step that takes 1 to 4.5
     for bad in ((6.0, 0.0, 0.0), (1.5, 1.5, 1.5), (float("nan"), 0.0, 0.0), (float("inf"), 0.0, 0.0)):
         assert L.mimk_orthogonalize(C.byref(desc(coefficients=(C.c_float * 3)(*bad))), None) == 8, bad
-    assert L.mimk_orthogonalize_workspace(C.byref(desc()), C.byref(need)) == 0 and need.value >= 8 * 64
+    assert L.mimk_orthogonalize_workspace(C.byref(desc(m=200, n=300)), C.byref(need)) == 0 and need.value >= 8 * 200 * 300
+    assert L.mimk_orthogonalize_workspace(C.byref(desc()), C.byref(need)) == 0      # (small matrices take none)
     assert L.mimk_orthogonalize_workspace(C.byref(desc()), None) == 1
     # a stack of any length takes a bounded buffer
     many = (C.c_void_p * 4096)(*[256] * 4096)
