@@ -114,24 +114,23 @@ __device__ __forceinline__ void st_shared(uint32_t a, uint32_t x, uint32_t y, ui
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
 
+// What a CTA has for its whole life, and what each of its threads carries from tile to tile, and from product to product.
+struct Core {
+    uint32_t tile_base, tmem_base;
+    Bars* bars;
+};
+struct Carry {
+    uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0, in_phase = 0;
+};
+struct MapsOf {
+    const CUtensorMap *left, *right, *hi, *lo, *out_hi, *out_lo;
+};
 // SMS: 2, a tile of 256 x 256 on a pair of SMs, or 1, one of 128 x 128 on one. A CTA stages 128 rows of the left operand and 128 columns of the right one.
-template <int KIND, int SMS>
-__device__ __forceinline__ void product(const Maps& maps, const Args& g) {
-    using S = Shape<KIND>;
-    constexpr int STAGES = S::STAGES, SIDE = BM * SMS, COLUMNS = SIDE;
-    extern __shared__ uint8_t smem_raw[];
+template <int SMS, int STAGES, int SLOTS>
+__device__ __forceinline__ Core set_up(uint8_t* smem_raw) {
     const uint32_t raw_addr = smem_u32(smem_raw), tile_base = (raw_addr + 1023u) & ~1023u;
-    Bars* bars = reinterpret_cast<Bars*>(smem_raw + (tile_base - raw_addr) + STAGES * STAGE + S::SLOTS * SLOT);
-    volatile int* abort_flag = &bars->abort_flag;
-
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t rank = SMS == 2 ? cluster_ctarank() : 0;
-    const int first = blockIdx.x / SMS, step = gridDim.x / SMS;
-
-    if (threadIdx.x == 32) {
-        tma_prefetch_desc(&maps.left), tma_prefetch_desc(&maps.right);
-        if (KIND == APPLY) tma_prefetch_desc(&maps.hi), tma_prefetch_desc(&maps.lo), tma_prefetch_desc(&maps.out_hi), tma_prefetch_desc(&maps.out_lo);
-    }
+    Core core{tile_base, 0, reinterpret_cast<Bars*>(smem_raw + (tile_base - raw_addr) + STAGES * STAGE + SLOTS * SLOT)};
+    Bars* bars = core.bars;
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; ++s) {
             mbar_init(smem_u32(&bars->full[s]), 1);
@@ -145,12 +144,12 @@ __device__ __forceinline__ void product(const Maps& maps, const Args& g) {
         bars->abort_flag = 0;
         fence_barrier_init();
     }
-    if (warp == 1) {
+    if (threadIdx.x >> 5 == 1) {
         if constexpr (SMS == 2) {
-            tmem_alloc_pair(smem_u32(&bars->tmem_base), 2 * COLUMNS);
+            tmem_alloc_pair(smem_u32(&bars->tmem_base), 2 * BM * SMS);
             tmem_relinquish_pair();
         } else {
-            tmem_alloc(smem_u32(&bars->tmem_base), 2 * COLUMNS);
+            tmem_alloc(smem_u32(&bars->tmem_base), 2 * BM * SMS);
             tmem_relinquish();
         }
     }
@@ -158,8 +157,34 @@ __device__ __forceinline__ void product(const Maps& maps, const Args& g) {
     __syncthreads();
     if constexpr (SMS == 2) cluster_sync();
     tc_fence_after();
-    const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(&bars->tmem_base);
-    after_previous();
+    core.tmem_base = *reinterpret_cast<volatile uint32_t*>(&bars->tmem_base);
+    return core;
+}
+template <int SMS>
+__device__ __forceinline__ void tear_down(const Core& core, int* status) {
+    tc_fence_before();
+    __syncthreads();
+    if constexpr (SMS == 2) cluster_sync();  // neither CTA may release shared or tensor memory while the other can still touch it
+    if (threadIdx.x >> 5 == 1) {
+        __syncwarp();
+        tc_fence_after();
+        if constexpr (SMS == 2) tmem_dealloc_pair(core.tmem_base, 2 * BM * SMS);
+        else tmem_dealloc(core.tmem_base, 2 * BM * SMS);
+    }
+    if (threadIdx.x == 0 && *const_cast<volatile int*>(&core.bars->abort_flag)) *status = MIMK_E_DEVICE_WAIT;
+}
+
+// This CTA's tiles of one product.
+template <int KIND, int SMS, int STAGES>
+__device__ __forceinline__ void product(const MapsOf& maps, const Args& g, const Core& core, Carry& carry) {
+    constexpr int SIDE = BM * SMS, COLUMNS = SIDE;
+    const uint32_t tile_base = core.tile_base, tmem_base = core.tmem_base;
+    Bars* bars               = core.bars;
+    volatile int* abort_flag = &bars->abort_flag;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = SMS == 2 ? cluster_ctarank() : 0;
+    const int first = blockIdx.x / SMS, step = gridDim.x / SMS;
+    uint32_t &stage = carry.stage, &phase = carry.phase, &acc = carry.acc, &acc_phase = carry.acc_phase, &in_phase = carry.in_phase;
 
     Tile t;
     if (warp == 0 || warp == 2) {
@@ -167,8 +192,7 @@ __device__ __forceinline__ void product(const Maps& maps, const Args& g) {
         if (lane == 0) {
             const bool left  = warp == 0;
             const int mn     = left ? g.a_mn : g.b_mn;
-            const auto* map  = left ? &maps.left : &maps.right;
-            uint32_t stage = 0, phase = 0;
+            const auto* map  = left ? maps.left : maps.right;
             bool ok = true;
             for (int index = first; ok && tile_at<KIND, SIDE>(g, index, t); index += step) {
                 const int at = (left ? t.m : t.n) + int(rank) * BM;
@@ -201,7 +225,6 @@ __device__ __forceinline__ void product(const Maps& maps, const Args& g) {
     } else if (warp == 1) {
         // ---------------- multiplications (of a pair: the even CTA) ----------------
         if (lane == 0 && rank == 0) {
-            uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0;
             bool ok = true;
             const uint64_t high  = smem_desc_sw128(0, 0, 1024);
             const uint32_t idesc = idesc_f16_f32(SIDE, SIDE, g.a_mn, g.b_mn);
@@ -237,7 +260,6 @@ __device__ __forceinline__ void product(const Maps& maps, const Args& g) {
         constexpr int HALF = SIDE / 2;
         const int quarter = warp & 3, half = (warp - FIRST) >> 2, side = half * HALF;
         const uint32_t slot = tile_base + STAGES * STAGE + (warp - FIRST) * 2 * SLOT, in_bar = smem_u32(&bars->in[(warp - FIRST) * 2]);
-        uint32_t acc = 0, acc_phase = 0, in_phase = 0;
         bool ok   = true;
         bool have = tile_at<KIND, SIDE>(g, first, t);
         // APPLY: 32 columns of X, in two sets of slots in turn
@@ -246,8 +268,8 @@ __device__ __forceinline__ void product(const Maps& maps, const Args& g) {
             if (KIND == APPLY && lane == 0 && row < g.rows && c < side + HALF && t.n + c < g.cols) {
                 const uint32_t set = c >> 5 & 1, to = slot + set * SLOT, bar = in_bar + set * 8;
                 mbar_expect_tx(bar, SLOT);
-                tma_load_3d(to, &maps.hi, t.n + c, row, t.z, bar);
-                tma_load_3d(to + SLOT / 2, &maps.lo, t.n + c, row, t.z, bar);
+                tma_load_3d(to, maps.hi, t.n + c, row, t.z, bar);
+                tma_load_3d(to + SLOT / 2, maps.lo, t.n + c, row, t.z, bar);
             }
         };
         if (have) request(side), request(side + 32);
@@ -263,13 +285,13 @@ __device__ __forceinline__ void product(const Maps& maps, const Args& g) {
                 if constexpr (KIND == SQUARE) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        a[i] = there && t.n + c + 8 * i < g.cols ? *reinterpret_cast<const uint4*>(g.in + (matrix + row) * g.pitch + t.n + c + 8 * i) : make_uint4(0, 0, 0, 0);
+                        a[i] = there && t.n + c + 8 * i < g.cols ? __ldcg(reinterpret_cast<const uint4*>(g.in + (matrix + row) * g.pitch + t.n + c + 8 * i)) : make_uint4(0, 0, 0, 0);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) dj[i] = t.n + c + 4 * i < g.cols ? *reinterpret_cast<const float4*>(diag + t.n + c + 4 * i) : make_float4(0.f, 0.f, 0.f, 0.f);
+                    for (int i = 0; i < 8; ++i) dj[i] = t.n + c + 4 * i < g.cols ? __ldcg(reinterpret_cast<const float4*>(diag + t.n + c + 4 * i)) : make_float4(0.f, 0.f, 0.f, 0.f);
                 }
             };
             if (row0 < g.rows && side < end) ask(side);
-            const float d = KIND == SQUARE && there ? diag[row] : 0.f;
+            const float d = KIND == SQUARE && there ? __ldcg(diag + row) : 0.f;
             if (!(ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&bars->acc_full[acc]), acc_phase, abort_flag)))) break;
             tc_fence_after();
             const uint32_t from = tmem_base + acc * COLUMNS + (uint32_t(quarter * 32) << 16);
@@ -342,7 +364,7 @@ __device__ __forceinline__ void product(const Maps& maps, const Args& g) {
                     }
                 }
             } else {
-                const float e = !g.tall && there ? diag[row] : 0.f;
+                const float e = !g.tall && there ? __ldcg(diag + row) : 0.f;
 #pragma unroll 1
                 for (int c = side; c < end; c += 32) {
                     const uint32_t set = c >> 5 & 1, at = slot + set * SLOT;
@@ -353,7 +375,7 @@ __device__ __forceinline__ void product(const Maps& maps, const Args& g) {
                     float4 ej[8];
                     if (g.tall) {
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) ej[i] = t.n + c + 4 * i < g.cols ? *reinterpret_cast<const float4*>(diag + t.n + c + 4 * i) : make_float4(0.f, 0.f, 0.f, 0.f);
+                        for (int i = 0; i < 8; ++i) ej[i] = t.n + c + 4 * i < g.cols ? __ldcg(reinterpret_cast<const float4*>(diag + t.n + c + 4 * i)) : make_float4(0.f, 0.f, 0.f, 0.f);
                     } else {
 #pragma unroll
                         for (int i = 0; i < 8; ++i) ej[i] = make_float4(e, e, e, e);
@@ -386,8 +408,8 @@ __device__ __forceinline__ void product(const Maps& maps, const Args& g) {
                     fence_proxy_async_smem();
                     __syncwarp();
                     if (lane == 0) {
-                        tma_store_3d(&maps.out_hi, at, t.n + c, row0, t.z);
-                        if (!g.last) tma_store_3d(&maps.out_lo, at + SLOT / 2, t.n + c, row0, t.z);
+                        tma_store_3d(maps.out_hi, at, t.n + c, row0, t.z);
+                        if (!g.last) tma_store_3d(maps.out_lo, at + SLOT / 2, t.n + c, row0, t.z);
                         bulk_commit();
                         if (c > side) bulk_wait_read_1();
                     }
@@ -402,54 +424,141 @@ __device__ __forceinline__ void product(const Maps& maps, const Args& g) {
         }
         if (KIND == APPLY && lane == 0) bulk_wait_all();
     }
-
-    tc_fence_before();
-    __syncthreads();
-    if constexpr (SMS == 2) cluster_sync();  // neither CTA may release shared or tensor memory while the other can still touch it
-    if (warp == 1) {
-        __syncwarp();
-        tc_fence_after();
-        if constexpr (SMS == 2) tmem_dealloc_pair(tmem_base, 2 * COLUMNS);
-        else tmem_dealloc(tmem_base, 2 * COLUMNS);
+}
+template <int KIND, int SMS>
+__device__ __forceinline__ void one_product(const Maps& maps, const Args& g) {
+    extern __shared__ uint8_t smem_raw[];
+    if (threadIdx.x == 32) {
+        tma_prefetch_desc(&maps.left), tma_prefetch_desc(&maps.right);
+        if (KIND == APPLY) tma_prefetch_desc(&maps.hi), tma_prefetch_desc(&maps.lo), tma_prefetch_desc(&maps.out_hi), tma_prefetch_desc(&maps.out_lo);
     }
-    if (threadIdx.x == 0 && *abort_flag) *g.status = MIMK_E_DEVICE_WAIT;
+    const Core core = set_up<SMS, Shape<KIND>::STAGES, Shape<KIND>::SLOTS>(smem_raw);
+    after_previous();
+    Carry carry;
+    product<KIND, SMS, Shape<KIND>::STAGES>({&maps.left, &maps.right, &maps.hi, &maps.lo, &maps.out_hi, &maps.out_lo}, g, core, carry);
+    tear_down<SMS>(core, g.status);
 }
 template <int KIND>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args g) {
-    product<KIND, 2>(maps, g);
+    one_product<KIND, 2>(maps, g);
 }
 template <int KIND>
 __global__ void __launch_bounds__(THREADS, 1) single_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args g) {
-    product<KIND, 1>(maps, g);
+    one_product<KIND, 1>(maps, g);
 }
 
-// A from partial results: 32 x 32 of its values a block, of a triangle of such tiles; its own and the other triangle's.
-__global__ void __launch_bounds__(256) sum_kernel(const __grid_constant__ Args g, int splits) {
-    __shared__ float tile[32][33];
-    after_previous();
-    Tile t;
-    if (!tile_at<SQUARE, 32>(g, blockIdx.x, t)) return;
-    const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
-    const int64_t matrix = int64_t(t.z) * g.rows, stride = int64_t(g.batch) * g.rows * g.pitch;
-    for (int i = y; i < 32; i += 8) {
-        const int row = t.m + i, column = t.n + x;
-        float v       = 0.f;
-        if (row < g.rows && column < g.cols) {
-            const float* p = g.part + (matrix + row) * g.pitch + column;
-#pragma unroll 4
-            for (int s = 0; s < splits; ++s) v += p[s * stride];
-            v *= g.f[0];
-            if (row == column) g.diag_out[int64_t(t.z) * g.diag_pitch + row] = v, v = 0.f;
-            g.out[(matrix + row) * g.pitch + column] = __float2half_rn(v * g.f[4]);
+// A from partial results: 8 rows and 32 columns of it for each warp, a column per lane; on and below the diagonal, and the other triangle's from there.
+__device__ __forceinline__ void sum_parts_of(const Args& g, int splits, int64_t first, int64_t step) {
+    const int lane = threadIdx.x & 31, across = (g.cols + 31) / 32, down = (g.rows + 7) / 8;
+    const int64_t stride = int64_t(g.batch) * g.rows * g.pitch, units = int64_t(across) * down;
+    for (int64_t u = first; u < units * g.batch; u += step) {
+        const int z = int(u / units), i = int(u - z * units), row0 = i / across * 8, column0 = i % across * 32, column = column0 + lane;
+        if (row0 + 7 < column0) continue;
+        const int64_t matrix = int64_t(z) * g.rows;
+        const float* p = g.part + (matrix + row0) * g.pitch + column;
+        float v[8] = {};
+#pragma unroll 2
+        for (int s = 0; s < splits; ++s)
+#pragma unroll
+            for (int r = 0; r < 8; ++r) v[r] += column < g.cols && row0 + r < g.rows ? __ldcg(p + s * stride + r * g.pitch) : 0.f;
+        __half h[8];
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+            v[r] *= g.f[0];
+            if (row0 + r == column && column < g.cols) g.diag_out[int64_t(z) * g.diag_pitch + column] = v[r], v[r] = 0.f;
+            h[r] = __float2half_rn(v[r] * g.f[4]);
+            if (column <= row0 + r && column < g.cols && row0 + r < g.rows) g.out[(matrix + row0 + r) * g.pitch + column] = h[r];
         }
-        tile[i][x] = v;
+        __half* other = g.out + (matrix + column) * g.pitch + row0;
+        if (column0 + 31 < row0 && row0 + 8 <= g.rows) {
+            *reinterpret_cast<uint4*>(other) = *reinterpret_cast<const uint4*>(h);
+        } else {
+#pragma unroll
+            for (int r = 0; r < 8; ++r)
+                if (column < row0 + r && column < g.cols && row0 + r < g.rows) other[r] = h[r];
+        }
+    }
+}
+__global__ void __launch_bounds__(256) sum_kernel(const __grid_constant__ Args g, int splits) {
+    after_previous();
+    sum_parts_of(g, splits, int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5), int64_t(gridDim.x) * 8);
+}
+
+// ---- all steps in one launch -----------------------------------------------------------------------------------------------------
+// Where the products are short, what lies between two launches (2 to 3 us, and 1.5 until the first operands are there) is most of a step: here the CTAs, all of them resident, meet
+// between the products instead.
+constexpr int MOST_STEPS = 64;
+struct Factors {
+    float p, q, r, a, b;  // a step's coefficients, and the factors of A and B
+};
+struct Steps {
+    CUtensorMap gram[2], apply[2], x_hi[2], x_lo[2], a, b, result;
+    Args g;           // what all products share; those of the result's extents are APPLY's
+    int k, kb_gram, kb, splits, per, steps, tall;
+    __half *matrix_a, *matrix_b;
+    float *d, *e;
+    float scale;
+    int* met;         // CTAs that have come so far, and whether one gave up
+    Factors f[MOST_STEPS];
+};
+// Everything written so far, by stores and by bulk stores that are done, is there for all CTAs' loads and bulk loads. False: a wait has run out somewhere.
+__device__ __forceinline__ bool all_meet(const Core& core, int* met, int nth) {
+    asm volatile("fence.proxy.async;" ::: "memory");
+    __threadfence();
+    __syncthreads();
+    volatile int* aborted = &core.bars->abort_flag;
+    if (threadIdx.x == 0) {
+        volatile int* given_up = met + 1;
+        if (*aborted) *given_up = 1;
+        atomicAdd(met, 1);
+        const int all      = nth * int(gridDim.x);
+        const long long t0 = clock64();
+        for (;;) {
+            int now;
+            asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(now) : "l"(met) : "memory");
+            if (now >= all) break;
+            if (*given_up || clock64() - t0 > WAIT_LIMIT_CYCLES) {
+                *given_up = 1, *aborted = 1;
+                break;
+            }
+        }
+        if (*given_up) *aborted = 1;
     }
     __syncthreads();
-    if (t.m == t.n) return;
-    for (int i = y; i < 32; i += 8) {
-        const int row = t.n + i, column = t.m + x;
-        if (row < g.rows && column < g.cols) g.out[(matrix + row) * g.pitch + column] = __float2half_rn(tile[x][i] * g.f[4]);
+    asm volatile("fence.proxy.async;" ::: "memory");
+    return !*aborted;
+}
+__global__ void __launch_bounds__(THREADS, 1) steps_kernel(const __grid_constant__ Steps k) {
+    extern __shared__ uint8_t smem_raw[];
+    constexpr int STAGES = Shape<APPLY>::STAGES;
+    const Core core = set_up<1, STAGES, Shape<APPLY>::SLOTS>(smem_raw);
+    Carry carry;
+    int nth = 0;
+#pragma unroll 1
+    for (int step = 0; step < k.steps; ++step) {
+        const Factors c = k.f[step];
+        const int now = step & 1, next = now ^ 1;
+        const bool last = step + 1 == k.steps;
+        Args g = k.g;
+        g.rows = g.cols = k.k, g.tiles_m = g.tiles_n = (k.k + BM - 1) / BM, g.kb = k.kb_gram, g.a_mn = g.b_mn = k.tall, g.out = k.matrix_a, g.diag_out = k.d;
+        g.splits = k.splits, g.per = k.per, g.f[0] = 1.f / (SX * SX), g.f[4] = c.a;
+        product<GRAM, 1, STAGES>({&k.gram[now], &k.gram[now], nullptr, nullptr, nullptr, nullptr}, g, core, carry);
+        if (!all_meet(core, k.met, ++nth)) break;
+        if (k.splits > 1) {
+            sum_parts_of(g, k.splits, int64_t(threadIdx.x >> 5) * gridDim.x + blockIdx.x, int64_t(gridDim.x) * (THREADS / 32));
+            if (!all_meet(core, k.met, ++nth)) break;
+        }
+        g.splits = 1, g.kb = k.kb, g.a_mn = g.b_mn = 0, g.in = k.matrix_a, g.out = k.matrix_b, g.diag_in = k.d, g.diag_out = k.e;
+        g.f[0] = 1.f / (c.a * c.a), g.f[1] = 1.f / c.a, g.f[2] = c.q, g.f[3] = c.r, g.f[4] = c.b;
+        product<SQUARE, 1, STAGES>({&k.a, &k.a, nullptr, nullptr, nullptr, nullptr}, g, core, carry);
+        if (!all_meet(core, k.met, ++nth)) break;
+        g.rows = k.g.rows, g.cols = k.g.cols, g.tiles_m = k.g.tiles_m, g.tiles_n = k.g.tiles_n, g.b_mn = !k.tall, g.tall = k.tall, g.last = last, g.diag_in = k.e;
+        g.f[0] = c.p, g.f[1] = 1.f / c.b, g.f[2] = k.scale / SX;
+        product<APPLY, 1, STAGES>({k.tall ? &k.apply[now] : &k.b, k.tall ? &k.b : &k.apply[now], &k.x_hi[now], &k.x_lo[now], last ? &k.result : &k.x_hi[next], last ? &k.result : &k.x_lo[next]}, g, core,
+                                  carry);
+        if (!last && !all_meet(core, k.met, ++nth)) break;
     }
+    tear_down<1>(core, k.g.status);
 }
 
 // ---- x to X ----------------------------------------------------------------------------------------------------------------------
@@ -497,8 +606,9 @@ struct Inverse {
     __device__ __forceinline__ float times(float v) const { return v * first * second; }
 };
 template <class T, int VEC>
-__global__ void __launch_bounds__(PREPARE) squares_kernel(const __grid_constant__ Matrices all, int64_t count, double* sums) {
+__global__ void __launch_bounds__(PREPARE) squares_kernel(const __grid_constant__ Matrices all, int64_t count, double* sums, int* met) {
     after_previous();
+    if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x < 2) met[threadIdx.x] = 0;
     const T* x = static_cast<const T*>(all.x[blockIdx.y]);
     for (int64_t chunk = blockIdx.x; chunk * CHUNK < count; chunk += gridDim.x) {
         const int64_t end = min(count, (chunk + 1) * CHUNK);
@@ -553,10 +663,6 @@ __global__ void __launch_bounds__(PREPARE) prepare_kernel(const __grid_constant_
 // 128-byte row, which serves as the operand of X X^T and as the right one of B X; A, then B, as f16 in another such matrix. Eight warps: 32 rows, one to a lane, and half of
 // the columns each. A step's three products take some 512 cycles each, what is between them 600 to 1500. [128, 128]: 
 constexpr int SMALL_K = 128, SMALL_L = 256, SMALL_THREADS = 256, CHUNK64 = 128 * 128;  // bytes of 128 rows of 64 columns
-constexpr int MOST_STEPS = 64;
-struct Factors {
-    float p, q, r, a, b;  // a step's coefficients, and the factors of A and B
-};
 struct SmallArgs {
     int k, l, chunks, steps;  // rows and columns of X (turned where x is taller than wide), its chunks of 64 columns
     int vec;                  // rows of x and of the result are whole 16 bytes
@@ -824,6 +930,7 @@ struct Plan {
     __half *x[2][2], *a, *b;
     float *d, *e;
     double* sums;
+    int* met;
     int splits;          // partial results of A that there is room for
     float* part;
     __nv_bfloat16* out;  // rows of pitch_x, where the result's are no whole 16 bytes
@@ -847,6 +954,7 @@ Plan plan(const Desc& d, Space& space) {
     p.d = static_cast<float*>(space.take(size_t(p.slice * p.pitch_d) * 4)), p.e = static_cast<float*>(space.take(size_t(p.slice * p.pitch_d) * 4));
     if (p.splits > 1) p.part = static_cast<float*>(space.take(size_t(p.slice) * size_t(p.splits) * size_t(part)));
     p.sums = static_cast<double*>(space.take(size_t(p.slice * p.chunks) * 8));
+    p.met = static_cast<int*>(space.take(8));
     // the same for every address of the result (a size is asked for before there is one)
     p.out = static_cast<__nv_bfloat16*>(space.take(size_t(p.slice * d.m * p.pitch_x) * 2));
     return p;
@@ -881,17 +989,17 @@ int launch_product(const Maps& maps, Args g, const DeviceInfo& dev, cudaStream_t
 // a tile's ends some 6000; adding up partial results another launch of 6000 and their bytes.
 struct How {
     int sms, splits, per, asked;
+    double time;
 };
-How how(int kind, int64_t rows, int64_t cols, int64_t batch, int64_t kb, int sm_count, int least_splits, int most_splits) {
-    How best{1, 1, int(kb), 1};
-    double least = 1e300;
-    for (int sms = 1; sms <= 2; ++sms) {
+How how(int kind, int64_t rows, int64_t cols, int64_t batch, int64_t kb, int sm_count, int least_splits, int most_splits, int most_sms = 2) {
+    How best{1, 1, int(kb), 1, 1e300};
+    for (int sms = 1; sms <= most_sms; ++sms) {
         const int64_t m = (rows + BM * sms - 1) / (BM * sms), n = (cols + BM * sms - 1) / (BM * sms), tiles = (kind == APPLY ? m * n : m * (m + 1) / 2) * batch;
         for (int64_t splits = least_splits; splits <= most_splits; splits *= 2) {
             const int64_t per = (kb + splits - 1) / splits, rounds = (tiles * splits + sm_count / sms - 1) / (sm_count / sms);
             double time = double(rounds) * double(per) * (sms == 2 ? 540 : 500) + 6000.0 * double(rounds < 2 ? rounds : 2);
             if (splits > 1) time += 6000 + double(splits) * double(rows) * double(rows) * double(batch) * 4 / 3000;
-            if (time < least) least = time, best = {sms, int((kb + per - 1) / per), int(per), int(splits)};
+            if (time < best.time) best = {sms, int((kb + per - 1) / per), int(per), int(splits), time};
         }
     }
     return best;
@@ -901,8 +1009,8 @@ int launch(const Maps& maps, Args g, const How& h, const DeviceInfo& dev, cudaSt
     g.splits = h.splits, g.per = h.per;
     MIMK_TRY((h.sms == 2 ? launch_product<KIND, 2>(maps, g, dev, s) : launch_product<KIND, 1>(maps, g, dev, s)));
     if (h.splits == 1) return MIMK_OK;
-    g.tiles_m = g.tiles_n = (g.rows + 31) / 32;
-    return launch_after(sum_kernel, unsigned(g.tiles_m * (g.tiles_m + 1) / 2 * g.batch), 256, 0, s, g, h.splits);
+    const int64_t units = int64_t((g.rows + 7) / 8) * ((g.cols + 31) / 32) * g.batch;
+    return launch_after(sum_kernel, unsigned((units + 7) / 8 < 65536 ? (units + 7) / 8 : 65536), 256, 0, s, g, h.splits);
 }
 
 template <class T>
@@ -916,10 +1024,10 @@ int prepare(const Desc& d, const Plan& p, int64_t first, int64_t count, cudaStre
     const int64_t values = d.m * d.n;
     const dim3 squares(unsigned(p.chunks < 4096 ? p.chunks : 4096), unsigned(count)), rows(unsigned(d.m < 4096 ? d.m : 4096), unsigned(count));
     if (vec) {
-        MIMK_TRY(launch_after(squares_kernel<T, 8>, squares, PREPARE, 0, s, all, values, p.sums));
+        MIMK_TRY(launch_after(squares_kernel<T, 8>, squares, PREPARE, 0, s, all, values, p.sums, p.met));
         return launch_after(prepare_kernel<T, 8>, rows, PREPARE, 0, s, all, int(d.m), int(d.n), int(p.pitch_x), static_cast<const double*>(p.sums), d.eps, p.x[0][0], p.x[0][1]);
     }
-    MIMK_TRY(launch_after(squares_kernel<T, 1>, squares, PREPARE, 0, s, all, values, p.sums));
+    MIMK_TRY(launch_after(squares_kernel<T, 1>, squares, PREPARE, 0, s, all, values, p.sums, p.met));
     return launch_after(prepare_kernel<T, 1>, rows, PREPARE, 0, s, all, int(d.m), int(d.n), int(p.pitch_x), static_cast<const double*>(p.sums), d.eps, p.x[0][0], p.x[0][1]);
 }
 
@@ -972,6 +1080,32 @@ int slice(const Desc& d, const Plan& p, const Factors* f, int64_t first, int64_t
     // (sums are split as for one matrix alone, so that it comes out the same in any batch)
     const int splits  = how(GRAM, p.k, p.k, 1, kb_gram, dev.sm_count, 1, p.splits).asked;
     const How hows[3] = {how(GRAM, p.k, p.k, count, kb_gram, dev.sm_count, splits, splits), how(SQUARE, p.k, p.k, count, kb, dev.sm_count, 1, 1), how(APPLY, d.m, d.n, count, kb, dev.sm_count, 1, 1)};
+    // In one launch, tiles of 128 x 128, where that ends first: a meeting takes 3000 cycles, the end of a launch and the beginning of the next 9000.
+    const How ones[3] = {how(GRAM, p.k, p.k, count, kb_gram, dev.sm_count, splits, splits, 1), how(SQUARE, p.k, p.k, count, kb, dev.sm_count, 1, 1, 1), how(APPLY, d.m, d.n, count, kb, dev.sm_count, 1, 1, 1)};
+    if (ones[0].time + ones[1].time + ones[2].time + 3 * 3000 < hows[0].time + hows[1].time + hows[2].time + 3 * 9000) {
+        Steps k{};
+        for (int i = 0; i < 2; ++i) k.gram[i] = gram[i], k.apply[i] = apply[i], k.x_hi[i] = x_hi[i], k.x_lo[i] = x_lo[i];
+        k.a = a_map, k.b = b_map, k.result = result;
+        k.g.batch = int(count), k.g.pitch = int(p.pitch_a), k.g.diag_pitch = int(p.pitch_d), k.g.status = dev.status_dev, k.g.part = p.part, k.g.splits = 1;
+        k.g.rows = int(d.m), k.g.cols = int(d.n), k.g.tiles_m = int((d.m + BM - 1) / BM), k.g.tiles_n = int((d.n + BM - 1) / BM);
+        k.k = int(p.k), k.kb_gram = int(kb_gram), k.kb = int(kb), k.splits = ones[0].splits, k.per = ones[0].per, k.steps = d.steps, k.tall = tall;
+        k.matrix_a = p.a, k.matrix_b = p.b, k.d = p.d, k.e = p.e, k.scale = d.scale, k.met = p.met;
+        for (int i = 0; i < d.steps; ++i) k.f[i] = f[i];
+        static bool configured[64] = {};
+        if (!configured[dev.device & 63]) {
+            MIMK_CUDA_TRY(cudaFuncSetAttribute(steps_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<APPLY>::SMEM));
+            configured[dev.device & 63] = true;
+        }
+        // no more CTAs than the product with the most tiles has
+        const int64_t square = (p.k + BM - 1) / BM, most = square * (square + 1) / 2 * k.splits > int64_t(k.g.tiles_m) * k.g.tiles_n ? square * (square + 1) / 2 * k.splits : int64_t(k.g.tiles_m) * k.g.tiles_n;
+        cudaLaunchAttribute together = {};
+        together.id = cudaLaunchAttributeCooperative, together.val.cooperative = 1;
+        cudaLaunchConfig_t config = {};
+        config.gridDim = dim3(unsigned(most * count < dev.sm_count ? most * count : dev.sm_count)), config.blockDim = dim3(THREADS), config.dynamicSmemBytes = Shape<APPLY>::SMEM;
+        config.stream = s, config.attrs = &together, config.numAttrs = 1;
+        MIMK_TRY(note_cuda_error(cudaLaunchKernelEx(&config, steps_kernel, k)));
+        return staged ? copy_rows(p.out, p.pitch_x, out, d.n, count * d.m, d.n, s) : MIMK_OK;
+    }
     Maps maps;
     for (int step = 0; step < d.steps; ++step) {
         const Factors& c = f[step];
