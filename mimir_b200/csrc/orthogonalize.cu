@@ -43,7 +43,7 @@ struct Shape {
 };
 
 struct Maps {
-    CUtensorMap left, right, hi, lo, out_hi, out_lo;  // the last four: tiles of 32 rows of X, APPLY
+    CUtensorMap left, right, tile, out;  // the last two: tiles of 32 rows and columns of X, and of the result, APPLY
 };
 struct Args {
     int rows, cols, batch;  // of the result
@@ -52,6 +52,7 @@ struct Args {
     int a_mn, b_mn;  // operand stored with its M (N) axis contiguous
     int pitch, diag_pitch;  // of A and B; of the diagonals
     int last, tall;  // APPLY: the result is BF16; e goes with columns
+    int z_left, z_right, z_hi, z_lo, z_out_hi, z_out_lo;  // where the batch's matrices begin in the buffers that the maps are of
     const __half* in;  // SQUARE: A
     __half* out;       // GRAM: A, SQUARE: B
     float* part;       // [splits][batch][rows][pitch], tiles on and below the diagonal
@@ -114,16 +115,9 @@ __device__ __forceinline__ void st_shared(uint32_t a, uint32_t x, uint32_t y, ui
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
 
-// What a CTA has for its whole life, and what each of its threads carries from tile to tile, and from product to product.
 struct Core {
     uint32_t tile_base, tmem_base;
     Bars* bars;
-};
-struct Carry {
-    uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0, in_phase = 0;
-};
-struct MapsOf {
-    const CUtensorMap *left, *right, *hi, *lo, *out_hi, *out_lo;
 };
 // SMS: 2, a tile of 256 x 256 on a pair of SMs, or 1, one of 128 x 128 on one. A CTA stages 128 rows of the left operand and 128 columns of the right one.
 template <int SMS, int STAGES, int SLOTS>
@@ -176,7 +170,7 @@ __device__ __forceinline__ void tear_down(const Core& core, int* status) {
 
 // This CTA's tiles of one product.
 template <int KIND, int SMS, int STAGES>
-__device__ __forceinline__ void product(const MapsOf& maps, const Args& g, const Core& core, Carry& carry) {
+__device__ __forceinline__ void product(const Maps& maps, const Args& g, const Core& core) {
     constexpr int SIDE = BM * SMS, COLUMNS = SIDE;
     const uint32_t tile_base = core.tile_base, tmem_base = core.tmem_base;
     Bars* bars               = core.bars;
@@ -184,7 +178,7 @@ __device__ __forceinline__ void product(const MapsOf& maps, const Args& g, const
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = SMS == 2 ? cluster_ctarank() : 0;
     const int first = blockIdx.x / SMS, step = gridDim.x / SMS;
-    uint32_t &stage = carry.stage, &phase = carry.phase, &acc = carry.acc, &acc_phase = carry.acc_phase, &in_phase = carry.in_phase;
+    uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0, in_phase = 0;
 
     Tile t;
     if (warp == 0 || warp == 2) {
@@ -192,7 +186,8 @@ __device__ __forceinline__ void product(const MapsOf& maps, const Args& g, const
         if (lane == 0) {
             const bool left  = warp == 0;
             const int mn     = left ? g.a_mn : g.b_mn;
-            const auto* map  = left ? maps.left : maps.right;
+            const auto* map  = left ? &maps.left : &maps.right;
+            const int z0     = left ? g.z_left : g.z_right;
             bool ok = true;
             for (int index = first; ok && tile_at<KIND, SIDE>(g, index, t); index += step) {
                 const int at = (left ? t.m : t.n) + int(rank) * BM;
@@ -205,17 +200,17 @@ __device__ __forceinline__ void product(const MapsOf& maps, const Args& g, const
                     if constexpr (SMS == 2) {
                         const uint32_t full_even = map_to_cta(full, 0);
                         if (!mn) {
-                            tma_load_3d_pair(to, map, k, at, t.z, full_even);
+                            tma_load_3d_pair(to, map, k, at, z0 + t.z, full_even);
                         } else {
-                            tma_load_3d_pair(to, map, at, k, t.z, full_even);
-                            tma_load_3d_pair(to + BK * 128, map, at + 64, k, t.z, full_even);
+                            tma_load_3d_pair(to, map, at, k, z0 + t.z, full_even);
+                            tma_load_3d_pair(to + BK * 128, map, at + 64, k, z0 + t.z, full_even);
                         }
                     } else {
                         if (!mn) {
-                            tma_load_3d(to, map, k, at, t.z, full);
+                            tma_load_3d(to, map, k, at, z0 + t.z, full);
                         } else {
-                            tma_load_3d(to, map, at, k, t.z, full);
-                            tma_load_3d(to + BK * 128, map, at + 64, k, t.z, full);
+                            tma_load_3d(to, map, at, k, z0 + t.z, full);
+                            tma_load_3d(to + BK * 128, map, at + 64, k, z0 + t.z, full);
                         }
                     }
                     if (++stage == STAGES) stage = 0, phase ^= 1u;
@@ -268,8 +263,8 @@ __device__ __forceinline__ void product(const MapsOf& maps, const Args& g, const
             if (KIND == APPLY && lane == 0 && row < g.rows && c < side + HALF && t.n + c < g.cols) {
                 const uint32_t set = c >> 5 & 1, to = slot + set * SLOT, bar = in_bar + set * 8;
                 mbar_expect_tx(bar, SLOT);
-                tma_load_3d(to, maps.hi, t.n + c, row, t.z, bar);
-                tma_load_3d(to + SLOT / 2, maps.lo, t.n + c, row, t.z, bar);
+                tma_load_3d(to, &maps.tile, t.n + c, row, g.z_hi + t.z, bar);
+                tma_load_3d(to + SLOT / 2, &maps.tile, t.n + c, row, g.z_lo + t.z, bar);
             }
         };
         if (have) request(side), request(side + 32);
@@ -408,8 +403,8 @@ __device__ __forceinline__ void product(const MapsOf& maps, const Args& g, const
                     fence_proxy_async_smem();
                     __syncwarp();
                     if (lane == 0) {
-                        tma_store_3d(maps.out_hi, at, t.n + c, row0, t.z);
-                        if (!g.last) tma_store_3d(maps.out_lo, at + SLOT / 2, t.n + c, row0, t.z);
+                        tma_store_3d(&maps.out, at, t.n + c, row0, g.z_out_hi + t.z);
+                        if (!g.last) tma_store_3d(&maps.out, at + SLOT / 2, t.n + c, row0, g.z_out_lo + t.z);
                         bulk_commit();
                         if (c > side) bulk_wait_read_1();
                     }
@@ -430,12 +425,11 @@ __device__ __forceinline__ void one_product(const Maps& maps, const Args& g) {
     extern __shared__ uint8_t smem_raw[];
     if (threadIdx.x == 32) {
         tma_prefetch_desc(&maps.left), tma_prefetch_desc(&maps.right);
-        if (KIND == APPLY) tma_prefetch_desc(&maps.hi), tma_prefetch_desc(&maps.lo), tma_prefetch_desc(&maps.out_hi), tma_prefetch_desc(&maps.out_lo);
+        if (KIND == APPLY) tma_prefetch_desc(&maps.tile), tma_prefetch_desc(&maps.out);
     }
     const Core core = set_up<SMS, Shape<KIND>::STAGES, Shape<KIND>::SLOTS>(smem_raw);
     after_previous();
-    Carry carry;
-    product<KIND, SMS, Shape<KIND>::STAGES>({&maps.left, &maps.right, &maps.hi, &maps.lo, &maps.out_hi, &maps.out_lo}, g, core, carry);
+    product<KIND, SMS, Shape<KIND>::STAGES>(maps, g, core);
     tear_down<SMS>(core, g.status);
 }
 template <int KIND>
@@ -484,83 +478,6 @@ __global__ void __launch_bounds__(256) sum_kernel(const __grid_constant__ Args g
     sum_parts_of(g, splits, int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5), int64_t(gridDim.x) * 8);
 }
 
-// ---- all steps in one launch -----------------------------------------------------------------------------------------------------
-// Where the products are short, what lies between two launches (2 to 3 us, and 1.5 until the first operands are there) is most of a step: here the CTAs, all of them resident, meet
-// between the products instead.
-constexpr int MOST_STEPS = 64;
-struct Factors {
-    float p, q, r, a, b;  // a step's coefficients, and the factors of A and B
-};
-struct Steps {
-    CUtensorMap gram[2], apply[2], x_hi[2], x_lo[2], a, b, result;
-    Args g;           // what all products share; those of the result's extents are APPLY's
-    int k, kb_gram, kb, splits, per, steps, tall;
-    __half *matrix_a, *matrix_b;
-    float *d, *e;
-    float scale;
-    int* met;         // CTAs that have come so far, and whether one gave up
-    Factors f[MOST_STEPS];
-};
-// Everything written so far, by stores and by bulk stores that are done, is there for all CTAs' loads and bulk loads. False: a wait has run out somewhere.
-__device__ __forceinline__ bool all_meet(const Core& core, int* met, int nth) {
-    asm volatile("fence.proxy.async;" ::: "memory");
-    __threadfence();
-    __syncthreads();
-    volatile int* aborted = &core.bars->abort_flag;
-    if (threadIdx.x == 0) {
-        volatile int* given_up = met + 1;
-        if (*aborted) *given_up = 1;
-        atomicAdd(met, 1);
-        const int all      = nth * int(gridDim.x);
-        const long long t0 = clock64();
-        for (;;) {
-            int now;
-            asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(now) : "l"(met) : "memory");
-            if (now >= all) break;
-            if (*given_up || clock64() - t0 > WAIT_LIMIT_CYCLES) {
-                *given_up = 1, *aborted = 1;
-                break;
-            }
-        }
-        if (*given_up) *aborted = 1;
-    }
-    __syncthreads();
-    asm volatile("fence.proxy.async;" ::: "memory");
-    return !*aborted;
-}
-__global__ void __launch_bounds__(THREADS, 1) steps_kernel(const __grid_constant__ Steps k) {
-    extern __shared__ uint8_t smem_raw[];
-    constexpr int STAGES = Shape<APPLY>::STAGES;
-    const Core core = set_up<1, STAGES, Shape<APPLY>::SLOTS>(smem_raw);
-    Carry carry;
-    int nth = 0;
-#pragma unroll 1
-    for (int step = 0; step < k.steps; ++step) {
-        const Factors c = k.f[step];
-        const int now = step & 1, next = now ^ 1;
-        const bool last = step + 1 == k.steps;
-        Args g = k.g;
-        g.rows = g.cols = k.k, g.tiles_m = g.tiles_n = (k.k + BM - 1) / BM, g.kb = k.kb_gram, g.a_mn = g.b_mn = k.tall, g.out = k.matrix_a, g.diag_out = k.d;
-        g.splits = k.splits, g.per = k.per, g.f[0] = 1.f / (SX * SX), g.f[4] = c.a;
-        product<GRAM, 1, STAGES>({&k.gram[now], &k.gram[now], nullptr, nullptr, nullptr, nullptr}, g, core, carry);
-        if (!all_meet(core, k.met, ++nth)) break;
-        if (k.splits > 1) {
-            sum_parts_of(g, k.splits, int64_t(threadIdx.x >> 5) * gridDim.x + blockIdx.x, int64_t(gridDim.x) * (THREADS / 32));
-            if (!all_meet(core, k.met, ++nth)) break;
-        }
-        g.splits = 1, g.kb = k.kb, g.a_mn = g.b_mn = 0, g.in = k.matrix_a, g.out = k.matrix_b, g.diag_in = k.d, g.diag_out = k.e;
-        g.f[0] = 1.f / (c.a * c.a), g.f[1] = 1.f / c.a, g.f[2] = c.q, g.f[3] = c.r, g.f[4] = c.b;
-        product<SQUARE, 1, STAGES>({&k.a, &k.a, nullptr, nullptr, nullptr, nullptr}, g, core, carry);
-        if (!all_meet(core, k.met, ++nth)) break;
-        g.rows = k.g.rows, g.cols = k.g.cols, g.tiles_m = k.g.tiles_m, g.tiles_n = k.g.tiles_n, g.b_mn = !k.tall, g.tall = k.tall, g.last = last, g.diag_in = k.e;
-        g.f[0] = c.p, g.f[1] = 1.f / c.b, g.f[2] = k.scale / SX;
-        product<APPLY, 1, STAGES>({k.tall ? &k.apply[now] : &k.b, k.tall ? &k.b : &k.apply[now], &k.x_hi[now], &k.x_lo[now], last ? &k.result : &k.x_hi[next], last ? &k.result : &k.x_lo[next]}, g, core,
-                                  carry);
-        if (!last && !all_meet(core, k.met, ++nth)) break;
-    }
-    tear_down<1>(core, k.g.status);
-}
-
 // ---- x to X ----------------------------------------------------------------------------------------------------------------------
 constexpr int TABLE = 1024;       // matrices of one launch
 constexpr int CHUNK = 1 << 16;    // values that one block squares
@@ -606,9 +523,8 @@ struct Inverse {
     __device__ __forceinline__ float times(float v) const { return v * first * second; }
 };
 template <class T, int VEC>
-__global__ void __launch_bounds__(PREPARE) squares_kernel(const __grid_constant__ Matrices all, int64_t count, double* sums, int* met) {
+__global__ void __launch_bounds__(PREPARE) squares_kernel(const __grid_constant__ Matrices all, int64_t count, double* sums) {
     after_previous();
-    if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x < 2) met[threadIdx.x] = 0;
     const T* x = static_cast<const T*>(all.x[blockIdx.y]);
     for (int64_t chunk = blockIdx.x; chunk * CHUNK < count; chunk += gridDim.x) {
         const int64_t end = min(count, (chunk + 1) * CHUNK);
@@ -663,6 +579,10 @@ __global__ void __launch_bounds__(PREPARE) prepare_kernel(const __grid_constant_
 // 128-byte row, which serves as the operand of X X^T and as the right one of B X; A, then B, as f16 in another such matrix. Eight warps: 32 rows, one to a lane, and half of
 // the columns each. A step's three products take some 512 cycles each, what is between them 600 to 1500. [128, 128]: 
 constexpr int SMALL_K = 128, SMALL_L = 256, SMALL_THREADS = 256, CHUNK64 = 128 * 128;  // bytes of 128 rows of 64 columns
+constexpr int MOST_STEPS = 64;
+struct Factors {
+    float p, q, r, a, b;  // a step's coefficients, and the factors of A and B
+};
 struct SmallArgs {
     int k, l, chunks, steps;  // rows and columns of X (turned where x is taller than wide), its chunks of 64 columns
     int vec;                  // rows of x and of the result are whole 16 bytes
@@ -930,7 +850,6 @@ struct Plan {
     __half *x[2][2], *a, *b;
     float *d, *e;
     double* sums;
-    int* met;
     int splits;          // partial results of A that there is room for
     float* part;
     __nv_bfloat16* out;  // rows of pitch_x, where the result's are no whole 16 bytes
@@ -948,13 +867,13 @@ Plan plan(const Desc& d, Space& space) {
     if (p.slice > d.batch) p.slice = d.batch;
     if (p.slice > TABLE) p.slice = TABLE;
     if (p.slice < 1) p.slice = 1;
-    for (auto& x : p.x)
-        for (__half*& piece : x) piece = static_cast<__half*>(space.take(size_t(p.slice * d.m * p.pitch_x) * 2));
-    p.a = static_cast<__half*>(space.take(size_t(p.slice * p.k * p.pitch_a) * 2)), p.b = static_cast<__half*>(space.take(size_t(p.slice * p.k * p.pitch_a) * 2));
+    // one after another: the four of X, A and B
+    __half* x = static_cast<__half*>(space.take(size_t(4 * p.slice * d.m * p.pitch_x) * 2));
+    for (int i = 0; i < 4; ++i) p.x[i >> 1][i & 1] = x ? x + i * p.slice * d.m * p.pitch_x : nullptr;
+    p.a = static_cast<__half*>(space.take(size_t(2 * p.slice * p.k * p.pitch_a) * 2)), p.b = p.a ? p.a + p.slice * p.k * p.pitch_a : nullptr;
     p.d = static_cast<float*>(space.take(size_t(p.slice * p.pitch_d) * 4)), p.e = static_cast<float*>(space.take(size_t(p.slice * p.pitch_d) * 4));
     if (p.splits > 1) p.part = static_cast<float*>(space.take(size_t(p.slice) * size_t(p.splits) * size_t(part)));
     p.sums = static_cast<double*>(space.take(size_t(p.slice * p.chunks) * 8));
-    p.met = static_cast<int*>(space.take(8));
     // the same for every address of the result (a size is asked for before there is one)
     p.out = static_cast<__nv_bfloat16*>(space.take(size_t(p.slice * d.m * p.pitch_x) * 2));
     return p;
@@ -986,19 +905,19 @@ int launch_product(const Maps& maps, Args g, const DeviceInfo& dev, cudaStream_t
 }
 // How a product runs: a tile on pairs of SMs or on single ones, and over how many tiles the k-blocks of one are dealt out; whichever ends first, in cycles. A
 // k-block takes 540 cycles on either, the single ones' 128 x 128 as the 64 bytes a cycle that an SM gets from the L2 cache carry its operands no faster (measured 500, pairs 542);
-// a tile's ends some 6000; adding up partial results another launch of 6000 and their bytes.
+// a tile's ends some 6000; adding up partial results another launch of 12000 and their bytes.
 struct How {
     int sms, splits, per, asked;
     double time;
 };
-How how(int kind, int64_t rows, int64_t cols, int64_t batch, int64_t kb, int sm_count, int least_splits, int most_splits, int most_sms = 2) {
+How how(int kind, int64_t rows, int64_t cols, int64_t batch, int64_t kb, int sm_count, int least_splits, int most_splits) {
     How best{1, 1, int(kb), 1, 1e300};
-    for (int sms = 1; sms <= most_sms; ++sms) {
+    for (int sms = 1; sms <= 2; ++sms) {
         const int64_t m = (rows + BM * sms - 1) / (BM * sms), n = (cols + BM * sms - 1) / (BM * sms), tiles = (kind == APPLY ? m * n : m * (m + 1) / 2) * batch;
         for (int64_t splits = least_splits; splits <= most_splits; splits *= 2) {
             const int64_t per = (kb + splits - 1) / splits, rounds = (tiles * splits + sm_count / sms - 1) / (sm_count / sms);
             double time = double(rounds) * double(per) * (sms == 2 ? 540 : 500) + 6000.0 * double(rounds < 2 ? rounds : 2);
-            if (splits > 1) time += 6000 + double(splits) * double(rows) * double(rows) * double(batch) * 4 / 3000;
+            if (splits > 1) time += 12000 + double(splits) * double(rows) * double(rows) * double(batch) * 4 / 3000;
             if (time < best.time) best = {sms, int((kb + per - 1) / per), int(per), int(splits), time};
         }
     }
@@ -1024,10 +943,10 @@ int prepare(const Desc& d, const Plan& p, int64_t first, int64_t count, cudaStre
     const int64_t values = d.m * d.n;
     const dim3 squares(unsigned(p.chunks < 4096 ? p.chunks : 4096), unsigned(count)), rows(unsigned(d.m < 4096 ? d.m : 4096), unsigned(count));
     if (vec) {
-        MIMK_TRY(launch_after(squares_kernel<T, 8>, squares, PREPARE, 0, s, all, values, p.sums, p.met));
+        MIMK_TRY(launch_after(squares_kernel<T, 8>, squares, PREPARE, 0, s, all, values, p.sums));
         return launch_after(prepare_kernel<T, 8>, rows, PREPARE, 0, s, all, int(d.m), int(d.n), int(p.pitch_x), static_cast<const double*>(p.sums), d.eps, p.x[0][0], p.x[0][1]);
     }
-    MIMK_TRY(launch_after(squares_kernel<T, 1>, squares, PREPARE, 0, s, all, values, p.sums, p.met));
+    MIMK_TRY(launch_after(squares_kernel<T, 1>, squares, PREPARE, 0, s, all, values, p.sums));
     return launch_after(prepare_kernel<T, 1>, rows, PREPARE, 0, s, all, int(d.m), int(d.n), int(p.pitch_x), static_cast<const double*>(p.sums), d.eps, p.x[0][0], p.x[0][1]);
 }
 
@@ -1065,47 +984,19 @@ int slice(const Desc& d, const Plan& p, const Factors* f, int64_t first, int64_t
     const bool tall = d.m > d.n;
     __nv_bfloat16* out = static_cast<__nv_bfloat16*>(d.out) + first * d.m * d.n;
     const bool staged  = !group::tma_can_read(out, d.n);
-    // every map once: X as an operand of each product and as tiles of 32 rows and columns, A, B, and the result's tiles
-    CUtensorMap gram[2], apply[2], x_hi[2], x_lo[2], a_map, b_map, result;
-    for (int i = 0; i < 2; ++i) {
-        MIMK_TRY(map_of(&gram[i], p.x[i][0], d.m, d.n, p.pitch_x, count, tall ? 64 : BM));
-        MIMK_TRY(map_of(&apply[i], p.x[i][0], d.m, d.n, p.pitch_x, count, tall ? BM : 64));
-        MIMK_TRY(tile_map(&x_hi[i], p.x[i][0], d.m, d.n, p.pitch_x, count));
-        MIMK_TRY(tile_map(&x_lo[i], p.x[i][1], d.m, d.n, p.pitch_x, count));
-    }
-    MIMK_TRY(map_of(&a_map, p.a, p.k, p.k, p.pitch_a, count, BM));
-    MIMK_TRY(map_of(&b_map, p.b, p.k, p.k, p.pitch_a, count, BM));
+    // Every map once, over all of a kind of buffers: the four of X (a first and a second f16, of one step and of the next) as an operand of each product and as tiles, A and B,
+    // and the result's tiles. (Two microseconds of host time each.)
+    CUtensorMap gram, apply, tiles, a_b, result;
+    MIMK_TRY(map_of(&gram, p.x[0][0], d.m, d.n, p.pitch_x, 4 * p.slice, tall ? 64 : BM));
+    MIMK_TRY(map_of(&apply, p.x[0][0], d.m, d.n, p.pitch_x, 4 * p.slice, tall ? BM : 64));
+    MIMK_TRY(tile_map(&tiles, p.x[0][0], d.m, d.n, p.pitch_x, 4 * p.slice));
+    MIMK_TRY(map_of(&a_b, p.a, p.k, p.k, p.pitch_a, 2 * p.slice, BM));
     MIMK_TRY(staged ? tile_map(&result, p.out, d.m, d.n, p.pitch_x, count) : tile_map(&result, out, d.m, d.n, d.n, count));
+    const int z = int(p.slice);
     const int64_t kb_gram = ((tall ? d.m : d.n) + BK - 1) / BK, kb = (p.k + BK - 1) / BK;
     // (sums are split as for one matrix alone, so that it comes out the same in any batch)
     const int splits  = how(GRAM, p.k, p.k, 1, kb_gram, dev.sm_count, 1, p.splits).asked;
     const How hows[3] = {how(GRAM, p.k, p.k, count, kb_gram, dev.sm_count, splits, splits), how(SQUARE, p.k, p.k, count, kb, dev.sm_count, 1, 1), how(APPLY, d.m, d.n, count, kb, dev.sm_count, 1, 1)};
-    // In one launch, tiles of 128 x 128, where that ends first: a meeting takes 3000 cycles, the end of a launch and the beginning of the next 9000.
-    const How ones[3] = {how(GRAM, p.k, p.k, count, kb_gram, dev.sm_count, splits, splits, 1), how(SQUARE, p.k, p.k, count, kb, dev.sm_count, 1, 1, 1), how(APPLY, d.m, d.n, count, kb, dev.sm_count, 1, 1, 1)};
-    if (ones[0].time + ones[1].time + ones[2].time + 3 * 3000 < hows[0].time + hows[1].time + hows[2].time + 3 * 9000) {
-        Steps k{};
-        for (int i = 0; i < 2; ++i) k.gram[i] = gram[i], k.apply[i] = apply[i], k.x_hi[i] = x_hi[i], k.x_lo[i] = x_lo[i];
-        k.a = a_map, k.b = b_map, k.result = result;
-        k.g.batch = int(count), k.g.pitch = int(p.pitch_a), k.g.diag_pitch = int(p.pitch_d), k.g.status = dev.status_dev, k.g.part = p.part, k.g.splits = 1;
-        k.g.rows = int(d.m), k.g.cols = int(d.n), k.g.tiles_m = int((d.m + BM - 1) / BM), k.g.tiles_n = int((d.n + BM - 1) / BM);
-        k.k = int(p.k), k.kb_gram = int(kb_gram), k.kb = int(kb), k.splits = ones[0].splits, k.per = ones[0].per, k.steps = d.steps, k.tall = tall;
-        k.matrix_a = p.a, k.matrix_b = p.b, k.d = p.d, k.e = p.e, k.scale = d.scale, k.met = p.met;
-        for (int i = 0; i < d.steps; ++i) k.f[i] = f[i];
-        static bool configured[64] = {};
-        if (!configured[dev.device & 63]) {
-            MIMK_CUDA_TRY(cudaFuncSetAttribute(steps_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<APPLY>::SMEM));
-            configured[dev.device & 63] = true;
-        }
-        // no more CTAs than the product with the most tiles has
-        const int64_t square = (p.k + BM - 1) / BM, most = square * (square + 1) / 2 * k.splits > int64_t(k.g.tiles_m) * k.g.tiles_n ? square * (square + 1) / 2 * k.splits : int64_t(k.g.tiles_m) * k.g.tiles_n;
-        cudaLaunchAttribute together = {};
-        together.id = cudaLaunchAttributeCooperative, together.val.cooperative = 1;
-        cudaLaunchConfig_t config = {};
-        config.gridDim = dim3(unsigned(most * count < dev.sm_count ? most * count : dev.sm_count)), config.blockDim = dim3(THREADS), config.dynamicSmemBytes = Shape<APPLY>::SMEM;
-        config.stream = s, config.attrs = &together, config.numAttrs = 1;
-        MIMK_TRY(note_cuda_error(cudaLaunchKernelEx(&config, steps_kernel, k)));
-        return staged ? copy_rows(p.out, p.pitch_x, out, d.n, count * d.m, d.n, s) : MIMK_OK;
-    }
     Maps maps;
     for (int step = 0; step < d.steps; ++step) {
         const Factors& c = f[step];
@@ -1115,19 +1006,20 @@ int slice(const Desc& d, const Plan& p, const Factors* f, int64_t first, int64_t
         // A
         g.rows = g.cols = int(p.k), g.kb = int(kb_gram), g.a_mn = g.b_mn = tall, g.out = p.a, g.diag_out = p.d, g.part = p.part;
         g.f[0] = 1.f / (SX * SX), g.f[4] = c.a;
-        maps.left = maps.right = gram[now];
+        maps.left = maps.right = gram, g.z_left = g.z_right = 2 * now * z;
         MIMK_TRY(launch<GRAM>(maps, g, hows[0], dev, s));
         // B
         g.kb = int(kb), g.a_mn = g.b_mn = 0, g.in = p.a, g.out = p.b, g.diag_in = p.d, g.diag_out = p.e;
         g.f[0] = 1.f / (c.a * c.a), g.f[1] = 1.f / c.a, g.f[2] = c.q, g.f[3] = c.r, g.f[4] = c.b;
-        maps.left = maps.right = a_map;
+        maps.left = maps.right = a_b, g.z_left = g.z_right = 0;
         MIMK_TRY(launch<SQUARE>(maps, g, hows[1], dev, s));
         // X
         g.rows = int(d.m), g.cols = int(d.n), g.b_mn = !tall, g.tall = tall, g.last = step + 1 == d.steps, g.diag_in = p.e;
         g.f[0] = c.p, g.f[1] = 1.f / c.b, g.f[2] = d.scale / SX;
-        maps.left = tall ? apply[now] : b_map, maps.right = tall ? b_map : apply[now];
-        maps.hi = x_hi[now], maps.lo = x_lo[now];
-        maps.out_hi = g.last ? result : x_hi[next], maps.out_lo = g.last ? result : x_lo[next];
+        (tall ? maps.left : maps.right) = apply, (tall ? g.z_left : g.z_right) = 2 * now * z;
+        (tall ? maps.right : maps.left) = a_b, (tall ? g.z_right : g.z_left) = z;
+        maps.tile = tiles, g.z_hi = 2 * now * z, g.z_lo = g.z_hi + z;
+        maps.out = g.last ? result : tiles, g.z_out_hi = g.last ? 0 : 2 * next * z, g.z_out_lo = g.z_out_hi + z;
         MIMK_TRY(launch<APPLY>(maps, g, hows[2], dev, s));
     }
     return staged ? copy_rows(p.out, p.pitch_x, out, d.n, count * d.m, d.n, s) : MIMK_OK;
