@@ -595,7 +595,8 @@ struct SmallShared {
     uint64_t done;
     uint32_t tmem_base;
     int abort_flag;
-    float d[SMALL_K], e[SMALL_K];
+    alignas(16) float d[SMALL_K];
+    float e[SMALL_K];
     double part[SMALL_THREADS / 32];
 };
 // 16-byte piece of row `row` of a 128-byte-swizzled matrix of 64-column chunks
@@ -710,6 +711,7 @@ __global__ void __launch_bounds__(SMALL_THREADS) small_kernel(const __grid_const
     for (int step = 0; step < g.steps; ++step) {
         const Factors f = g.f[step];
         const bool last = step + 1 == g.steps;
+        uint32_t both[2][32];
         // A
         multiply([&] {
             for (int c = 0; c < g.chunks; ++c)
@@ -718,12 +720,14 @@ __global__ void __launch_bounds__(SMALL_THREADS) small_kernel(const __grid_const
                     mma_f16_ss(mma_acc, d, d, square, c > 0 || i > 0);
                 }
         });
-#pragma unroll 1
-        for (int c = half * 64; c < half * 64 + 64; c += 32) {
-            uint32_t r[32];
+        tmem_ld_32x32(acc + half * 64, both[0]);
+        tmem_ld_32x32(acc + half * 64 + 32, both[1]);
+        tmem_ld_wait();
+#pragma unroll
+        for (int part = 0; part < 2; ++part) {
+            const int c = half * 64 + part * 32;
+            uint32_t(&r)[32] = both[part];
             float v[32];
-            tmem_ld_32x32(acc + c, r);
-            tmem_ld_wait();
 #pragma unroll
             for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]) * (1.f / (SX * SX));
             if (c == (warp & 3) * 32) {  // the diagonal: lane i has it in column i
@@ -742,21 +746,23 @@ __global__ void __launch_bounds__(SMALL_THREADS) small_kernel(const __grid_const
                 }
         });
         const float di = sh.d[row], less = 1.f / f.a;
-#pragma unroll 1
-        for (int c = half * 64; c < half * 64 + 64; c += 32) {
-            uint32_t r[32];
+        tmem_ld_32x32(acc + half * 64, both[0]);
+        tmem_ld_32x32(acc + half * 64 + 32, both[1]);
+        tmem_ld_wait();
+#pragma unroll
+        for (int part = 0; part < 2; ++part) {
+            const int c = half * 64 + part * 32;
+            uint32_t(&r)[32] = both[part];
             float v[32];
-            tmem_ld_32x32(acc + c, r);
-            tmem_ld_wait();
 #pragma unroll
             for (int i = 0; i < 32; i += 8) {
                 const uint4 w = ld_shared(at64(a16, row, c + i));
 #pragma unroll
                 for (int j = 0; j < 8; j += 2) {
                     const float2 o = unpack_f16((&w.x)[j >> 1]);
-#pragma unroll
-                    for (int h = 0; h < 2; ++h)
-                        v[i + j + h] = fmaf(fmaf(f.r, di + sh.d[c + i + j + h], f.q), (h ? o.y : o.x) * less, f.r * (__uint_as_float(r[i + j + h]) * less * less));
+                    const float2 dj = *reinterpret_cast<const float2*>(&sh.d[c + i + j]);
+                    v[i + j]     = fmaf(fmaf(f.r, di + dj.x, f.q), o.x * less, f.r * (__uint_as_float(r[i + j]) * less * less));
+                    v[i + j + 1] = fmaf(fmaf(f.r, di + dj.y, f.q), o.y * less, f.r * (__uint_as_float(r[i + j + 1]) * less * less));
                 }
             }
             if (c == (warp & 3) * 32) {
