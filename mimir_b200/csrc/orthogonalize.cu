@@ -577,7 +577,7 @@ __global__ void __launch_bounds__(PREPARE) prepare_kernel(const __grid_constant_
 // ---- small matrices --------------------------------------------------------------------------------------------------------------
 // All steps of a matrix with up to 128 rows and 256 columns (or turned: 256 and 128) in one CTA: X as f32 in tensor memory and as f16 in shared memory, 64 columns to a
 // 128-byte row, which serves as the operand of X X^T and as the right one of B X; A, then B, as f16 in another such matrix. Eight warps: 32 rows, one to a lane, and half of
-// the columns each. A step's three products take some 512 cycles each, what is between them 600 to 1500. [128, 128]: 
+// the columns each. A step of [128, 128] takes 4.5 us: its three products 900 cycles each (issued by one thread), the rest what is between them.
 constexpr int SMALL_K = 128, SMALL_L = 256, SMALL_THREADS = 256, CHUNK64 = 128 * 128;  // bytes of 128 rows of 64 columns
 constexpr int MOST_STEPS = 64;
 struct Factors {
@@ -731,9 +731,10 @@ __global__ void __launch_bounds__(SMALL_THREADS) small_kernel(const __grid_const
 #pragma unroll
             for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]) * (1.f / (SX * SX));
             if (c == (warp & 3) * 32) {  // the diagonal: lane i has it in column i
+                float on = 0.f;
 #pragma unroll
-                for (int i = 0; i < 32; ++i)
-                    if (i == lane) sh.d[row] = v[i], v[i] = 0.f;
+                for (int i = 0; i < 32; ++i) on = i == lane ? v[i] : on, v[i] = i == lane ? 0.f : v[i];
+                sh.d[row] = on;
             }
             put_row(a16, row, c, v, f.a);
         }
@@ -766,9 +767,10 @@ __global__ void __launch_bounds__(SMALL_THREADS) small_kernel(const __grid_const
                 }
             }
             if (c == (warp & 3) * 32) {
+                float on = 0.f;
 #pragma unroll
-                for (int i = 0; i < 32; ++i)
-                    if (i == lane) sh.e[row] = f.q * di + f.r * fmaf(di, di, __uint_as_float(r[i]) * less * less), v[i] = 0.f;
+                for (int i = 0; i < 32; ++i) on = i == lane ? __uint_as_float(r[i]) : on, v[i] = i == lane ? 0.f : v[i];
+                sh.e[row] = f.q * di + f.r * fmaf(di, di, on * less * less);
             }
             put_row(a16, row, c, v, f.b);
         }
@@ -956,7 +958,7 @@ int prepare(const Desc& d, const Plan& p, int64_t first, int64_t count, cudaStre
     return launch_after(prepare_kernel<T, 1>, rows, PREPARE, 0, s, all, int(d.m), int(d.n), int(p.pitch_x), static_cast<const double*>(p.sums), d.eps, p.x[0][0], p.x[0][1]);
 }
 
-// Matrices that a CTA takes whole. Against three launches a step: 64 of [128, 128] 141 us, here ; one of [255, 120] , here .
+// Matrices that a CTA takes whole: 64 of [128, 128] in 30 us, with three launches a step 141.
 bool small(const Desc& d) { return (d.m < d.n ? d.m : d.n) <= SMALL_K && (d.m < d.n ? d.n : d.m) <= SMALL_L; }
 template <class T, bool TALL>
 int small_launch(const Matrices& all, const SmallArgs& g, int64_t count, const DeviceInfo& dev, cudaStream_t s) {
