@@ -256,8 +256,8 @@ __device__ __forceinline__ void leave16(uint32_t at, float a, float b, float c, 
 constexpr int THREADS = 512;                // of a block: one team of all of them, or several
 constexpr uint32_t PLANE = THREADS * 16;    // 16 bytes for each
 constexpr int MOST_SMEM = 200 << 10;
-template <int ROW>                          // planes of a row
-constexpr int STAGES = MOST_SMEM / (ROW * int(PLANE)) < 6 ? MOST_SMEM / (ROW * int(PLANE)) : 6;
+template <int ROW, int BLOCKS = 1>          // planes of a row; blocks that share an SM
+constexpr int STAGES = MOST_SMEM / BLOCKS / (ROW * int(PLANE)) < 6 ? MOST_SMEM / BLOCKS / (ROW * int(PLANE)) : 6;
 
 // Two f32 values to an instruction.
 struct F2 {
@@ -494,13 +494,13 @@ struct Weights {
 };
 
 template <class RT, class HT, int CH, bool RAGGED, bool GROUPS>
-__global__ void __launch_bounds__(THREADS, 1) forward_ring_kernel(const __grid_constant__ Args<RT, HT> g, const __grid_constant__ Ring k) {
+__global__ void __launch_bounds__(THREADS, CH == 1 ? 2 : 1) forward_ring_kernel(const __grid_constant__ Args<RT, HT> g, const __grid_constant__ Ring k) {
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ Sums sums;
     after_previous();
     const Mine<CH> m(k, g.d, smem);
     if (m.team >= k.teams) return;  // (whole teams: their barriers are their own)
-    constexpr int PAIR = PLANES<RT> + PLANES<HT>, ROW = CH * PAIR;
+    constexpr int PAIR = PLANES<RT> + PLANES<HT>, ROW = CH * PAIR, AHEAD = STAGES<ROW, CH == 1 ? 2 : 1>;
     Walk<GROUPS> cur(g, k, m.team), ahead = cur;
     const int64_t total = g.n * g.d;
     const float per     = 1.f / float(g.d);
@@ -525,14 +525,14 @@ __global__ void __launch_bounds__(THREADS, 1) forward_ring_kernel(const __grid_c
         }
         copies_end();
     };
-    for (int stage = 0; stage < STAGES<ROW>; ++stage) request(stage * ROW * PLANE);
+    for (int stage = 0; stage < AHEAD; ++stage) request(stage * ROW * PLANE);
     Weights<CH> f;
     int64_t group  = -1;
     uint32_t stage = 0;
     int turn       = 0;
     while (cur.next()) {
         if (cur.group != group) f.load(g, m, group = cur.group);
-        copies_wait<STAGES<ROW> - 1>();
+        copies_wait<AHEAD - 1>();
         F2 v[CH][4], h[CH][4], squares(0.f);
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
@@ -547,7 +547,7 @@ __global__ void __launch_bounds__(THREADS, 1) forward_ring_kernel(const __grid_c
             e = rsqrtf(fmaf(sum, per, g.eps));
         }
         request(stage);
-        stage   = stage == (STAGES<ROW> - 1) * ROW * PLANE ? 0 : stage + ROW * PLANE;
+        stage   = stage == (AHEAD - 1) * ROW * PLANE ? 0 : stage + ROW * PLANE;
         squares = F2(0.f);
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
@@ -837,12 +837,15 @@ Plan plan(const Desc& d, bool backward, bool aligned, Space& space, int sm_count
     p.ring             = aligned && in_block > 0 && row <= MOST_SMEM;
     if (p.ring) {
         p.k.team = int(team), p.k.classes = classes;
-        p.threads = THREADS, p.smem = size_t(row * (MOST_SMEM / row < 6 ? MOST_SMEM / row : 6));
-        const int64_t most = int64_t(sm_count) * in_block, need = up(d.n, classes);
+        const int64_t share = !backward && p.columns == 1 ? 2 : 1, stages = MOST_SMEM / share / row;  // blocks to an SM
+        p.threads = THREADS, p.smem = size_t(row * (stages < 6 ? stages : 6));
+        const int64_t most = int64_t(sm_count) * share * in_block, need = up(d.n, classes);
         p.k.teams = int((need < most ? need : most) / classes * classes);
         p.teams   = p.k.teams;
         p.blocks  = int((p.teams + in_block - 1) / in_block);
-        p.pieces  = up((p.teams + p.groups - 1) / (p.groups ? p.groups : 1), classes);
+        // (no more units than teams, as far as that goes: a team with two of them would be the last)
+        p.pieces = p.groups ? p.teams / p.groups / classes * classes : classes;
+        if (p.pieces < classes) p.pieces = classes;
     } else {
         const int64_t each = d.d <= 2048 ? 8 : d.d <= 8192 ? 16 : 32, lanes = up((d.d + each - 1) / each, 32);
         p.threads = int(lanes), p.rows = lanes == 32 ? 4 : 1;
