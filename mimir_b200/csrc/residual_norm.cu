@@ -311,35 +311,38 @@ struct Walk<false> {
 };
 template <>
 struct Walk<true> {
-    int64_t row, end, offset, unit, group;  // offset: of the row's first element
-    int64_t w, step, per, n, d, run, pieces, units;
-    int cls, classes;
+    int64_t offset, d;
+    int row, end, unit, group;
+    int w, step, per, n, run, pieces, units, cls, classes;  // (there are fewer than 2^31 rows, and no more units)
     template <class A>
     __device__ __forceinline__ Walk(const A& g, const Ring& k, int team)
-        : row(0), end(0), offset(0), w(team / k.classes - k.teams / k.classes), step(k.teams / k.classes), n(g.n), d(g.d), run(g.gate_rows), pieces(g.pieces), units(g.groups * g.pieces),
-          cls(team % k.classes), classes(k.classes) {
+        : offset(0), d(g.d), row(0), end(0), unit(0), group(0), w(team / k.classes - k.teams / k.classes), step(k.teams / k.classes), n(int(g.n)), run(int(g.gate_rows)), pieces(int(g.pieces)),
+          units(int(g.groups * g.pieces)), cls(team % k.classes), classes(k.classes) {
         per = pieces % classes ? 0 : pieces / classes;
     }
     // the next row of the unit, or the first of the team's next one; false: there is none
     __device__ __forceinline__ bool next() {
-        row += pieces, offset += pieces * d;
-        return row < end || next_unit();
+        if (end - row > pieces) {
+            row += pieces, offset += pieces * d;
+            return true;
+        }
+        return next_unit();
     }
     __device__ __forceinline__ bool next_unit() {
         do {
             w += step;
-            int64_t piece;
+            int piece;
             if (per) {
-                group = w / per, piece = (w - group * per) * classes;
-                if (group * pieces >= units) return false;
-                const int shift = int((cls - (group * run + piece)) % classes);
-                piece += shift < 0 ? shift + classes : shift;
+                group = int(unsigned(w) / unsigned(per)), piece = (w - group * per) * classes;
+                if (int64_t(group) * pieces >= units) return false;
+                // (classes is a power of two)
+                piece += (cls - (group * run + piece)) & (classes - 1);
             } else {  // units of one row
-                const int64_t u = w * classes + cls;
+                const int64_t u = int64_t(w) * classes + cls;
                 if (u >= units) return false;
-                group = u / run, piece = u - group * run;
+                group = int(unsigned(u) / unsigned(run)), piece = int(u) - group * run;
             }
-            unit = group * pieces + piece, row = group * run + piece, end = min(n, (group + 1) * run);
+            unit = group * pieces + piece, row = group * run + piece, end = run < n - group * run ? (group + 1) * run : n;
         } while (row >= end);
         offset = row * d;
         return true;
@@ -400,16 +403,30 @@ __device__ __forceinline__ void put_anywhere(T* p, const float (&v)[8], int lo, 
     }
 }
 // eight factors from column `at` on, of which those in [lo, hi) are there; zeros for the others
-__device__ __forceinline__ void factors_part(const Factors& f, int64_t at, int lo, int hi, float (&v)[8]) {
-    if (lo == 0 && hi == 8 && (reinterpret_cast<uintptr_t>(f.p) + uintptr_t(at) * (f.bf16 ? 2 : 4)) % 16 == 0) {
-        factors_at(f, at, v);
-        return;
-    }
+template <class T>
+__device__ __forceinline__ void factors_of(const T* p, int lo, int hi, float (&v)[8]) {
+    if (lo == 0 && hi == 8 && reinterpret_cast<uintptr_t>(p) % 16 == 0) {
+        Run<T, 8> run;
+        run.load(p), run.get(v);
+    } else {
+        Run<T, 1> run[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        float one[1] = {0.f};
-        if (j >= lo && j < hi) factors_at(f, at + j, one);
-        v[j] = one[0];
+        for (int j = 0; j < 8; ++j) {
+            run[j].clear();
+            if (j >= lo && j < hi) run[j].load(p + j);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) run[j].get(*reinterpret_cast<float(*)[1]>(v + j));
+    }
+}
+__device__ __forceinline__ void factors_part(const Factors& f, int64_t at, int lo, int hi, float (&v)[8]) {
+    if (!f.p) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = j >= lo && j < hi ? 1.f : 0.f;
+    } else if (f.bf16) {
+        factors_of(static_cast<const __nv_bfloat16*>(f.p) + at, lo, hi, v);
+    } else {
+        factors_of(static_cast<const float*>(f.p) + at, lo, hi, v);
     }
 }
 
@@ -494,13 +511,13 @@ struct Weights {
 };
 
 template <class RT, class HT, int CH, bool RAGGED, bool GROUPS>
-__global__ void __launch_bounds__(THREADS, CH == 1 ? 2 : 1) forward_ring_kernel(const __grid_constant__ Args<RT, HT> g, const __grid_constant__ Ring k) {
+__global__ void __launch_bounds__(THREADS, CH == 1 && !GROUPS ? 2 : 1) forward_ring_kernel(const __grid_constant__ Args<RT, HT> g, const __grid_constant__ Ring k) {
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ Sums sums;
     after_previous();
     const Mine<CH> m(k, g.d, smem);
     if (m.team >= k.teams) return;  // (whole teams: their barriers are their own)
-    constexpr int PAIR = PLANES<RT> + PLANES<HT>, ROW = CH * PAIR, AHEAD = STAGES<ROW, CH == 1 ? 2 : 1>;
+    constexpr int PAIR = PLANES<RT> + PLANES<HT>, ROW = CH * PAIR, AHEAD = STAGES<ROW, CH == 1 && !GROUPS ? 2 : 1>;
     Walk<GROUPS> cur(g, k, m.team), ahead = cur;
     const int64_t total = g.n * g.d;
     const float per     = 1.f / float(g.d);
@@ -527,7 +544,7 @@ __global__ void __launch_bounds__(THREADS, CH == 1 ? 2 : 1) forward_ring_kernel(
     };
     for (int stage = 0; stage < AHEAD; ++stage) request(stage * ROW * PLANE);
     Weights<CH> f;
-    int64_t group  = -1;
+    int group      = -1;
     uint32_t stage = 0;
     int turn       = 0;
     while (cur.next()) {
@@ -645,7 +662,7 @@ __global__ void __launch_bounds__(THREADS, 1) backward_ring_kernel(const __grid_
         }
     };
     Weights<CH> f;
-    int64_t group = -1, unit = -1;
+    int group = -1, unit = -1;
     uint32_t stage = 0;
     int turn       = 0;
     // (a row's e and s are asked for a row ahead)
@@ -741,7 +758,7 @@ struct Join {
 struct Joins {
     Join j[3];
 };
-constexpr int JOINED = 256, AT_ONCE = 8;  // threads; rows that each has on their way
+constexpr int JOINED = 512, AT_ONCE = 16;  // threads; rows that each has on their way
 __global__ void __launch_bounds__(JOINED) join_kernel(const __grid_constant__ Joins all, int64_t d) {
     __shared__ float sums[JOINED / 32][32];
     after_previous();
@@ -837,7 +854,7 @@ Plan plan(const Desc& d, bool backward, bool aligned, Space& space, int sm_count
     p.ring             = aligned && in_block > 0 && row <= MOST_SMEM;
     if (p.ring) {
         p.k.team = int(team), p.k.classes = classes;
-        const int64_t share = !backward && p.columns == 1 ? 2 : 1, stages = MOST_SMEM / share / row;  // blocks to an SM
+        const int64_t share = !backward && p.columns == 1 && p.groups == 1 ? 2 : 1, stages = MOST_SMEM / share / row;  // blocks to an SM
         p.threads = THREADS, p.smem = size_t(row * (stages < 6 ? stages : 6));
         const int64_t most = int64_t(sm_count) * share * in_block, need = up(d.n, classes);
         p.k.teams = int((need < most ? need : most) / classes * classes);
