@@ -17,6 +17,7 @@ template <>
 struct Run<float, 8> {
     uint4 a, b;
     __device__ __forceinline__ void load(const float* p) { a = *reinterpret_cast<const uint4*>(p), b = *reinterpret_cast<const uint4*>(p + 4); }
+    __device__ __forceinline__ void store(float* p) const { *reinterpret_cast<uint4*>(p) = a, *reinterpret_cast<uint4*>(p + 4) = b; }
     __device__ __forceinline__ void clear() { a = b = make_uint4(0, 0, 0, 0); }
     __device__ __forceinline__ void get(float (&v)[8]) const {
         v[0] = __uint_as_float(a.x), v[1] = __uint_as_float(a.y), v[2] = __uint_as_float(a.z), v[3] = __uint_as_float(a.w);
@@ -27,6 +28,7 @@ template <>
 struct Run<__nv_bfloat16, 8> {
     uint4 a;
     __device__ __forceinline__ void load(const __nv_bfloat16* p) { a = *reinterpret_cast<const uint4*>(p); }
+    __device__ __forceinline__ void store(__nv_bfloat16* p) const { *reinterpret_cast<uint4*>(p) = a; }
     __device__ __forceinline__ void clear() { a = make_uint4(0, 0, 0, 0); }
     __device__ __forceinline__ void get(float (&v)[8]) const {
         v[0] = bf16_low(a.x), v[1] = bf16_high(a.x), v[2] = bf16_low(a.y), v[3] = bf16_high(a.y);
@@ -37,6 +39,7 @@ template <>
 struct Run<float, 1> {
     float a;
     __device__ __forceinline__ void load(const float* p) { a = *p; }
+    __device__ __forceinline__ void store(float* p) const { *p = a; }
     __device__ __forceinline__ void clear() { a = 0.f; }
     __device__ __forceinline__ void get(float (&v)[1]) const { v[0] = a; }
 };
@@ -44,6 +47,7 @@ template <>
 struct Run<__nv_bfloat16, 1> {
     uint16_t a;
     __device__ __forceinline__ void load(const __nv_bfloat16* p) { a = *reinterpret_cast<const uint16_t*>(p); }
+    __device__ __forceinline__ void store(__nv_bfloat16* p) const { *reinterpret_cast<uint16_t*>(p) = a; }
     __device__ __forceinline__ void clear() { a = 0; }
     __device__ __forceinline__ void get(float (&v)[1]) const { v[0] = __uint_as_float(uint32_t(a) << 16); }
 };

@@ -46,22 +46,38 @@ __global__ void __launch_bounds__(THREADS) rows_kernel(const T* table, Ids ids, 
         if (from - lane * VEC >= d) continue;
         const int c = class_at(ids, i);
         if (c == BAD && lane == 0) *status = MIMK_E_SHAPE;
+        const int left = int(min(d - from, int64_t(32 * VEC * COLS)));  // (not above zero: this lane has none of the row)
+        O* to          = out + i * d + from;
+        if (c < 0) {
+            float v[VEC];
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) v[j] = c == BAD ? NAN : 0.f;
+#pragma unroll
+            for (int k = 0; k < COLS; ++k)
+                if (k * 32 * VEC < left) put(to + k * 32 * VEC, v);
+            continue;
+        }
+        const T* row = table + int64_t(c) * d + from;
         Run<T, VEC> run[COLS];
 #pragma unroll
-        for (int k = 0; k < COLS; ++k) {
-            const int64_t at = from + k * 32 * VEC;
-            run[k].clear();
-            if (c >= 0 && at < d) run[k].load(table + int64_t(c) * d + at);
+        for (int k = 0; k < COLS; ++k)
+            if (k * 32 * VEC < left) run[k].load(row + k * 32 * VEC);
+        if constexpr (sizeof(T) == sizeof(O)) {
+            if (scale == 1.f) {  // the values as they are
+#pragma unroll
+                for (int k = 0; k < COLS; ++k)
+                    if (k * 32 * VEC < left) run[k].store(to + k * 32 * VEC);
+                continue;
+            }
         }
 #pragma unroll
         for (int k = 0; k < COLS; ++k) {
-            const int64_t at = from + k * 32 * VEC;
-            if (at >= d) break;
+            if (k * 32 * VEC >= left) break;
             float v[VEC];
             run[k].get(v);
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) v[j] = c == BAD ? NAN : c == NO_TOKEN ? 0.f : v[j] * scale;
-            put(out + i * d + at, v);
+            for (int j = 0; j < VEC; ++j) v[j] *= scale;
+            put(to + k * 32 * VEC, v);
         }
     }
 }
