@@ -423,8 +423,8 @@ int mimk_clip_grads(const void* const* tensors, void* const* out, const int64_t*
  * has_ignore: a position whose id is ignore_index, a class or not, has no token: its row of the result is zeros, and its row of dy is not read.
  * Any other id outside [0, v) is recorded (mimk_device_status: MIMK_E_SHAPE); its row of the result is NaN, and nothing of it enters dtable.
  * Sums are f32, over positions in rising order in groups that the extents and ids alone decide, rounded once: equal descriptors and ids give equal bits. No
- * operand overlaps a result. Extents below 2^31 (v d may be more), rows are dense. Workspace as above, of embedding_grad only: 8 bytes per class and position
- * and what long runs of one class leave between launches. */
+ * operand overlaps a result. Extents below 2^31 (v d may be more), rows are dense. Workspace as above, of embedding_grad only: none up to 2048 positions; otherwise 8 bytes per
+ * class, 17 per position, and an f32 row of d for each 256 positions. */
 typedef struct mimk_embedding_desc {
     int64_t n, d, v;   /* positions, features, classes */
     const void* table; /* [v, d] of dtype */
@@ -479,11 +479,12 @@ int mimk_residual_rmsnorm_bwd(const mimk_residual_rmsnorm_desc* desc, void* stre
 
 /* Matrices with their singular values brought near 1 (an optimiser's orthogonalised update) by Newton-Schulz steps: X = x / (|x| + eps), |x| the 2-norm of all
  * values; for each step (p, q, r): A = X X^T (X^T X where m > n), X <- p X + (q A + r A^2) X (X (q A + r A^2)); out = scale * X as BF16.
- * x: F32 or BF16. Operands of the products are rounded to 11 significant bits (f16 with powers of two as factors), except the diagonals of A and of q A + r A^2, which
- * are f32; p X is added in f32 from an X of 22 bits; sums are f32, |x| is f64. What X has below 2^-32 is lost. A matrix with a value that is not finite comes out NaN, one of zeros zeros.
+ * x: F32 or BF16. Operands of the products are rounded to 11 significant bits (f16 with powers of two as factors, down to 2^-32 for X), except the diagonals of A and of
+ * q A + r A^2, which are f32; p X is added in f32 from an X of 22 bits at least; sums are f32, |x| is f64. A matrix with a value that is not finite comes out NaN, one of zeros zeros.
  * The steps must keep singular values from 0 to 1 within 4 (MIMK_E_UNSUPPORTED otherwise): the largest value of |p s + q s^3 + r s^5| is followed from step to step.
  * Equal descriptors give equal bits, a matrix the same whatever others are in the batch. The arrays are on the host and are read before the call returns. No result overlaps an operand.
- * Workspace as above: 8 bytes per value of X, 4 per value of A, of as many matrices as take about 1 GiB. */
+ * Workspace as above: none for matrices of up to 128 x 256 or 256 x 128; otherwise 10 bytes per value of X, 4 per value of A, and partial sums of A in no more bytes than X
+ * has where its sums are long; of as many matrices as take about 1 GiB, or of one. */
 typedef struct mimk_orthogonalize_desc {
     int64_t batch, m, n;
     const void* const* x;      /* batch matrices [m, n] of dtype, dense */

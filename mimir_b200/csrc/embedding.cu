@@ -538,8 +538,12 @@ __global__ void __launch_bounds__(THREADS) few_kernel(const T* dy, Ids ids, O* d
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------------------
+constexpr int WIDE = 2, NARROW = 8;  // loads a lane for a gradient's part of a row: of 8 elements, or of one
+// the way without groups (its grid has a part of a row for each second index)
+bool few(const mimk_embedding_desc& d) { return d.n <= FEW && d.d <= int64_t(65535) * 32 * NARROW; }
 Groups groups_in(Space& space, const mimk_embedding_desc& d) {
-    Groups g;
+    Groups g{};
+    if (few(d)) return g;
     g.count = static_cast<int*>(space.take(size_t(d.v) * 4)), g.start = static_cast<int*>(space.take(size_t(d.v) * 4));
     g.slot = static_cast<int*>(space.take(size_t(d.n) * 4)), g.order = static_cast<int*>(space.take(size_t(d.n) * 4));
     g.sorted = static_cast<int*>(space.take(size_t(d.n) * 4));
@@ -565,8 +569,6 @@ unsigned blocks_for(int64_t units, int64_t each, int64_t most) {
     return unsigned(b < 1 ? 1 : b < most ? b : most);
 }
 
-constexpr int WIDE = 2, NARROW = 8;  // loads a lane for a gradient's part of a row: of 8 elements, or of one
-
 template <int VEC, int COLS>
 int parts_of(int64_t d) {
     return int((d + 32 * VEC * COLS - 1) / (32 * VEC * COLS));
@@ -586,7 +588,7 @@ int rows(const mimk_embedding_desc& d, const DeviceInfo& dev, cudaStream_t s) {
 template <class T, class O, int VEC, int COLS>
 int grad(const mimk_embedding_desc& d, const Groups& g, const DeviceInfo& dev, cudaStream_t s) {
     const int parts = parts_of<VEC, COLS>(d.d);
-    if (d.n <= FEW && parts <= 65535) {
+    if (few(d)) {
         // Eight blocks to an SM, but no more groups than classes. 2048 positions here and 3000 the other way: 131072 x 4096 bf16 191 and 185 us, 50021 x 2048 54 and 62,
         // 10007 x 777 f32 28 and 62, 1000 x 4096 25 and 36, 131072 x 64 28 and 32.
         int log = 0;
@@ -651,8 +653,8 @@ extern "C" int mimk_embedding_grad(const mimk_embedding_desc* d, void* stream) {
     if (off(d->dy, d->dtype) || off(d->dtable, d->out_dtype) || off(d->ids, d->id_dtype)) return MIMK_E_ALIGN;
     Space space(d->workspace);
     const Groups g = groups_in(space, *d);
-    if (!d->workspace || space.used() > d->workspace_bytes) return MIMK_E_WORKSPACE;
-    if (!aligned16(d->workspace)) return MIMK_E_ALIGN;
+    if (space.used() > d->workspace_bytes || (space.used() && !d->workspace)) return MIMK_E_WORKSPACE;
+    if (space.used() && !aligned16(d->workspace)) return MIMK_E_ALIGN;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     MIMK_BY_TYPES(grad, d->d % 8 == 0 && aligned16(d->dy) && aligned16(d->dtable), *d, g, *dev, s);
 }

@@ -288,7 +288,8 @@ def test_refusals():
     lib, need = _lib.lib(), C.c_uint64()
     d = _lib.EmbeddingDesc()
     out = torch.empty_like(table)
-    d.n, d.d, d.v, d.ids, d.dy, d.scale, d.dtype, d.out_dtype, d.id_dtype = 20, 40, 50, ids.data_ptr(), dy.data_ptr(), 1.0, _lib.BF16, _lib.BF16, _lib.I64
+    ids, dy = ids_of((3000,), 50, 28), randn((3000, 40), 30, 1.0, BF16)
+    d.n, d.d, d.v, d.ids, d.dy, d.scale, d.dtype, d.out_dtype, d.id_dtype = 3000, 40, 50, ids.data_ptr(), dy.data_ptr(), 1.0, _lib.BF16, _lib.BF16, _lib.I64
     assert lib.mimk_embedding_grad(C.byref(d), None) == 1
     d.dtable = out.data_ptr()
     assert lib.mimk_embedding_grad_workspace(C.byref(d), C.byref(need)) == 0
