@@ -442,10 +442,11 @@ __global__ void __launch_bounds__(THREADS, 1) single_kernel(const __grid_constan
 }
 
 // A from partial results: 8 rows and 32 columns of it for each warp, a column per lane; on and below the diagonal, and the other triangle's from there.
-__device__ __forceinline__ void sum_parts_of(const Args& g, int splits, int64_t first, int64_t step) {
+__global__ void __launch_bounds__(256) sum_kernel(const __grid_constant__ Args g, int splits) {
+    after_previous();
     const int lane = threadIdx.x & 31, across = (g.cols + 31) / 32, down = (g.rows + 7) / 8;
     const int64_t stride = int64_t(g.batch) * g.rows * g.pitch, units = int64_t(across) * down;
-    for (int64_t u = first; u < units * g.batch; u += step) {
+    for (int64_t u = int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5); u < units * g.batch; u += int64_t(gridDim.x) * 8) {
         const int z = int(u / units), i = int(u - z * units), row0 = i / across * 8, column0 = i % across * 32, column = column0 + lane;
         if (row0 + 7 < column0) continue;
         const int64_t matrix = int64_t(z) * g.rows;
@@ -473,15 +474,12 @@ __device__ __forceinline__ void sum_parts_of(const Args& g, int splits, int64_t 
         }
     }
 }
-__global__ void __launch_bounds__(256) sum_kernel(const __grid_constant__ Args g, int splits) {
-    after_previous();
-    sum_parts_of(g, splits, int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5), int64_t(gridDim.x) * 8);
-}
 
 // ---- x to X ----------------------------------------------------------------------------------------------------------------------
 constexpr int TABLE = 1024;       // matrices of one launch
-constexpr int CHUNK = 1 << 16;    // values that one block squares
 constexpr int PREPARE = 256;
+// Values that one block squares: eight for each thread, more where that would be more than some 1200 blocks.
+__host__ __device__ __forceinline__ int64_t chunk_of(int64_t count) { return (count / 1184 + 8 * PREPARE) / (8 * PREPARE) * (8 * PREPARE); }
 
 struct Matrices {
     const void* x[TABLE];
@@ -525,36 +523,37 @@ struct Inverse {
 template <class T, int VEC>
 __global__ void __launch_bounds__(PREPARE) squares_kernel(const __grid_constant__ Matrices all, int64_t count, double* sums) {
     after_previous();
-    const T* x = static_cast<const T*>(all.x[blockIdx.y]);
-    for (int64_t chunk = blockIdx.x; chunk * CHUNK < count; chunk += gridDim.x) {
-        const int64_t end = min(count, (chunk + 1) * CHUNK);
-        double sum        = 0;
-#pragma unroll 4
-        for (int64_t i = chunk * CHUNK + threadIdx.x * VEC; i < end; i += PREPARE * VEC) {
-            Run<T, VEC> run;
-            float v[VEC];
-            run.load(x + i), run.get(v);
-            sum += squares(v);
-        }
-        sum = block_total(sum);
-        if (threadIdx.x == 0) sums[blockIdx.y * ((count + CHUNK - 1) / CHUNK) + chunk] = sum;
+    const T* x           = static_cast<const T*>(all.x[blockIdx.y]);
+    const int64_t chunk  = chunk_of(count), begin = blockIdx.x * chunk, end = min(count, begin + chunk);
+    double sum           = 0;
+#pragma unroll 8
+    for (int64_t i = begin + threadIdx.x * VEC; i < end; i += PREPARE * VEC) {
+        Run<T, VEC> run;
+        float v[VEC];
+        run.load(x + i), run.get(v);
+        sum += squares(v);
     }
+    sum = block_total(sum);
+    if (threadIdx.x == 0) sums[blockIdx.y * gridDim.x + blockIdx.x] = sum;
 }
 // X times SX as two f16: rows of `pitch`. Every block adds the chunks' sums up itself, in the same order.
 template <class T, int VEC>
 __global__ void __launch_bounds__(PREPARE) prepare_kernel(const __grid_constant__ Matrices all, int rows, int cols, int pitch, const double* sums, float eps, __half* hi, __half* lo) {
     after_previous();
     const int64_t count = int64_t(rows) * cols;
-    const int chunks    = int((count + CHUNK - 1) / CHUNK);
+    const int chunks    = int((count + chunk_of(count) - 1) / chunk_of(count));
     double total        = 0;
     for (int i = threadIdx.x; i < chunks; i += PREPARE) total += sums[blockIdx.y * chunks + i];
     const Inverse by(sqrt(block_total(total)), eps);
     const T* x          = static_cast<const T*>(all.x[blockIdx.y]);
     const int64_t base  = int64_t(blockIdx.y) * rows * pitch;
     const int units     = (cols + VEC - 1) / VEC;  // of a row
-    for (int row = blockIdx.x; row < rows; row += gridDim.x)
+    int log             = 0;                       // a row to 2^log threads
+    while (log < 8 && 1 << log < units) ++log;
+    const int together = PREPARE >> log;
+    for (int row = blockIdx.x * together + (threadIdx.x >> log); row < rows; row += gridDim.x * together)
 #pragma unroll 2
-        for (int u = threadIdx.x; u < units; u += PREPARE) {
+        for (int u = threadIdx.x & ((1 << log) - 1); u < units; u += 1 << log) {
             Run<T, VEC> run;
             float v[VEC];
             run.load(x + int64_t(row) * cols + u * VEC), run.get(v);
@@ -865,7 +864,7 @@ struct Plan {
 Plan plan(const Desc& d, Space& space) {
     Plan p{};
     p.k = d.m < d.n ? d.m : d.n, p.pitch_x = up(d.n, 8), p.pitch_a = up(p.k, 8), p.pitch_d = up(p.k, 4);
-    p.chunks = (d.m * d.n + CHUNK - 1) / CHUNK;
+    p.chunks = (d.m * d.n + chunk_of(d.m * d.n) - 1) / chunk_of(d.m * d.n);
     // Partial results where A has few tiles and they are long: no more bytes than X has.
     const int64_t l = d.m < d.n ? d.n : d.m, part = 4 * p.k * p.pitch_a;
     p.splits = 1;
@@ -949,7 +948,7 @@ int prepare(const Desc& d, const Plan& p, int64_t first, int64_t count, cudaStre
         vec      = vec && aligned16(d.x[first + i]);
     }
     const int64_t values = d.m * d.n;
-    const dim3 squares(unsigned(p.chunks < 4096 ? p.chunks : 4096), unsigned(count)), rows(unsigned(d.m < 4096 ? d.m : 4096), unsigned(count));
+    const dim3 squares(unsigned(p.chunks), unsigned(count)), rows(unsigned(d.m < 4096 ? d.m : 4096), unsigned(count));
     if (vec) {
         MIMK_TRY(launch_after(squares_kernel<T, 8>, squares, PREPARE, 0, s, all, values, p.sums));
         return launch_after(prepare_kernel<T, 8>, rows, PREPARE, 0, s, all, int(d.m), int(d.n), int(p.pitch_x), static_cast<const double*>(p.sums), d.eps, p.x[0][0], p.x[0][1]);
