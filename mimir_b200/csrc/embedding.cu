@@ -20,6 +20,8 @@ constexpr int ZEROS = 4096;          // bytes of one bulk store
 constexpr int LIGHT = 32;            // positions of a class that one warp adds up
 constexpr int PIECE = 512;           // and that one block does
 constexpr int WINDOW = 1 << 17;      // positions in one map of bits
+constexpr int SORTED = 4096;         // positions that fit in its place
+constexpr int WARP_SORTED = SORTED / (WORKERS / 32);  // and in a warp's part of it
 constexpr int64_t LIM = int64_t(1) << 31;
 
 struct Ids {
@@ -138,9 +140,9 @@ __global__ void __launch_bounds__(THREADS) clear_kernel(Groups g, int64_t v) {
     for (int64_t i = int64_t(blockIdx.x) * THREADS + threadIdx.x; i < v; i += int64_t(gridDim.x) * THREADS) g.count[i] = 0;
 }
 
-// All blocks of the launch (which are resident at once) have come here. False: one of them has not come in a second or so, the status word says so, and the kernel is
-// left by all.
-__device__ __forceinline__ bool all_blocks_meet(const Groups& g, int nth, int* status) {
+// All blocks of the launch (which are resident at once) have come here. False: one of them has not come in a second or so (longer for many positions, whose phases take
+// up to some cycles each where one class has most of them), the status word says so, and the kernel is left by all.
+__device__ __forceinline__ bool all_blocks_meet(const Groups& g, int64_t n, int nth, int* status) {
     __shared__ int met;
     workers_meet<WORKERS>();
     if (threadIdx.x == 0) {
@@ -155,7 +157,7 @@ __device__ __forceinline__ bool all_blocks_meet(const Groups& g, int nth, int* s
             int now;
             asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(now) : "l"(arrived) : "memory");
             if (now >= all) break;
-            if (*given_up || clock64() - t0 > 2000000000LL) {
+            if (*given_up || clock64() - t0 > 2000000000LL + 16 * n) {
                 *given_up = 1, *status = MIMK_E_DEVICE_WAIT, met = 0;
                 break;
             }
@@ -231,13 +233,64 @@ __device__ __forceinline__ void fill_groups(const Ids& ids, const Groups& g, int
     }
 }
 
-// A block for a heavy class: its positions as bits of a map, read off in order.
-__device__ __forceinline__ void sort_heavies(const Groups& g, int64_t n, uint32_t* bits) {
-    const int heavies = g.cursor[1];
-    for (int h = blockIdx.x; h < heavies; h += gridDim.x) {
-        if (g.heavy[h].y) continue;
+// `size` values in shared memory, a power of two, in rising order (a bitonic network), by `threads` of which this is the t-th.
+template <class Meet>
+__device__ __forceinline__ void sort_shared(int* held, int size, int t, int threads, Meet&& meet) {
+    for (int run = 2; run <= size; run *= 2)
+        for (int step = run / 2; step; step /= 2) {
+            for (int k = t; k < size / 2; k += threads) {
+                const int at = 2 * k - (k & (step - 1)), a = held[at], b = held[at + step];
+                if ((a > b) == ((at & run) == 0)) held[at] = b, held[at + step] = a;
+            }
+            meet();
+        }
+}
+// The groups of heavy classes put in order. Up to WARP_SORTED positions: by a warp, in its part of the room. More: by a block, as bits of a map that are read off in order; where there
+// are more positions than one map's, groups of up to SORTED in the map's place, and groups of more than a map's positions as the ids name them, which are fewer than the
+// group over again for each map. (1048576 positions in 26214 classes, 64 columns of bf16: 704 us; 3531 with maps alone, 1099 with all sorted by blocks.)
+__device__ __forceinline__ void sort_heavies(const Ids& ids, const Groups& g, int64_t n, uint32_t* bits) {
+    const int heavies = g.cursor[1], warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    for (int h = blockIdx.x + warp * gridDim.x; h < heavies; h += gridDim.x * (WORKERS / 32)) {
         const int c = g.heavy[h].x, count = g.count[c], start = g.start[c];
+        if (g.heavy[h].y || count > WARP_SORTED) continue;
+        int* held = reinterpret_cast<int*>(bits) + warp * WARP_SORTED;
+        int size  = 2 * LIGHT;
+        while (size < count) size *= 2;
+        for (int k = lane; k < size; k += 32) held[k] = k < count ? g.order[start + k] : INT_MAX;
+        __syncwarp();
+        sort_shared(held, size, lane, 32, [] { __syncwarp(); });
+        for (int k = lane; k < count; k += 32) g.sorted[start + k] = held[k];
+        __syncwarp();
+    }
+    workers_meet<WORKERS>();
+    for (int h = blockIdx.x; h < heavies; h += gridDim.x) {
+        const int c = g.heavy[h].x, count = g.count[c], start = g.start[c];
+        if (g.heavy[h].y || count <= WARP_SORTED) continue;
+        if (n > WINDOW && count <= SORTED) {
+            int* held = reinterpret_cast<int*>(bits);
+            int size  = WARP_SORTED;
+            while (size < count) size *= 2;
+            for (int k = threadIdx.x; k < size; k += WORKERS) held[k] = k < count ? g.order[start + k] : INT_MAX;
+            workers_meet<WORKERS>();
+            sort_shared(held, size, threadIdx.x, WORKERS, [] { workers_meet<WORKERS>(); });
+            for (int k = threadIdx.x; k < count; k += WORKERS) g.sorted[start + k] = held[k];
+            workers_meet<WORKERS>();
+            continue;
+        }
         int done = 0;
+        if (count > WINDOW) {
+            constexpr int EACH = 4;
+            for (int64_t base = 0; base < n && done < count; base += WORKERS * EACH) {
+                const int64_t first = base + threadIdx.x * EACH;
+                unsigned its        = 0;
+#pragma unroll
+                for (int k = 0; k < EACH; ++k) its |= unsigned(first + k < n && class_at(ids, first + k) == c) << k;
+                int all, to = start + done + block_before(__popc(its), &all);
+                for (; its; its &= its - 1) g.sorted[to++] = int(first) + __ffs(its) - 1;
+                done += all;
+            }
+            continue;
+        }
         for (int64_t window = 0; window < n && done < count; window += WINDOW) {
             const int words = int(n - window < WINDOW ? (n - window + 31) / 32 : WINDOW / 32);
             const int each  = (words + WORKERS - 1) / WORKERS;
@@ -379,17 +432,17 @@ __global__ void __launch_bounds__(BLOCK, 1) grad_kernel(const T* dy, Ids ids, Gr
     }
     // (launched together: the blocks meet)
     count_positions(ids, g, n, status);
-    const bool met = all_blocks_meet(g, 1, status);
+    const bool met = all_blocks_meet(g, n, 1, status);
     if (threadIdx.x == 0) counted = met;
     with_writer<BLOCK>();
     if (!met) return;
     take_places(g, v);
-    if (!all_blocks_meet(g, 2, status)) return;
+    if (!all_blocks_meet(g, n, 2, status)) return;
     fill_groups(ids, g, n);
-    if (!all_blocks_meet(g, 3, status)) return;
+    if (!all_blocks_meet(g, n, 3, status)) return;
     if (g.cursor[1]) {
-        sort_heavies(g, n, room.bits);
-        if (!all_blocks_meet(g, 4, status)) return;
+        sort_heavies(ids, g, n, room.bits);
+        if (!all_blocks_meet(g, n, 4, status)) return;
     }
     const int64_t heavy_units = int64_t(g.cursor[1]) << shift;
     for (int64_t u = blockIdx.x; u < heavy_units; u += gridDim.x) {
@@ -428,7 +481,7 @@ __global__ void __launch_bounds__(BLOCK, 1) grad_kernel(const T* dy, Ids ids, Gr
     }
     if (!g.cursor[5]) return;
     // what pieces of one class left, in their order
-    if (!all_blocks_meet(g, 5, status)) return;
+    if (!all_blocks_meet(g, n, 5, status)) return;
     for (int64_t u = int64_t(blockIdx.x) * (WORKERS / 32) + warp; u < heavy_units; u += warps) {
         const int64_t h = u >> shift, begin = (u - (h << shift)) * PART, from = begin + lane * VEC;
         const int4 piece = g.heavy[h];

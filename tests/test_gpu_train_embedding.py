@@ -97,6 +97,29 @@ def test_many_positions():
     check_grad(randn((n, 24), 2, 1.0, BF16), ids, 40, 1.0, None, F32)
 
 
+def test_many_classes_of_many_positions():
+    """More positions than one map of bits holds: classes of some hundred, of a few thousand, of more than are sorted in shared memory, and of more than a map's."""
+    from mimir_b200 import tensor as T
+    n, v = 400001, 1000
+    ids = ids_of((n,), v, 7, skew=False)
+    order = torch.randperm(n, generator=torch.Generator().manual_seed(7)).cuda()
+    ids[order[:4000]], ids[order[4000:8500]], ids[order[8500:150000]] = 3, 500, v - 1
+    dy = randn((n, 16), 2, 1.0, F32)
+    assert torch.equal(check_grad(dy, ids, v, 1.0, None), T.embedding_grad(dy, ids, v))
+
+
+def test_one_class_of_very_many_positions():
+    """Whole numbers, so that sums are exact in whichever order."""
+    from mimir_b200 import tensor as T
+    n, v = 2 ** 25 + 3, 4
+    ids = torch.full((n,), 2, dtype=torch.int32, device="cuda")
+    ids[::1001] = 1
+    dy = torch.randint(-1, 2, (n, 1), device="cuda", generator=torch.Generator(device="cuda").manual_seed(8)).float()
+    got = T.embedding_grad(dy, ids, v)
+    T.device_status()
+    assert torch.equal(got[:, 0], torch.stack([dy[ids == c].double().sum() for c in range(v)]).float())
+
+
 def test_add_to():
     from mimir_b200 import tensor as T
     for n, d, v in ((700, 264, 200), (700, 33, 5000), (10, 64, 90)):
