@@ -15,7 +15,7 @@ namespace mimk {
 
 namespace {
 
-constexpr int64_t MOST_COLUMNS = 32768, LIM = int64_t(1) << 31;
+constexpr int64_t MOST_COLUMNS = 32768, LIM = (int64_t(1) << 31) - (1 << 17);  // (rows in 32 bits, with a team's step behind the last)
 
 // A vector of d factors, f32 or bf16; absent: ones.
 struct Factors {

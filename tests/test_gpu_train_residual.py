@@ -178,6 +178,36 @@ def test_many_rows():
     check(*inputs((3000, 1032), F32, F32, True, 0))
 
 
+@pytest.mark.parametrize("d,types", [(2048, (BF16, BF16)), (2049, (BF16, BF16)), (8200, (F32, BF16))])
+def test_rows_that_begin_past_32_bits(d, types):
+    """More than 2^31 values, of which the last rows are compared with a call of their own: whole rows, ragged ones, and those held in registers. Bits, where both calls have a row's
+    columns in the same places; else within what both may be off."""
+    from mimir_b200 import tensor as T
+    n, few = 2 ** 31 // d + 24, 16
+    p, _, _ = inputs((few, d), *types, False, 0)
+    p["post_gamma"] = p["gamma"]
+    last = torch.zeros((n, d), dtype=types[0], device="cuda")
+    r, h, dr, dx = last, *(torch.zeros((n, d), dtype=t, device="cuda") for t in (types[1], types[0], types[1]))
+    for k, (t, of) in enumerate(((r, p["r"]), (h, p["h"]), (dr, None), (dx, None))):
+        t[-few:] = of if of is not None else randn((few, d), 30 + k, 1.0, t.dtype)
+    own = dict(p, r=r[-few:].clone(), h=h[-few:].clone())
+    want = run(own, dr[-few:].clone(), dx[-few:].clone(), 1.0, 1.0)
+    more = dict(post_gamma=p["post_gamma"], gate=p["gate"])
+    new, x, kept = T.residual_rmsnorm_fwd(r, h, p["gamma"], EPS, **more)
+    got = dict(r=new[-few:].clone(), x=x[-few:].clone())
+    assert not bool(new[:64].any()) and not bool(x[:64].any())
+    del new, x
+    got.update(zip(("dr", "dh", "dgamma", "dpost_gamma", "dgate"), T.residual_rmsnorm_bwd(dr, dx, r, h, p["gamma"], kept, **more)))
+    assert not bool(got["dr"][:64].any()) and not bool(got["dh"][:64].any())
+    got["dr"], got["dh"] = got["dr"][-few:].clone(), got["dh"][-few:].clone()
+    bounds = formulas(own, dr[-few:], dx[-few:], 1.0, 1.0)
+    for name, value in got.items():
+        exact, off = bounds[name]
+        assert bool(((value.double() - exact).abs() <= 1.02 * (off + U[value.dtype] * (exact.abs() + off)) + 1e-37).all()), name
+        if d % 8 == 0 and name in ("r", "x", "dr", "dh"):
+            assert same_bits(value, want[name]), name
+
+
 def test_empty_extents():
     for shape in ((0, 16), (3, 0, 16), (4, 0)):
         p, dr, dx = inputs(shape, F32, BF16, True, 0)

@@ -76,3 +76,17 @@ def test_orthogonalize(lib):
     # a stack of any length takes a bounded buffer
     many = (C.c_void_p * 4096)(*[256] * 4096)
     assert L.mimk_orthogonalize_workspace(C.byref(desc(batch=4096, m=1024, n=1024, x=many)), C.byref(need)) == 0 and need.value < 3 << 29
+
+
+def test_as_many_rows_as_places_in_32_bits(lib):
+    """Rows are numbered in 32 bits, with some to spare for the steps from one to the next."""
+    L, need = lib.lib(), C.c_uint64()
+    most = (1 << 31) - (1 << 17)
+    d = lib.EmbeddingDesc()
+    d.n, d.d, d.v, d.dtype, d.out_dtype, d.id_dtype = most, 1, 8, lib.BF16, lib.BF16, lib.I64
+    assert L.mimk_embedding(C.byref(d), None) == L.mimk_embedding_grad(C.byref(d), None) == L.mimk_embedding_grad_workspace(C.byref(d), C.byref(need)) == 8
+    d.n = most - 1
+    assert L.mimk_embedding_grad_workspace(C.byref(d), C.byref(need)) == 0 and need.value >= 16 * most
+    r = lib.ResidualRmsnormDesc()
+    r.n, r.d, r.gate_rows, r.r, r.gamma, r.x, r.eps, r.residual_scale, r.branch_scale = most, 1, 1, 256, 256, 256, 1e-6, 1.0, 1.0
+    assert L.mimk_residual_rmsnorm_fwd(C.byref(r), None) == L.mimk_residual_rmsnorm_bwd(C.byref(r), None) == L.mimk_residual_rmsnorm_workspace(C.byref(r), C.byref(need)) == 8
