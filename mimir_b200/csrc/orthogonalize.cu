@@ -509,11 +509,11 @@ __device__ __forceinline__ double squares(const float (&v)[VEC]) {
     for (int j = 0; j < VEC; ++j) d += double(v[j]) * double(v[j]);
     return d;
 }
-// SX / (norm + eps), in two factors, as one may be beyond f32; NaN of a norm that is not finite
+// SX / (norm + eps), in two factors, as one may be beyond f32; NaN of a norm that is not finite, zero (for zeros to stay so) where norm and eps are zero
 struct Inverse {
     float first, second;
     __device__ __forceinline__ Inverse(double norm, float eps) {
-        const double by = isfinite(norm) ? 1.0 / (norm + double(eps)) : double(NAN);
+        const double by = !isfinite(norm) ? double(NAN) : norm + double(eps) > 0 ? 1.0 / (norm + double(eps)) : 0.0;
         int power         = 0;
         const double lead = isfinite(by) ? frexp(by, &power) : by;
         first = ldexpf(1.f, power / 2), second = float(ldexp(lead, power - power / 2)) * SX;

@@ -177,6 +177,12 @@ def test_zeros_and_values_that_are_not_finite():
     assert not bool(got[1].any()) and bool(got[[2, 3, 5]].isnan().all()) and torch.equal(got[[0, 4]], want[[0, 4]])
 
 
+def test_zeros_without_eps():
+    from mimir_b200 import tensor as T
+    for shape in ((40, 56), (200, 300), (130, 1)):
+        assert not bool(T.orthogonalize(torch.zeros(shape, device="cuda"), eps=0.0).any())
+
+
 def test_a_row_of_zeros_and_padding():
     from mimir_b200 import tensor as T
     x = matrix("random", (50, 80), 13)
