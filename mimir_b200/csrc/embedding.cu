@@ -6,7 +6,8 @@
 // bits), and results are the same call after call. A warp then owns 32 x VEC x COLS columns of a class: it adds up to 32 rows of dy, or writes zeros;
 // classes of more rows are taken by whole blocks, a run of the rows for each warp, joined in shared memory. All of it is one launch whose blocks meet between
 // its phases (and one that clears the counts). Up to 2048 positions: a launch of blocks that each look through all of them for the classes that are their own.
-// What bounds it: the bytes, most of all the table's gradient.
+// What bounds it: the bytes. 8192 rows of 4096 bf16: 18 us, 7.3 TB/s (some of it from L2); their gradient for 131072 classes, 1.07 GB of zeros and sums: 206 us, 5.5 TB/s,
+// of which some 25 go by before the first zeros, until all classes are counted. 3500 x 2048 of 50021 classes: 61 us, 3.6 TB/s. 515 x 777 f32 of 10007: 18 us.
 #include "elements.cuh"
 #include "train_common.cuh"
 
@@ -37,7 +38,8 @@ __device__ __forceinline__ int class_at(const Ids& ids, int64_t i) {
     return id >= 0 && id < ids.v ? int(id) : BAD;
 }
 
-// COLS loads of VEC elements, 32 lanes side by side, are a part of a row: one warp's work.
+// COLS loads of VEC elements, 32 lanes side by side, are a part of a row: one warp's work. Where nothing changes, the bits are stored as they came (8192 x 4096 bf16: 25 us
+// by way of f32, 18 so).
 template <class T, class O, int VEC, int COLS>
 __global__ void __launch_bounds__(THREADS) rows_kernel(const T* table, Ids ids, O* out, int64_t n, int64_t d, int shift, float scale, int* status) {
     after_previous();

@@ -9,7 +9,10 @@
 //   with A = O + diag(d):  A^2 = O O + (d_i + d_j) O_ij + diag(d_i^2),  B X = (B - diag(e)) X + diag(e) X
 // Against 64 bits the result, before its own rounding to bf16 (1.66e-3), is off by 2e-4 to 1e-3; without the diagonals' part a random matrix by 2.7e-3, without the
 // second f16 of X one with falling values by 6e-3 to 3e-2.
-// What bounds it: the tensor cores; with few rows, three dependent launches a step.
+// What bounds it: the tensor cores, where there are many tiles: 4096 x 14336, five steps of k^2 l + k^3 + 2 k^2 l (k <= l) operations: 3.2 ms from idle, 1.24 PFLOP/s, three
+// quarters of what a library's product reaches; under the power limit 3.7 ms, 1.06 of 1.40. The tensor cores have work for 0.94 of a tile's time; the rest are
+// last rounds of tiles (136 of A and 896 of X over 74 pairs of SMs). Medium sizes: loads from L2, 64 bytes a cycle for each SM (how, below), and the start and end of three dependent launches
+// a step, 7 us or more each: 703 x 255 in 125 us, 3 of 1024 x 2816 in 300.
 #include <math.h>
 
 #include <cuda_fp16.h>
@@ -576,7 +579,8 @@ __global__ void __launch_bounds__(PREPARE) prepare_kernel(const __grid_constant_
 // ---- small matrices --------------------------------------------------------------------------------------------------------------
 // All steps of a matrix with up to 128 rows and 256 columns (or turned: 256 and 128) in one CTA: X as f32 in tensor memory and as f16 in shared memory, 64 columns to a
 // 128-byte row, which serves as the operand of X X^T and as the right one of B X; A, then B, as f16 in another such matrix. Eight warps: 32 rows, one to a lane, and half of
-// the columns each. A step of [128, 128] takes 4.5 us: its three products 900 cycles each (issued by one thread), the rest what is between them.
+// the columns each. A step of [128, 128] takes 5 us: its three products 900 cycles each (issued by one thread), the rest what is between them. 64 matrices: 31 us (141 by launches of
+// their own for each product, from which matrices that do not fit here are taken).
 constexpr int SMALL_K = 128, SMALL_L = 256, SMALL_THREADS = 256, CHUNK64 = 128 * 128;  // bytes of 128 rows of 64 columns
 constexpr int MOST_STEPS = 64;
 struct Factors {
@@ -910,9 +914,9 @@ int launch_product(const Maps& maps, Args g, const DeviceInfo& dev, cudaStream_t
     const int64_t most = dev.sm_count / SMS;
     return launch_after(kern, unsigned(SMS * (tiles < most ? tiles : most)), THREADS, Shape<KIND>::SMEM, s, maps, g);
 }
-// How a product runs: a tile on pairs of SMs or on single ones, and over how many tiles the k-blocks of one are dealt out; whichever ends first, in cycles. A
-// k-block takes 540 cycles on either, the single ones' 128 x 128 as the 64 bytes a cycle that an SM gets from the L2 cache carry its operands no faster (measured 500, pairs 542);
-// a tile's ends some 6000; adding up partial results another launch of 12000 and their bytes.
+// How a product runs: a tile on pairs of SMs or on single ones, and over how many tiles the k-blocks of one are dealt out; whichever ends first, in cycles. Measured: a
+// k-block takes 540 cycles on a pair (256 x 256, of which the tensor cores need 512) and 500 on a single SM, whose 128 x 128 would be done in 256, had the 64 bytes a cycle that an SM gets
+// from the L2 cache not to carry its operands; what a tile has at its ends some 6000; adding up partial results another launch of 12000 and their bytes.
 struct How {
     int sms, splits, per, asked;
     double time;
@@ -957,7 +961,7 @@ int prepare(const Desc& d, const Plan& p, int64_t first, int64_t count, cudaStre
     return launch_after(prepare_kernel<T, 1>, rows, PREPARE, 0, s, all, int(d.m), int(d.n), int(p.pitch_x), static_cast<const double*>(p.sums), d.eps, p.x[0][0], p.x[0][1]);
 }
 
-// Matrices that a CTA takes whole: 64 of [128, 128] in 30 us, with three launches a step 141.
+// Matrices that a CTA takes whole.
 bool small(const Desc& d) { return (d.m < d.n ? d.m : d.n) <= SMALL_K && (d.m < d.n ? d.n : d.m) <= SMALL_L; }
 template <class T, bool TALL>
 int small_launch(const Matrices& all, const SmallArgs& g, int64_t count, const DeviceInfo& dev, cudaStream_t s) {

@@ -6,7 +6,9 @@
 // e h and s r_out, and D = (dr_out + s t) - k r_out^,  k = s mean(t r_out^),  the second mean is mean(q h^ (dr_out + s t)) - k mean(q h^ r_out^). r_out is
 // computed over again from r and h, the same bytes as reading it, so that a stream kept in bf16 is not rounded on the way into the gradients.
 // Gradients over rows are summed by each block over its rows, in registers, and over the blocks by a second launch.
-// What bounds it: the bytes.
+// What bounds it: the bytes, 8 of each value forward and 12 backward (bf16). 8192 x 4096 bf16, both norms and a gate: forward 55 us, 4.9 TB/s; backward 84 and the join of
+// sums 7, 4.8 TB/s. One block's registers fill an SM, so that two teams of 256 threads there wait for their sums with little beside them to do: 3300 cycles a row
+// and team forward, 600 of them with an instruction to issue. Rows held in registers, without a ring: 254 us for both passes.
 #include "attn_common.cuh"
 #include "elements.cuh"
 #include "train_common.cuh"
@@ -228,7 +230,8 @@ __global__ void __launch_bounds__(MAXT, 1) backward_kernel(const __grid_constant
 }
 
 // ---- the same with rows on their way in shared memory --------------------------------------------------------------------------------
-// Each thread copies the columns that are its own, some rows ahead, into places of its own (cp.async), so that what is on its way takes no registers and no barrier.
+// What a thread needs of the next rows is asked for up to six rows ahead: at the bytes that an SM gets, some 50 KiB have to be on their way for each, and 200 can be.
+// Each thread copies the columns that are its own, into places of its own (cp.async), so that what is on its way takes no registers and no barrier.
 // Columns are taken in chunks of eight that start on 16-byte boundaries: of a row that begins `lead` elements past one, the first chunk has the end of the row
 // before it and the last one the beginning of the next, which are left out when values are read. With 8 / gcd(d, 8) classes of rows, a row's number modulo that count
 // decides its lead: a team's rows are all of one class, so that its columns are the same in every row.
@@ -743,7 +746,8 @@ __global__ void __launch_bounds__(THREADS, 1) backward_ring_kernel(const __grid_
     }
 }
 
-// out[group, c] = factor[c] times the sum of `count` rows of partial sums, into up to two results; 32 columns a block, a run of the rows for each warp
+// out[group, c] = factor[c] times the sum of `count` rows of partial sums, into up to two results; 32 columns a block, every 16th row a warp, 16 of them on their way.
+// Bound by the latency of two such reads and a launch: 4.8 MB in 7 us.
 struct Result {
     void* out;
     int bf16, times;  // times: by `by` and the factors
@@ -846,7 +850,7 @@ Plan plan(const Desc& d, bool backward, bool aligned, Space& space, int sm_count
     int classes       = 8;
     while (classes > 1 && d.d % (16 / classes) == 0) classes /= 2;
     // A team's threads hold eight columns each, sixteen where those are too many threads for one team, or (forward, whose columns cost less than what each
-    // row costs a thread) for two on an SM.
+    // row costs a thread) for two on an SM. Longer rows and tensors that do not start on 16 bytes stay in registers: 8192 x 4096 in 2.4 times the time.
     const int64_t chunks = (d.d + (classes > 1 ? 7 : 0) + 7) / 8;
     p.columns            = chunks <= (backward ? 512 : 256) ? 1 : 2;
     const int64_t team = up((chunks + p.columns - 1) / p.columns, 32), in_block = team <= THREADS ? THREADS / team : 0;
