@@ -7,7 +7,7 @@
 // classes of more rows are taken by whole blocks, a run of the rows for each warp, joined in shared memory. All of it is one launch whose blocks meet between
 // its phases (and one that clears the counts). Up to 2048 positions: a launch of blocks that each look through all of them for the classes that are their own.
 // What bounds it: the bytes. 8192 rows of 4096 bf16: 18 us, 7.3 TB/s (some of it from L2); their gradient for 131072 classes, 1.07 GB of zeros and sums: 206 us, 5.5 TB/s,
-// of which some 25 go by before the first zeros, until all classes are counted. 3500 x 2048 of 50021 classes: 61 us, 3.6 TB/s. 515 x 777 f32 of 10007: 18 us.
+// of which some 25 go by before the first zeros, until all classes are counted. 3001 x 2048 of 50021 classes, 217 MB: 61 us. 515 x 777 f32 of 10007: 18 us.
 #include "elements.cuh"
 #include "train_common.cuh"
 

@@ -2,10 +2,10 @@
 //   u = e h post_gamma,  r_out = a r + b gate u,  x = s r_out gamma         e = 1 / sqrt(mean h^2 + eps),  s = 1 / sqrt(mean r_out^2 + eps)
 //   t = dx gamma,  D = dr_out + s t - s^3 r_out mean(t r_out):  dr = a D,  dgamma = sum dx s r_out,  dgate = sum b u D
 //   q = b gate post_gamma:  dpost_gamma = sum b gate e h D,  dh = e q D - e^3 h mean(q h D)
-// A row belongs to a team of threads, a warp or a block, and stays in their registers. The backward pass has one join of sums for a row: with hats for
+// A row belongs to a team of threads, a warp or a block, and stays in their registers, or is read twice (long rows backward). The backward pass has one join of sums for a row: with hats for
 // e h and s r_out, and D = (dr_out + s t) - k r_out^,  k = s mean(t r_out^),  the second mean is mean(q h^ (dr_out + s t)) - k mean(q h^ r_out^). r_out is
 // computed over again from r and h, the same bytes as reading it, so that a stream kept in bf16 is not rounded on the way into the gradients.
-// Gradients over rows are summed by each block over its rows, in registers, and over the blocks by a second launch.
+// Gradients over rows are summed by each team over its rows and over the teams by a second launch.
 // What bounds it: the bytes, 8 of each value forward and 12 backward (bf16). 8192 x 4096 bf16, both norms and a gate: forward 55 us, 4.9 TB/s; backward 84 and the join of
 // sums 7, 4.8 TB/s. One block's registers fill an SM, so that two teams of 256 threads there wait for their sums with little beside them to do: 3300 cycles a row
 // and team forward, 600 of them with an instruction to issue. Rows held in registers, without a ring: 254 us for both passes.
@@ -51,8 +51,9 @@ struct Args {
     const HT* dx;
     RT* dr;
     HT* dh;
-    // sums over rows: one row of d for each block, or (gate) for each unit of rows; a unit that is a whole group of the gate's writes dgate
-    float *part_gamma, *part_post, *part_gate;
+    // sums over rows: one row of d for each team, or (gate) for each unit of rows; a unit that is a whole group of the gate's writes dgate
+    float *part_gamma, *part_post, *part_gate, *part_z;
+    int shared;  // (backward_kernel) sums for each column are kept in shared memory
     void* dgate;
     int64_t groups, pieces;
     float eps, a, b;
@@ -142,91 +143,113 @@ __global__ void __launch_bounds__(MAXT, 1) forward_kernel(const __grid_constant_
     }
 }
 
-template <class RT, class HT, int VEC, int CH, int MAXT>
-__global__ void __launch_bounds__(MAXT, 1) backward_kernel(const __grid_constant__ Args<RT, HT> g) {
+// A block for each row, which is read twice, the second time from the caches: what is kept from row to row, sums for each column, takes shared memory or, of longer rows, the block's
+// rows of partial sums themselves, and no thread touches another's columns. (4096 x 16384 bf16: 285 us, 2.8 TB/s; with a row and the
+// sums in registers, 32 columns a thread, which spilled, 957.)
+constexpr int THREADS = 512;  // of a block: one team of all of them, or several
+template <class RT, class HT, int VEC>
+__global__ void __launch_bounds__(THREADS, 1) backward_kernel(const __grid_constant__ Args<RT, HT> g) {
+    extern __shared__ __align__(16) float room[];
     after_previous();
-    const float per   = 1.f / float(g.d);
-    const int64_t team = int64_t(blockIdx.x) * blockDim.y + threadIdx.y, teams = int64_t(gridDim.x) * blockDim.y;
-    float dgamma[CH][VEC] = {}, dpost[CH][VEC] = {};
-    for (int64_t unit = team; unit < g.groups * g.pieces; unit += teams) {
+    const int d = int(g.d), array = (d + 3) & ~3, t = threadIdx.x * VEC, step = blockDim.x * VEC;
+    const float per       = 1.f / float(d);
+    const bool several    = g.groups > 1;
+    const int64_t own     = int64_t(blockIdx.x) * d;
+    float* const dgamma   = g.shared ? room : g.part_gamma + own;
+    float* const z        = g.shared ? room + array : (several ? g.part_z : g.part_post) + own;  // sum D h^: of the unit's rows, or of all
+    float* const dpost    = g.shared ? room + 2 * array : g.part_post + own;
+    const bool with_gamma = g.part_gamma != nullptr, with_z = g.post_gamma.p || g.gate.p, with_post = several && g.part_post != nullptr;
+    const auto columns    = [&](auto&& f) {
+        for (int at = t; at < d; at += step) f(at);
+    };
+    const auto add = [](float* to, const float (&v)[VEC]) {
+        Run<float, VEC> run;
+        float old[VEC];
+        run.load(to), run.get(old);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) old[j] += v[j];
+        put(to, old);
+    };
+    const float nothing[VEC] = {};
+    columns([&](int at) {
+        if (with_gamma) put(dgamma + at, nothing);
+        if (with_z) put(z + at, nothing);
+        if (with_post) put(dpost + at, nothing);
+    });
+    for (int64_t unit = blockIdx.x; unit < g.groups * g.pieces; unit += gridDim.x) {
         const int64_t group = unit / g.pieces, piece = unit - group * g.pieces, end = min(g.n, (group + 1) * g.gate_rows);
-        float dgate[CH][VEC] = {};
         for (int64_t row = group * g.gate_rows + piece; row < end; row += g.pieces) {
-            Run<RT, VEC> rr[CH], drr[CH];
-            Run<HT, VEC> hr[CH], dxr[CH];
-#pragma unroll
-            for (int c = 0; c < CH; ++c) {
-                const int64_t at = (c * int(blockDim.x) + int(threadIdx.x)) * VEC, p = row * g.d + at;
-                rr[c].clear(), drr[c].clear(), hr[c].clear(), dxr[c].clear();
-                if (at < g.d) {
-                    rr[c].load(g.r + p);
-                    if (g.h) hr[c].load(g.h + p);
-                    if (g.dr_out) drr[c].load(g.dr_out + p);
-                    if (g.dx) dxr[c].load(g.dx + p);
-                }
-            }
             const float e = g.post_gamma.p ? g.kept[row] : 1.f, s = g.gamma.p ? g.kept[g.n + row] : 1.f;
-            float sum[3] = {};
-            float hat[CH][VEC], rhat[CH][VEC], before[CH][VEC], q[CH][VEC];  // h^, r_out^, dr_out + s t, q
-#pragma unroll
-            for (int c = 0; c < CH; ++c) {
-                const int64_t at = (c * int(blockDim.x) + int(threadIdx.x)) * VEC;
-                float w[VEC], gate[VEC], dx[VEC];
-                rr[c].get(rhat[c]), hr[c].get(hat[c]), drr[c].get(before[c]), dxr[c].get(dx);
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) w[j] = gate[j] = q[c][j] = 0.f;
-                if (at < g.d) factors_at(g.gamma, at, w), factors_at(g.post_gamma, at, q[c]), factors_at(g.gate, group * g.d + at, gate);
+            // h^, r_out^, dr_out + s t, q, t and dx of a thread's columns
+            float hat[VEC], rhat[VEC], before[VEC], q[VEC], w[VEC], dx[VEC];
+            const auto read = [&](int at) {
+                const int64_t p = row * g.d + at;
+                Run<RT, VEC> rr, drr;
+                Run<HT, VEC> hr, dxr;
+                hr.clear(), drr.clear(), dxr.clear(), rr.load(g.r + p);
+                if (g.h) hr.load(g.h + p);
+                if (g.dr_out) drr.load(g.dr_out + p);
+                if (g.dx) dxr.load(g.dx + p);
+                float gate[VEC];
+                factors_at(g.gamma, at, w), factors_at(g.post_gamma, at, q), factors_at(g.gate, group * g.d + at, gate);
+                rr.get(rhat), hr.get(hat), drr.get(before), dxr.get(dx);
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) {
-                    q[c][j] *= g.b * gate[j];
-                    hat[c][j] *= e;
-                    rhat[c][j] = g.h ? s * fmaf(g.a, rhat[c][j], q[c][j] * hat[c][j]) : s * rhat[c][j];
-                    const float t = dx[j] * w[j];
-                    before[c][j] = fmaf(s, t, before[c][j]);
-                    dgamma[c][j] = fmaf(dx[j], rhat[c][j], dgamma[c][j]);
-                    const float qh = q[c][j] * hat[c][j];
-                    sum[0] = fmaf(t, rhat[c][j], sum[0]), sum[1] = fmaf(qh, before[c][j], sum[1]), sum[2] = fmaf(qh, rhat[c][j], sum[2]);
+                    q[j] *= g.b * gate[j], hat[j] *= e, w[j] *= dx[j];
+                    rhat[j]   = g.h ? s * fmaf(g.a, rhat[j], q[j] * hat[j]) : s * rhat[j];
+                    before[j] = fmaf(s, w[j], before[j]);
                 }
-            }
+            };
+            float sum[3] = {};
+            columns([&](int at) {
+                read(at);
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) {
+                    const float qh = q[j] * hat[j];
+                    sum[0] = fmaf(w[j], rhat[j], sum[0]), sum[1] = fmaf(qh, before[j], sum[1]), sum[2] = fmaf(qh, rhat[j], sum[2]);
+                    dx[j] *= rhat[j];
+                }
+                if (with_gamma) add(dgamma + at, dx);
+            });
             team_sum(sum);
             const float k = g.gamma.p ? s * sum[0] * per : 0.f, m = g.post_gamma.p ? (sum[1] - k * sum[2]) * per : 0.f;
-#pragma unroll
-            for (int c = 0; c < CH; ++c) {
-                const int64_t at = (c * int(blockDim.x) + int(threadIdx.x)) * VEC, p = row * g.d + at;
-                if (at >= g.d) break;
-                float f[VEC], gate[VEC], out[VEC];
-                factors_at(g.post_gamma, at, f), factors_at(g.gate, group * g.d + at, gate);
+            columns([&](int at) {
+                read(at);
+                float out[VEC];
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) {
-                    const float D = fmaf(-k, rhat[c][j], before[c][j]);
+                    const float D = fmaf(-k, rhat[j], before[j]);
                     out[j] = g.a * D;
-                    const float bD = g.b * D;
-                    dpost[c][j] = fmaf(gate[j] * bD, hat[c][j], dpost[c][j]);
-                    dgate[c][j] = fmaf(f[j] * bD, hat[c][j], dgate[c][j]);
-                    q[c][j] = e * fmaf(q[c][j], D, -hat[c][j] * m);
+                    q[j]   = e * fmaf(q[j], D, -hat[j] * m);
+                    hat[j] *= D;
                 }
-                if (g.dr) put(g.dr + p, out);
-                if (g.dh) put(g.dh + p, q[c]);
-            }
+                put(g.dr + row * g.d + at, out);
+                if (g.dh) put(g.dh + row * g.d + at, q);
+                if (with_z) add(z + at, hat);
+            });
         }
-        if (g.gate.p) {
+        if (several && with_z) {
+            columns([&](int at) {
+                Run<float, VEC> run;
+                float sums[VEC], f[VEC], gate[VEC];
+                run.load(z + at), run.get(sums), put(z + at, nothing);
+                factors_at(g.post_gamma, at, f), factors_at(g.gate, group * g.d + at, gate);
 #pragma unroll
-            for (int c = 0; c < CH; ++c) {
-                const int64_t at = (c * int(blockDim.x) + int(threadIdx.x)) * VEC;
-                if (at >= g.d) break;
-                if (g.pieces > 1) put(g.part_gate + unit * g.d + at, dgate[c]);
-                else if (g.gate.bf16) put(static_cast<__nv_bfloat16*>(g.dgate) + group * g.d + at, dgate[c]);
-                else put(static_cast<float*>(g.dgate) + group * g.d + at, dgate[c]);
-            }
+                for (int j = 0; j < VEC; ++j) gate[j] *= g.b * sums[j], f[j] *= g.b * sums[j];
+                if (with_post) add(dpost + at, gate);
+                if (g.pieces > 1) put(g.part_gate + unit * g.d + at, f);
+                else if (g.gate.bf16) put(static_cast<__nv_bfloat16*>(g.dgate) + group * g.d + at, f);
+                else put(static_cast<float*>(g.dgate) + group * g.d + at, f);
+            });
         }
     }
-#pragma unroll
-    for (int c = 0; c < CH; ++c) {
-        const int64_t at = (c * int(blockDim.x) + int(threadIdx.x)) * VEC;
-        if (at >= g.d) break;
-        if (g.part_gamma) put(g.part_gamma + team * g.d + at, dgamma[c]);
-        if (g.part_post) put(g.part_post + team * g.d + at, dpost[c]);
-    }
+    if (!g.shared) return;
+    columns([&](int at) {
+        Run<float, VEC> run;
+        float v[VEC];
+        if (with_gamma) run.load(dgamma + at), run.get(v), put(g.part_gamma + own + at, v);
+        if (g.part_post) run.load((several ? dpost : z) + at), run.get(v), put(g.part_post + own + at, v);
+    });
 }
 
 // ---- the same with rows on their way in shared memory --------------------------------------------------------------------------------
@@ -256,7 +279,6 @@ __device__ __forceinline__ void leave16(uint32_t at, float a, float b, float c, 
     asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(at), "f"(a), "f"(b), "f"(c), "f"(d) : "memory");
 }
 
-constexpr int THREADS = 512;                // of a block: one team of all of them, or several
 constexpr uint32_t PLANE = THREADS * 16;    // 16 bytes for each
 constexpr int MOST_SMEM = 200 << 10;
 template <int ROW, int BLOCKS = 1>          // planes of a row; blocks that share an SM
@@ -840,7 +862,8 @@ struct Plan {
     Ring k;
     size_t smem;
     int64_t teams, groups, pieces;
-    float *gamma, *post, *gate;
+    float *gamma, *post, *gate, *z;
+    bool shared;
 };
 Plan plan(const Desc& d, bool backward, bool aligned, Space& space, int sm_count) {
     Plan p{};
@@ -850,7 +873,7 @@ Plan plan(const Desc& d, bool backward, bool aligned, Space& space, int sm_count
     int classes       = 8;
     while (classes > 1 && d.d % (16 / classes) == 0) classes /= 2;
     // A team's threads hold eight columns each, sixteen where those are too many threads for one team, or (forward, whose columns cost less than what each
-    // row costs a thread) for two on an SM. Longer rows and tensors that do not start on 16 bytes stay in registers: 8192 x 4096 in 2.4 times the time.
+    // row costs a thread) for two on an SM. Longer rows, and tensors that do not start on 16 bytes, go without a ring: 8192 x 4096 bf16, one value at a time, in 352 and 538 us.
     const int64_t chunks = (d.d + (classes > 1 ? 7 : 0) + 7) / 8;
     p.columns            = chunks <= (backward ? 512 : 256) ? 1 : 2;
     const int64_t team = up((chunks + p.columns - 1) / p.columns, 32), in_block = team <= THREADS ? THREADS / team : 0;
@@ -867,20 +890,27 @@ Plan plan(const Desc& d, bool backward, bool aligned, Space& space, int sm_count
         // (no more units than teams, as far as that goes: a team with two of them would be the last)
         p.pieces = p.groups ? p.teams / p.groups / classes * classes : classes;
         if (p.pieces < classes) p.pieces = classes;
+    } else if (backward) {
+        const int64_t lanes = up((d.d + 7) / (aligned && d.d % 8 == 0 ? 8 : 1), 32), bytes = (p.groups > 1 ? 3 : 2) * up(d.d, 4) * 4;
+        p.threads = int(lanes < THREADS ? lanes : THREADS), p.rows = 1;
+        p.shared  = bytes <= MOST_SMEM;
+        p.smem    = p.shared ? size_t(bytes) : 0;
+        const int64_t most = int64_t(sm_count) * (!p.shared ? 1 : bytes <= MOST_SMEM / 4 ? 4 : MOST_SMEM / bytes);
+        p.teams = p.blocks = int(d.n < most ? d.n : most);
+        p.pieces = p.groups ? (p.teams + p.groups - 1) / p.groups : 1;
     } else {
         const int64_t each = d.d <= 2048 ? 8 : d.d <= 8192 ? 16 : 32, lanes = up((d.d + each - 1) / each, 32);
         p.threads = int(lanes), p.rows = lanes == 32 ? 4 : 1;
         const int64_t most = int64_t(sm_count) * (lanes <= 128 ? 4 : lanes <= 256 ? 2 : 1), need = (d.n + p.rows - 1) / p.rows;
         p.blocks = int(need < most ? (need < 1 ? 1 : need) : most);
-        p.teams  = int64_t(p.blocks) * p.rows;
-        p.pieces = p.groups ? (p.teams + p.groups - 1) / p.groups : 1;
     }
     if (p.pieces > run) p.pieces = run;
     if (!backward) return p;
     auto part = [&](int64_t rows) { return static_cast<float*>(space.take(size_t(rows) * size_t(d.d) * 4)); };
     if (d.gamma) p.gamma = part(p.teams);
-    if (d.post_gamma || (d.gate && p.ring && p.groups == 1)) p.post = part(p.teams);
-    if (d.gate && p.pieces > 1 && !(p.ring && p.groups == 1)) p.gate = part(p.groups * p.pieces);
+    if (d.post_gamma || (d.gate && p.groups == 1)) p.post = part(p.teams);
+    if (d.gate && p.pieces > 1 && p.groups > 1) p.gate = part(p.groups * p.pieces);
+    if (!p.ring && !p.shared && p.groups > 1) p.z = part(p.teams);
     return p;
 }
 
@@ -939,19 +969,23 @@ int forward(const Desc& d, const Plan& p, const DeviceInfo& dev, cudaStream_t s)
 template <class RT, class HT, int VEC>
 int backward(const Desc& d, const Plan& p, const DeviceInfo& dev, cudaStream_t s) {
     Args<RT, HT> g = args_of<RT, HT>(d);
-    g.part_gamma = p.gamma, g.part_post = p.post, g.part_gate = p.gate, g.groups = p.groups, g.pieces = p.pieces;
+    g.part_gamma = p.gamma, g.part_post = p.post, g.part_gate = p.gate, g.part_z = p.z, g.shared = p.shared, g.groups = p.groups, g.pieces = p.pieces;
     const bool several = p.groups > 1;
     if (p.ring) {
         MIMK_TRY(with_columns(p, [&](auto columns, auto ragged, auto several) { return launch_ring<backward_ring_kernel<RT, HT, columns.value, ragged.value, several.value>>(p, g, dev, s); }));
     } else {
-        const auto kern = d.d <= 2048 ? backward_kernel<RT, HT, VEC, 8 / VEC, 256> : d.d <= 8192 ? backward_kernel<RT, HT, VEC, 16 / VEC, 512> : backward_kernel<RT, HT, VEC, 32 / VEC, 1024>;
-        MIMK_TRY(launch(kern, dim3(unsigned(p.blocks)), dim3(p.threads, p.rows), s, g));
+        static bool configured[64] = {};
+        if (!configured[dev.device & 63]) {
+            MIMK_CUDA_TRY(cudaFuncSetAttribute(backward_kernel<RT, HT, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize, MOST_SMEM));
+            configured[dev.device & 63] = true;
+        }
+        MIMK_TRY(launch_after(backward_kernel<RT, HT, VEC>, unsigned(p.blocks), unsigned(p.threads), p.smem, s, g));
     }
     Joins all{};
     int count    = 0;
     int64_t most = 1;
     if (p.gamma) all.j[count++] = {p.gamma, 1, p.teams, p.teams, 0, {{d.dgamma, d.gamma_dtype == MIMK_BF16}}};
-    if (p.post && p.ring && !several) {
+    if (p.post && !several) {
         all.j[count++] = {p.post, 1, p.teams, p.teams, 0, {{d.post_gamma ? d.dpost_gamma : nullptr, d.post_gamma_dtype == MIMK_BF16, 1, g.b, g.gate}, {d.gate ? d.dgate : nullptr, d.gate_dtype == MIMK_BF16, 1, g.b, g.post_gamma}}};
     } else if (p.post) {
         all.j[count++] = {p.post, 1, p.teams, p.teams, 0, {{d.dpost_gamma, d.post_gamma_dtype == MIMK_BF16}}};

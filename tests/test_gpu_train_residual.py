@@ -148,6 +148,23 @@ def test_gates_of_runs_of_rows(lead, gate):
     check(*inputs((*lead, 264), F32, BF16, True, gate))
 
 
+@pytest.mark.parametrize("d,gate", list(itertools.product([8200, 8193, 17088, 30008], [None, 0, 1, 2])))
+def test_long_rows(d, gate):
+    """Rows that are read twice: sums for their columns in shared memory and outside, for all rows and for groups of them, more rows than blocks."""
+    for lead, types, post in (((2, 5), (F32, F32), True), ((3, 101), (BF16, BF16), gate != 1)):
+        check(*inputs((*lead, d), *types, post, gate), a=-0.5)
+
+
+@pytest.mark.parametrize("d,gate", list(itertools.product([8, 100, 1024, 4099], [None, 0, 1, 2])))
+def test_rows_that_begin_elsewhere(d, gate):
+    """Tensors that do not start on 16 bytes, by every kind of gate."""
+    p, dr, dx = inputs((3, 301, d), BF16, BF16, True, gate)
+
+    def moved(t):
+        return None if t is None else torch.empty(t.numel() + 1, dtype=t.dtype, device="cuda")[1:].view(t.shape).copy_(t)
+    check({k: moved(t) for k, t in p.items()}, moved(dr), moved(dx), b=0.5)
+
+
 @pytest.mark.parametrize("weights", [F32, BF16])
 def test_weights_of_either_type(weights):
     check(*inputs((70, 512), F32, BF16, True, 0, weights=weights))
