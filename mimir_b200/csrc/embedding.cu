@@ -247,12 +247,13 @@ __device__ __forceinline__ void sort_shared(int* held, int size, int t, int thre
             meet();
         }
 }
-// The groups of heavy classes put in order. Up to WARP_SORTED positions: by a warp, in its part of the room. More: by a block, as bits of a map that are read off in order; where there
+// The groups of heavy classes put in order. Where there are more of them than blocks, those of up to WARP_SORTED positions by a warp, in its part of the room. Others by a block, as bits of a map that are read off in order; where there
 // are more positions than one map's, groups of up to SORTED in the map's place, and groups of more than a map's positions as the ids name them, which are fewer than the
 // group over again for each map. (1048576 positions in 26214 classes, 64 columns of bf16: 704 us; 3531 with maps alone, 1099 with all sorted by blocks.)
 __device__ __forceinline__ void sort_heavies(const Ids& ids, const Groups& g, int64_t n, uint32_t* bits) {
     const int heavies = g.cursor[1], warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    for (int h = blockIdx.x + warp * gridDim.x; h < heavies; h += gridDim.x * (WORKERS / 32)) {
+    const bool many   = heavies > int(gridDim.x);
+    for (int h = blockIdx.x + warp * gridDim.x; many && h < heavies; h += gridDim.x * (WORKERS / 32)) {
         const int c = g.heavy[h].x, count = g.count[c], start = g.start[c];
         if (g.heavy[h].y || count > WARP_SORTED) continue;
         int* held = reinterpret_cast<int*>(bits) + warp * WARP_SORTED;
@@ -264,13 +265,14 @@ __device__ __forceinline__ void sort_heavies(const Ids& ids, const Groups& g, in
         for (int k = lane; k < count; k += 32) g.sorted[start + k] = held[k];
         __syncwarp();
     }
-    workers_meet<WORKERS>();
+    if (many) workers_meet<WORKERS>();
     for (int h = blockIdx.x; h < heavies; h += gridDim.x) {
+        if (g.heavy[h].y) continue;
         const int c = g.heavy[h].x, count = g.count[c], start = g.start[c];
-        if (g.heavy[h].y || count <= WARP_SORTED) continue;
+        if (many && count <= WARP_SORTED) continue;
         if (n > WINDOW && count <= SORTED) {
             int* held = reinterpret_cast<int*>(bits);
-            int size  = WARP_SORTED;
+            int size  = 2 * LIGHT;
             while (size < count) size *= 2;
             for (int k = threadIdx.x; k < size; k += WORKERS) held[k] = k < count ? g.order[start + k] : INT_MAX;
             workers_meet<WORKERS>();
