@@ -324,7 +324,7 @@ template <>
 struct Walk<false> {
     int64_t offset, d;  // of the row's first element
     int row, n, teams;
-    static constexpr int unit = 0, group = 0;
+    static constexpr int group = 0;
     template <class A>
     __device__ __forceinline__ Walk(const A& g, const Ring& k, int team)
         : offset((int64_t(team) - k.teams) * g.d), d(int64_t(k.teams) * g.d), row(team - k.teams), n(int(g.n)), teams(k.teams) {}

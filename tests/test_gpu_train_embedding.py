@@ -265,6 +265,27 @@ def test_same_bits_again_on_another_stream_and_in_a_graph():
     assert all(torch.equal(g, w) for g, w in zip(got, want))
 
 
+def test_calls_on_several_streams_at_once():
+    """Launches whose blocks meet, beside one another and beside products that fill the GPU."""
+    from mimir_b200 import tensor as T
+    cases = [(randn((n, 512), n, 1.0, BF16), ids_of((n,), v, n), v) for n, v in ((5000, 20011), (8192, 300), (2500, 50021), (1000, 4000))]
+    want = [T.embedding_grad(dy, ids, v) for dy, ids, v in cases]
+    a = randn((4096, 4096), 1, 1.0, BF16)
+    product = T.product_2d(a, a)
+    streams = [torch.cuda.Stream() for _ in range(len(cases) + 1)]
+    torch.cuda.synchronize()
+    got = [[] for _ in cases]
+    for _ in range(6):
+        with torch.cuda.stream(streams[-1]):
+            same = T.product_2d(a, a)
+        for stream, out, (dy, ids, v) in zip(streams, got, cases):
+            with torch.cuda.stream(stream):
+                out.append(T.embedding_grad(dy, ids, v))
+    torch.cuda.synchronize()
+    T.device_status()
+    assert torch.equal(same, product) and all(torch.equal(g, w) for out, w in zip(got, want) for g in out)
+
+
 def test_gradient_against_differences():
     """<out, dy> along a step of the table: the forward pass is linear, so the quotient is the product with the gradient but for the roundings of both."""
     from mimir_b200 import tensor as T

@@ -217,6 +217,23 @@ def test_same_bits_again_on_another_stream_and_in_a_graph():
     assert all(torch.equal(g, w) for g, w in zip(got, want))
 
 
+def test_calls_on_several_streams_at_once():
+    """Pairs of SMs and tensor memory asked for by several launches."""
+    from mimir_b200 import tensor as T
+    cases = [randn(shape, 40, 1.0, dtype) for shape, dtype in (((600, 900), F32), ((96, 64, 128), BF16), ((1500, 1100), BF16), ((40, 5000), F32))]
+    want = [T.orthogonalize(x) for x in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    got = [[] for _ in cases]
+    for _ in range(5):
+        for stream, out, x in zip(streams, got, cases):
+            with torch.cuda.stream(stream):
+                out.append(T.orthogonalize(x))
+    torch.cuda.synchronize()
+    T.device_status()
+    assert all(torch.equal(g, w) for out, w in zip(got, want) for g in out)
+
+
 def test_refusals():
     import ctypes as C
 
