@@ -879,6 +879,9 @@ Plan plan(const Desc& d, bool backward, bool aligned, Space& space, int sm_count
     const int64_t team = up((chunks + p.columns - 1) / p.columns, 32), in_block = team <= THREADS ? THREADS / team : 0;
     const int64_t row  = p.columns * int64_t(PLANE) * int64_t(pair) / 2 * (backward ? 2 : 1);
     p.ring             = aligned && in_block > 0 && row <= MOST_SMEM;
+    // Sixteen columns and their sums are more than a thread's registers backward: whole rows are read twice instead where a gate has groups or the stream is F32 (4096 x 8192,
+    // one group and four: bf16 155 and 185 us, by a ring 155 and 290; F32 stream 210 and 216, by a ring 240 and 392).
+    if (backward && p.columns == 2 && classes == 1 && (p.groups > 1 || d.stream_dtype == MIMK_F32)) p.ring = false;
     if (p.ring) {
         p.k.team = int(team), p.k.classes = classes;
         const int64_t share = !backward && p.columns == 1 && p.groups == 1 ? 2 : 1, stages = MOST_SMEM / share / row;  // blocks to an SM
@@ -972,7 +975,10 @@ int backward(const Desc& d, const Plan& p, const DeviceInfo& dev, cudaStream_t s
     g.part_gamma = p.gamma, g.part_post = p.post, g.part_gate = p.gate, g.part_z = p.z, g.shared = p.shared, g.groups = p.groups, g.pieces = p.pieces;
     const bool several = p.groups > 1;
     if (p.ring) {
-        MIMK_TRY(with_columns(p, [&](auto columns, auto ragged, auto several) { return launch_ring<backward_ring_kernel<RT, HT, columns.value, ragged.value, several.value>>(p, g, dev, s); }));
+        MIMK_TRY(with_columns(p, [&](auto columns, auto ragged, auto several) {
+            if constexpr (columns.value == 2 && !ragged.value && (several.value || sizeof(RT) == 4)) return int(MIMK_E_UNSUPPORTED);  // (planned without a ring)
+            else return launch_ring<backward_ring_kernel<RT, HT, columns.value, ragged.value, several.value>>(p, g, dev, s);
+        }));
     } else {
         static bool configured[64] = {};
         if (!configured[dev.device & 63]) {

@@ -148,7 +148,7 @@ def test_gates_of_runs_of_rows(lead, gate):
     check(*inputs((*lead, 264), F32, BF16, True, gate))
 
 
-@pytest.mark.parametrize("d,gate", list(itertools.product([8200, 8193, 17088, 30008], [None, 0, 1, 2])))
+@pytest.mark.parametrize("d,gate", list(itertools.product([4104, 5001, 8192, 8200, 8193, 17088, 30008], [None, 0, 1, 2])))
 def test_long_rows(d, gate):
     """Rows that are read twice: sums for their columns in shared memory and outside, for all rows and for groups of them, more rows than blocks."""
     for lead, types, post in (((2, 5), (F32, F32), True), ((3, 101), (BF16, BF16), gate != 1)):
