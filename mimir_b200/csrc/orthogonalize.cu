@@ -7,8 +7,12 @@
 // their largest possible value below 2^15; p X is added from an X of two f16 (22 bits), so that rounding one operand of B X does not enter X itself;
 // and the diagonals of A and B, near which the values of most matrices lie, are kept in f32 and out of the products:
 //   with A = O + diag(d):  A^2 = O O + (d_i + d_j) O_ij + diag(d_i^2),  B X = (B - diag(e)) X + diag(e) X
-// Against 64 bits the result, before its own rounding to bf16 (1.66e-3), is off by 2e-4 to 1e-3; without the diagonals' part a random matrix by 2.7e-3, without the
-// second f16 of X one with falling values by 6e-3 to 3e-2.
+// What the first f16 of X leaves out, L, must not enter the small directions, where it would grow with them: (B - diag(e)) L does, with -e where B has all but nothing (matrices of a few rows and
+// hardly any rank came out off by 4e-2, in eight steps by 0.9). Matrices that a CTA takes whole have L multiplied, too. For others diag(e) L is left out as long as singular values can
+// still grow by more than 4, so that B L stays in B's own large directions, and is added in the steps from there on, where singular values lie near one another and B near its diagonal.
+// Against 64 bits the result, before its own rounding to bf16 (1.66e-3), is off by 2e-4 to 1e-3 for random matrices and such with falling values, and by up to 2.5e-3 for any of some thousand
+// spectra and bases tried (nearly parallel rows, two or three levels, a few rows large). With diag(e) L left out of all steps: 1.4e-3 in place of 5e-4 (random, 64 x 256) and
+// 2.5e-3; in all but the last three: 4.6e-3; without the second f16 of X 6e-3 to 3e-2 for falling values.
 // What bounds it: the tensor cores, where there are many tiles: 4096 x 14336, five steps of k^2 l + k^3 + 2 k^2 l (k <= l) operations: 3.2 ms from idle, 1.24 PFLOP/s, three
 // quarters of what a library's product reaches; under the power limit 3.7 ms, 1.06 of 1.40. The tensor cores have work for 0.94 of a tile's time; the rest are
 // last rounds of tiles (136 of A and 896 of X over 74 pairs of SMs). Medium sizes: loads from L2, 64 bytes a cycle for each SM (how, below), and the start and end of three dependent launches
@@ -62,7 +66,7 @@ struct Args {
     const float* diag_in;  // SQUARE: d, APPLY: e
     float* diag_out;
     // GRAM: A = acc * f[0], times f[4] as f16. SQUARE: O O = acc * f[0], A = in * f[1], q = f[2], r = f[3], times f[4] as f16.
-    // APPLY: SX X' = (f[0] + e) SX X + acc * f[1]; the result times f[2]
+    // APPLY: SX X' = (f[0] + e) SX X + acc * f[1], of X's second f16 only f[3] e; the result times f[2]
     float f[5];
     int* status;
 };
@@ -390,8 +394,9 @@ __device__ __forceinline__ void product(const Maps& maps, const Args& g, const C
                         for (int j = 0; j < 4; ++j) {
                             const int k    = 8 * i + 2 * j;
                             const float2 a = unpack_f16(h[j]), b = unpack_f16(l[j]);
-                            const float x = fmaf(g.f[0] + (&ej[k >> 2].x)[k & 3], fmaf(b.x, 1.f / LOW, a.x), __uint_as_float(raw[k]) * g.f[1]);
-                            const float y = fmaf(g.f[0] + (&ej[k >> 2].x)[(k & 3) + 1], fmaf(b.y, 1.f / LOW, a.y), __uint_as_float(raw[k + 1]) * g.f[1]);
+                            const float e0 = (&ej[k >> 2].x)[k & 3], e1 = (&ej[k >> 2].x)[(k & 3) + 1];
+                            const float x = fmaf(g.f[0] + e0, a.x, fmaf(fmaf(g.f[3], e0, g.f[0]) * (1.f / LOW), b.x, __uint_as_float(raw[k]) * g.f[1]));
+                            const float y = fmaf(g.f[0] + e1, a.y, fmaf(fmaf(g.f[3], e1, g.f[0]) * (1.f / LOW), b.y, __uint_as_float(raw[k + 1]) * g.f[1]));
                             if (g.last) {
                                 h[j] = pack_bf16x2(x * g.f[2], y * g.f[2]);
                             } else {
@@ -577,14 +582,15 @@ __global__ void __launch_bounds__(PREPARE) prepare_kernel(const __grid_constant_
 }
 
 // ---- small matrices --------------------------------------------------------------------------------------------------------------
-// All steps of a matrix with up to 128 rows and 256 columns (or turned: 256 and 128) in one CTA: X as f32 in tensor memory and as f16 in shared memory, 64 columns to a
-// 128-byte row, which serves as the operand of X X^T and as the right one of B X; A, then B, as f16 in another such matrix. Eight warps: 32 rows, one to a lane, and half of
+// All steps of a matrix with up to 128 rows and 256 columns (or turned: 256 and 128) in one CTA: X as f32 in tensor memory and as two f16 in shared memory, 64 columns to a
+// 128-byte row, of which the first serves as the operand of X X^T and both as the right one of B X; A, then B, as f16 in another such matrix. Eight warps: 32 rows, one to a lane, and half of
 // the columns each. A step of [128, 128] takes 5 us: its three products 900 cycles each (issued by one thread), the rest what is between them. 64 matrices: 31 us (141 by launches of
 // their own for each product, from which matrices that do not fit here are taken).
 constexpr int SMALL_K = 128, SMALL_L = 256, SMALL_THREADS = 256, CHUNK64 = 128 * 128;  // bytes of 128 rows of 64 columns
 constexpr int MOST_STEPS = 64;
 struct Factors {
     float p, q, r, a, b;  // a step's coefficients, and the factors of A and B
+    float low;            // 1: diag(B) times X's second f16 is added, 0: not (matrices that a CTA does not take whole)
 };
 struct SmallArgs {
     int k, l, chunks, steps;  // rows and columns of X (turned where x is taller than wide), its chunks of 64 columns
@@ -615,6 +621,21 @@ __device__ __forceinline__ void put_tmem(uint32_t to, const float (&v)[32]) {
         tmem_st_32x32_x16(to + h, r);
     }
 }
+// 32 values of X's row as f16, and what that leaves out of them as another (as it is: X is SX times values up to 1, of 1 / 181 and more on the average, whose 12th to 23rd bits lie above 2^-24)
+__device__ __forceinline__ void put_x(uint32_t first, uint32_t second, int row, int column, const float (&v)[32]) {
+#pragma unroll
+    for (int i = 0; i < 32; i += 8) {
+        uint32_t h[4], l[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            h[j] = pack_f16(v[i + 2 * j], v[i + 2 * j + 1]);
+            const float2 r = unpack_f16(h[j]);
+            l[j] = pack_f16(v[i + 2 * j] - r.x, v[i + 2 * j + 1] - r.y);
+        }
+        st_shared(at64(first, row, column + i), h[0], h[1], h[2], h[3]);
+        st_shared(at64(second, row, column + i), l[0], l[1], l[2], l[3]);
+    }
+}
 // 32 values of a row as f16
 __device__ __forceinline__ void put_row(uint32_t base, int row, int column, const float (&v)[32], float by) {
 #pragma unroll
@@ -626,7 +647,7 @@ template <class T, bool TALL>
 __global__ void __launch_bounds__(SMALL_THREADS) small_kernel(const __grid_constant__ Matrices all, const __grid_constant__ SmallArgs g) {
     extern __shared__ uint8_t smem_raw[];
     __shared__ SmallShared sh;
-    const uint32_t raw = smem_u32(smem_raw), x16 = (raw + 1023u) & ~1023u, a16 = x16 + g.chunks * CHUNK64;
+    const uint32_t raw = smem_u32(smem_raw), x16 = (raw + 1023u) & ~1023u, a16 = x16 + g.chunks * CHUNK64, low16 = a16 + 2 * CHUNK64;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row = (warp & 3) * 32 + lane, half = warp >> 2;
     const int width = g.chunks * 64, columns = g.chunks > 2 ? 512 : 256;  // of tensor memory: X, and the products behind it
     if (threadIdx.x == 0) mbar_init(smem_u32(&sh.done), 1), sh.abort_flag = 0, fence_barrier_init();
@@ -687,7 +708,7 @@ __global__ void __launch_bounds__(SMALL_THREADS) small_kernel(const __grid_const
 #pragma unroll
         for (int i = 0; i < 32; ++i) v[i] = by.times(__uint_as_float(r[i]));
         put_tmem(tmem + c, v);
-        put_row(x16, row, c, v, 1.f);
+        put_x(x16, low16, row, c, v);
     }
     tmem_st_wait();
 
@@ -779,9 +800,11 @@ __global__ void __launch_bounds__(SMALL_THREADS) small_kernel(const __grid_const
         }
         // X
         multiply([&] {
-            for (int c = 0; c < kblocks; ++c)
-                for (int i = 0; i < 4; ++i)
-                    mma_f16_ss(mma_acc, high | (((a16 + c * CHUNK64 + i * 32) >> 4) | 1u << 16), high | (((x16 + (c * 64 + i * 16) * 128) >> 4) | uint32_t(CHUNK64 >> 4) << 16), wide, c > 0 || i > 0);
+            for (const uint32_t x : {x16, low16})
+                for (int c = 0; c < kblocks; ++c)
+                    for (int i = 0; i < 4; ++i)
+                        mma_f16_ss(mma_acc, high | (((a16 + c * CHUNK64 + i * 32) >> 4) | 1u << 16), high | (((x + (c * 64 + i * 16) * 128) >> 4) | uint32_t(CHUNK64 >> 4) << 16), wide,
+                                   x == low16 || c > 0 || i > 0);
         });
         const float plus = f.p + sh.e[row], back = 1.f / f.b;
         __nv_bfloat16* out = g.out + int64_t(blockIdx.x) * g.k * g.l;
@@ -796,7 +819,7 @@ __global__ void __launch_bounds__(SMALL_THREADS) small_kernel(const __grid_const
             for (int i = 0; i < 32; ++i) v[i] = fmaf(plus, __uint_as_float(was[i]), __uint_as_float(r[i]) * back);
             if (!last) {
                 put_tmem(tmem + c, v);
-                put_row(x16, row, c, v, 1.f);
+                put_x(x16, low16, row, c, v);
                 continue;
             }
 #pragma unroll
@@ -834,7 +857,7 @@ int factors_of(const Desc& d, Factors (&f)[MOST_STEPS]) {
         if (!(fabs(p) <= 1e4 && fabs(q) <= 1e4 && fabs(r) <= 1e4)) return MIMK_E_UNSUPPORTED;
         const double a = most * most, b = fabs(q) * a + fabs(r) * a * a;
         const auto power = [](double v) { return float(exp2(floor(log2(32768.0 / (v > 1.0 / 1024 ? v : 1.0 / 1024))))); };
-        f[s] = {float(p), float(q), float(r), power(a), power(b)};
+        f[s] = {float(p), float(q), float(r), power(a), power(b), 0.f};
         double next = 0;
         for (int i = 0; i <= 4096; ++i) {
             const double v = most * i / 4096, w = fabs(v * (p + v * v * (q + r * v * v)));
@@ -844,6 +867,9 @@ int factors_of(const Desc& d, Factors (&f)[MOST_STEPS]) {
         if (!(most <= 4)) return MIMK_E_UNSUPPORTED;
         if (most < 1e-3) most = 1e-3;
     }
+    // by how much small singular values grow in the steps that follow
+    double growth = 1;
+    for (int s = d.steps - 1; s >= 0; --s) f[s].low = growth <= 4 ? 1.f : 0.f, growth *= fabs(double(d.coefficients[3 * s]));
     return MIMK_OK;
 }
 
@@ -968,10 +994,10 @@ int small_launch(const Matrices& all, const SmallArgs& g, int64_t count, const D
     const auto kern = small_kernel<T, TALL>;
     static bool configured[64] = {};
     if (!configured[dev.device & 63]) {
-        MIMK_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (SMALL_L / 64 + 2) * CHUNK64 + 1024));
+        MIMK_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (2 * SMALL_L / 64 + 2) * CHUNK64 + 1024));
         configured[dev.device & 63] = true;
     }
-    return launch_after(kern, unsigned(count), SMALL_THREADS, size_t(g.chunks + 2) * CHUNK64 + 1024, s, all, g);
+    return launch_after(kern, unsigned(count), SMALL_THREADS, size_t(2 * g.chunks + 2) * CHUNK64 + 1024, s, all, g);
 }
 int small_all(const Desc& d, const Factors* f, const DeviceInfo& dev, cudaStream_t s) {
     static thread_local Matrices all;
@@ -1026,7 +1052,7 @@ int slice(const Desc& d, const Plan& p, const Factors* f, int64_t first, int64_t
         MIMK_TRY(launch<SQUARE>(maps, g, hows[1], dev, s));
         // X
         g.rows = int(d.m), g.cols = int(d.n), g.b_mn = !tall, g.tall = tall, g.last = step + 1 == d.steps, g.diag_in = p.e;
-        g.f[0] = c.p, g.f[1] = 1.f / c.b, g.f[2] = d.scale / SX;
+        g.f[0] = c.p, g.f[1] = 1.f / c.b, g.f[2] = d.scale / SX, g.f[3] = c.low;
         (tall ? maps.left : maps.right) = apply, (tall ? g.z_left : g.z_right) = 2 * now * z;
         (tall ? maps.right : maps.left) = a_b, (tall ? g.z_right : g.z_left) = z;
         maps.tile = tiles, g.z_hi = 2 * now * z, g.z_lo = g.z_hi + z;
