@@ -80,3 +80,15 @@ def test_more_and_other_steps(shape):
         check(x, T.orthogonalize(x, steps=8), (DEFAULT,) * 8, 3e-3 * DEFAULT[0] ** 3)
         check(x, T.orthogonalize(x, steps=25, coefficients=(1.5, -0.5, 0.0)), ((1.5, -0.5, 0.0),) * 25)
     T.device_status()
+
+
+def test_a_matrix_comes_out_the_same_where_a_stack_has_other_tiles():
+    """Alone, A's tiles are of single SMs; of many matrices they are of pairs."""
+    from mimir_b200 import tensor as T
+    g = torch.Generator(device="cuda").manual_seed(5)
+    for shape in ((16, 1024, 4096), (16, 4096, 1024), (40, 512, 2048), (30, 300, 5000)):
+        x = torch.randn(shape, generator=g, device="cuda", dtype=BF16)
+        got = T.orthogonalize(x)
+        for i in (0, shape[0] // 2, shape[0] - 1):
+            assert torch.equal(T.orthogonalize(x[i]), got[i]), (shape, i)
+    T.device_status()
