@@ -521,10 +521,10 @@ __global__ void __launch_bounds__(THREADS) few_kernel(const T* dy, Ids ids, O* d
     __shared__ int heavies;
     __shared__ float joined[WARPS][32 * VEC];
     after_previous();
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, groups = 1 << log_groups, own = (v - int(blockIdx.x) + groups - 1) >> log_groups;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, groups = 1 << log_groups, own = ((v - 1 - int(blockIdx.x)) >> log_groups) + 1;  // (no more groups than classes)
     const int64_t from = int64_t(blockIdx.y) * PART + lane * VEC;
     // (a window of the block's classes: all of them, unless there are more than 2048)
-    for (int window = 0; window < own; window += OWN) {
+    for (int window = 0;; window += OWN) {
         const int here = min(OWN, own - window);
         for (int i = threadIdx.x; i < here; i += THREADS) counts[i] = 0;
         if (threadIdx.x == 0) heavies = 0;
@@ -591,6 +591,7 @@ __global__ void __launch_bounds__(THREADS) few_kernel(const T* dy, Ids ids, O* d
             store_row<O, VEC, COLS>(acc, dtable + ((int64_t(window + local) << log_groups) + blockIdx.x) * d, d, from, positions ? scale : 0.f, add);
         }
         workers_meet<THREADS>();
+        if (own - window <= OWN) break;
     }
 }
 
