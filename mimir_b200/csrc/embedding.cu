@@ -131,14 +131,16 @@ struct Groups {
     int* sorted;  // [n] the same, groups of more than LIGHT positions in rising order
     int4* heavy;  // pieces of such groups: class, which piece, of how many, place of the partial sums where there are several
     int* light;   // [n] the other classes that occur
+    int* whole;   // the classes of such groups: those of up to WARP_SORTED positions from the front, others from the end
     float* part;  // rows of partial sums
-    int* cursor;  // places taken; pieces; blocks that have met; whether one gave up; the other classes; rows of partial sums
-    int64_t part_pitch;
+    int* cursor;  // places taken; pieces; blocks that have met; whether one gave up; the other classes; rows of partial sums; classes at the front and at the end of `whole`; of those put in order by blocks, how many are taken
+    int64_t part_pitch, wholes;
 };
+constexpr int CURSORS = 9;
 
 __global__ void __launch_bounds__(THREADS) clear_kernel(Groups g, int64_t v) {
     after_previous();
-    if (blockIdx.x == 0 && threadIdx.x < 6) g.cursor[threadIdx.x] = 0;
+    if (blockIdx.x == 0 && threadIdx.x < CURSORS) g.cursor[threadIdx.x] = 0;
     for (int64_t i = int64_t(blockIdx.x) * THREADS + threadIdx.x; i < v; i += int64_t(gridDim.x) * THREADS) g.count[i] = 0;
 }
 
@@ -207,23 +209,31 @@ __device__ __forceinline__ int block_before(int v, int* total) {
 }
 
 __device__ __forceinline__ void take_places(const Groups& g, int64_t v) {
-    __shared__ int first[4];
+    __shared__ int first[6];
     for (int64_t base = int64_t(blockIdx.x) * WORKERS; base < v; base += int64_t(gridDim.x) * WORKERS) {
         const int64_t c = base + threadIdx.x;
         const int count = c < v ? g.count[c] : 0;
         const int pieces = count > LIGHT ? (count + PIECE - 1) / PIECE : 0, parts = pieces > 1 ? pieces : 0;
-        int all, heavies, lights, partials;
+        int all, heavies, partials;
         const int before = block_before(count, &all);
         if (!all) continue;
-        const int nth = block_before(pieces, &heavies), other = block_before(count > 0 && !pieces, &lights), row = block_before(parts, &partials);
+        const int nth = block_before(pieces, &heavies), row = block_before(parts, &partials);
+        // light classes, those for a warp and those for a block: ten bits each
+        const bool light = count > 0 && !pieces, some = pieces && count <= WARP_SORTED, much = pieces && !some;
+        int kinds;
+        const int other = block_before(int(light) | int(some) << 10 | int(much) << 20, &kinds), lights = kinds & 1023, somes = kinds >> 10 & 1023, muches = kinds >> 20;
         if (threadIdx.x == 0) first[0] = atomicAdd(g.cursor, all);
         if (threadIdx.x == 32 && heavies) first[1] = atomicAdd(g.cursor + 1, heavies);
         if (threadIdx.x == 64 && lights) first[2] = atomicAdd(g.cursor + 4, lights);
         if (threadIdx.x == 96 && partials) first[3] = atomicAdd(g.cursor + 5, partials);
+        if (threadIdx.x == 128 && somes) first[4] = atomicAdd(g.cursor + 6, somes);
+        if (threadIdx.x == 160 && muches) first[5] = atomicAdd(g.cursor + 7, muches);
         workers_meet<WORKERS>();
         if (count) g.start[c] = first[0] + before;
         for (int k = 0; k < pieces; ++k) g.heavy[first[1] + nth + k] = make_int4(int(c), k, pieces, first[3] + row);
-        if (count && !pieces) g.light[first[2] + other] = int(c);
+        if (light) g.light[first[2] + (other & 1023)] = int(c);
+        if (some) g.whole[first[4] + (other >> 10 & 1023)] = int(c);
+        if (much) g.whole[g.wholes - 1 - first[5] - (other >> 20)] = int(c);
         workers_meet<WORKERS>();
     }
 }
@@ -249,13 +259,15 @@ __device__ __forceinline__ void sort_shared(int* held, int size, int t, int thre
 }
 // The groups of heavy classes put in order. Where there are more of them than blocks, those of up to WARP_SORTED positions by a warp, in its part of the room. Others by a block, as bits of a map that are read off in order; where there
 // are more positions than one map's, groups of up to SORTED in the map's place, and groups of more than a map's positions as the ids name them, which are fewer than the
-// group over again for each map. (1048576 positions in 26214 classes, 64 columns of bf16: 704 us; 3531 with maps alone, 1099 with all sorted by blocks.)
+// group over again for each map. (1048576 positions in 26214 classes, 64 columns of bf16: 681 us; 3531 with maps alone, 1099 with all sorted by blocks.)
+// A block that is done takes the next group that nobody has, so that blocks end within one group's time of each other, however the classes follow one another: a few cycles for each of
+// all positions at most, far below the limit of the meeting that follows. (22429696 positions in 148 classes: 19 ms; with a fixed share of the list of pieces one block had all of these, 2.1 s, and the others gave up.)
 __device__ __forceinline__ void sort_heavies(const Ids& ids, const Groups& g, int64_t n, uint32_t* bits) {
-    const int heavies = g.cursor[1], warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const bool many   = heavies > int(gridDim.x);
-    for (int h = blockIdx.x + warp * gridDim.x; many && h < heavies; h += gridDim.x * (WORKERS / 32)) {
-        const int c = g.heavy[h].x, count = g.count[c], start = g.start[c];
-        if (g.heavy[h].y || count > WARP_SORTED) continue;
+    __shared__ int taken;
+    const int some = g.cursor[6], much = g.cursor[7], warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const bool many = some + much > int(gridDim.x);
+    for (int h = blockIdx.x + warp * gridDim.x; many && h < some; h += gridDim.x * (WORKERS / 32)) {
+        const int c = g.whole[h], count = g.count[c], start = g.start[c];
         int* held = reinterpret_cast<int*>(bits) + warp * WARP_SORTED;
         int size  = 2 * LIGHT;
         while (size < count) size *= 2;
@@ -265,11 +277,17 @@ __device__ __forceinline__ void sort_heavies(const Ids& ids, const Groups& g, in
         for (int k = lane; k < count; k += 32) g.sorted[start + k] = held[k];
         __syncwarp();
     }
-    if (many) workers_meet<WORKERS>();
-    for (int h = blockIdx.x; h < heavies; h += gridDim.x) {
-        if (g.heavy[h].y) continue;
-        const int c = g.heavy[h].x, count = g.count[c], start = g.start[c];
-        if (many && count <= WARP_SORTED) continue;
+    const int groups   = much + (many ? 0 : some);
+    const auto advance = [&] {
+        workers_meet<WORKERS>();
+        if (threadIdx.x == 0) taken = groups > int(gridDim.x) ? int(gridDim.x) + atomicAdd(g.cursor + 8, 1) : groups;
+    };
+    if (threadIdx.x == 0) taken = blockIdx.x;
+    for (;; advance()) {
+        workers_meet<WORKERS>();
+        const int h = taken;
+        if (h >= groups) break;
+        const int c = h < much ? g.whole[g.wholes - 1 - h] : g.whole[h - much], count = g.count[c], start = g.start[c];
         if (n > WINDOW && count <= SORTED) {
             int* held = reinterpret_cast<int*>(bits);
             int size  = 2 * LIGHT;
@@ -609,7 +627,8 @@ Groups groups_in(Space& space, const mimk_embedding_desc& d) {
     g.heavy = static_cast<int4*>(space.take((size_t(d.n) / LIGHT + size_t(d.n) / PIECE) * 16));
     g.part_pitch = up(d.d, 8), g.part = static_cast<float*>(space.take(size_t(d.n) / PIECE * 2 * size_t(g.part_pitch) * 4));
     g.light = static_cast<int*>(space.take(size_t(d.n) * 4));
-    g.cursor = static_cast<int*>(space.take(24));
+    g.wholes = d.n / LIGHT, g.whole = static_cast<int*>(space.take(size_t(g.wholes) * 4));
+    g.cursor = static_cast<int*>(space.take(CURSORS * 4));
     return g;
 }
 
