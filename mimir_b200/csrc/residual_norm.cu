@@ -836,6 +836,11 @@ int check(const Desc* d) {
     if (!d->h && !d->gamma) return MIMK_E_ARG;  // (nothing to do)
     return MIMK_OK;
 }
+// Rows of one group: all of them without a gate, and no more than there are.
+int64_t group_rows(const Desc& d) {
+    const int64_t all = d.n > 0 ? d.n : 1;
+    return d.gate && d.gate_rows < all ? d.gate_rows : all;
+}
 bool off(const void* p, int dtype) { return reinterpret_cast<uintptr_t>(p) % dtype_size(dtype) != 0; }
 int misplaced(const Desc& d) {
     for (const void* p : {d.r, static_cast<const void*>(d.r_out), d.dr_out, static_cast<const void*>(d.dr)})
@@ -868,7 +873,7 @@ struct Plan {
 Plan plan(const Desc& d, bool backward, bool aligned, Space& space, int sm_count) {
     Plan p{};
     const size_t pair = dtype_size(d.stream_dtype) + dtype_size(d.block_dtype);
-    const int64_t run = d.gate ? d.gate_rows : (d.n > 0 ? d.n : 1);
+    const int64_t run = group_rows(d);
     p.groups          = (d.n + run - 1) / run;
     int classes       = 8;
     while (classes > 1 && d.d % (16 / classes) == 0) classes /= 2;
@@ -920,7 +925,7 @@ Plan plan(const Desc& d, bool backward, bool aligned, Space& space, int sm_count
 template <class RT, class HT>
 Args<RT, HT> args_of(const Desc& d) {
     Args<RT, HT> g{};
-    g.n = d.n, g.d = d.d, g.gate_rows = d.gate ? d.gate_rows : (d.n > 0 ? d.n : 1);
+    g.n = d.n, g.d = d.d, g.gate_rows = group_rows(d);
     g.r = static_cast<const RT*>(d.r), g.h = static_cast<const HT*>(d.h);
     g.gamma = {d.gamma, d.gamma_dtype == MIMK_BF16}, g.post_gamma = {d.post_gamma, d.post_gamma_dtype == MIMK_BF16}, g.gate = {d.gate, d.gate_dtype == MIMK_BF16};
     g.r_out = static_cast<RT*>(d.r_out), g.x = static_cast<HT*>(d.x), g.kept = d.kept;
