@@ -909,8 +909,8 @@ Plan plan(const Desc& d, bool backward, bool aligned, Space& space, int sm_count
     } else {
         const int64_t each = d.d <= 2048 ? 8 : d.d <= 8192 ? 16 : 32, lanes = up((d.d + each - 1) / each, 32);
         p.threads = int(lanes), p.rows = lanes == 32 ? 4 : 1;
-        const int64_t most = int64_t(sm_count) * (lanes <= 128 ? 4 : lanes <= 256 ? 2 : 1), need = (d.n + p.rows - 1) / p.rows;
-        p.blocks = int(need < most ? (need < 1 ? 1 : need) : most);
+        const int64_t need = (d.n + p.rows - 1) / p.rows;
+        p.blocks = int(need < (1 << 20) ? need : 1 << 20);
     }
     if (p.pieces > run) p.pieces = run;
     if (!backward) return p;
@@ -970,9 +970,11 @@ int forward(const Desc& d, const Plan& p, const DeviceInfo& dev, cudaStream_t s)
     Args<RT, HT> g = args_of<RT, HT>(d);
     g.groups = p.groups, g.pieces = p.pieces;
     if (p.ring) return with_columns(p, [&](auto columns, auto ragged, auto several) { return launch_ring<forward_ring_kernel<RT, HT, columns.value, ragged.value, several.value>>(p, g, dev, s); });
-    const auto kern = d.d <= 2048 ? forward_kernel<RT, HT, VEC, 8 / VEC, 256> : d.d <= 8192 ? forward_kernel<RT, HT, VEC, 16 / VEC, 512> : forward_kernel<RT, HT, VEC, 32 / VEC, 1024>;
-    const int64_t blocks = (d.n + p.rows - 1) / p.rows;
-    return launch(kern, dim3(unsigned(blocks < (1 << 20) ? blocks : 1 << 20)), dim3(p.threads, p.rows), s, g);
+    auto kern = forward_kernel<RT, HT, VEC, 32 / VEC, 1024>;
+    if constexpr (VEC == 1) {  // (whole rows of up to 8192 columns are planned with a ring)
+        if (d.d <= 8192) kern = d.d <= 2048 ? forward_kernel<RT, HT, 1, 8, 256> : forward_kernel<RT, HT, 1, 16, 512>;
+    }
+    return launch(kern, dim3(unsigned(p.blocks)), dim3(p.threads, p.rows), s, g);
 }
 template <class RT, class HT, int VEC>
 int backward(const Desc& d, const Plan& p, const DeviceInfo& dev, cudaStream_t s) {
