@@ -584,8 +584,8 @@ __global__ void __launch_bounds__(PREPARE) prepare_kernel(const __grid_constant_
 // ---- small matrices --------------------------------------------------------------------------------------------------------------
 // All steps of a matrix with up to 128 rows and 256 columns (or turned: 256 and 128) in one CTA: X as f32 in tensor memory and as two f16 in shared memory, 64 columns to a
 // 128-byte row, of which the first serves as the operand of X X^T and both as the right one of B X; A, then B, as f16 in another such matrix. Eight warps: 32 rows, one to a lane, and half of
-// the columns each. A step of [128, 128] takes 5 us: its three products 900 cycles each (issued by one thread), the rest what is between them. 64 matrices: 27 us (141 by launches of
-// their own for each product, from which matrices that do not fit here are taken).
+// the columns each. A step of [128, 128] takes 5 us: its three products 900 cycles each (issued by one thread), the rest what is between them. 64 matrices: 27 us a call
+// among others, 34 with cold caches (30 without X's second f16; 141 by launches of their own for each product, from which matrices that do not fit here are taken).
 constexpr int SMALL_K = 128, SMALL_L = 256, SMALL_THREADS = 256, CHUNK64 = 128 * 128;  // bytes of 128 rows of 64 columns
 constexpr int MOST_STEPS = 64;
 struct Factors {
