@@ -423,8 +423,9 @@ int mimk_clip_grads(const void* const* tensors, void* const* out, const int64_t*
  * has_ignore: a position whose id is ignore_index, a class or not, has no token: its row of the result is zeros, and its row of dy is not read.
  * Any other id outside [0, v) is recorded (mimk_device_status: MIMK_E_SHAPE); its row of the result is NaN, and nothing of it enters dtable.
  * Sums are f32, over positions in rising order in groups that the extents and ids alone decide, rounded once: equal descriptors and ids give equal bits. No
- * operand overlaps a result. n < 2^31 - 2^17, d and v < 2^31 (v d may be more), rows are dense. Workspace as above, of embedding_grad only: none up to 2048 positions; otherwise 8 bytes per
- * class, 17 per position, and an f32 row of d for each 256 positions. */
+ * operand overlaps a result. n < 2^31 - 2^17, d and v < 2^31 (v d may be more), rows are dense. Workspace as above, of embedding_grad only: none up to 2048 positions of up to 16776960
+ * features; otherwise 8 bytes per class, 17 per position, and an f32 row of d for each 256 positions. Its blocks wait for one another then: should one not come in a second or more, the gradient is
+ * left unfinished and the status recorded (MIMK_E_DEVICE_WAIT). */
 typedef struct mimk_embedding_desc {
     int64_t n, d, v;   /* positions, features, classes */
     const void* table; /* [v, d] of dtype */
@@ -450,7 +451,7 @@ int mimk_embedding_grad(const mimk_embedding_desc* desc, void* stream);
  * and F32, F32 and BF16, or BF16 and BF16; gamma, post_gamma, gate and their gradients each F32 or BF16.
  * x is of r_out before its rounding. kept: fwd leaves what bwd takes of each row's sums, 2 n f32 (NULL: nothing is left); bwd computes r_out over again from r and h.
  * All sums are f32; gradients of gamma, post_gamma and gate are summed over rows in an order that the extents alone decide: equal descriptors give equal bits.
- * r_out may be r, and dr may be dr_out; no other result overlaps an operand. d <= 32768, n < 2^31 - 2^17. Workspace as above, of bwd only. */
+ * r_out may be r where no bwd follows (bwd takes the r that fwd read), and dr may be dr_out; no other result overlaps an operand. d <= 32768, n < 2^31 - 2^17. Workspace as above, of bwd only. */
 typedef struct mimk_residual_rmsnorm_desc {
     int64_t n, d, gate_rows;
     const void* r; /* [n, d], so h, r_out, x and their gradients */

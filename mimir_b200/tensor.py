@@ -638,7 +638,8 @@ def embedding(table: torch.Tensor, ids: torch.Tensor, *, scale: float = 1.0, ign
 def embedding_grad(dy: torch.Tensor, ids: torch.Tensor, classes: int, *, scale: float = 1.0, ignore_index: int | None = None, out_dtype=None,
                    add_to: torch.Tensor | None = None) -> torch.Tensor:
     """The gradient of embedding's table [classes, features] from its result's gradient dy [*ids.shape, features]: row c is scale times the sum of dy's rows whose id is c,
-    in f32, the same call after call. Positions without a token and ids that are no class add nothing; the latter make device_status() raise. add_to: a gradient of the table's
+    in f32, the same call after call. Positions without a token and ids that are no class add nothing; the latter make device_status() raise, as does a launch of more
+    than 2048 positions whose blocks have waited for one another in vain, which leaves the result unfinished. add_to: a gradient of the table's
     (of a tied output layer, or of an earlier part of the batch) that the sums are added to, in place, and which is returned; rows of classes that do not occur are not touched."""
     if add_to is None and (out := _native.embedding_grad(dy, ids, classes, scale, ignore_index, out_dtype)) is not None:
         return out
